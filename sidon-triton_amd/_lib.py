@@ -1,5 +1,5 @@
-"""ctypes binding of libsidon_flexrel.so (the C ABI in include/sidon_flexrel.h and
-include/sidon_encoder.h).
+"""ctypes binding of libsidon_flexrel.so (the C ABI in include/sidon_flexrel.h,
+include/sidon_encoder.h and include/sidon_operators.h).
 
 There is no fallback: if the library is missing or fails to load, every entry
 point raises.  The library is built by ``build.py`` (or ``__graft_entry__.build()``).
@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import ctypes
 from pathlib import Path
+
+import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libsidon_flexrel.so"
 
@@ -79,9 +81,17 @@ SIGNATURES = {
     "sidon_fbank_normalize_noalloc": (ctypes.c_int, [_VP, _VP, _VP, ctypes.c_int, ctypes.c_int, _VP]),
     "sidon_stage_items": (ctypes.c_int, [_VP, ctypes.c_int64, _VP, ctypes.c_int64, _I64P, _VP, _IP, _VP, _IP,
                                          ctypes.c_int, _VP]),
+    "sidon_group_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 5),
+    "sidon_group_norm_act": (ctypes.c_int, [_VP, ctypes.c_int64, _VP, _VP, _VP, ctypes.c_float, _VP, ctypes.c_int64,
+                                            _VP, ctypes.c_size_t, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                            ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP]),
     "sidon_last_error": (ctypes.c_char_p, []),
     "sidon_version": (ctypes.c_char_p, []),
 }
+
+# Element type and activation codes of include/sidon_operators.h.
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "relu": 3}
 
 _lib = None
 

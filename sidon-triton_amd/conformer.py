@@ -16,6 +16,11 @@ Same names and argument meaning as src/sidon_triton/triton_encoder.py:
   * ``residual_gemm`` / ``residual_partials``: the projections into the fp32
     stream (:491-492), in place or as partial sums for the next norm;
 
+  * ``group_norm_act(x, batch, groups, w, b, eps)``: group norm with an
+    activation over the valid frames, the norm that a conv module without
+    LayerNorm has in its place (no counterpart in the reference;
+    csrc/group_norm.hip, include/sidon_operators.h);
+
 plus ``glu_causal_dw_norm(h, ...)``, the two fused: it reads the pointwise
 conv's output h [B*T, 2C] and forms g on the fly (bit-identical to
 ``causal_dw_norm(glu(h), ...)``, without the g round trip through HBM).
@@ -116,6 +121,73 @@ def glu_causal_dw_norm(h: torch.Tensor, batch: int, dwt: torch.Tensor, ln_w: tor
                        eps: float, out: torch.Tensor | None = None) -> torch.Tensor:
     """causal_dw_norm(glu(h), ...) in one pass: h [B*T, 2C] fp16."""
     return _dw(h, True, batch, dwt, ln_w, ln_b, eps, out)
+
+
+def group_norm_act(x: torch.Tensor, batch: int, groups: int, w: torch.Tensor, b: torch.Tensor, eps: float = 1e-5,
+                   lens: torch.Tensor | None = None, act: str | None = "silu", out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """act((x - mean) * rsqrt(var + eps) * w + b) [B*T, C]: group norm, channels
+    last, over each item's valid frames.
+
+    x [B*T, C] fp16, bf16 or fp32 (channels contiguous, any row stride), w and b
+    [C] fp32, lens int32 [B] valid frames on the device (None: all T, clamped to
+    [0, T]); mean and biased variance over the frames t < lens[b] of a group's
+    C / groups channels.  Frames past an item's length take no part, whatever
+    they hold, and come back as zeros.  act: None, "silu", "gelu" (the erf form)
+    or "relu".  out may be x itself.  workspace: a contiguous uint8 tensor of
+    ``group_norm_workspace`` bytes; allocated per call when None.  Forward only."""
+    device = x.device
+    _check_device_tensor("x", x, device)
+    if x.dtype not in _lib.DTYPES or x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError("x must be a float16, bfloat16 or float32 [R, C] tensor with channels contiguous")
+    rows, c = x.shape
+    if batch < 1 or rows < 1 or rows % batch:
+        raise ValueError(f"{rows} rows do not split into {batch} items")
+    if groups < 1 or c % groups:
+        raise ValueError(f"{c} channels do not split into {groups} groups")
+    if act not in _lib.ACTIVATIONS:
+        raise ValueError(f"act must be one of {list(_lib.ACTIVATIONS)} (got {act!r})")
+    for name, t in (("w", w), ("b", b)):
+        _check_device_tensor(name, t, device)
+        if t.dtype != torch.float32 or tuple(t.shape) != (c,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 [{c}] tensor")
+    if lens is not None:
+        _check_device_tensor("lens", lens, device)
+        if lens.dtype != torch.int32 or tuple(lens.shape) != (batch,) or not lens.is_contiguous():
+            raise ValueError("lens must be a contiguous int32 tensor of shape [B]")
+    if not plain(x, w, b):
+        raise ValueError("group_norm_act has no backward: call it under torch.no_grad()")
+    if out is None:
+        out = torch.empty(rows, c, device=device, dtype=x.dtype)
+    else:
+        _check_device_tensor("out", out, device)
+        if out.dtype != x.dtype or tuple(out.shape) != (rows, c) or out.stride(1) != 1:
+            raise ValueError(f"out must be a {x.dtype} [{rows}, {c}] tensor with channels contiguous")
+    lib = _lib.load()
+    need = group_norm_workspace(batch, rows // batch, c, groups, x.dtype)
+    if workspace is None:
+        workspace = torch.empty(max(need, 8), device=device, dtype=torch.uint8)
+    else:
+        _check_device_tensor("workspace", workspace, device)
+        if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+            raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
+    with _on_device(device):
+        rc = lib.sidon_group_norm_act(x.data_ptr(), _row_stride(x), None if lens is None else lens.data_ptr(),
+                                      w.data_ptr(), b.data_ptr(), ctypes.c_float(float(eps)), out.data_ptr(),
+                                      _row_stride(out), workspace.data_ptr(), workspace.numel(), batch, rows // batch,
+                                      c, groups, _lib.DTYPES[x.dtype], _lib.ACTIVATIONS[act], _stream_handle(device))
+    _lib.check("sidon_group_norm_act", rc)
+    return out
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between rows; a single row's stride means nothing."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def group_norm_workspace(batch: int, length: int, channels: int, groups: int, dtype: torch.dtype) -> int:
+    """Bytes of ``group_norm_act``'s workspace for [batch * length, channels]."""
+    return int(_lib.load().sidon_group_norm_workspace_bytes(batch, length, channels, groups, _lib.DTYPES[dtype]))
 
 
 def linear_silu_fits(x: torch.Tensor, w: torch.Tensor) -> bool:

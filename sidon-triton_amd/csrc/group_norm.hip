@@ -1,0 +1,589 @@
+// group_norm.hip -- group norm with an activation, channels last, over the
+// valid rows of B items (MI355X / gfx950):
+//
+//   y = act((x - mean_bg) * rsqrt(var_bg + eps) * w_c + bias_c)
+//
+// with mean and variance over an item's rows t < lens[b] and the C / G
+// channels of a group.  Memory bound: the floor is x once and y once.
+//
+// Two ways through it:
+//
+//   slab     one workgroup owns a whole (item, group), keeps its values in
+//            registers between the statistics and the store: one launch, x
+//            read once.  For groups whose rows fit a workgroup's registers.
+//   passes   workgroups over row chunks leave (mean, M2) per group, a second
+//            launch joins them and writes y: x read twice.
+//
+// Statistics never form a difference of large sums: every thread takes the
+// mean of what it holds and the squares around that mean, and partial results
+// (n, mean, M2) are joined by  M2 = sum M2_i + n_i (mean_i - mean)^2, in fp32.
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "sidon_host.h"
+#include "sidon_operators.h"
+#include "sidon_wave.h"
+
+#define SIDON_API extern "C" __attribute__((visibility("default")))
+#define SIDON_INLINE __attribute__((always_inline))
+
+namespace {
+
+constexpr int kMaxC = 8192;
+constexpr int kThreads = 256;      // of the two-pass kernels
+constexpr int kMaxChunks = 128;    // row chunks per item that the second pass joins
+constexpr int kStatWgs = 1024;     // workgroups a statistics launch aims for
+constexpr int kApplyWgs = 2048;
+constexpr int kSlabThreads = 1024;
+constexpr int kSlabVecs = 16;      // 16-byte vectors per thread that a slab may take
+
+struct Params {
+  const void* x;
+  const int32_t* lens;
+  const float* w;
+  const float* bias;
+  void* y;
+  float2* part;   // [B, chunks, G] (mean, M2)
+  int64_t ldx, ldy;
+  float eps;
+  int B, T, C, G, act;
+  int chunks, rows_per_chunk;       // statistics
+  int apply_rows;                   // rows per workgroup of the second pass
+};
+
+template <typename T, int V>
+struct Vec {
+  typedef T type __attribute__((ext_vector_type(V)));
+};
+template <typename T>
+struct Vec<T, 1> {
+  typedef T type;
+};
+
+// V elements at p (aligned to their size) as fp32, and back with one rounding.
+template <typename T, int V>
+__device__ __forceinline__ void load(const T* p, float (&v)[V]) {
+  const typename Vec<T, V>::type r = *reinterpret_cast<const typename Vec<T, V>::type*>(p);
+  if constexpr (V == 1) {
+    v[0] = (float)r;
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (float)r[e];
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float (&v)[V]) {
+  typename Vec<T, V>::type r;
+  if constexpr (V == 1) {
+    r = (T)v[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) r[e] = (T)v[e];
+  }
+  *reinterpret_cast<typename Vec<T, V>::type*>(p) = r;
+}
+
+// kExact: results kept in fp32, where the hardware exponential's and
+// reciprocal's error (about |v| 2^-24) would show; 16-bit results hide it.
+template <bool kExact, int V>
+__device__ __forceinline__ void activate(float (&v)[V], int act) {
+  if (act == SIDON_ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      v[e] = kExact ? v[e] / (1.f + expf(-v[e])) : v[e] * __builtin_amdgcn_rcpf(1.f + __expf(-v[e]));
+  } else if (act == SIDON_ACT_GELU) {
+    // erfc keeps the far negative side's digits, where 1 + erf loses them
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] *= 0.5f * erfcf(-0.70710678118654752f * v[e]);
+  } else if (act == SIDON_ACT_RELU) {
+    // (a comparison, so that NaN stays NaN)
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+  }
+}
+
+__device__ __forceinline__ int valid_rows(const Params& p, int b) {
+  return p.lens == nullptr ? p.T : min(max(p.lens[b], 0), p.T);
+}
+
+// ---- slab -------------------------------------------------------------------------
+
+// TH threads hold TH x NV vectors of 16 bytes: all T rows of one group.
+// Neighbouring groups share cache lines where a group's row is under 128
+// bytes, so each XCD (workgroups go round-robin over the 8) takes a contiguous
+// range of groups.
+template <typename T, int NV, int TH>
+__global__ void __launch_bounds__(TH) gn_slab_kernel(const Params p) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int kWaves = TH / 64;
+  __shared__ float red[2][kWaves];
+  const int xcd = blockIdx.x & 7, per = gridDim.x >> 3, rem = gridDim.x & 7;
+  const int lin = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + ((int)blockIdx.x >> 3);
+  const int b = lin / p.G;
+  const int g = lin - b * p.G;
+  const int cg = p.C / p.G;
+  const int vpr = cg / V;
+  const int n = valid_rows(p, b);
+  const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.T * p.ldx + g * cg;
+  T* y = static_cast<T*>(p.y) + (int64_t)b * p.T * p.ldy + g * cg;
+
+  // Vector j of a thread: number threadIdx.x + TH j of the slab.
+  const int row0 = (int)threadIdx.x / vpr, col0 = (int)threadIdx.x - row0 * vpr;
+  const int drow = TH / vpr, dcol = TH - drow * vpr;
+  typedef typename Vec<T, V>::type vec_t;
+  vec_t raw[NV];
+  {
+    int row = row0, col = col0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      raw[j] = vec_t{};
+      if (row < n) raw[j] = *reinterpret_cast<const vec_t*>(x + row * p.ldx + col * V);
+      row += drow;
+      col += dcol;
+      if (col >= vpr) {
+        col -= vpr;
+        ++row;
+      }
+    }
+  }
+  auto block_sum = [&](float v, int which) SIDON_INLINE {
+    v = sidon::wave_sum(v);
+    if ((threadIdx.x & 63) == 0) red[which][threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) s += red[which][i];
+    return s;
+  };
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum += (float)raw[j][e];
+  const float inv = n > 0 ? 1.f / ((float)n * (float)cg) : 0.f;
+  const float mean = block_sum(sum, 0) * inv;
+  float sq = 0.f;
+  {
+    int row = row0, col = col0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (row < n) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float d = (float)raw[j][e] - mean;
+          sq = fmaf(d, d, sq);
+        }
+      }
+      row += drow;
+      col += dcol;
+      if (col >= vpr) {
+        col -= vpr;
+        ++row;
+      }
+    }
+  }
+  const float rstd = rsqrtf(block_sum(sq, 1) * inv + p.eps);
+  int row = row0, col = col0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (row < p.T) {
+      float v[V] = {};
+      if (row < n) {
+        float w[V], bias[V];
+        load<float, V>(p.w + g * cg + col * V, w);
+        load<float, V>(p.bias + g * cg + col * V, bias);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = fmaf(((float)raw[j][e] - mean) * rstd, w[e], bias[e]);
+        activate<sizeof(T) == 4, V>(v, p.act);
+      }
+      store<T, V>(y + row * p.ldy + col * V, v);
+    }
+    row += drow;
+    col += dcol;
+    if (col >= vpr) {
+      col -= vpr;
+      ++row;
+    }
+  }
+}
+
+// ---- two passes -------------------------------------------------------------------
+
+// Lanes of a power-of-two team (of consecutive lanes of a wavefront).
+__device__ __forceinline__ float team_sum(float v, int team) {
+  for (int o = team >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// The threads of a workgroup over C channels: a thread owns one vector of V
+// columns and every `lanes`-th row (or, past kThreads vectors, a vector per
+// pass and every row).
+struct Layout {
+  int nv, lanes, passes;
+};
+template <int V>
+__device__ __forceinline__ Layout layout(int C) {
+  Layout l;
+  l.nv = C / V;
+  l.lanes = l.nv < kThreads ? kThreads / l.nv : 1;
+  l.passes = (l.nv + kThreads - 1) / kThreads;
+  return l;
+}
+
+// Team size for G groups on the workgroup's threads: all of them busy.
+__device__ __forceinline__ int team_size(int G) {
+  int t = 64;
+  while (t > 1 && t * G > kThreads) t >>= 1;
+  return t;
+}
+
+// (mean, M2) of each group over the rows of chunk blockIdx.x of item
+// blockIdx.y.  A unit is what a thread keeps one (mean, M2) for: its whole
+// vector where the vector lies in one group (kWide), else a channel.
+template <typename T, int V, bool kWide>
+__global__ void __launch_bounds__(kThreads) gn_stat_kernel(const Params p) {
+  constexpr int U = kWide ? 1 : V;
+  constexpr int kPer = kWide ? V : 1;        // values per row of a unit
+  constexpr int NB = V == 1 ? 16 : 8;        // rows held at once
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float2* unit = reinterpret_cast<float2*>(smem);
+  const int b = blockIdx.y;
+  const int r0 = blockIdx.x * p.rows_per_chunk;
+  const int r1 = min(r0 + p.rows_per_chunk, valid_rows(p, b));
+  if (r0 >= r1) return;   // the second pass counts the rows itself
+  const Layout l = layout<V>(p.C);
+  const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.T * p.ldx;
+  const int lr = l.passes == 1 ? (int)threadIdx.x / l.nv : 0;
+  for (int pass = 0; pass < l.passes; ++pass) {
+    const int vec = l.passes == 1 ? (int)threadIdx.x - lr * l.nv : pass * kThreads + (int)threadIdx.x;
+    if (lr >= l.lanes || vec >= l.nv) continue;
+    const T* xc = x + vec * V;
+    float mean[U] = {}, m2[U] = {};
+    float have = 0.f;   // values per unit so far
+    for (int r = r0 + lr; r < r1; r += NB * l.lanes) {
+      typedef typename Vec<T, V>::type vec_t;
+      float v[NB][V];
+      int rows = 0;
+      vec_t raw[NB];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int row = r + i * l.lanes;
+        raw[i] = vec_t{};
+        if (row < r1) {
+          raw[i] = *reinterpret_cast<const vec_t*>(xc + row * p.ldx);
+          ++rows;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        if constexpr (V == 1) {
+          v[i][0] = (float)raw[i];
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[i][e] = (float)raw[i][e];
+        }
+      }
+      const float more = (float)(rows * kPer);
+      const float inv = 1.f / more;
+      const float frac = more / (have + more);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) s += v[i][u * kPer + e];
+        const float m = s * inv;
+        float q = 0.f;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          if (i < rows) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+              const float d = v[i][u * kPer + e] - m;
+              q = fmaf(d, d, q);
+            }
+          }
+        }
+        const float delta = m - mean[u];
+        mean[u] = fmaf(delta, frac, mean[u]);
+        m2[u] += q + delta * delta * (have * frac);
+      }
+      have += more;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) unit[(lr * l.nv + vec) * U + u] = make_float2(mean[u], m2[u]);
+  }
+  __syncthreads();
+  // Join a group's units: per row lane, `cols` of them side by side.
+  const int cols = l.nv * U / p.G;
+  const int stride = l.nv * U;
+  const int cnt_rows = r1 - r0;
+  const int team = team_size(p.G);
+  const int tl = (int)threadIdx.x & (team - 1);
+  const float inv_n = 1.f / ((float)cnt_rows * (float)(p.C / p.G));
+  float2* out = p.part + ((int64_t)b * p.chunks + blockIdx.x) * p.G;
+  for (int g = (int)threadIdx.x / team; g < p.G; g += kThreads / team) {
+    float s = 0.f;
+    for (int i = 0; i < l.lanes; ++i) {
+      const float cnt = (float)(((cnt_rows - i + l.lanes - 1) / l.lanes) * kPer);
+      for (int c = tl; c < cols; c += team) s = fmaf(unit[i * stride + g * cols + c].x, cnt, s);
+    }
+    const float mean = team_sum(s, team) * inv_n;
+    float q = 0.f;
+    for (int i = 0; i < l.lanes; ++i) {
+      const float cnt = (float)(((cnt_rows - i + l.lanes - 1) / l.lanes) * kPer);
+      for (int c = tl; c < cols; c += team) {
+        const float2 v = unit[i * stride + g * cols + c];
+        const float d = v.x - mean;
+        q += fmaf(d * d, cnt, v.y);
+      }
+    }
+    const float m2 = team_sum(q, team);
+    if (tl == 0) out[g] = make_float2(mean, m2);
+  }
+}
+
+// Join the chunks' statistics of item blockIdx.y, then y for apply_rows rows.
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) gn_apply_kernel(const Params p) {
+  constexpr int NB = V == 1 ? 8 : 4;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float2* stat = reinterpret_cast<float2*>(smem);   // [G] (mean, rstd)
+  const int b = blockIdx.y;
+  const int r0 = blockIdx.x * p.apply_rows;
+  const int r1 = min(r0 + p.apply_rows, p.T);
+  const int n = valid_rows(p, b);
+  const int cg = p.C / p.G;
+  if (r0 < n) {
+    const int used = (n + p.rows_per_chunk - 1) / p.rows_per_chunk;
+    const int team = team_size(p.G);
+    const int tl = (int)threadIdx.x & (team - 1);
+    const float2* part = p.part + (int64_t)b * p.chunks * p.G;
+    const float inv_n = 1.f / ((float)n * (float)cg);
+    for (int g = (int)threadIdx.x / team; g < p.G; g += kThreads / team) {
+      float s = 0.f;
+#pragma unroll 4
+      for (int c = tl; c < used; c += team) {
+        const float cnt = (float)(min(p.rows_per_chunk, n - c * p.rows_per_chunk)) * (float)cg;
+        s = fmaf(part[(int64_t)c * p.G + g].x, cnt, s);
+      }
+      const float mean = team_sum(s, team) * inv_n;
+      float q = 0.f;
+#pragma unroll 4
+      for (int c = tl; c < used; c += team) {
+        const float cnt = (float)(min(p.rows_per_chunk, n - c * p.rows_per_chunk)) * (float)cg;
+        const float2 v = part[(int64_t)c * p.G + g];
+        const float d = v.x - mean;
+        q += fmaf(d * d, cnt, v.y);
+      }
+      const float var = team_sum(q, team) * inv_n;
+      if (tl == 0) stat[g] = make_float2(mean, rsqrtf(var + p.eps));
+    }
+  }
+  __syncthreads();
+  const Layout l = layout<V>(p.C);
+  const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.T * p.ldx;
+  T* y = static_cast<T*>(p.y) + (int64_t)b * p.T * p.ldy;
+  const int lr = l.passes == 1 ? (int)threadIdx.x / l.nv : 0;
+  for (int pass = 0; pass < l.passes; ++pass) {
+    const int vec = l.passes == 1 ? (int)threadIdx.x - lr * l.nv : pass * kThreads + (int)threadIdx.x;
+    if (lr >= l.lanes || vec >= l.nv) continue;
+    float mean[V], rstd[V], w[V], bias[V];
+    if (r0 < n) {
+      load<float, V>(p.w + vec * V, w);
+      load<float, V>(p.bias + vec * V, bias);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float2 s = stat[(vec * V + e) / cg];
+        mean[e] = s.x;
+        rstd[e] = s.y;
+      }
+    }
+    for (int r = r0 + lr; r < r1; r += NB * l.lanes) {
+      float v[NB][V];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int row = r + i * l.lanes;
+        if (row < r1 && row < n) load<T, V>(x + row * p.ldx + vec * V, v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int row = r + i * l.lanes;
+        if (row >= r1) break;
+        if (row < n) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[i][e] = fmaf((v[i][e] - mean[e]) * rstd[e], w[e], bias[e]);
+          activate<sizeof(T) == 4, V>(v[i], p.act);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[i][e] = 0.f;
+        }
+        store<T, V>(y + row * p.ldy + vec * V, v[i]);
+      }
+    }
+  }
+}
+
+// ---- host -------------------------------------------------------------------------
+
+int element_size(int dtype) { return dtype == SIDON_FP32 ? 4 : 2; }
+
+// Row chunks of the statistics: enough workgroups to fill the chip, a few rows
+// per thread at least, at most kMaxChunks for the second pass to join.
+void plan_chunks(Params& p, int vec) {
+  const int nv = p.C / vec;
+  const int lanes = nv < kThreads ? kThreads / nv : 1;
+  int chunks = kStatWgs / p.B;
+  if (chunks > kMaxChunks) chunks = kMaxChunks;
+  const int most = (p.T + 8 * lanes - 1) / (8 * lanes);
+  if (chunks > most) chunks = most;
+  if (chunks < 1) chunks = 1;
+  p.rows_per_chunk = (p.T + chunks - 1) / chunks;
+  p.chunks = (p.T + p.rows_per_chunk - 1) / p.rows_per_chunk;
+  int blocks = kApplyWgs / p.B;
+  const int most_apply = (p.T + 4 * lanes - 1) / (4 * lanes);
+  if (blocks > most_apply) blocks = most_apply;
+  if (blocks < 1) blocks = 1;
+  p.apply_rows = (p.T + blocks - 1) / blocks;
+}
+
+template <typename T, int NV, int TH>
+void slab_launch(const Params& p, hipStream_t stream) {
+  hipLaunchKernelGGL((gn_slab_kernel<T, NV, TH>), dim3((unsigned)(p.B * p.G)), dim3(TH), 0, stream, p);
+}
+
+template <typename T>
+void slab(const Params& p, int64_t vecs, hipStream_t stream) {
+  if (vecs <= 256 * 4) {
+    slab_launch<T, 4, 256>(p, stream);
+  } else if (vecs <= 1024 * 4) {
+    slab_launch<T, 4, 1024>(p, stream);
+  } else if (vecs <= 1024 * 8) {
+    slab_launch<T, 8, 1024>(p, stream);
+  } else {
+    slab_launch<T, kSlabVecs, kSlabThreads>(p, stream);
+  }
+}
+
+template <typename T, int V>
+void passes(const Params& p, hipStream_t stream) {
+  const bool wide = (p.C / p.G) % V == 0;
+  const int nv = p.C / V;
+  const int threads_used = nv < kThreads ? (kThreads / nv) * nv : nv;
+  const size_t unit_bytes = (size_t)threads_used * (wide ? 1 : V) * sizeof(float2);
+  const dim3 grid((unsigned)p.chunks, (unsigned)p.B);
+  if (wide) {
+    hipLaunchKernelGGL((gn_stat_kernel<T, V, true>), grid, dim3(kThreads), unit_bytes, stream, p);
+  } else {
+    hipLaunchKernelGGL((gn_stat_kernel<T, V, false>), grid, dim3(kThreads), unit_bytes, stream, p);
+  }
+  hipLaunchKernelGGL((gn_apply_kernel<T, V>), dim3((unsigned)((p.T + p.apply_rows - 1) / p.apply_rows), (unsigned)p.B),
+                     dim3(kThreads), (size_t)p.G * sizeof(float2), stream, p);
+}
+
+template <typename T>
+void run(Params& p, bool vector, hipStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const int cg = p.C / p.G;
+  const int64_t vecs = (int64_t)p.T * (cg / V);
+  if (vector && cg % V == 0 && vecs <= kSlabVecs * kSlabThreads && (int64_t)p.B * p.G <= INT32_MAX) {
+    slab<T>(p, vecs, stream);
+  } else if (vector) {
+    plan_chunks(p, V);
+    passes<T, V>(p, stream);
+  } else {
+    plan_chunks(p, 1);
+    passes<T, 1>(p, stream);
+  }
+}
+
+bool shape_ok(int B, int T, int C, int G, int dtype) {
+  return B >= 1 && T >= 1 && C >= 1 && C <= kMaxC && G >= 1 && C % G == 0 && dtype >= SIDON_FP32 && dtype <= SIDON_BF16 &&
+         B <= 65535;
+}
+
+// Whether x and y, as rows of C elements ld apart, share memory in any way
+// other than being the same tensor.
+bool overlap(const void* x, int64_t ldx, const void* y, int64_t ldy, int64_t rows, int C, int size) {
+  const uintptr_t xb = reinterpret_cast<uintptr_t>(x), yb = reinterpret_cast<uintptr_t>(y);
+  const uintptr_t xe = xb + (uintptr_t)(((rows - 1) * ldx + C) * size);
+  const uintptr_t ye = yb + (uintptr_t)(((rows - 1) * ldy + C) * size);
+  if (xb >= ye || yb >= xe || (xb == yb && ldx == ldy)) return false;
+  if (ldx == ldy) {   // column blocks of one wider tensor
+    const uintptr_t row = (uintptr_t)ldx * size, width = (uintptr_t)C * size;
+    const uintptr_t d = xb < yb ? (yb - xb) % row : (row - (xb - yb) % row) % row;
+    if (d >= width && row - d >= width) return false;
+  }
+  return true;
+}
+
+}  // namespace
+
+SIDON_API size_t sidon_group_norm_workspace_bytes(int B, int T, int C, int G, int dtype) {
+  if (!shape_ok(B, T, C, G, dtype)) return 0;
+  // The larger of what the two ways of splitting rows take; at most this many chunks.
+  int64_t chunks = kStatWgs / B;
+  if (chunks > kMaxChunks) chunks = kMaxChunks;
+  if (chunks < 1) chunks = 1;
+  if (chunks > T) chunks = T;
+  return (size_t)B * (size_t)chunks * (size_t)G * sizeof(float2);
+}
+
+SIDON_API int sidon_group_norm_act(const void* x, int64_t ldx, const int32_t* lens, const float* w, const float* bias,
+                                   float eps, void* y, int64_t ldy, void* ws, size_t ws_bytes, int B, int T, int C,
+                                   int G, int dtype, int act, sidon_stream_t stream) {
+  using sidon::fail;
+  sidon::clear_error();
+  if (!x || !w || !bias || !y || !ws) return fail(SIDON_E_NULL, "x, w, bias, y and ws must be non-NULL");
+  if (dtype < SIDON_FP32 || dtype > SIDON_BF16) return fail(SIDON_E_SHAPE, "dtype=%d is no SIDON_FP32 / FP16 / BF16", dtype);
+  if (act < SIDON_ACT_NONE || act > SIDON_ACT_RELU) return fail(SIDON_E_SHAPE, "act=%d is no SIDON_ACT_*", act);
+  if (!shape_ok(B, T, C, G, dtype))
+    return fail(SIDON_E_SHAPE, "B=%d T=%d C=%d G=%d: need B in [1, 65535], T >= 1, C in [1, %d], C a multiple of G", B,
+                T, C, G, kMaxC);
+  const int size = element_size(dtype);
+  const int64_t rows = (int64_t)B * T;
+  if (ldx < C || ldy < C || ldx > (int64_t(1) << 31) || ldy > (int64_t(1) << 31))
+    return fail(SIDON_E_STRIDE, "row strides ldx=%lld ldy=%lld must be >= C and at most 2^31", (long long)ldx,
+                (long long)ldy);
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % (uintptr_t)size != 0 ||
+      ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(bias)) & 3u) != 0 ||
+      (reinterpret_cast<uintptr_t>(lens) & 3u) != 0 || (reinterpret_cast<uintptr_t>(ws) & 7u) != 0)
+    return fail(SIDON_E_ALIGN, "x and y must be aligned to their elements, w, bias and lens to 4 bytes, ws to 8");
+  if (ws_bytes < sidon_group_norm_workspace_bytes(B, T, C, G, dtype))
+    return fail(SIDON_E_SHAPE, "ws holds %zu bytes, the call needs %zu", ws_bytes,
+                sidon_group_norm_workspace_bytes(B, T, C, G, dtype));
+  if (overlap(x, ldx, y, ldy, rows, C, size)) return fail(SIDON_E_SHAPE, "y may be x itself but must not overlap it otherwise");
+  int rc;
+  if ((rc = sidon::check_device())) return rc;
+  Params p{};
+  p.x = x;
+  p.lens = lens;
+  p.w = w;
+  p.bias = bias;
+  p.y = y;
+  p.part = static_cast<float2*>(ws);
+  p.ldx = ldx;
+  p.ldy = ldy;
+  p.eps = eps;
+  p.B = B;
+  p.T = T;
+  p.C = C;
+  p.G = G;
+  p.act = act;
+  const int v = 16 / size;
+  const bool vector = C % v == 0 && ldx % v == 0 && ldy % v == 0 && sidon::aligned16(x) && sidon::aligned16(y) &&
+                      sidon::aligned16(w) && sidon::aligned16(bias);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == SIDON_FP32) {
+    run<float>(p, vector, s);
+  } else if (dtype == SIDON_FP16) {
+    run<_Float16>(p, vector, s);
+  } else {
+    run<__bf16>(p, vector, s);
+  }
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return fail(SIDON_E_LAUNCH, "group norm launch failed: %s", hipGetErrorString(err));
+  return SIDON_OK;
+}
