@@ -32,7 +32,8 @@ namespace {
 
 constexpr int kMaxC = 8192;
 constexpr int kThreads = 256;      // of the two-pass kernels
-constexpr int kMaxChunks = 128;    // row chunks per item that the second pass joins
+constexpr int kMaxChunks = 64;     // row chunks per item that the second pass joins
+constexpr int kBlockVecs = 32;     // vectors per row of a column block, or one group
 constexpr int kStatWgs = 1024;     // workgroups a statistics launch aims for
 constexpr int kApplyWgs = 2048;
 constexpr int kSlabThreads = 1024;
@@ -48,6 +49,7 @@ struct Params {
   int64_t ldx, ldy;
   float eps;
   int B, T, C, G, act;
+  int block_groups;                 // groups per column block of the two passes
   int chunks, rows_per_chunk;       // statistics
   int apply_rows;                   // rows per workgroup of the second pass
 };
@@ -84,6 +86,24 @@ __device__ __forceinline__ void store(T* p, const float (&v)[V]) {
   *reinterpret_cast<typename Vec<T, V>::type*>(p) = r;
 }
 
+// erfc(z) for z >= 0: e^(-z^2) times a polynomial in t = 1 / (1 + 0.4 z), fitted
+// to erfc(z) e^(z^2) over [0, 40] for the least relative error (1.3e-7, 3e-7
+// with fp32 arithmetic).  erfcf costs a memory-bound kernel three times as much
+// arithmetic (1463 x 64 values of bf16 on a CU: 27 us against 15 with SiLU).
+__device__ __forceinline__ float erfc_positive(float z) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.4f, z, 1.f));
+  float c = 0.0500626639f;
+  c = fmaf(c, t, -0.182005256f);
+  c = fmaf(c, t, 0.167402819f);
+  c = fmaf(c, t, -0.00389658613f);
+  c = fmaf(c, t, 0.140410721f);
+  c = fmaf(c, t, 0.168903336f);
+  c = fmaf(c, t, 0.207769737f);
+  c = fmaf(c, t, 0.225677118f);
+  c = fmaf(c, t, 0.225675568f);
+  return c * t * __expf(-z * z);
+}
+
 // kExact: results kept in fp32, where the hardware exponential's and
 // reciprocal's error (about |v| 2^-24) would show; 16-bit results hide it.
 template <bool kExact, int V>
@@ -93,14 +113,33 @@ __device__ __forceinline__ void activate(float (&v)[V], int act) {
     for (int e = 0; e < V; ++e)
       v[e] = kExact ? v[e] / (1.f + expf(-v[e])) : v[e] * __builtin_amdgcn_rcpf(1.f + __expf(-v[e]));
   } else if (act == SIDON_ACT_GELU) {
-    // erfc keeps the far negative side's digits, where 1 + erf loses them
+    // v / 2 erfc(-v / sqrt 2): erfc keeps the far negative side's digits, where 1 + erf loses them
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] *= 0.5f * erfcf(-0.70710678118654752f * v[e]);
+    for (int e = 0; e < V; ++e) {
+      if constexpr (kExact) {
+        v[e] *= 0.5f * erfcf(-0.70710678118654752f * v[e]);
+      } else {
+        const float half = 0.5f * erfc_positive(0.70710678118654752f * fabsf(v[e]));
+        v[e] *= v[e] < 0.f ? half : 1.f - half;
+      }
+    }
   } else if (act == SIDON_ACT_RELU) {
     // (a comparison, so that NaN stays NaN)
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
   }
+}
+
+// Keeps what is computed from r on either side of this apart: without it the
+// compiler keeps a slab's fp32 values live between its passes, twice the
+// registers (181 of them spilled at 16 vectors of fp16 a thread).
+template <typename R>
+__device__ __forceinline__ void opaque(R& r) {
+  typedef int int4_t __attribute__((ext_vector_type(4)));
+  static_assert(sizeof(R) == sizeof(int4_t), "16-byte vectors");
+  int4_t v = __builtin_bit_cast(int4_t, r);
+  asm volatile("" : "+v"(v));
+  r = __builtin_bit_cast(R, v);
 }
 
 __device__ __forceinline__ int valid_rows(const Params& p, int b) {
@@ -166,8 +205,10 @@ __global__ void __launch_bounds__(TH) gn_slab_kernel(const Params p) {
   float sq = 0.f;
   {
     int row = row0, col = col0;
+    asm volatile("" : "+v"(row), "+v"(col));   // (the same for the indices)
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      opaque(raw[j]);
       if (row < n) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -185,11 +226,13 @@ __global__ void __launch_bounds__(TH) gn_slab_kernel(const Params p) {
   }
   const float rstd = rsqrtf(block_sum(sq, 1) * inv + p.eps);
   int row = row0, col = col0;
+  asm volatile("" : "+v"(row), "+v"(col));
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     if (row < p.T) {
       float v[V] = {};
       if (row < n) {
+        opaque(raw[j]);
         float w[V], bias[V];
         load<float, V>(p.w + g * cg + col * V, w);
         load<float, V>(p.bias + g * cg + col * V, bias);
@@ -238,6 +281,20 @@ __device__ __forceinline__ int team_size(int G) {
   return t;
 }
 
+// The columns of block blockIdx.z: whole groups, whole vectors.
+struct Block {
+  int g0, groups, c0, cols;
+};
+__device__ __forceinline__ Block column_block(const Params& p) {
+  Block k;
+  const int cg = p.C / p.G;
+  k.g0 = (int)blockIdx.z * p.block_groups;
+  k.groups = min(p.block_groups, p.G - k.g0);
+  k.c0 = k.g0 * cg;
+  k.cols = k.groups * cg;
+  return k;
+}
+
 // (mean, M2) of each group over the rows of chunk blockIdx.x of item
 // blockIdx.y.  A unit is what a thread keeps one (mean, M2) for: its whole
 // vector where the vector lies in one group (kWide), else a channel.
@@ -252,8 +309,9 @@ __global__ void __launch_bounds__(kThreads) gn_stat_kernel(const Params p) {
   const int r0 = blockIdx.x * p.rows_per_chunk;
   const int r1 = min(r0 + p.rows_per_chunk, valid_rows(p, b));
   if (r0 >= r1) return;   // the second pass counts the rows itself
-  const Layout l = layout<V>(p.C);
-  const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.T * p.ldx;
+  const Block k = column_block(p);
+  const Layout l = layout<V>(k.cols);
+  const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.T * p.ldx + k.c0;
   const int lr = l.passes == 1 ? (int)threadIdx.x / l.nv : 0;
   for (int pass = 0; pass < l.passes; ++pass) {
     const int vec = l.passes == 1 ? (int)threadIdx.x - lr * l.nv : pass * kThreads + (int)threadIdx.x;
@@ -317,14 +375,14 @@ __global__ void __launch_bounds__(kThreads) gn_stat_kernel(const Params p) {
   }
   __syncthreads();
   // Join a group's units: per row lane, `cols` of them side by side.
-  const int cols = l.nv * U / p.G;
+  const int cols = l.nv * U / k.groups;
   const int stride = l.nv * U;
   const int cnt_rows = r1 - r0;
-  const int team = team_size(p.G);
+  const int team = team_size(k.groups);
   const int tl = (int)threadIdx.x & (team - 1);
   const float inv_n = 1.f / ((float)cnt_rows * (float)(p.C / p.G));
-  float2* out = p.part + ((int64_t)b * p.chunks + blockIdx.x) * p.G;
-  for (int g = (int)threadIdx.x / team; g < p.G; g += kThreads / team) {
+  float2* out = p.part + ((int64_t)b * p.chunks + blockIdx.x) * p.G + k.g0;
+  for (int g = (int)threadIdx.x / team; g < k.groups; g += kThreads / team) {
     float s = 0.f;
     for (int i = 0; i < l.lanes; ++i) {
       const float cnt = (float)(((cnt_rows - i + l.lanes - 1) / l.lanes) * kPer);
@@ -350,19 +408,20 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) gn_apply_kernel(const Params p) {
   constexpr int NB = V == 1 ? 8 : 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float2* stat = reinterpret_cast<float2*>(smem);   // [G] (mean, rstd)
+  float2* stat = reinterpret_cast<float2*>(smem);   // of the block's groups: (mean, rstd)
   const int b = blockIdx.y;
   const int r0 = blockIdx.x * p.apply_rows;
   const int r1 = min(r0 + p.apply_rows, p.T);
   const int n = valid_rows(p, b);
   const int cg = p.C / p.G;
+  const Block k = column_block(p);
   if (r0 < n) {
     const int used = (n + p.rows_per_chunk - 1) / p.rows_per_chunk;
-    const int team = team_size(p.G);
+    const int team = team_size(k.groups);
     const int tl = (int)threadIdx.x & (team - 1);
-    const float2* part = p.part + (int64_t)b * p.chunks * p.G;
+    const float2* part = p.part + (int64_t)b * p.chunks * p.G + k.g0;
     const float inv_n = 1.f / ((float)n * (float)cg);
-    for (int g = (int)threadIdx.x / team; g < p.G; g += kThreads / team) {
+    for (int g = (int)threadIdx.x / team; g < k.groups; g += kThreads / team) {
       float s = 0.f;
 #pragma unroll 4
       for (int c = tl; c < used; c += team) {
@@ -383,17 +442,17 @@ __global__ void __launch_bounds__(kThreads) gn_apply_kernel(const Params p) {
     }
   }
   __syncthreads();
-  const Layout l = layout<V>(p.C);
-  const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.T * p.ldx;
-  T* y = static_cast<T*>(p.y) + (int64_t)b * p.T * p.ldy;
+  const Layout l = layout<V>(k.cols);
+  const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.T * p.ldx + k.c0;
+  T* y = static_cast<T*>(p.y) + (int64_t)b * p.T * p.ldy + k.c0;
   const int lr = l.passes == 1 ? (int)threadIdx.x / l.nv : 0;
   for (int pass = 0; pass < l.passes; ++pass) {
     const int vec = l.passes == 1 ? (int)threadIdx.x - lr * l.nv : pass * kThreads + (int)threadIdx.x;
     if (lr >= l.lanes || vec >= l.nv) continue;
     float mean[V], rstd[V], w[V], bias[V];
     if (r0 < n) {
-      load<float, V>(p.w + vec * V, w);
-      load<float, V>(p.bias + vec * V, bias);
+      load<float, V>(p.w + k.c0 + vec * V, w);
+      load<float, V>(p.bias + k.c0 + vec * V, bias);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float2 s = stat[(vec * V + e) / cg];
@@ -430,23 +489,33 @@ __global__ void __launch_bounds__(kThreads) gn_apply_kernel(const Params p) {
 
 int element_size(int dtype) { return dtype == SIDON_FP32 ? 4 : 2; }
 
-// Row chunks of the statistics: enough workgroups to fill the chip, a few rows
-// per thread at least, at most kMaxChunks for the second pass to join.
-void plan_chunks(Params& p, int vec) {
-  const int nv = p.C / vec;
+// Column blocks of whole groups and about kBlockVecs vectors: whole cache
+// lines per row, and only these groups' partial results to join.  Row chunks:
+// enough workgroups to fill the chip, a few rows per thread at least, at most
+// kMaxChunks for the second pass to join.  (With all columns in a block and 128
+// chunks, joining 128 x 32 groups in every workgroup of the second pass took
+// as long as its rows: 1 x 4800 x 1024 fp16 21 us against 13.)
+void plan_passes(Params& p, int vec) {
+  const int cg = p.C / p.G;
+  int step = 1;   // groups whose channels are whole vectors
+  while (step * cg % vec != 0) ++step;
+  int groups = (kBlockVecs * vec + cg * step - 1) / (cg * step) * step;
+  if (groups > p.G) groups = p.G;
+  p.block_groups = groups;
+  const int blocks = (p.G + groups - 1) / groups;
+  const int nv = groups * cg / vec;
   const int lanes = nv < kThreads ? kThreads / nv : 1;
-  int chunks = kStatWgs / p.B;
-  if (chunks > kMaxChunks) chunks = kMaxChunks;
-  const int most = (p.T + 8 * lanes - 1) / (8 * lanes);
-  if (chunks > most) chunks = most;
-  if (chunks < 1) chunks = 1;
-  p.rows_per_chunk = (p.T + chunks - 1) / chunks;
+  const auto split = [&](int wgs, int rows, int most) {
+    int64_t n = wgs / ((int64_t)p.B * blocks);
+    const int64_t cap = (p.T + rows * lanes - 1) / (rows * lanes);
+    if (n > cap) n = cap;
+    if (n > most) n = most;
+    if (n < 1) n = 1;
+    return (int)((p.T + n - 1) / n);
+  };
+  p.rows_per_chunk = split(kStatWgs, 8, kMaxChunks);
   p.chunks = (p.T + p.rows_per_chunk - 1) / p.rows_per_chunk;
-  int blocks = kApplyWgs / p.B;
-  const int most_apply = (p.T + 4 * lanes - 1) / (4 * lanes);
-  if (blocks > most_apply) blocks = most_apply;
-  if (blocks < 1) blocks = 1;
-  p.apply_rows = (p.T + blocks - 1) / blocks;
+  p.apply_rows = split(kApplyWgs, 4, 65535);
 }
 
 template <typename T, int NV, int TH>
@@ -470,17 +539,19 @@ void slab(const Params& p, int64_t vecs, hipStream_t stream) {
 template <typename T, int V>
 void passes(const Params& p, hipStream_t stream) {
   const bool wide = (p.C / p.G) % V == 0;
-  const int nv = p.C / V;
+  const int nv = p.block_groups * (p.C / p.G) / V;
   const int threads_used = nv < kThreads ? (kThreads / nv) * nv : nv;
   const size_t unit_bytes = (size_t)threads_used * (wide ? 1 : V) * sizeof(float2);
-  const dim3 grid((unsigned)p.chunks, (unsigned)p.B);
+  const unsigned blocks = (unsigned)((p.G + p.block_groups - 1) / p.block_groups);
+  const dim3 grid((unsigned)p.chunks, (unsigned)p.B, blocks);
   if (wide) {
     hipLaunchKernelGGL((gn_stat_kernel<T, V, true>), grid, dim3(kThreads), unit_bytes, stream, p);
   } else {
     hipLaunchKernelGGL((gn_stat_kernel<T, V, false>), grid, dim3(kThreads), unit_bytes, stream, p);
   }
-  hipLaunchKernelGGL((gn_apply_kernel<T, V>), dim3((unsigned)((p.T + p.apply_rows - 1) / p.apply_rows), (unsigned)p.B),
-                     dim3(kThreads), (size_t)p.G * sizeof(float2), stream, p);
+  hipLaunchKernelGGL((gn_apply_kernel<T, V>), 
+                     dim3((unsigned)((p.T + p.apply_rows - 1) / p.apply_rows), (unsigned)p.B, blocks), dim3(kThreads),
+                     (size_t)p.block_groups * sizeof(float2), stream, p);
 }
 
 template <typename T>
@@ -488,13 +559,21 @@ void run(Params& p, bool vector, hipStream_t stream) {
   constexpr int V = 16 / sizeof(T);
   const int cg = p.C / p.G;
   const int64_t vecs = (int64_t)p.T * (cg / V);
-  if (vector && cg % V == 0 && vecs <= kSlabVecs * kSlabThreads && (int64_t)p.B * p.G <= INT32_MAX) {
+  // A workgroup takes about 3.5 us + 0.085 us/KB for its slab (fp16, SiLU; the
+  // CU's own rate), the two passes 10.5 us + 0.6 us/MB for the whole tensor, so
+  // a large slab pays only where many of them run at once.  us, slab | passes:
+  // 1 x 500 x 32 channels a group 6.0 | 11.5, 1 x 1463 x 32 10.7 | 11.7, 1 x 1463 x
+  // 64 18.5 | 12.0, 8 x 1500 x 64 21.5 | 25.8, fp32 1 x 1463 x 32 18.0 | 12.5, 4 x
+  // 1463 x 32 21.0 | 22.7, 8 x 1500 x 32 25.6 | 34.5.
+  const double slab_kb = vecs * 16.0 / 1024, all_mb = slab_kb * p.B * p.G / 1024;
+  if (vector && cg % V == 0 && vecs <= kSlabVecs * kSlabThreads && slab_kb <= 80 + 6 * all_mb &&
+      (int64_t)p.B * p.G <= INT32_MAX) {
     slab<T>(p, vecs, stream);
   } else if (vector) {
-    plan_chunks(p, V);
+    plan_passes(p, V);
     passes<T, V>(p, stream);
   } else {
-    plan_chunks(p, 1);
+    plan_passes(p, 1);
     passes<T, 1>(p, stream);
   }
 }
@@ -523,11 +602,7 @@ bool overlap(const void* x, int64_t ldx, const void* y, int64_t ldy, int64_t row
 
 SIDON_API size_t sidon_group_norm_workspace_bytes(int B, int T, int C, int G, int dtype) {
   if (!shape_ok(B, T, C, G, dtype)) return 0;
-  // The larger of what the two ways of splitting rows take; at most this many chunks.
-  int64_t chunks = kStatWgs / B;
-  if (chunks > kMaxChunks) chunks = kMaxChunks;
-  if (chunks < 1) chunks = 1;
-  if (chunks > T) chunks = T;
+  const int64_t chunks = T < kMaxChunks ? T : kMaxChunks;
   return (size_t)B * (size_t)chunks * (size_t)G * sizeof(float2);
 }
 
