@@ -383,20 +383,21 @@ __global__ void __launch_bounds__(kThreads) gn_stat_kernel(const Params p) {
   const float inv_n = 1.f / ((float)cnt_rows * (float)(p.C / p.G));
   float2* out = p.part + ((int64_t)b * p.chunks + blockIdx.x) * p.G + k.g0;
   for (int g = (int)threadIdx.x / team; g < k.groups; g += kThreads / team) {
+    // Unit u of the group: row lane u / cols, column u % cols.  A lane beyond the
+    // chunk's rows kept nothing: its count is 0.
+    const auto count = [&](int lane) { return (float)((cnt_rows - lane + l.lanes - 1) / l.lanes * kPer); };
     float s = 0.f;
-    for (int i = 0; i < l.lanes; ++i) {
-      const float cnt = (float)(((cnt_rows - i + l.lanes - 1) / l.lanes) * kPer);
-      for (int c = tl; c < cols; c += team) s = fmaf(unit[i * stride + g * cols + c].x, cnt, s);
+    for (int u = tl; u < l.lanes * cols; u += team) {
+      const int i = u / cols;
+      s = fmaf(unit[i * stride + g * cols + u - i * cols].x, count(i), s);
     }
     const float mean = team_sum(s, team) * inv_n;
     float q = 0.f;
-    for (int i = 0; i < l.lanes; ++i) {
-      const float cnt = (float)(((cnt_rows - i + l.lanes - 1) / l.lanes) * kPer);
-      for (int c = tl; c < cols; c += team) {
-        const float2 v = unit[i * stride + g * cols + c];
-        const float d = v.x - mean;
-        q += fmaf(d * d, cnt, v.y);
-      }
+    for (int u = tl; u < l.lanes * cols; u += team) {
+      const int i = u / cols;
+      const float2 v = unit[i * stride + g * cols + u - i * cols];
+      const float d = v.x - mean;
+      q += fmaf(d * d, count(i), v.y);
     }
     const float m2 = team_sum(q, team);
     if (tl == 0) out[g] = make_float2(mean, m2);
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(kThreads) gn_apply_kernel(const Params p) {
   for (int pass = 0; pass < l.passes; ++pass) {
     const int vec = l.passes == 1 ? (int)threadIdx.x - lr * l.nv : pass * kThreads + (int)threadIdx.x;
     if (lr >= l.lanes || vec >= l.nv) continue;
-    float mean[V], rstd[V], w[V], bias[V];
+    float mean[V], w[V], bias[V];   // w: times rstd
     if (r0 < n) {
       load<float, V>(p.w + k.c0 + vec * V, w);
       load<float, V>(p.bias + k.c0 + vec * V, bias);
@@ -457,7 +458,7 @@ __global__ void __launch_bounds__(kThreads) gn_apply_kernel(const Params p) {
       for (int e = 0; e < V; ++e) {
         const float2 s = stat[(vec * V + e) / cg];
         mean[e] = s.x;
-        rstd[e] = s.y;
+        w[e] *= s.y;
       }
     }
     for (int r = r0 + lr; r < r1; r += NB * l.lanes) {
@@ -473,7 +474,7 @@ __global__ void __launch_bounds__(kThreads) gn_apply_kernel(const Params p) {
         if (row >= r1) break;
         if (row < n) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) v[i][e] = fmaf((v[i][e] - mean[e]) * rstd[e], w[e], bias[e]);
+          for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] - mean[e], w[e], bias[e]);
           activate<sizeof(T) == 4, V>(v[i], p.act);
         } else {
 #pragma unroll
