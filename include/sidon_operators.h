@@ -49,6 +49,39 @@ int sidon_group_norm_act(const void* x, int64_t ldx, const int32_t* lens, const 
                          void* y, int64_t ldy, void* ws, size_t ws_bytes, int B, int T, int C, int G, int dtype,
                          int act, sidon_stream_t stream);
 
+/*
+ * Differential attention: the difference of two softmax maps over one set of
+ * values, with a learned weight per head.  For batch b, head h and query i:
+ *
+ *   o = sum_j softmax_j(q1 . k1_j / sqrt D) v_j - lambda sum_j softmax_j(q2 . k2_j / sqrt D) v_j
+ *   lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lam_init
+ *   out = o                                                              norm_w == NULL
+ *   out = (1 - lam_init) * norm_w * o / sqrt(mean(o^2) + eps)            otherwise
+ *
+ * over the keys j < LK = lens[b] (int32 [B] on the device, clamped to [0, S];
+ * NULL = S) and, if causal != 0, j <= LK - L + i: the L queries are the last L
+ * of the LK positions.  A query that sees no key gives zeros.  Keys and values
+ * past LK are not read.  Heads h / (H / Hk) share keys and values.
+ *
+ * q [B, H, 2, L, D], k [B, Hk, 2, S, D], v [B, Hk, S, 2 D], out [B, H, L, 2 D] of
+ * `dtype` (SIDON_FP16 or SIDON_BF16), the last dimension contiguous, the other
+ * strides int64 arrays in elements ((batch, head, map, row) for q and k, (batch,
+ * head, row) for v and out), multiples of 8 from 0 to 2^40, rows of k and v less
+ * than 2^25 apart; D 64 or 128.  lam fp32 [lam_heads, 4, D]: lq1, lk1, lq2, lk2,
+ * lam_heads 1 or H.  norm_w fp32 [2 D].  out must not overlap an input.
+ *
+ * Scores, softmax statistics, sums and the norm in fp32, probabilities rounded to
+ * `dtype` in front of the product with v, one rounding at the end.  ws:
+ * sidon_diff_attention_workspace_bytes bytes for these sizes on the current
+ * device (0: ws may be NULL), 16-byte aligned, contents irrelevant.
+ */
+size_t sidon_diff_attention_workspace_bytes(int B, int H, int Hk, int L, int S, int D);
+int sidon_diff_attention(const void* q, const void* k, const void* v, const float* lam, int lam_heads, float lam_init,
+                         const int32_t* lens, const float* norm_w, float eps, void* out, void* ws, size_t ws_bytes,
+                         int B, int H, int Hk, int L, int S, int D, int causal, int dtype, const int64_t* q_strides,
+                         const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                         sidon_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

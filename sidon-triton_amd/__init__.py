@@ -27,12 +27,18 @@ Entry points (same argument meaning as the reference):
     -- the module drop-in for transformers' relative_key self-attention
     (src/sidon_triton/modeling.py:40-131).
 
+and, with no counterpart in the reference, the language-model operators of
+include/sidon_operators.h beside them:
+  * ``diff_attention.diff_attention`` -- differential attention, prompts and
+    single tokens against a cache;
+  * ``conformer.group_norm_act`` -- group norm with an activation, channels last.
+
 The package directory name is not a Python identifier; the repository's
 entry scripts load it under the module name ``sidon_triton_amd``.
 """
 
-from . import (_lib, blas, conformer, encoder, encoder_attention, encoder_block, flexrel, frontend, graphs,
-               modeling, runtime)
+from . import (_lib, blas, conformer, diff_attention, encoder, encoder_attention, encoder_block, flexrel, frontend,
+               graphs, modeling, runtime)
 from .flexrel import HEAD_DIM, LEFT, NUM_POS, RIGHT, flexrel_attention
 
 __all__ = [
@@ -42,6 +48,7 @@ __all__ = [
     "RIGHT",
     "blas",
     "conformer",
+    "diff_attention",
     "encoder",
     "encoder_attention",
     "encoder_block",

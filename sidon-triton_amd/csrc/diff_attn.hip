@@ -1,0 +1,699 @@
+// diff_attn.hip -- differential attention (MI355X / gfx950): the difference of
+// two softmax maps over one set of values, with a learned weight,
+//
+//   o_i = sum_j softmax_j(q1_i . k1_j / sqrt D) v_j - lambda sum_j softmax_j(q2_i . k2_j / sqrt D) v_j
+//   lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init
+//   out_i = o_i,  or  (1 - lambda_init) norm_w o_i / sqrt(mean(o_i^2) + eps)
+//
+// with head dim D (64 or 128) per map and 2 D values, keys j < lens[b], and
+// optionally j <= lens[b] - L + i.  Grouped heads share keys and values: the
+// G heads of a group and their L queries are G L rows over one key head.
+//
+// A wavefront owns 32 rows and both maps (D = 64) or one of them (D = 128, whose
+// accumulators for both would not fit its registers): S^T = K . Q^T by
+// v_mfma_f32_32x32x16, an online softmax per map with the running maximum
+// raised only when a step's probabilities would leave the fp16 range,
+// O^T += V^T . P^T, for both maps from one read of the values.  Key rows enter
+// the A operand with bits 2 and 3 of their index swapped, which makes the
+// accumulator, rounded to 16 bits, the B operand of the second product.
+//
+// Keys go by steps of 32: a step's keys and values (8 D x 32 bytes) are copied
+// global -> LDS by global_load_lds_dwordx4 into a ring, as tiles of 32 rows x
+// 128 bytes with swizzled 16-byte chunks; keys are read with ds_read_b128,
+// values transposed with ds_read_b64_tr_b16.  RB wavefronts (row blocks)
+// share a ring; KS such groups take every KS-th step and are merged through
+// LDS; and over the grid a row block's steps can be split again, each part
+// leaving (max, sum, O) of both maps in fp32 for a joining launch.
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "flexrel_device.h"
+#include "sidon_host.h"
+#include "sidon_operators.h"
+#include "sidon_wave.h"
+
+#define SIDON_API extern "C" __attribute__((visibility("default")))
+#define SIDON_INLINE __attribute__((always_inline))
+
+namespace {
+
+using namespace sidon_flexrel;
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBlock = 32;          // rows per wavefront
+constexpr float kFloorMax = -1e30f; // a running maximum that no key has raised yet (finite: -inf - -inf is NaN)
+constexpr int kMaxGridSplits = 64;
+
+struct DiffParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const float* lam;      // [4, D] per head (or shared: lam_h == 0)
+  const float* norm_w;   // [2 D] or null
+  const int32_t* lens;
+  float2* part_ml;       // [B Hk, splits, R, 2] (maximum, sum)
+  float* part_o;         // [B Hk, splits, R, 2, 2 D]
+  int64_t qb, qh, qm, kb, kh, km, vb, vh, ob, oh;   // strides (elements): batch, head, map
+  int64_t ql, ol;        // row strides
+  int kl, vl;            // row strides (< 2^25)
+  int lam_h;
+  int B, H, Hk, G, L, S, R;
+  int blocks, splits;
+  int causal;
+  float scale;           // log2(e) / sqrt(D)
+  float lam_init, eps;
+};
+
+template <typename E>
+struct Half;
+template <>
+struct Half<_Float16> {
+  typedef h8 v8;
+  typedef h2 v2;
+  typedef h4 v4;
+  static __device__ __forceinline__ f32x16 mfma(i4 a, i4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Half<__bf16> {
+  typedef b8 v8;
+  typedef b2 v2;
+  typedef b4 v4;
+  static __device__ __forceinline__ f32x16 mfma(i4 a, i4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  }
+};
+
+// x of lane l plus x of lane l ^ 32.
+__device__ __forceinline__ float pair_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The learned weight of head h, in every lane of a wavefront.
+template <int D>
+__device__ __forceinline__ float head_lambda(const DiffParams& p, int h, int lane) {
+  const float* l = p.lam + (int64_t)h * p.lam_h;
+  float a = 0.f, b = 0.f;
+#pragma unroll
+  for (int d = 0; d < D; d += 64) {
+    a = fmaf(l[d + lane], l[D + d + lane], a);
+    b = fmaf(l[2 * D + d + lane], l[3 * D + d + lane], b);
+  }
+  return expf(sidon::wave_sum(a)) - expf(sidon::wave_sum(b)) + p.lam_init;
+}
+
+// The same for a wavefront whose rows may be of several heads of its group.
+template <int D>
+__device__ __forceinline__ float wave_lambda(const DiffParams& p, int hk, int row0, int row, int lane) {
+  if (p.lam_h == 0) return head_lambda<D>(p, 0, lane);
+  float lambda = 0.f;
+  const int first = min(row0, p.R - 1) / p.L, last = min(row0 + kBlock - 1, p.R - 1) / p.L;
+  for (int j = first; j <= last; ++j) {
+    const float l = head_lambda<D>(p, hk * p.G + j, lane);
+    if (row / p.L == j) lambda = l;
+  }
+  return lambda;
+}
+
+template <int N>
+__device__ __forceinline__ void wait_copies(int newer_steps) {
+  // all but the copies (N a step) of the `newer_steps` youngest steps have landed
+  if (newer_steps >= 3) {
+    wait_vmcnt<3 * N>();
+  } else if (newer_steps == 2) {
+    wait_vmcnt<2 * N>();
+  } else if (newer_steps == 1) {
+    wait_vmcnt<N>();
+  } else {
+    wait_vmcnt<0>();
+  }
+}
+
+// A workgroup: RB row blocks x MW wavefronts per row block (2: one per map, 1:
+// both maps in one) x KS key groups.
+template <int D, int RB, int MW, int KS, int ST>
+struct Shape {
+  static constexpr int kMaps = 2 / MW;                // maps per wavefront
+  static constexpr int kRingWaves = RB * MW;          // wavefronts that share a ring
+  static constexpr int kWaves = kRingWaves * KS;
+  static constexpr int kP = D / 64;                   // 128-byte panels per key map
+  static constexpr int kPanels = 4 * kP;              // of a step: K of map 0, K of map 1, V
+  static constexpr int kStage = kPanels * kTile;
+  static constexpr int kRing = ST * kStage;
+  static constexpr int kDb = 2 * D / 32;              // 32-wide blocks of the values
+  static constexpr int kO = kMaps * kDb * 16;         // fp32 accumulators per lane
+  static constexpr int kPart = (kO + 4) * 64 * 4;     // bytes of a wavefront's partial result
+  static constexpr int kMerge = KS > 1 ? KS / 2 * kRingWaves * kPart : 0;
+  static constexpr int kCross = MW > 1 ? RB * kPart : 0;
+  static constexpr int kNeed = kMerge > kCross ? kMerge : kCross;
+  static constexpr int kLds = KS * kRing > kNeed ? KS * kRing : kNeed;
+  static constexpr int kMine = kPanels / kRingWaves;  // panels a wavefront copies
+  static constexpr int kCopies = kMine * 4;           // 1 KB copies per wavefront and step
+  static_assert(kLds <= 160 * 1024 && kCopies * (ST - 1) < 64 && ST >= 2 && ST <= 4, "LDS, vmcnt range");
+  static_assert(kPanels % kRingWaves == 0, "whole panels per wavefront");
+};
+
+template <typename E, int D, int RB, int MW, int KS, int ST, int kMinWaves>
+__global__ void __launch_bounds__(64 * RB * MW * KS, kMinWaves) diff_attn_kernel(const DiffParams p) {
+  using C = Shape<D, RB, MW, KS, ST>;
+  typedef typename Half<E>::v2 v2;
+  typedef typename Half<E>::v4 v4;
+  constexpr int P = C::kP, NM = C::kMaps, kDb = C::kDb;
+  constexpr int kQ = D / 16;          // Q operands per map
+  __shared__ __attribute__((aligned(16))) char smem[C::kLds];
+
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = w % C::kRingWaves, ks = w / C::kRingWaves;
+  const int rb = wr % RB, m0 = wr / RB;   // row block, first (or only) map
+  const int n = lane & 31, g = lane >> 5;
+
+  // Each XCD takes a contiguous range: key heads slowest, so that a head's keys
+  // and values stay in one L2; of a causal call the longest rows first.
+  const int lin = xcd_linear(blockIdx.x, gridDim.x);
+  const int per_head = p.splits * p.blocks;
+  const int bh = lin / per_head;
+  const int rest = lin - bh * per_head;
+  const int split = rest / p.blocks;
+  const int blk = p.blocks - 1 - (rest - split * p.blocks);
+  const int b = bh / p.Hk, hk = bh - b * p.Hk;
+  const int row0 = (blk * RB + rb) * kBlock;   // of this wavefront
+  const int row = row0 + n;                    // of this lane: head row / L of the group, query row % L
+
+  int lk = p.S;
+  if (p.lens != nullptr) lk = __builtin_amdgcn_readfirstlane(min(max(p.lens[b], 0), p.S));
+
+  // Keys that this lane's row sees, the most and the fewest that a row of the
+  // wavefront does, and the steps that some row of the workgroup needs.
+  int lim, wave_most, wave_least, steps;
+  {
+    const auto limit = [&](int r) SIDON_INLINE { return p.causal ? min(max(lk - p.L + 1 + r % p.L, 0), lk) : lk; };
+    // Over rows [a, e): a causal row's limit grows with its query and starts
+    // again at the next head.
+    const auto most = [&](int a, int e) SIDON_INLINE {
+      e = min(e, p.R);
+      if (a >= e) return 0;
+      return a / p.L != (e - 1) / p.L ? lk : limit(e - 1);
+    };
+    wave_most = most(row0, row0 + kBlock);
+    const int last = min(row0 + kBlock, p.R) - 1;
+    wave_least = row0 > last ? 0 : limit(row0 / p.L != last / p.L ? last / p.L * p.L : row0);
+    lim = row < p.R ? limit(row) : wave_most;   // (rows past R are never stored)
+    steps = (most(blk * RB * kBlock, (blk + 1) * RB * kBlock) + kStep - 1) / kStep;
+  }
+  const int t0 = (int)((int64_t)steps * split / p.splits);
+  const int t1 = (int)((int64_t)steps * (split + 1) / p.splits);
+  const int count = (t1 - t0 + KS - 1) / KS;   // of every key group; its last step may be past t1
+  const auto mine = [&](int u) SIDON_INLINE { return t0 + u * KS + ks; };   // step u of this group
+  const int own = count > 0 && mine(count - 1) >= t1 ? count - 1 : count;
+
+  // ---- copies: panels K of map 0, K of map 1, V, over the ring's wavefronts ----
+  const uint32_t ring = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem) + ks * C::kRing;
+  const char* const kbase = static_cast<const char*>(p.k) + 2 * (b * p.kb + hk * p.kh);
+  const char* const vbase = static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh);
+  const int crow = lane >> 3;                                // row of a copy's 8
+  // Step t into ring slot `slot`.  Rows past the valid keys read the last
+  // valid one again: their probabilities are 0, and what lies there may be anything.
+  const auto copy = [&](int t, int slot) SIDON_INLINE {
+    const int most = min(lk - t * kStep, kStep) - 1;
+#pragma unroll
+    for (int j = 0; j < C::kMine; ++j) {
+      const int pid = wr * C::kMine + j;
+      const bool key = pid < 2 * P;
+      const int64_t stride = 2 * (int64_t)(key ? p.kl : p.vl);
+      const char* src = key ? kbase + 2 * ((pid / P) * p.km) + (pid % P) * 128 : vbase + (pid - 2 * P) * 128;
+      src += t * (kStep * stride);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + crow;
+        const uint32_t off = (uint32_t)min(r, most) * (uint32_t)stride + 16u * ((lane & 7) ^ tile_swz(r));
+        dma_1k(ring + slot * C::kStage + pid * kTile + i * 1024, src, off);
+      }
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < ST - 1; ++u)
+    if (u < own) copy(mine(u), u);
+
+  // ---- Q^T operands: lane (n, g) holds query n, dims 16 s + 8 g + [0, 8) ----
+  const int rr = min(row, p.R - 1);
+  i4 qop[NM][kQ];
+  {
+    const E* qp = static_cast<const E*>(p.q) + b * p.qb + (hk * p.G + rr / p.L) * p.qh + (rr % p.L) * p.ql + 8 * g;
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+      for (int s = 0; s < kQ; ++s) qop[m][s] = *reinterpret_cast<const i4*>(qp + (m0 + m) * p.qm + 16 * s);
+  }
+
+  // ---- operand offsets in a tile ----
+  const int krow = mfma_row_perm(n);
+  const int kswz = tile_swz(krow);
+  int tr[2][2];
+  {
+    const int G4 = lane >> 4, a = (lane >> 2) & 3, bq = lane & 3;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        const int r = 8 * (G4 >> 1) + 4 * hf + a;
+        const int chunk = 4 * db + 2 * (G4 & 1) + (bq >> 1);
+        tr[hf][db] = r * 128 + ((chunk ^ tile_swz(r)) << 4) + 8 * (bq & 1);
+      }
+  }
+
+  f32x16 o[NM][kDb];
+#pragma unroll
+  for (int m = 0; m < NM; ++m)
+#pragma unroll
+    for (int d = 0; d < kDb; ++d) o[m][d] = f32x16{};
+  float mx[NM], sum[NM];   // maximum of the scaled scores (of lanes n and n + 32), sum over this lane's keys
+#pragma unroll
+  for (int m = 0; m < NM; ++m) {
+    mx[m] = kFloorMax;
+    sum[m] = 0.f;
+  }
+
+  const auto compute = [&](int t, int slot) SIDON_INLINE {
+    const char* stage = smem + ks * C::kRing + slot * C::kStage;
+    const int k0 = t * kStep;
+    const bool masked = k0 + kStep > wave_least;
+    i4 pk[NM][2];
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      f32x16 s = {};
+#pragma unroll
+      for (int i = 0; i < kQ; ++i) {
+        const char* tile = stage + ((m0 + m) * P + i / 4) * kTile;
+        const i4 kop = *reinterpret_cast<const i4*>(tile + krow * 128 + (((2 * (i % 4) + g) ^ kswz) << 4));
+        s = Half<E>::mfma(kop, qop[m][i], s);
+      }
+      if (masked) {
+        const int left = lim - k0 - 8 * g;   // element i is key 16 (i / 8) + i % 8 of what this lane holds
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (16 * (i >> 3) + (i & 7) >= left) s[i] = -INFINITY;
+      }
+      const auto probs = [&](float top) SIDON_INLINE {
+        float total = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const f2 e = {fast_exp2(fmaf(s[i], p.scale, -top)), fast_exp2(fmaf(s[i + 1], p.scale, -top))};
+          total += e[0] + e[1];
+          const v2 r = __builtin_convertvector(e, v2);
+          pk[m][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, r);
+        }
+        return total;
+      };
+      float total = probs(mx[m]);
+      // A lane's 16 probabilities that sum below 2^15 are finite in fp16.
+      bool need = !(total < kSumLimit);
+      if (__builtin_amdgcn_ballot_w64(need) != 0) {
+        // Both lanes of a query raise its maximum together.
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        top = pair_max(top) * p.scale;
+        need = pair_max(need ? 1.f : 0.f) != 0.f;
+        const float next = need ? fmaxf(mx[m], top) : mx[m];
+        const float alpha = fast_exp2(mx[m] - next);   // 1 where nothing changed, 0 from kFloorMax
+        if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+#pragma unroll
+          for (int d = 0; d < kDb; ++d) o[m][d] *= alpha;
+        }
+        sum[m] *= alpha;
+        mx[m] = next;
+        total = probs(next);
+      }
+      sum[m] += total;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int d = 0; d < kDb; ++d) {
+        const char* tile = stage + (2 * P + d / 2) * kTile + 2048 * hh;
+        const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + tr[0][d & 1]));
+        const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + tr[1][d & 1]));
+        typedef int i2 __attribute__((ext_vector_type(2)));
+        const i2 l2 = __builtin_bit_cast(i2, lo), u2 = __builtin_bit_cast(i2, hi);
+        const i4 vop = {l2[0], l2[1], u2[0], u2[1]};
+#pragma unroll
+        for (int m = 0; m < NM; ++m) o[m][d] = Half<E>::mfma(vop, pk[m][hh], o[m][d]);
+        if (d % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // few operands at a time: the registers are full
+      }
+  };
+
+  // ---- key steps ----
+  int slot = 0;
+  for (int u = 0; u < count; ++u) {
+    // Step u has landed; behind the barrier it has for every wavefront of the
+    // ring, and nobody reads slot u - 1 any more, which is filled again.
+    wait_copies<C::kCopies>(min(ST - 2, own - 1 - u));
+    if constexpr (C::kRingWaves > 1) {
+      lds_barrier();
+    } else {
+      wait_lgkm0();
+    }
+    if (u + ST - 1 < own) copy(mine(u + ST - 1), slot == 0 ? ST - 1 : slot - 1);
+    const int t = mine(u);
+    if (t < t1 && t * kStep < wave_most) compute(t, slot);
+    slot = slot == ST - 1 ? 0 : slot + 1;
+  }
+#pragma unroll
+  for (int m = 0; m < NM; ++m) sum[m] = pair_sum(sum[m]);
+
+  // A wavefront's partial result in LDS, lane by lane: kO values, then (maximum, sum) per map.
+  float* const mem = reinterpret_cast<float*>(smem) + lane * 4;
+  const auto put = [&](float* at, int m, int d, int i) SIDON_INLINE {
+    *reinterpret_cast<f4*>(at + ((m * kDb + d) * 4 + i) * 256) =
+        f4{o[m][d][4 * i], o[m][d][4 * i + 1], o[m][d][4 * i + 2], o[m][d][4 * i + 3]};
+  };
+  const auto get = [&](const float* at, int m, int d, int i) SIDON_INLINE {
+    return *reinterpret_cast<const f4*>(at + ((m * kDb + d) * 4 + i) * 256);
+  };
+
+  // ---- merge the key groups, half of them into the other half at a time ----
+  if constexpr (KS > 1) {
+#pragma unroll
+    for (int half = KS / 2; half >= 1; half >>= 1) {
+      wait_vmcnt<0>();
+      lds_barrier();   // the rings, or the last round's values, are done with
+      float* at = mem + ((ks % half) * C::kRingWaves + wr) * (C::kPart / 4);
+      float* ml = at + NM * kDb * 4 * 256;
+      if (ks >= half && ks < 2 * half) {
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+#pragma unroll
+          for (int d = 0; d < kDb; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put(at, m, d, i);
+          ml[2 * m] = mx[m];
+          ml[2 * m + 1] = sum[m];
+        }
+      }
+      lds_barrier();
+      if (ks < half) {
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+          const float top = fmaxf(mx[m], ml[2 * m]);
+          const float fa = fast_exp2(mx[m] - top), fb = fast_exp2(ml[2 * m] - top);
+          mx[m] = top;
+          sum[m] = sum[m] * fa + ml[2 * m + 1] * fb;
+#pragma unroll
+          for (int d = 0; d < kDb; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const f4 v = get(at, m, d, i);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[m][d][4 * i + e] = o[m][d][4 * i + e] * fa + v[e] * fb;
+            }
+        }
+      }
+    }
+    if (ks > 0) return;
+  }
+
+  // Lane (n, g) holds of row n the values 32 d + 8 i + 4 g + [0, 4).
+  if (p.splits > 1) {
+    if (row >= p.R) return;
+    const int64_t at = ((int64_t)bh * p.splits + split) * p.R + row;
+    float* dst = p.part_o + at * (4 * D) + 4 * g;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      if (g == 0) p.part_ml[at * 2 + m0 + m] = make_float2(mx[m], sum[m]);
+#pragma unroll
+      for (int d = 0; d < kDb; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f4*>(dst + (m0 + m) * 2 * D + 32 * d + 8 * i) =
+              f4{o[m][d][4 * i], o[m][d][4 * i + 1], o[m][d][4 * i + 2], o[m][d][4 * i + 3]};
+    }
+    return;
+  }
+
+  // What each map's accumulators weigh in the difference (0 where no key was seen).
+  float f[NM];
+#pragma unroll
+  for (int m = 0; m < NM; ++m) {
+    f[m] = sum[m] == 0.f ? 0.f : 1.f / sum[m];
+    if (m0 + m == 1) f[m] *= wave_lambda<D>(p, hk, row0, rr, lane);
+  }
+  if constexpr (MW > 1) {
+    lds_barrier();   // the ring, or the merge, is done with
+    float* at = mem + rb * (C::kPart / 4);
+    if (m0 == 1) {
+#pragma unroll
+      for (int d = 0; d < kDb; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[0][d][4 * i] *= f[0], o[0][d][4 * i + 1] *= f[0], o[0][d][4 * i + 2] *= f[0], o[0][d][4 * i + 3] *= f[0];
+          put(at, 0, d, i);
+        }
+    }
+    lds_barrier();
+    if (m0 == 1) return;
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f4 v = get(at, 0, d, i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][d][4 * i + e] = o[0][d][4 * i + e] * f[0] - v[e];
+      }
+  } else {
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[0][d][i] = o[0][d][i] * f[0] - o[NM - 1][d][i] * f[NM - 1];
+  }
+  float gain = 1.f;
+  if (p.norm_w != nullptr) {
+    float sq = 0.f;
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sq = fmaf(o[0][d][i], o[0][d][i], sq);
+    gain = (1.f - p.lam_init) * rsqrtf(pair_sum(sq) * (1.f / (2 * D)) + p.eps);
+  }
+  if (row >= p.R) return;
+  E* dst = static_cast<E*>(p.out) + b * p.ob + (hk * p.G + row / p.L) * p.oh + (row % p.L) * p.ol + 4 * g;
+#pragma unroll
+  for (int d = 0; d < kDb; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f4 wv = {1.f, 1.f, 1.f, 1.f};
+      if (p.norm_w != nullptr) wv = *reinterpret_cast<const f4*>(p.norm_w + 32 * d + 8 * i + 4 * g);
+      v4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = (E)(o[0][d][4 * i + e] * gain * wv[e]);
+      *reinterpret_cast<v4*>(dst + 32 * d + 8 * i) = r;
+      if (i == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Join the grid splits of a row: one wavefront per row, 2 D / 64 values a lane.
+constexpr int kJoinRows = 4;
+template <typename E, int D>
+__global__ void __launch_bounds__(64 * kJoinRows) diff_attn_join_kernel(const DiffParams p) {
+  constexpr int N = 2 * D / 64;
+  typedef float fn __attribute__((ext_vector_type(N)));
+  const int lane = threadIdx.x & 63;
+  const int64_t lin = (int64_t)blockIdx.x * kJoinRows + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t bh = lin / p.R;
+  const int row = (int)(lin - bh * p.R);
+  if (bh >= (int64_t)p.B * p.Hk) return;
+  const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
+  const int head = hk * p.G + row / p.L;
+
+  // Lane s < splits holds part s (kMaxGridSplits <= 64).
+  float4 ml = make_float4(kFloorMax, 0.f, kFloorMax, 0.f);
+  if (lane < p.splits) ml = *reinterpret_cast<const float4*>(p.part_ml + ((bh * p.splits + lane) * p.R + row) * 2);
+  float m1 = ml.x, m2 = ml.z;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    m1 = fmaxf(m1, __shfl_xor(m1, d));
+    m2 = fmaxf(m2, __shfl_xor(m2, d));
+  }
+  const float f1 = fast_exp2(ml.x - m1), f2 = fast_exp2(ml.z - m2);
+  const float s1 = sidon::wave_sum(ml.y * f1), s2 = sidon::wave_sum(ml.w * f2);
+  const float lambda = head_lambda<D>(p, head, lane);
+  const float i1 = s1 == 0.f ? 0.f : 1.f / s1;
+  const float i2 = s2 == 0.f ? 0.f : lambda / s2;
+  // What each part weighs in the difference.
+  const float w1 = f1 * i1, w2 = f2 * i2;
+  const uint64_t used = __builtin_amdgcn_ballot_w64(ml.y != 0.f || ml.w != 0.f);
+  fn x = {};
+  const float* src = p.part_o + (bh * p.splits * p.R + row) * (4 * D) + N * lane;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    if (!(used >> s & 1)) continue;
+    const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w1), s));
+    const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w2), s));
+    const float* at = src + (int64_t)s * p.R * (4 * D);
+    const fn u = *reinterpret_cast<const fn*>(at), v = *reinterpret_cast<const fn*>(at + 2 * D);
+    x += u * a - v * c;
+  }
+  float gain = 1.f;
+  if (p.norm_w != nullptr) {
+    float sq = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) sq = fmaf(x[e], x[e], sq);
+    gain = (1.f - p.lam_init) * rsqrtf(sidon::wave_sum(sq) * (1.f / (2 * D)) + p.eps);
+  }
+  E* dst = static_cast<E*>(p.out) + b * p.ob + head * p.oh + (row % p.L) * p.ol + N * lane;
+  typedef E en __attribute__((ext_vector_type(N)));
+  en r;
+#pragma unroll
+  for (int e = 0; e < N; ++e) r[e] = (E)(x[e] * gain * (p.norm_w != nullptr ? p.norm_w[N * lane + e] : 1.f));
+  *reinterpret_cast<en*>(dst) = r;
+}
+
+// ---- host -------------------------------------------------------------------------
+
+struct Plan {
+  int rows;     // per workgroup
+  int blocks, splits;
+};
+
+// Rows per workgroup and grid splits.
+Plan plan(int B, int Hk, int R, int S, int cus) {
+  Plan c;
+  const int64_t heads = (int64_t)B * Hk;
+  const int64_t wide = heads * ((R + 127) / 128);
+  c.rows = R > kBlock && wide >= cus ? 128 : kBlock;
+  c.blocks = (R + c.rows - 1) / c.rows;
+  c.splits = 1;
+  const int64_t wgs = heads * c.blocks;
+  const int steps = (S + kStep - 1) / kStep;
+  if (c.rows == kBlock && wgs < cus) {
+    // at least one step for each wavefront of a part
+    int64_t s = cus / wgs;
+    if (s > (steps + 3) / 4) s = (steps + 3) / 4;
+    if (s > kMaxGridSplits) s = kMaxGridSplits;
+    c.splits = s < 1 ? 1 : (int)s;
+  }
+  return c;
+}
+
+bool shape_ok(int B, int H, int Hk, int L, int S, int D) {
+  return B >= 1 && H >= 1 && Hk >= 1 && H % Hk == 0 && L >= 1 && S >= 1 && (D == 64 || D == 128) &&
+         S <= (1 << 30) && (int64_t)(H / Hk) * L <= (1 << 24) && (int64_t)B * Hk <= (1 << 24);
+}
+
+size_t part_bytes(int B, int Hk, int R, int D, int splits) {
+  return splits > 1 ? (size_t)B * Hk * R * splits * (16 + (size_t)D * 16) : 0;
+}
+
+template <typename E>
+void launch(const DiffParams& p, int D, int rows, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.blocks * p.splits));
+  if (D == 64) {
+    if (rows == kBlock) {
+      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 1, 1, 4, 2, 1>), grid, dim3(256), 0, stream, p);
+    } else {
+      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 4, 1, 1, 4, 2>), grid, dim3(256), 0, stream, p);
+    }
+  } else {
+    if (rows == kBlock) {
+      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 1, 2, 2, 2, 1>), grid, dim3(256), 0, stream, p);
+    } else {
+      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 4, 2, 1, 4, 2>), grid, dim3(512), 0, stream, p);
+    }
+  }
+  if (p.splits > 1) {
+    const int64_t all = (int64_t)p.B * p.Hk * p.R;
+    const dim3 join((unsigned)((all + kJoinRows - 1) / kJoinRows));
+    if (D == 64) {
+      hipLaunchKernelGGL((diff_attn_join_kernel<E, 64>), join, dim3(64 * kJoinRows), 0, stream, p);
+    } else {
+      hipLaunchKernelGGL((diff_attn_join_kernel<E, 128>), join, dim3(64 * kJoinRows), 0, stream, p);
+    }
+  }
+}
+
+}  // namespace
+
+SIDON_API size_t sidon_diff_attention_workspace_bytes(int B, int H, int Hk, int L, int S, int D) {
+  if (!shape_ok(B, H, Hk, L, S, D)) return 0;
+  const int R = H / Hk * L;
+  return part_bytes(B, Hk, R, D, plan(B, Hk, R, S, sidon::compute_units()).splits);
+}
+
+SIDON_API int sidon_diff_attention(const void* q, const void* k, const void* v, const float* lam, int lam_heads,
+                                   float lam_init, const int32_t* lens, const float* norm_w, float eps, void* out,
+                                   void* ws, size_t ws_bytes, int B, int H, int Hk, int L, int S, int D, int causal,
+                                   int dtype, const int64_t* q_strides, const int64_t* k_strides,
+                                   const int64_t* v_strides, const int64_t* o_strides, sidon_stream_t stream) {
+  using sidon::fail;
+  sidon::clear_error();
+  if (!q || !k || !v || !lam || !out || !q_strides || !k_strides || !v_strides || !o_strides)
+    return fail(SIDON_E_NULL, "q, k, v, lam, out and the strides must be non-NULL");
+  if (dtype != SIDON_FP16 && dtype != SIDON_BF16) return fail(SIDON_E_SHAPE, "dtype=%d is neither SIDON_FP16 nor SIDON_BF16", dtype);
+  if (!shape_ok(B, H, Hk, L, S, D))
+    return fail(SIDON_E_SHAPE, "B=%d H=%d Hk=%d L=%d S=%d D=%d: need sizes >= 1, H a multiple of Hk, D 64 or 128, H / Hk * L and B * Hk <= 2^24, S <= 2^30",
+                B, H, Hk, L, S, D);
+  if (lam_heads != 1 && lam_heads != H) return fail(SIDON_E_SHAPE, "lam_heads=%d must be 1 or H=%d", lam_heads, H);
+  // Strides in the order (batch, head, map, row) for q and k, (batch, head, row) for v and out.
+  const struct {
+    const char* name;
+    const int64_t* s;
+    int n;
+    int64_t row_most;
+  } all[] = {{"q", q_strides, 4, int64_t(1) << 40}, {"k", k_strides, 4, (int64_t(1) << 25) - 1},
+             {"v", v_strides, 3, (int64_t(1) << 25) - 1}, {"out", o_strides, 3, int64_t(1) << 40}};
+  for (const auto& t : all) {
+    for (int i = 0; i < t.n; ++i)
+      if (t.s[i] < 0 || t.s[i] % 8 != 0 || t.s[i] > (i == t.n - 1 ? t.row_most : int64_t(1) << 40))
+        return fail(SIDON_E_STRIDE, "%s stride %lld (number %d) must be a multiple of 8 in [0, %s]", t.name,
+                    (long long)t.s[i], i, i == t.n - 1 && t.row_most < (int64_t(1) << 40) ? "2^25)" : "2^40]");
+  }
+  if (!sidon::aligned16(q) || !sidon::aligned16(k) || !sidon::aligned16(v) || !sidon::aligned16(out) ||
+      (norm_w && !sidon::aligned16(norm_w)) || (reinterpret_cast<uintptr_t>(lam) & 3u) != 0 ||
+      (reinterpret_cast<uintptr_t>(lens) & 3u) != 0 || !sidon::aligned16(ws))
+    return fail(SIDON_E_ALIGN, "q, k, v, out, norm_w and ws must be 16-byte aligned, lam and lens 4-byte aligned");
+  int rc;
+  if ((rc = sidon::check_device())) return rc;
+  const int R = H / Hk * L;
+  const Plan c = plan(B, Hk, R, S, sidon::compute_units());
+  if (ws_bytes < part_bytes(B, Hk, R, D, c.splits) || (c.splits > 1 && ws == nullptr))
+    return fail(SIDON_E_SHAPE, "ws holds %zu bytes, the call needs %zu", ws_bytes, part_bytes(B, Hk, R, D, c.splits));
+  if ((int64_t)B * Hk * c.blocks * c.splits > INT32_MAX) return fail(SIDON_E_SHAPE, "too many rows for one launch");
+  DiffParams p{};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.out = out;
+  p.lam = lam;
+  p.norm_w = norm_w;
+  p.lens = lens;
+  p.part_ml = static_cast<float2*>(ws);
+  p.part_o = static_cast<float*>(ws) + (size_t)B * Hk * R * c.splits * 4;
+  p.qb = q_strides[0], p.qh = q_strides[1], p.qm = q_strides[2], p.ql = q_strides[3];
+  p.kb = k_strides[0], p.kh = k_strides[1], p.km = k_strides[2], p.kl = (int)k_strides[3];
+  p.vb = v_strides[0], p.vh = v_strides[1], p.vl = (int)v_strides[2];
+  p.ob = o_strides[0], p.oh = o_strides[1], p.ol = o_strides[2];
+  p.lam_h = lam_heads == 1 ? 0 : 4 * D;
+  p.B = B, p.H = H, p.Hk = Hk, p.G = H / Hk, p.L = L, p.S = S, p.R = R;
+  p.blocks = c.blocks, p.splits = c.splits;
+  p.causal = causal != 0;
+  p.scale = 1.4426950408889634f / (D == 64 ? 8.f : 11.313708498984761f);
+  p.lam_init = lam_init;
+  p.eps = eps;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == SIDON_FP16) {
+    launch<_Float16>(p, D, c.rows, s);
+  } else {
+    launch<__bf16>(p, D, c.rows, s);
+  }
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return fail(SIDON_E_LAUNCH, "differential attention launch failed: %s", hipGetErrorString(err));
+  return SIDON_OK;
+}

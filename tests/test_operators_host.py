@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -40,3 +42,57 @@ def test_group_norm_rejects_host_tensors(sidon):
     x = torch.zeros(4, 8)
     with pytest.raises(ValueError, match="HIP device"):
         sidon.conformer.group_norm_act(x, 1, 2, torch.ones(8), torch.zeros(8))
+
+
+def _attention(lib, **over):
+    i64 = ctypes.c_int64
+    a = dict(q=16, k=16, v=16, lam=16, lam_heads=1, lens=None, norm_w=16, out=16, ws=None, wsb=0, B=2, H=4, Hk=2, L=10,
+             S=100, D=64, causal=0, dtype=1, qs=(512, 128, 64, 1024), ks=(8192, 128, 64, 256), vs=(8192, 128, 256),
+             os=(8192, 128, 512))
+    a.update(over)
+    st = [None if a[n] is None else (i64 * len(a[n]))(*a[n]) for n in ("qs", "ks", "vs", "os")]
+    return lib.sidon_diff_attention(a["q"], a["k"], a["v"], a["lam"], a["lam_heads"], 0.5, a["lens"], a["norm_w"], 1e-5,
+                                    a["out"], a["ws"], a["wsb"], a["B"], a["H"], a["Hk"], a["L"], a["S"], a["D"],
+                                    a["causal"], a["dtype"], *st, None)
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(q=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(lam=None), -1), (dict(out=None), -1),
+    (dict(qs=None), -1), (dict(os=None), -1), (dict(dtype=0), -2), (dict(dtype=3), -2), (dict(B=0), -2), (dict(L=0), -2),
+    (dict(S=0), -2), (dict(H=5), -2), (dict(Hk=0), -2), (dict(D=32), -2), (dict(D=96), -2), (dict(S=(1 << 30) + 1), -2),
+    (dict(L=1 << 24), -2), (dict(lam_heads=2), -2), (dict(qs=(512, 128, 60, 1024)), -3), (dict(ks=(-8, 0, 0, 0)), -3),
+    (dict(ks=(8192, 128, 64, 1 << 25)), -3), (dict(vs=(8192, 128, 1 << 25)), -3), (dict(vs=(8192, 4, 256)), -3),
+    (dict(os=(1 << 41, 128, 512)), -3), (dict(q=24), -4), (dict(v=8), -4), (dict(out=8), -4), (dict(norm_w=20), -4),
+    (dict(lam=18), -4), (dict(lens=6), -4), (dict(ws=24, wsb=1 << 20), -4),
+])
+def test_diff_attention_refuses(sidon, over, code):
+    lib = sidon._lib.load()
+    assert _attention(lib, **over) == code
+    assert lib.sidon_last_error().decode()
+
+
+def test_diff_attention_workspace(sidon):
+    lib = sidon._lib.load()
+    ws = lib.sidon_diff_attention_workspace_bytes
+    assert ws(1, 8, 3, 1, 100, 64) == 0 and ws(1, 8, 8, 4800, 4800, 64) == 0
+    one = ws(1, 8, 8, 1, 4800, 64)   # split over the chip
+    assert one % (8 * (16 + 64 * 16)) == 0 and 1 < one // (8 * (16 + 64 * 16)) <= 64
+
+
+def test_diff_attention_rejects_wrong_tensors(sidon):
+    call = sidon.diff_attention.diff_attention
+    q = torch.zeros(1, 2, 2, 3, 64, dtype=torch.float16)
+    k, v = torch.zeros(1, 1, 2, 5, 64, dtype=torch.float16), torch.zeros(1, 1, 5, 128, dtype=torch.float16)
+    lam = torch.zeros(4, 64)
+    with pytest.raises(ValueError, match="HIP device"):
+        call(q, k, v, lam, 0.5)
+    with pytest.raises(ValueError, match="belong together"):
+        call(q, k, v[..., :64], lam, 0.5)
+    with pytest.raises(ValueError, match="share"):
+        call(q, torch.zeros(1, 3, 2, 5, 64, dtype=torch.float16), torch.zeros(1, 3, 5, 128, dtype=torch.float16), lam, 0.5)
+    with pytest.raises(ValueError, match="H, 2, L"):
+        call(q[..., :32], k[..., :32], v[..., :64], lam[:, :32], 0.5)
+    with pytest.raises(TypeError, match="float16"):
+        call(q.float(), k.float(), v.float(), lam, 0.5)
+    with pytest.raises(ValueError, match="empty"):
+        call(q[:, :, :, :0], k, v, lam, 0.5)
