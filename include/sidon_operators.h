@@ -50,6 +50,39 @@ int sidon_group_norm_act(const void* x, int64_t ldx, const int32_t* lens, const 
                          int act, sidon_stream_t stream);
 
 /*
+ * A shared projection with a low-rank adapter per request.  For row m of
+ * x [M, K], with e = ids[m / (M / items)] (int32 [items] on the device):
+ *
+ *   sidon_adapter_linear     y[m] = act(x[m] . w^T + bias + scale[e] (x[m] . a[e]^T) . b[e]^T)
+ *   sidon_adapter_residual   y[m] = add[m] + x[m] . w^T + scale[e] (x[m] . a[e]^T) . b[e]^T
+ *
+ * Items are M / items consecutive rows each: utterances of a padded batch, or
+ * (items == M) single tokens.  An e outside [0, adapters) means no adapter: the
+ * row's low-rank term is left out, and no other row's adapter touches it.
+ *
+ * x [M, K], w [N, K], a [adapters, R, K], b [adapters, N, R] and bias [N] (or NULL)
+ * of `dtype` (SIDON_FP16 or SIDON_BF16), K contiguous, rows of x and w ldx / ldw
+ * apart, a and b contiguous; scale fp32 [adapters].  linear: y [M, N] of `dtype`,
+ * act SIDON_ACT_NONE or SIDON_ACT_SILU.  residual: y and add fp32 [M, N], y may be
+ * add itself (same stride), any other overlap of y with an input is refused.
+ * N and K multiples of 64, R a multiple of 8 in [8, 128], M a multiple of items;
+ * strides multiples of 8 (y and add of residual: 4); x and w each under 4 GiB;
+ * pointers 16-byte aligned (bias 8, ids and scale 4).
+ *
+ * Sums in fp32.  linear rounds scale (x . a^T) to `dtype` in front of the product
+ * with b; residual, whose result is fp32, keeps all of it (two or three summands).
+ * ws: sidon_adapter_workspace_bytes bytes, 16-byte aligned, contents irrelevant.
+ */
+size_t sidon_adapter_workspace_bytes(int M, int R, int residual, int dtype);
+int sidon_adapter_linear(const void* x, int ldx, const void* w, int ldw, const void* bias, const void* a, const void* b,
+                         const float* scale, const int32_t* ids, void* y, int ldy, void* ws, size_t ws_bytes, int M,
+                         int N, int K, int R, int adapters, int items, int act, int dtype, sidon_stream_t stream);
+int sidon_adapter_residual(const void* x, int ldx, const void* w, int ldw, const void* a, const void* b,
+                           const float* scale, const int32_t* ids, const float* add, int ldadd, float* y, int ldy,
+                           void* ws, size_t ws_bytes, int M, int N, int K, int R, int adapters, int items, int dtype,
+                           sidon_stream_t stream);
+
+/*
  * Differential attention: the difference of two softmax maps over one set of
  * values, with a learned weight per head.  For batch b, head h and query i:
  *

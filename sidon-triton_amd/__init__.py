@@ -29,6 +29,8 @@ Entry points (same argument meaning as the reference):
 
 and, with no counterpart in the reference, the language-model operators of
 include/sidon_operators.h beside them:
+  * ``adapters.adapter_linear`` / ``adapters.adapter_residual`` -- a shared
+    projection with a low-rank adapter per request;
   * ``diff_attention.diff_attention`` -- differential attention, prompts and
     single tokens against a cache;
   * ``conformer.group_norm_act`` -- group norm with an activation, channels last.
@@ -37,8 +39,8 @@ The package directory name is not a Python identifier; the repository's
 entry scripts load it under the module name ``sidon_triton_amd``.
 """
 
-from . import (_lib, blas, conformer, diff_attention, encoder, encoder_attention, encoder_block, flexrel, frontend,
-               graphs, modeling, runtime)
+from . import (_lib, adapters, blas, conformer, diff_attention, encoder, encoder_attention, encoder_block, flexrel,
+               frontend, graphs, modeling, runtime)
 from .flexrel import HEAD_DIM, LEFT, NUM_POS, RIGHT, flexrel_attention
 
 __all__ = [
@@ -46,6 +48,7 @@ __all__ = [
     "LEFT",
     "NUM_POS",
     "RIGHT",
+    "adapters",
     "blas",
     "conformer",
     "diff_attention",

@@ -85,6 +85,12 @@ SIGNATURES = {
     "sidon_group_norm_act": (ctypes.c_int, [_VP, ctypes.c_int64, _VP, _VP, _VP, ctypes.c_float, _VP, ctypes.c_int64,
                                             _VP, ctypes.c_size_t, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                             ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP]),
+    "sidon_adapter_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 4),
+    "sidon_adapter_linear": (ctypes.c_int, [_VP, ctypes.c_int, _VP, ctypes.c_int, _VP, _VP, _VP, _VP, _VP, _VP,
+                                            ctypes.c_int, _VP, ctypes.c_size_t, *[ctypes.c_int] * 8, _VP]),
+    "sidon_adapter_residual": (ctypes.c_int, [_VP, ctypes.c_int, _VP, ctypes.c_int, _VP, _VP, _VP, _VP, _VP,
+                                              ctypes.c_int, _VP, ctypes.c_int, _VP, ctypes.c_size_t,
+                                              *[ctypes.c_int] * 7, _VP]),
     "sidon_diff_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
     "sidon_diff_attention": (ctypes.c_int, [_VP, _VP, _VP, _VP, ctypes.c_int, ctypes.c_float, _VP, _VP, ctypes.c_float,
                                             _VP, _VP, ctypes.c_size_t, *[ctypes.c_int] * 8, _I64P, _I64P, _I64P, _I64P,

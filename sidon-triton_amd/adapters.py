@@ -1,0 +1,170 @@
+"""Shared projections with a low-rank adapter per request (csrc/adapters.hip).
+
+The reference merges one adapter into the weights before serving
+(W + 0.25 A B, tools/convert_torchscript.py:179-205), so a batch cannot mix fine-tuned
+variants.  Here the shared weights stay as they are and every item of a batch
+names its adapter:
+
+    y[m] = act(x[m] W^T + bias + scale_e (x[m] A_e^T) B_e^T),   e = ids[item of row m]
+
+next to ``conformer.linear`` / ``conformer.linear_silu_lt`` (``adapter_linear``)
+and ``conformer.residual_gemm`` (``adapter_residual``).  ``encoder.HipEncoder``
+takes packed adapters for its projections.  All launch on the current stream and
+allocate only the output and the workspace (neither when given).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .conformer import _row_stride, plain
+from .flexrel import _check_device_tensor, _on_device, _stream_handle
+
+MAX_RANK = 128
+_TYPES = (torch.float16, torch.bfloat16)
+
+
+def workspace_bytes(rows: int, rank: int, residual: bool = False, dtype: torch.dtype = torch.float16) -> int:
+    """Bytes of the workspace of a call on ``rows`` rows (all items together)."""
+    return int(_lib.load().sidon_adapter_workspace_bytes(rows, rank, int(residual), _lib.DTYPES[dtype]))
+
+
+def pack_adapters(pairs, scales, device=None, dtype: torch.dtype = torch.float16):
+    """[(A [r, K], B [N, r]), ...] of any ranks up to 128 and their scales ->
+    (a [E, R, K], b [E, N, R], scale [E]) for the calls below, R the largest rank
+    rounded up to 8 and the rest zeros."""
+    pairs, scales = list(pairs), [float(s) for s in scales]
+    if not pairs or len(pairs) != len(scales):
+        raise ValueError("pack_adapters needs one scale per (A, B) pair, and one pair at least")
+    for a, b in pairs:
+        if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[1] or not 1 <= a.shape[0] <= MAX_RANK \
+                or a.shape[1] != pairs[0][0].shape[1] or b.shape[0] != pairs[0][1].shape[0]:
+            raise ValueError(f"every pair must be A [r <= {MAX_RANK}, K] and B [N, r] of one K and N "
+                             f"(got {tuple(a.shape)} and {tuple(b.shape)})")
+    rank = -(-max(a.shape[0] for a, _ in pairs) // 8) * 8
+    device = pairs[0][0].device if device is None else device
+    a_all = torch.zeros(len(pairs), rank, pairs[0][0].shape[1], dtype=dtype, device=device)
+    b_all = torch.zeros(len(pairs), pairs[0][1].shape[0], rank, dtype=dtype, device=device)
+    for e, (a, b) in enumerate(pairs):
+        a_all[e, :a.shape[0]] = a.detach().to(device=device, dtype=dtype)
+        b_all[e, :, :b.shape[1]] = b.detach().to(device=device, dtype=dtype)
+    return a_all, b_all, torch.tensor(scales, dtype=torch.float32, device=device)
+
+
+def stack_adapters(pairs):
+    """The adapters of projections that are fused along their outputs (q, k and v
+    as one): [(A_i [r_i, K], B_i [N_i, r_i]), ...] -> one pair of the fused
+    projection, A stacked and B block-diagonal.  Scales that differ belong into
+    the B_i."""
+    pairs = list(pairs)
+    if not pairs:
+        raise ValueError("stack_adapters needs at least one pair")
+    return torch.cat([a for a, _ in pairs]), torch.block_diag(*[b for _, b in pairs])
+
+
+def _operands(x, w, a, b, scale, ids):
+    device = x.device
+    for name, t in (("x", x), ("w", w), ("a", a), ("b", b)):
+        _check_device_tensor(name, t, device)
+        if t.dtype not in _TYPES or t.dtype != x.dtype:
+            raise TypeError(f"{name} must be float16 or bfloat16, of x's type (got {t.dtype})")
+    for name, t in (("x", x), ("w", w)):
+        if t.dim() != 2 or t.stride(1) != 1:
+            raise ValueError(f"{name} must be a [rows, K] tensor with K contiguous")
+    rows, k = x.shape
+    n = w.shape[0]
+    if w.shape[1] != k:
+        raise ValueError(f"x has {k} columns, w {w.shape[1]}")
+    if a.dim() != 3 or a.shape[2] != k or not a.is_contiguous():
+        raise ValueError(f"a must be a contiguous [E, R, {k}] tensor")
+    if tuple(b.shape) != (a.shape[0], n, a.shape[1]) or not b.is_contiguous():
+        raise ValueError(f"b must be a contiguous [{a.shape[0]}, {n}, {a.shape[1]}] tensor")
+    _check_device_tensor("scale", scale, device)
+    if scale.dtype != torch.float32 or tuple(scale.shape) != (a.shape[0],) or not scale.is_contiguous():
+        raise ValueError(f"scale must be a contiguous float32 [{a.shape[0]}] tensor")
+    _check_device_tensor("ids", ids, device)
+    if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous() or ids.numel() < 1:
+        raise ValueError("ids must be a contiguous int32 [items] tensor")
+    if rows < 1 or rows % ids.numel():
+        raise ValueError(f"{rows} rows do not split into {ids.numel()} items")
+    return rows, n, k
+
+
+def _workspace(workspace, need, device):
+    if workspace is None:
+        return torch.empty(max(need, 16), device=device, dtype=torch.uint8)
+    _check_device_tensor("workspace", workspace, device)
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+        raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
+    return workspace
+
+
+def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, a: torch.Tensor, b: torch.Tensor,
+                   scale: torch.Tensor, ids: torch.Tensor, act: str | None = None, out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x W^T + bias + scale_e (x A_e^T) B_e^T) [M, N] for x [M, K], w [N, K],
+    a [E, R, K], b [E, N, R] (``pack_adapters``) and bias [N] or None, fp16 or bf16;
+    scale fp32 [E].
+
+    ids: int32 [items] on the device, M a multiple of items: rows in order, M /
+    items per item (an utterance of a padded batch; items = M: single tokens).  An
+    id outside [0, E) means no adapter.  act: None or "silu".  N and K multiples of
+    64, R of 8 up to 128.  Sums in fp32, scale (x A_e^T) rounded to x's type.  Rows of x, w and out
+    may be strided.  workspace: a contiguous uint8 tensor of ``workspace_bytes``.
+    Forward only."""
+    rows, n, k = _operands(x, w, a, b, scale, ids)
+    device = x.device
+    if bias is not None:
+        _check_device_tensor("bias", bias, device)
+        if bias.dtype != x.dtype or tuple(bias.shape) != (n,) or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous {x.dtype} [{n}] tensor")
+    if act not in (None, "silu"):
+        raise ValueError(f"act must be None or 'silu' (got {act!r})")
+    if not plain(*(t for t in (x, w, bias, a, b, scale) if t is not None)):
+        raise ValueError("adapter_linear has no backward: call it under torch.no_grad()")
+    if out is None:
+        out = torch.empty(rows, n, device=device, dtype=x.dtype)
+    else:
+        _check_device_tensor("out", out, device)
+        if out.dtype != x.dtype or tuple(out.shape) != (rows, n) or out.stride(1) != 1:
+            raise ValueError(f"out must be a {x.dtype} [{rows}, {n}] tensor with rows contiguous")
+    workspace = _workspace(workspace, workspace_bytes(rows, a.shape[1], False, x.dtype), device)
+    lib = _lib.load()
+    with _on_device(device):
+        rc = lib.sidon_adapter_linear(
+            x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), None if bias is None else bias.data_ptr(),
+            a.data_ptr(), b.data_ptr(), scale.data_ptr(), ids.data_ptr(), out.data_ptr(), _row_stride(out),
+            workspace.data_ptr(), workspace.numel(), rows, n, k, a.shape[1], a.shape[0], ids.numel(),
+            _lib.ACTIVATIONS[act], _lib.DTYPES[x.dtype], _stream_handle(device))
+    _lib.check("sidon_adapter_linear", rc)
+    return out
+
+
+def adapter_residual(y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                     scale: torch.Tensor, ids: torch.Tensor, out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """y + x W^T + scale_e (x A_e^T) B_e^T into the fp32 stream y [M, N], in place
+    or, with ``out`` fp32 [M, N], beside it; the other arguments as for
+    ``adapter_linear``.  The low-rank term keeps fp32 accuracy."""
+    rows, n, k = _operands(x, w, a, b, scale, ids)
+    device = x.device
+    out = y if out is None else out
+    for name, t in (("y", y), ("out", out)):
+        _check_device_tensor(name, t, device)
+        if t.dtype != torch.float32 or tuple(t.shape) != (rows, n) or t.stride(1) != 1:
+            raise ValueError(f"{name} must be a float32 [{rows}, {n}] tensor with rows contiguous")
+    if not plain(y, x, w, a, b, scale):
+        raise ValueError("adapter_residual has no backward: call it under torch.no_grad()")
+    workspace = _workspace(workspace, workspace_bytes(rows, a.shape[1], True, x.dtype), device)
+    lib = _lib.load()
+    with _on_device(device):
+        rc = lib.sidon_adapter_residual(
+            x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), a.data_ptr(), b.data_ptr(), scale.data_ptr(),
+            ids.data_ptr(), y.data_ptr(), _row_stride(y), out.data_ptr(), _row_stride(out), workspace.data_ptr(),
+            workspace.numel(), rows, n, k, a.shape[1], a.shape[0], ids.numel(), _lib.DTYPES[x.dtype],
+            _stream_handle(device))
+    _lib.check("sidon_adapter_residual", rc)
+    return out

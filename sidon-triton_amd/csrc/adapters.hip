@@ -1,0 +1,292 @@
+// adapters.hip -- a shared projection with a low-rank adapter per request
+// (MI355X / gfx950):
+//
+//   y[m] = act(x[m] . w^T + bias + scale_e (x[m] . a_e^T) . b_e^T),   e = ids[m / rows_per_id]
+//
+// and the same into an fp32 stream.  Two launches:
+//
+//   shrink   low[m] = scale_e x[m] . a_e^T   [M, R]
+//   expand   the tiled GEMM of gemm_tile.h over x . w^T, whose accumulators take
+//            low[m] . b_e^T in front of the epilogue, so y is written once
+//
+// Rows of different adapters share tiles: the shared product does not see
+// them, and the low-rank terms cost a product per adapter among a block's rows.
+#include "gemm_tile.h"
+
+#include "sidon_host.h"
+#include "sidon_operators.h"
+
+#define SIDON_API extern "C" __attribute__((visibility("default")))
+
+namespace {
+
+using namespace sidon_gemm;
+using sidon::fail;
+
+constexpr int kMaxRank = 128;
+constexpr int kShrinkWaves = 8;     // K ranges of a row block
+constexpr int kShrinkRows = 16;     // rows of a matrix product
+
+struct ShrinkParams {
+  const void* x;
+  const void* a;             // [adapters, R, K]
+  const float* scale;
+  const int32_t* ids;
+  void* low;                 // [planes, M, R]
+  int64_t plane;
+  int ldx, M, K, R, adapters, rows_per_id, planes;
+  int rows;                  // per workgroup, <= 16
+};
+
+// RB blocks of 16 ranks.  A workgroup owns `rows` rows; its wavefronts take
+// every kShrinkWaves-th 32 columns of K and are summed through LDS in order.
+// Products are 16 ranks x 16 rows: a lane's accumulators are 4 ranks of one
+// row, so of several adapters among the rows each costs a pass over K whose
+// other rows' results are dropped.
+template <typename E, int RB>
+__global__ void __launch_bounds__(64 * kShrinkWaves) shrink_kernel(const ShrinkParams p) {
+  typedef typename Elem<E>::e8 e8;
+  __shared__ f4 part[kShrinkWaves][RB][64];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 15, lg = lane >> 4;
+  const int row0 = blockIdx.x * p.rows;
+  const int row = min(row0 + min(ln, p.rows - 1), p.M - 1);
+  int id = p.ids[row / p.rows_per_id];
+  if (id < 0 || id >= p.adapters) id = -1;
+  const E* x = static_cast<const E*>(p.x) + (int64_t)row * p.ldx + 8 * lg;
+  // (the same for every wavefront: they hold the same rows)
+  uint64_t todo = __builtin_amdgcn_ballot_w64(id >= 0);
+  while (todo != 0) {
+    const int e = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
+    todo &= ~__builtin_amdgcn_ballot_w64(id == e);
+    const E* a[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+      a[b] = static_cast<const E*>(p.a) + ((int64_t)e * p.R + min(16 * b + ln, p.R - 1)) * p.K + 8 * lg;
+    f4 acc[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) acc[b] = f4{};
+    constexpr int kUnroll = RB <= 2 ? 4 : 2;
+    for (int k0 = 32 * w; k0 < p.K; k0 += 32 * kShrinkWaves * kUnroll) {
+      e8 xv[kUnroll], av[kUnroll][RB];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int k = k0 + 32 * kShrinkWaves * u;
+        xv[u] = e8{};
+        if (k < p.K) xv[u] = *reinterpret_cast<const e8*>(x + k);
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          av[u][b] = e8{};
+          if (k < p.K) av[u][b] = *reinterpret_cast<const e8*>(a[b] + k);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) acc[b] = mma(av[u][b], xv[u], acc[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) part[w][b][lane] = acc[b];
+    __syncthreads();
+    const float scale = p.scale[e];
+    for (int t = threadIdx.x; t < RB * 64; t += 64 * kShrinkWaves) {
+      const int b = t >> 6, l = t & 63;
+      const int n = l & 15, r = 16 * b + 4 * (l >> 4);
+      f4 s = part[0][b][l];
+#pragma unroll
+      for (int i = 1; i < kShrinkWaves; ++i) s += part[i][b][l];
+      const int m = row0 + n;
+      if (n < p.rows && m < p.M && r < p.R && p.ids[m / p.rows_per_id] == e) {
+        E* dst = static_cast<E*>(p.low) + (int64_t)m * p.R + r;
+        for (int plane = 0; plane < p.planes; ++plane) {
+          typename Elem<E>::e4 v;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (plane == 0) s[c] *= scale;
+            v[c] = to_elem<E>(s[c]);
+            s[c] -= (float)v[c];   // exact: what the rounding left
+          }
+          *reinterpret_cast<typename Elem<E>::e4*>(dst + plane * p.plane) = v;
+        }
+      }
+    }
+    if (todo != 0) __syncthreads();
+  }
+}
+
+// ---- expand -----------------------------------------------------------------------
+
+typedef void (*ExpandFn)(LowParams);
+struct ExpandKernel {
+  int bm, bn, threads;
+  ExpandFn fn[2][2];   // [fp16, bf16][half out, fp32 add]
+};
+
+#define SIDON_LOW(BM, BN, WM, WN, MF, ST, MODE, E) gemm_tile_kernel<BM, BN, WM, WN, MF, ST, MODE, E, LowParams>
+#define SIDON_BOTH(BM, BN, WM, WN, MF, ST)                                              \
+  {BM, BN, 64 * WM * WN,                                                                \
+   {{SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, _Float16), SIDON_LOW(BM, BN, WM, WN, MF, ST, kAdd, _Float16)}, \
+    {SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, __bf16), SIDON_LOW(BM, BN, WM, WN, MF, ST, kAdd, __bf16)}}}
+#define SIDON_HALF(BM, BN, WM, WN, MF, ST)                                              \
+  {BM, BN, 64 * WM * WN,                                                                \
+   {{SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, _Float16), nullptr},                      \
+    {SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, __bf16), nullptr}}}
+
+// gemm.hip's shapes, a third of them: what the rest would gain is small next
+// to the low-rank term.
+const ExpandKernel kExpand[] = {
+    SIDON_BOTH(32, 64, 2, 2, 16, 6),   SIDON_BOTH(64, 64, 2, 2, 16, 4),   SIDON_BOTH(64, 128, 2, 4, 16, 4),
+    SIDON_BOTH(128, 128, 2, 4, 16, 4), SIDON_BOTH(192, 128, 2, 4, 16, 3), SIDON_HALF(128, 256, 2, 4, 16, 3),
+    SIDON_HALF(256, 256, 2, 4, 16, 2),
+};
+
+struct Call {
+  LowParams p;
+  const void* a;
+  const float* scale;
+  void* ws;
+  size_t ws_bytes;
+  int items, dtype;
+  bool residual;
+};
+
+int planes_of(bool residual, int dtype) { return !residual ? 1 : dtype == SIDON_FP16 ? 2 : 3; }
+
+bool ranges_meet(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t ab = reinterpret_cast<uintptr_t>(a), bb = reinterpret_cast<uintptr_t>(b);
+  return ab < bb + (uintptr_t)b_bytes && bb < ab + (uintptr_t)a_bytes;
+}
+
+int check_and_launch(Call& c, sidon_stream_t stream) {
+  LowParams& p = c.p;
+  if (!p.x || !p.w || !c.a || !p.up || !c.scale || !p.ids || !p.y || !c.ws || (c.residual && !p.add))
+    return fail(SIDON_E_NULL, "only bias may be NULL");
+  if (c.dtype != SIDON_FP16 && c.dtype != SIDON_BF16)
+    return fail(SIDON_E_SHAPE, "dtype=%d is neither SIDON_FP16 nor SIDON_BF16", c.dtype);
+  if (p.M < 1 || p.N < 64 || p.N % 64 != 0 || p.K < 64 || p.K % 64 != 0 || p.rank < 8 || p.rank > kMaxRank ||
+      p.rank % 8 != 0 || p.adapters < 1 || c.items < 1 || p.M % c.items != 0)
+    return fail(SIDON_E_SHAPE,
+                "M=%d N=%d K=%d R=%d adapters=%d items=%d: need M >= 1 and a multiple of items, N and K multiples of 64, "
+                "R a multiple of 8 up to %d, adapters >= 1",
+                p.M, p.N, p.K, p.rank, p.adapters, c.items, kMaxRank);
+  if (p.act != SIDON_ACT_NONE && p.act != SIDON_ACT_SILU) return fail(SIDON_E_SHAPE, "act=%d: 0 (none) or 1 (SiLU)", p.act);
+  const int step = c.residual ? 4 : 8;
+  if (p.ldx < p.K || p.ldw < p.K || p.ldy < p.N || (p.ldx | p.ldw) % 8 != 0 || p.ldy % step != 0 ||
+      (c.residual && (p.ldadd < p.N || p.ldadd % step != 0)))
+    return fail(SIDON_E_STRIDE, "row strides ldx=%d ldw=%d (multiples of 8, >= K) ldy=%d ldadd=%d (multiples of %d, >= N)",
+                p.ldx, p.ldw, p.ldy, p.ldadd, step);
+  if ((int64_t)p.M * p.ldx * 2 >= (int64_t(1) << 32) || (int64_t)p.N * p.ldw * 2 >= (int64_t(1) << 32))
+    return fail(SIDON_E_SHAPE, "x and w must each span less than 4 GiB");
+  if (!sidon::aligned16(p.x) || !sidon::aligned16(p.w) || !sidon::aligned16(c.a) || !sidon::aligned16(p.up) ||
+      !sidon::aligned16(p.y) || !sidon::aligned16(c.ws) || (c.residual && !sidon::aligned16(p.add)) ||
+      (reinterpret_cast<uintptr_t>(p.bias) & 7u) != 0 || (reinterpret_cast<uintptr_t>(p.ids) & 3u) != 0 ||
+      (reinterpret_cast<uintptr_t>(c.scale) & 3u) != 0)
+    return fail(SIDON_E_ALIGN, "x, w, a, b, y, add and ws must be 16-byte aligned, bias 8, ids and scale 4");
+  const size_t need = sidon_adapter_workspace_bytes(p.M, p.rank, c.residual, c.dtype);
+  if (c.ws_bytes < need) return fail(SIDON_E_SHAPE, "ws holds %zu bytes, the call needs %zu", c.ws_bytes, need);
+  // Workgroups read the inputs while others already write y.
+  const int64_t ysize = c.residual ? 4 : 2;
+  const int64_t ybytes = ((int64_t)(p.M - 1) * p.ldy + p.N) * ysize;
+  const int64_t up_bytes = (int64_t)p.adapters * p.N * p.rank * 2, a_bytes = (int64_t)p.adapters * p.rank * p.K * 2;
+  if (ranges_meet(p.y, ybytes, p.x, ((int64_t)(p.M - 1) * p.ldx + p.K) * 2) ||
+      ranges_meet(p.y, ybytes, p.w, ((int64_t)(p.N - 1) * p.ldw + p.K) * 2) || ranges_meet(p.y, ybytes, p.up, up_bytes) ||
+      ranges_meet(p.y, ybytes, c.a, a_bytes) || ranges_meet(p.y, ybytes, c.ws, (int64_t)need) ||
+      (p.bias != nullptr && ranges_meet(p.y, ybytes, p.bias, (int64_t)p.N * 2)))
+    return fail(SIDON_E_SHAPE, "y must not overlap an input or ws");
+  if (c.residual && !(p.add == p.y && p.ldadd == p.ldy) &&
+      ranges_meet(p.y, ybytes, p.add, ((int64_t)(p.M - 1) * p.ldadd + p.N) * 4))
+    return fail(SIDON_E_SHAPE, "y may be add itself but must not overlap it otherwise");
+  int rc;
+  if ((rc = sidon::check_device())) return rc;
+  const int cus = sidon::compute_units();
+
+  p.rows_per_id = p.M / c.items;
+  p.planes = planes_of(c.residual, c.dtype);
+  p.plane = (int64_t)p.M * p.rank;
+  p.low = c.ws;
+  ShrinkParams s{};
+  s.x = p.x;
+  s.a = c.a;
+  s.scale = c.scale;
+  s.ids = p.ids;
+  s.low = c.ws;
+  s.plane = p.plane;
+  s.ldx = p.ldx, s.M = p.M, s.K = p.K, s.R = p.rank, s.adapters = p.adapters, s.rows_per_id = p.rows_per_id;
+  s.planes = p.planes;
+  // Few rows: one per workgroup, so that rows of different adapters run side by side.
+  s.rows = (p.M + cus - 1) / cus;
+  if (s.rows > kShrinkRows) s.rows = kShrinkRows;
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)((p.M + s.rows - 1) / s.rows)), block(64 * kShrinkWaves);
+  const auto shrink = [&](auto zero) {
+    typedef decltype(zero) E;
+    if (s.R <= 16) {
+      hipLaunchKernelGGL((shrink_kernel<E, 1>), grid, block, 0, st, s);
+    } else if (s.R <= 32) {
+      hipLaunchKernelGGL((shrink_kernel<E, 2>), grid, block, 0, st, s);
+    } else if (s.R <= 64) {
+      hipLaunchKernelGGL((shrink_kernel<E, 4>), grid, block, 0, st, s);
+    } else {
+      hipLaunchKernelGGL((shrink_kernel<E, 8>), grid, block, 0, st, s);
+    }
+  };
+  if (c.dtype == SIDON_FP16) {
+    shrink(_Float16(0));
+  } else {
+    shrink(__bf16(0));
+  }
+
+  const ExpandKernel* best = nullptr;
+  double best_us = 0;
+  for (const ExpandKernel& t : kExpand) {
+    if (t.fn[0][c.residual] == nullptr || p.N % t.bn != 0) continue;
+    const double us = tile_us(t.bm, t.bn, p.M, p.N, p.K, 1, !c.residual, cus);
+    if (best == nullptr || us < best_us) best = &t, best_us = us;
+  }
+  p.tiles_m = (p.M + best->bm - 1) / best->bm;
+  p.tiles_n = p.N / best->bn;
+  p.splits = 1;
+  p.group = p.tiles_m < 8 ? p.tiles_m : 8;
+  const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n;
+  if (wgs >= (int64_t(1) << 31)) return fail(SIDON_E_SHAPE, "too many tiles");
+  hipLaunchKernelGGL(best->fn[c.dtype == SIDON_BF16][c.residual], dim3((unsigned)wgs), dim3(best->threads), 0, st, p);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return fail(SIDON_E_LAUNCH, "adapter projection launch failed: %s", hipGetErrorString(err));
+  return SIDON_OK;
+}
+
+}  // namespace
+
+SIDON_API size_t sidon_adapter_workspace_bytes(int M, int R, int residual, int dtype) {
+  if (M < 1 || R < 8 || R > kMaxRank || R % 8 != 0 || (dtype != SIDON_FP16 && dtype != SIDON_BF16)) return 0;
+  return (size_t)M * R * 2 * planes_of(residual != 0, dtype);
+}
+
+SIDON_API int sidon_adapter_linear(const void* x, int ldx, const void* w, int ldw, const void* bias, const void* a,
+                                   const void* b, const float* scale, const int32_t* ids, void* y, int ldy, void* ws,
+                                   size_t ws_bytes, int M, int N, int K, int R, int adapters, int items, int act,
+                                   int dtype, sidon_stream_t stream) {
+  sidon::clear_error();
+  Call c{};
+  LowParams& p = c.p;
+  p.x = x, p.w = w, p.bias = bias, p.y = y, p.up = b, p.ids = ids;
+  p.ldx = ldx, p.ldw = ldw, p.ldy = ldy, p.M = M, p.N = N, p.K = K, p.rank = R, p.adapters = adapters, p.act = act;
+  c.a = a, c.scale = scale, c.ws = ws, c.ws_bytes = ws_bytes, c.items = items, c.dtype = dtype;
+  static_assert(kNone == SIDON_ACT_NONE && kSilu == SIDON_ACT_SILU, "the tile kernel's activation codes");
+  return check_and_launch(c, stream);
+}
+
+SIDON_API int sidon_adapter_residual(const void* x, int ldx, const void* w, int ldw, const void* a, const void* b,
+                                     const float* scale, const int32_t* ids, const float* add, int ldadd, float* y,
+                                     int ldy, void* ws, size_t ws_bytes, int M, int N, int K, int R, int adapters,
+                                     int items, int dtype, sidon_stream_t stream) {
+  sidon::clear_error();
+  Call c{};
+  LowParams& p = c.p;
+  p.x = x, p.w = w, p.y = y, p.up = b, p.ids = ids, p.add = add;
+  p.ldx = ldx, p.ldw = ldw, p.ldy = ldy, p.ldadd = ldadd;
+  p.M = M, p.N = N, p.K = K, p.rank = R, p.adapters = adapters;
+  c.a = a, c.scale = scale, c.ws = ws, c.ws_bytes = ws_bytes, c.items = items, c.dtype = dtype, c.residual = true;
+  return check_and_launch(c, stream);
+}

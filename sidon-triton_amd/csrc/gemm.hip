@@ -96,15 +96,10 @@ Choice search(int M, int N, int K, int mode, int max_splits, int cus) {
   for (const TileKernel& t : kTiles) {
     if (t.fn[mode] == nullptr || N % t.bn != 0) continue;
     const int64_t tiles = (int64_t)((M + t.bm - 1) / t.bm) * (N / t.bn);
-    const double mm = t.bm * t.bn / 4096.0, cp = (t.bm + t.bn) / 64.0;
     for (int s = 1; s <= max_splits; ++s) {
       // At least two slices per split, and the splits of one round of CUs.
       if (s > 1 && (2 * s > slices || tiles * s > cus || (int64_t)s * M > kMaxPartRows)) break;
-      const double n = (double)tiles * s;
-      const double load = (double)((tiles * s + cus - 1) / cus);
-      const double nk = (double)slices / s;
-      double us = 3.0 + load * (0.062 * nk * mm + 0.031 * nk + (mode <= kGlu ? 0.39 : 0.48) * mm) +
-                  0.065 * (n / cus) * nk * cp;
+      double us = tile_us(t.bm, t.bn, M, N, K, s, mode <= kGlu, cus);
       if (s > 1) us += (s + 1.0) * M * N * 4.0 / 8e6;  // partial tiles read back, the stream written by the norm
       if (best.tile == nullptr || us < best.us) best = Choice{&t, s, us};
     }
@@ -151,9 +146,9 @@ int launch(const Choice& c, int mode, TileParams p, hipStream_t stream, const ch
 TileParams params(const void* x, int ldx, const void* w, int ldw, const void* bias, void* y, int ldy, int M, int N,
                   int K, int act) {
   TileParams p{};
-  p.x = static_cast<const _Float16*>(x);
-  p.w = static_cast<const _Float16*>(w);
-  p.bias = static_cast<const _Float16*>(bias);
+  p.x = x;
+  p.w = w;
+  p.bias = bias;
   p.y = y;
   p.ldx = ldx;
   p.ldw = ldw;

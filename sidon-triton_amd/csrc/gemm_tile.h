@@ -1,6 +1,7 @@
-// gemm_tile.h -- the tiled fp16 GEMM kernel behind the encoder's projections
+// gemm_tile.h -- the tiled GEMM kernel behind the encoder's projections
 // (MI355X / gfx950):  acc[m, n] = sum_k X[m, k] . W[n, k], X [M, K] and
-// W [N, K] fp16 with K contiguous, fp32 sums, and an epilogue per use.
+// W [N, K] fp16 (bf16 too where a low-rank term per row joins them, adapters.hip)
+// with K contiguous, fp32 sums, and an epilogue per use.
 //
 // A workgroup owns a BM x BN tile (of one K range, when K is split over
 // workgroups) and runs WM x WN wavefronts, each TM x TN of it in MF x MF MFMA
@@ -32,9 +33,27 @@
 
 namespace sidon_gemm {
 
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+// Operand types E: _Float16 and __bf16.
+template <typename E>
+struct Elem {
+  typedef E e4 __attribute__((ext_vector_type(4)));
+  typedef E e8 __attribute__((ext_vector_type(8)));
+};
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f4 mma(Elem<_Float16>::e8 a, Elem<_Float16>::e8 b, f4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16 mma(Elem<_Float16>::e8 a, Elem<_Float16>::e8 b, f16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f4 mma(Elem<__bf16>::e8 a, Elem<__bf16>::e8 b, f4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16 mma(Elem<__bf16>::e8 a, Elem<__bf16>::e8 b, f16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
 
 // Epilogues.
 enum : int {
@@ -51,9 +70,9 @@ enum : int {
 };
 
 struct TileParams {
-  const _Float16* x;
-  const _Float16* w;
-  const _Float16* bias;
+  const void* x;      // of the kernel's operand type, as w and bias
+  const void* w;
+  const void* bias;
   void* y;
   int64_t split_stride;
   int ldx, ldw, ldy;  // row strides (elements)
@@ -63,6 +82,24 @@ struct TileParams {
   int group;    // row tiles walked together (tile order)
   int act;
 };
+
+// The same with a low-rank term per row in front of the epilogue:
+//   acc[m, n] += sum_r low[m, r] . up[e, n, r],   e = ids[m / rows_per_id], none where e is outside [0, adapters)
+// low holds `planes` summands of its values (rounded values and what the
+// roundings left), each [M, rank].
+struct LowParams : TileParams {
+  const void* low;
+  const void* up;            // [adapters, N, rank]
+  const int32_t* ids;
+  const float* add;          // kAdd: Y = add + acc
+  int64_t plane;             // elements between planes
+  int ldadd;
+  int rows_per_id, adapters, rank, planes;
+};
+template <class Params>
+struct IsLow { static constexpr bool value = false; };
+template <>
+struct IsLow<LowParams> { static constexpr bool value = true; };
 
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
@@ -104,12 +141,16 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
 
-// fp32 value rounded to fp16 on its own: the empty asm keeps a product and
+// fp32 value rounded to E on its own: the empty asm keeps a product and
 // its conversion from fusing into one mixed-precision rounding.
-__device__ __forceinline__ _Float16 to_half(float y) {
+template <typename E>
+__device__ __forceinline__ E to_elem(float y) {
   asm volatile("" : "+v"(y));
-  return (_Float16)y;
+  return (E)y;
 }
+
+// Up to this many adapters among a block's rows, a matrix product each.
+constexpr int kFewKinds = 4;
 
 template <int BM, int BN, int WM, int WN, int MF, int ST, int kMode>
 struct Tile {
@@ -128,9 +169,11 @@ struct Tile {
   static_assert(kMode != kGlu || (TN / MF) % 2 == 0, "a GLU wavefront holds pairs of blocks");
 };
 
-template <int BM, int BN, int WM, int WN, int MF, int ST, int kMode>
-__global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const TileParams p) {
+template <int BM, int BN, int WM, int WN, int MF, int ST, int kMode, typename E = _Float16, class Params = TileParams>
+__global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p) {
   using T = Tile<BM, BN, WM, WN, MF, ST, kMode>;
+  typedef typename Elem<E>::e4 h4;
+  typedef typename Elem<E>::e8 h8;
   constexpr int NW = T::kWaves, TM = T::TM, TN = T::TN;
   constexpr int IM = TM / MF, IN = TN / MF;      // MFMA blocks per wavefront
   constexpr int NG = 64 / MF;                    // lane groups along K
@@ -245,11 +288,7 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const TileParam
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
         const int i = t / IN, j = t % IN;
-        if constexpr (MF == 32) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wb[s & 1][j], xa[s & 1][i], acc[i][j], 0, 0, 0);
-        } else {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wb[s & 1][j], xa[s & 1][i], acc[i][j], 0, 0, 0);
-        }
+        acc[i][j] = mma(wb[s & 1][j], xa[s & 1][i], acc[i][j]);
 #pragma unroll
         for (int r = R * t / TT; r < R * (t + 1) / TT; ++r) {
           if (!last) {
@@ -309,12 +348,112 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const TileParam
   constexpr int kOld = kMode == kAdd ? TM / kFRows : 1;
   f4 old[kOld];
   if constexpr (kMode == kAdd) {
-    const float* yb = static_cast<const float*>(p.y) + tn * BN + TN * wn + 4 * (lane % kFLanes);
+    const float* yb = static_cast<const float*>(p.y);
+    int64_t ld = p.ldy;
+    if constexpr (IsLow<Params>::value) {
+      yb = p.add;
+      ld = p.ldadd;
+    }
+    yb += tn * BN + TN * wn + 4 * (lane % kFLanes);
 #pragma unroll
     for (int t = 0; t < kOld; ++t)
-      old[t] = *reinterpret_cast<const f4*>(yb + (int64_t)min(m0 + TM * wm + kFRows * t + lane / kFLanes, p.M - 1) * p.ldy);
+      old[t] = *reinterpret_cast<const f4*>(yb + min(m0 + TM * wm + kFRows * t + lane / kFLanes, p.M - 1) * ld);
   }
   body(kt, No{}, No{}, No{});
+  if constexpr (IsLow<Params>::value) {
+    // The low-rank term.  A lane's row of block i is MF i + ln, as its
+    // accumulators' row, so rows of different adapters in a block cost one
+    // product per adapter and a selection; up's rows come straight from global
+    // memory (each is used once by a workgroup).
+    const int col0 = tn * BN + TN * wn;
+    const E* const lowb = static_cast<const E*>(p.low);
+    const E* const upb = static_cast<const E*>(p.up);
+    constexpr int kW = 8 * NG;   // ranks per product
+    int id[IM];
+    int e0 = -1;
+    bool same = true;
+#pragma unroll
+    for (int i = 0; i < IM; ++i) {
+      const int e = p.ids[min(m0 + TM * wm + MF * i + ln, p.M - 1) / p.rows_per_id];
+      id[i] = e >= 0 && e < p.adapters ? e : -1;
+      if (i == 0) e0 = __builtin_amdgcn_readfirstlane(id[0]);
+      same = same && id[i] == e0;
+    }
+    const auto low_at = [&](int i, int plane, int r) SIDON_INLINE {
+      const E* at = lowb + plane * p.plane + (int64_t)min(m0 + TM * wm + MF * i + ln, p.M - 1) * p.rank + r;
+      return r < p.rank ? *reinterpret_cast<const h8*>(at) : h8{};
+    };
+    const auto up_at = [&](int e, int col, int r) SIDON_INLINE {
+      const E* at = upb + ((int64_t)e * p.N + col0 + col) * p.rank + r;
+      return r < p.rank ? *reinterpret_cast<const h8*>(at) : h8{};
+    };
+    if (__builtin_amdgcn_ballot_w64(!same) == 0) {
+      if (e0 >= 0) {
+        for (int r0 = 0; r0 < p.rank; r0 += kW) {
+          const int r = r0 + 8 * lg;
+          h8 u[IN];
+#pragma unroll
+          for (int j = 0; j < IN; ++j) u[j] = up_at(e0, MF * j + ln, r);
+          for (int plane = 0; plane < p.planes; ++plane) {
+#pragma unroll
+            for (int i = 0; i < IM; ++i) {
+              const h8 v = low_at(i, plane, r);
+#pragma unroll
+              for (int j = 0; j < IN; ++j) acc[i][j] = mma(u[j], v, acc[i][j]);
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < IM; ++i) {
+        uint64_t todo = __builtin_amdgcn_ballot_w64(id[i] >= 0);
+        int kinds = 0;
+        for (uint64_t t = todo; t != 0; ++kinds)
+          t &= ~__builtin_amdgcn_ballot_w64(id[i] == __builtin_amdgcn_readlane(id[i], __builtin_ctzll(t)));
+        if (kinds <= kFewKinds) {
+          while (todo != 0) {
+            const int e = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(todo));
+            todo &= ~__builtin_amdgcn_ballot_w64(id[i] == e);
+#pragma unroll
+            for (int j = 0; j < IN; ++j) {
+              // (apart from acc, so that what another adapter holds, infinities
+              // among it, never meets this row's sum)
+              acc_t t = {};
+              for (int r0 = 0; r0 < p.rank; r0 += kW) {
+                const int r = r0 + 8 * lg;
+                const h8 u = up_at(e, MF * j + ln, r);
+                for (int plane = 0; plane < p.planes; ++plane) t = mma(u, low_at(i, plane, r), t);
+              }
+#pragma unroll
+              for (int a = 0; a < AR; ++a) acc[i][j][a] += id[i] == e ? t[a] : 0.f;
+            }
+          }
+        } else if (id[i] >= 0) {
+          // Nearly every row has an adapter of its own: each lane takes its
+          // row's products itself, from whole rows of up.
+          for (int r = 0; r < p.rank; r += 8) {
+            float v[8] = {};
+            for (int plane = 0; plane < p.planes; ++plane) {
+              const h8 part = low_at(i, plane, r);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) v[c] += (float)part[c];
+            }
+#pragma unroll
+            for (int j = 0; j < IN; ++j)
+#pragma unroll
+              for (int a = 0; a < AR; ++a) {
+                const h8 u = up_at(id[i], MF * j + 8 * (a >> 2) + 4 * lg + (a & 3), r);
+                float t = acc[i][j][a];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) t = fmaf(v[c], (float)u[c], t);
+                acc[i][j][a] = t;
+              }
+          }
+        }
+      }
+    }
+  }
   lds_barrier();  // every wavefront is done with the ring, which the epilogue reuses
 
   // acc[i][j]: row MF i + ln, columns MF j + 8 (e / 4) + 4 lg + e % 4 of the
@@ -343,9 +482,9 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const TileParam
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               // Both halves rounded to fp16 first, as the projection stores them.
-              const float a = (float)to_half(acc[i][j][4 * q + e]);
-              const float b = (float)to_half(acc[i][j + IN / 2][4 * q + e]);
-              v[e] = to_half(a * sigmoid(b));
+              const float a = (float)to_elem<E>(acc[i][j][4 * q + e]);
+              const float b = (float)to_elem<E>(acc[i][j + IN / 2][4 * q + e]);
+              v[e] = to_elem<E>(a * sigmoid(b));
             }
             put(i, MF * j + 8 * q + 4 * lg, v);
           }
@@ -358,16 +497,16 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const TileParam
           for (int q = 0; q < Q; ++q) {
             const int col = MF * j + 8 * q + 4 * lg;
             h4 bv = {};
-            if (p.bias != nullptr) bv = *reinterpret_cast<const h4*>(p.bias + tn * BN + TN * wn + col);
+            if (p.bias != nullptr) bv = *reinterpret_cast<const h4*>(static_cast<const E*>(p.bias) + tn * BN + TN * wn + col);
 #pragma unroll
             for (int i = 0; i < IM; ++i) {
               h4 v;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 float s = acc[i][j][4 * q + e] + (float)bv[e];
-                if constexpr (kAct == kSiluHalf) s = (float)to_half(s);
+                if constexpr (kAct == kSiluHalf) s = (float)to_elem<E>(s);
                 if constexpr (kAct != kNone) s = s * sigmoid(s);
-                v[e] = to_half(s);
+                v[e] = to_elem<E>(s);
               }
               put(i, col, v);
             }
@@ -392,7 +531,7 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const TileParam
         const h4 lo = *reinterpret_cast<const h4*>(ep + row * kRow + (((2 * c) ^ (row & kUnitMask)) << 3));
         const h4 hi = *reinterpret_cast<const h4*>(ep + row * kRow + (((2 * c + 1) ^ (row & kUnitMask)) << 3));
         const h8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        *reinterpret_cast<h8*>(static_cast<_Float16*>(p.y) + (int64_t)gmr * p.ldy +
+        *reinterpret_cast<h8*>(static_cast<E*>(p.y) + (int64_t)gmr * p.ldy +
                                tn * (kMode == kGlu ? BN / 2 : BN) + OC * wn + 8 * c) = v;
       }
     }
@@ -427,6 +566,17 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const TileParam
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
   }
+}
+
+// What a launch of bm x bn tiles takes (us; gemm.hip states the fit): K in
+// `splits` ranges, `half` for 16-bit outputs.
+inline double tile_us(int bm, int bn, int M, int N, int K, int splits, bool half, int cus) {
+  const int64_t tiles = (int64_t)((M + bm - 1) / bm) * (N / bn);
+  const double mm = bm * bn / 4096.0, cp = (bm + bn) / 64.0;
+  const double n = (double)tiles * splits;
+  const double load = (double)((tiles * splits + cus - 1) / cus);
+  const double nk = (double)(K / 64) / splits;
+  return 3.0 + load * (0.062 * nk * mm + 0.031 * nk + (half ? 0.39 : 0.48) * mm) + 0.065 * (n / cus) * nk * cp;
 }
 
 }  // namespace sidon_gemm

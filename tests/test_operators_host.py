@@ -96,3 +96,64 @@ def test_diff_attention_rejects_wrong_tensors(sidon):
         call(q.float(), k.float(), v.float(), lam, 0.5)
     with pytest.raises(ValueError, match="empty"):
         call(q[:, :, :, :0], k, v, lam, 0.5)
+
+
+def _adapter(lib, residual, **over):
+    mb = 1 << 20
+    a = dict(x=16 * mb, ldx=128, w=32 * mb, ldw=128, bias=48 * mb, a=64 * mb, b=80 * mb, scale=16, ids=16, y=96 * mb,
+             ldy=256, add=112 * mb, ldadd=256, ws=128 * mb, wsb=mb, M=12, N=256, K=128, R=16, adapters=3, items=4, act=0,
+             dtype=1)
+    a.update(over)
+    if residual:
+        return lib.sidon_adapter_residual(*[a[n] for n in (
+            "x", "ldx", "w", "ldw", "a", "b", "scale", "ids", "add", "ldadd", "y", "ldy", "ws", "wsb", "M", "N", "K", "R",
+            "adapters", "items", "dtype")], None)
+    return lib.sidon_adapter_linear(*[a[n] for n in (
+        "x", "ldx", "w", "ldw", "bias", "a", "b", "scale", "ids", "y", "ldy", "ws", "wsb", "M", "N", "K", "R", "adapters",
+        "items", "act", "dtype")], None)
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(x=None), -1), (dict(w=None), -1), (dict(a=None), -1), (dict(b=None), -1), (dict(scale=None), -1),
+    (dict(ids=None), -1), (dict(y=None), -1), (dict(ws=None), -1), (dict(M=0), -2), (dict(N=32), -2), (dict(N=250), -2),
+    (dict(K=96), -2), (dict(R=0), -2), (dict(R=12), -2), (dict(R=136), -2), (dict(adapters=0), -2), (dict(items=0), -2),
+    (dict(items=5), -2), (dict(dtype=0), -2), (dict(wsb=100), -2), (dict(ldx=120), -3), (dict(ldw=132), -3),
+    (dict(ldy=255), -3), (dict(ldx=1 << 30), -2), (dict(x=8), -4), (dict(a=8), -4), (dict(ids=2), -4),
+    (dict(y=16 * (1 << 20)), -2), (dict(y=32 * (1 << 20) + 64), -2), (dict(y=80 * (1 << 20)), -2),
+    (dict(y=128 * (1 << 20)), -2),
+])
+@pytest.mark.parametrize("residual", [False, True])
+def test_adapter_calls_refuse(sidon, residual, over, code):
+    lib = sidon._lib.load()
+    assert _adapter(lib, residual, **over) == code
+    assert lib.sidon_last_error().decode()
+
+
+def test_adapter_calls_refuse_their_own(sidon):
+    lib = sidon._lib.load()
+    assert _adapter(lib, False, act=2) == -2 and _adapter(lib, False, bias=12) == -4
+    assert _adapter(lib, True, add=None) == -1 and _adapter(lib, True, ldadd=250) == -3
+    assert _adapter(lib, True, add=96 * (1 << 20), ldadd=260) == -2   # the same memory, other rows
+
+
+def test_adapter_workspace_and_packing(sidon):
+    ws = sidon.adapters.workspace_bytes
+    assert ws(100, 16) == 3200 and ws(100, 16, True) == 6400 and ws(100, 16, True, torch.bfloat16) == 9600
+    assert ws(0, 16) == 0 and ws(10, 12) == 0 and ws(10, 136) == 0
+    a, b = torch.ones(3, 64), torch.ones(128, 3)
+    pa, pb, sc = sidon.adapters.pack_adapters([(a, b), (torch.ones(9, 64), torch.ones(128, 9))], [1.0, 0.5])
+    assert tuple(pa.shape) == (2, 16, 64) and tuple(pb.shape) == (2, 128, 16) and sc.tolist() == [1.0, 0.5]
+    assert pa[0].sum() == 3 * 64 and pb[0].sum() == 3 * 128
+    with pytest.raises(ValueError):
+        sidon.adapters.pack_adapters([(a, b), (a[:, :32], b)], [1.0, 1.0])
+    with pytest.raises(ValueError):
+        sidon.adapters.pack_adapters([(a, b)], [])
+    with pytest.raises(ValueError):
+        sidon.adapters.pack_adapters([(torch.ones(129, 64), torch.ones(8, 129))], [1.0])
+
+
+def test_adapter_linear_rejects_wrong_tensors(sidon):
+    x, w = torch.zeros(4, 64, dtype=torch.float16), torch.zeros(64, 64, dtype=torch.float16)
+    a, b = torch.zeros(1, 8, 64, dtype=torch.float16), torch.zeros(1, 64, 8, dtype=torch.float16)
+    with pytest.raises(ValueError, match="HIP device"):
+        sidon.adapters.adapter_linear(x, w, None, a, b, torch.ones(1), torch.zeros(1, dtype=torch.int32))
