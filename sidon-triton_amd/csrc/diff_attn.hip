@@ -90,6 +90,15 @@ struct Half<__bf16> {
   }
 };
 
+// A pointer that is the same in every lane, in scalar registers (the copies
+// take it there, and under pressure the compiler forms it in vector ones).
+__device__ __forceinline__ const char* uniform(const char* x) {
+  const uint64_t u = reinterpret_cast<uint64_t>(x);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)u);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
+  return reinterpret_cast<const char*>((uint64_t)hi << 32 | lo);
+}
+
 // x of lane l plus x of lane l ^ 32.
 __device__ __forceinline__ float pair_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -122,57 +131,41 @@ __device__ __forceinline__ float wave_lambda(const DiffParams& p, int hk, int ro
   return lambda;
 }
 
-template <int N>
-__device__ __forceinline__ void wait_copies(int newer_steps) {
-  // all but the copies (N a step) of the `newer_steps` youngest steps have landed
-  if (newer_steps >= 3) {
-    wait_vmcnt<3 * N>();
-  } else if (newer_steps == 2) {
-    wait_vmcnt<2 * N>();
-  } else if (newer_steps == 1) {
-    wait_vmcnt<N>();
-  } else {
-    wait_vmcnt<0>();
-  }
-}
-
-// A workgroup: RB row blocks x MW wavefronts per row block (2: one per map, 1:
-// both maps in one) x KS key groups.
-template <int D, int RB, int MW, int KS, int ST>
+// A workgroup: RB row blocks x 2 maps x KS key groups, a wavefront each.  The
+// wavefronts of a key group share a ring of two key slots and three value
+// slots, a step of 32 keys each.
+template <int D, int RB, int KS>
 struct Shape {
-  static constexpr int kMaps = 2 / MW;                // maps per wavefront
-  static constexpr int kRingWaves = RB * MW;          // wavefronts that share a ring
+  static constexpr int kRingWaves = 2 * RB;
   static constexpr int kWaves = kRingWaves * KS;
-  static constexpr int kP = D / 64;                   // 128-byte panels per key map
-  static constexpr int kPanels = 4 * kP;              // of a step: K of map 0, K of map 1, V
-  static constexpr int kStage = kPanels * kTile;
-  static constexpr int kRing = ST * kStage;
+  static constexpr int kP = D / 64;                   // 128-byte panels per key map (twice as many for V)
+  static constexpr int kSlot = 2 * kP * kTile;        // bytes of a step's keys (both maps), or of its values
+  static constexpr int kV = 2 * kSlot;                // value slots behind the key slots
+  static constexpr int kRing = 5 * kSlot;
   static constexpr int kDb = 2 * D / 32;              // 32-wide blocks of the values
-  static constexpr int kO = kMaps * kDb * 16;         // fp32 accumulators per lane
-  static constexpr int kPart = (kO + 4) * 64 * 4;     // bytes of a wavefront's partial result
+  static constexpr int kPart = (kDb * 16 + 4) * 64 * 4;   // bytes of a wavefront's partial result
   static constexpr int kMerge = KS > 1 ? KS / 2 * kRingWaves * kPart : 0;
-  static constexpr int kCross = MW > 1 ? RB * kPart : 0;
+  static constexpr int kCross = RB * kPart;
   static constexpr int kNeed = kMerge > kCross ? kMerge : kCross;
   static constexpr int kLds = KS * kRing > kNeed ? KS * kRing : kNeed;
-  static constexpr int kMine = kPanels / kRingWaves;  // panels a wavefront copies
-  static constexpr int kCopies = kMine * 4;           // 1 KB copies per wavefront and step
-  static_assert(kLds <= 160 * 1024 && kCopies * (ST - 1) < 64 && ST >= 2 && ST <= 4, "LDS, vmcnt range");
-  static_assert(kPanels % kRingWaves == 0, "whole panels per wavefront");
+  static constexpr int kCopies = kSlot / 1024 / kRingWaves;   // 1 KB copies per wavefront and slot
+  static_assert(kLds <= 160 * 1024, "LDS");
+  static_assert(kSlot / 1024 % kRingWaves == 0, "an even split of the copies");
 };
 
-template <typename E, int D, int RB, int MW, int KS, int ST, int kMinWaves>
-__global__ void __launch_bounds__(64 * RB * MW * KS, kMinWaves) diff_attn_kernel(const DiffParams p) {
-  using C = Shape<D, RB, MW, KS, ST>;
+template <typename E, int D, int RB, int KS, int kMinWaves>
+__global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(const DiffParams p) {
+  using C = Shape<D, RB, KS>;
   typedef typename Half<E>::v2 v2;
   typedef typename Half<E>::v4 v4;
-  constexpr int P = C::kP, NM = C::kMaps, kDb = C::kDb;
-  constexpr int kQ = D / 16;          // Q operands per map
+  constexpr int P = C::kP, kDb = C::kDb;
+  constexpr int kQ = D / 16;          // Q operands
   __shared__ __attribute__((aligned(16))) char smem[C::kLds];
 
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = w % C::kRingWaves, ks = w / C::kRingWaves;
-  const int rb = wr % RB, m0 = wr / RB;   // row block, first (or only) map
+  const int rb = wr >> 1, map = wr & 1;
   const int n = lane & 31, g = lane >> 5;
 
   // Each XCD takes a contiguous range: key heads slowest, so that a head's keys
@@ -190,9 +183,9 @@ __global__ void __launch_bounds__(64 * RB * MW * KS, kMinWaves) diff_attn_kernel
   int lk = p.S;
   if (p.lens != nullptr) lk = __builtin_amdgcn_readfirstlane(min(max(p.lens[b], 0), p.S));
 
-  // Keys that this lane's row sees, the most and the fewest that a row of the
-  // wavefront does, and the steps that some row of the workgroup needs.
-  int lim, wave_most, wave_least, steps;
+  // Keys that this lane's row sees, the fewest that a row of the wavefront
+  // does, and the steps that some row of the wavefront, of the workgroup needs.
+  int lim, wave_least, wave_steps, steps;
   {
     const auto limit = [&](int r) SIDON_INLINE { return p.causal ? min(max(lk - p.L + 1 + r % p.L, 0), lk) : lk; };
     // Over rows [a, e): a causal row's limit grows with its query and starts
@@ -202,60 +195,63 @@ __global__ void __launch_bounds__(64 * RB * MW * KS, kMinWaves) diff_attn_kernel
       if (a >= e) return 0;
       return a / p.L != (e - 1) / p.L ? lk : limit(e - 1);
     };
-    wave_most = most(row0, row0 + kBlock);
+    const int wave_most = most(row0, row0 + kBlock);
     const int last = min(row0 + kBlock, p.R) - 1;
     wave_least = row0 > last ? 0 : limit(row0 / p.L != last / p.L ? last / p.L * p.L : row0);
     lim = row < p.R ? limit(row) : wave_most;   // (rows past R are never stored)
+    wave_steps = (wave_most + kStep - 1) / kStep;
     steps = (most(blk * RB * kBlock, (blk + 1) * RB * kBlock) + kStep - 1) / kStep;
   }
   const int t0 = (int)((int64_t)steps * split / p.splits);
   const int t1 = (int)((int64_t)steps * (split + 1) / p.splits);
-  const int count = (t1 - t0 + KS - 1) / KS;   // of every key group; its last step may be past t1
   const auto mine = [&](int u) SIDON_INLINE { return t0 + u * KS + ks; };   // step u of this group
-  const int own = count > 0 && mine(count - 1) >= t1 ? count - 1 : count;
+  const auto until = [&](int t) SIDON_INLINE { return max(t - t0 - ks + KS - 1, 0) / KS; };   // steps u with mine(u) < t
+  const int all = (t1 - t0 + KS - 1) / KS;         // most steps of a group: the workgroup's rounds
+  const int have = until(t1);                      // of this group, in its ring
+  const int count = until(min(t1, wave_steps));    // of this wavefront
 
-  // ---- copies: panels K of map 0, K of map 1, V, over the ring's wavefronts ----
+  // ---- copies into the ring, split over its wavefronts ----
   const uint32_t ring = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem) + ks * C::kRing;
   const char* const kbase = static_cast<const char*>(p.k) + 2 * (b * p.kb + hk * p.kh);
   const char* const vbase = static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh);
-  const int crow = lane >> 3;                                // row of a copy's 8
-  // Step t into ring slot `slot`.  Rows past the valid keys read the last
-  // valid one again: their probabilities are 0, and what lies there may be anything.
-  const auto copy = [&](int t, int slot) SIDON_INLINE {
+  // Rows past the valid keys read the last valid one again: their
+  // probabilities are 0, and what lies there may be anything.
+  const auto copy = [&](int t, uint32_t at, const char* base, int64_t panel0, int64_t panel, int64_t stride) SIDON_INLINE {
     const int most = min(lk - t * kStep, kStep) - 1;
+    const char* src = base + t * (kStep * stride);
 #pragma unroll
-    for (int j = 0; j < C::kMine; ++j) {
-      const int pid = wr * C::kMine + j;
-      const bool key = pid < 2 * P;
-      const int64_t stride = 2 * (int64_t)(key ? p.kl : p.vl);
-      const char* src = key ? kbase + 2 * ((pid / P) * p.km) + (pid % P) * 128 : vbase + (pid - 2 * P) * 128;
-      src += t * (kStep * stride);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 8 * i + crow;
-        const uint32_t off = (uint32_t)min(r, most) * (uint32_t)stride + 16u * ((lane & 7) ^ tile_swz(r));
-        dma_1k(ring + slot * C::kStage + pid * kTile + i * 1024, src, off);
-      }
+    for (int j = 0; j < C::kCopies; ++j) {
+      const int i = wr * C::kCopies + j;
+      const int pid = i / 4, r = i % 4 * 8 + (lane >> 3);
+      const uint32_t off = (uint32_t)min(r, most) * (uint32_t)stride + 16u * ((lane & 7) ^ tile_swz(r));
+      dma_1k(at + i * 1024, uniform(src + (pid / P) * panel0 + (pid % P) * panel), off);
     }
   };
-#pragma unroll
-  for (int u = 0; u < ST - 1; ++u)
-    if (u < own) copy(mine(u), u);
+  const auto copy_k = [&](int u) SIDON_INLINE {   // panel pid: dims 64 (pid % P) of map pid / P
+    if (u < have) copy(mine(u), ring + (u & 1) * C::kSlot, kbase, 2 * p.km, 128, 2 * (int64_t)p.kl);
+  };
+  const auto copy_v = [&](int u, int slot) SIDON_INLINE {   // panel pid: values 64 pid
+    if (u < have) copy(mine(u), ring + C::kV + slot * C::kSlot, vbase, 128 * P, 128, 2 * (int64_t)p.vl);
+  };
+  copy_k(0);
+  copy_k(1);
+  copy_v(0, 0);
 
   // ---- Q^T operands: lane (n, g) holds query n, dims 16 s + 8 g + [0, 8) ----
   const int rr = min(row, p.R - 1);
-  i4 qop[NM][kQ];
+  i4 qop[kQ];
   {
-    const E* qp = static_cast<const E*>(p.q) + b * p.qb + (hk * p.G + rr / p.L) * p.qh + (rr % p.L) * p.ql + 8 * g;
+    const E* qp = static_cast<const E*>(p.q) + b * p.qb + (hk * p.G + rr / p.L) * p.qh + (rr % p.L) * p.ql + 8 * g +
+                  map * p.qm;
 #pragma unroll
-    for (int m = 0; m < NM; ++m)
-#pragma unroll
-      for (int s = 0; s < kQ; ++s) qop[m][s] = *reinterpret_cast<const i4*>(qp + (m0 + m) * p.qm + 16 * s);
+    for (int s = 0; s < kQ; ++s) qop[s] = *reinterpret_cast<const i4*>(qp + 16 * s);
   }
 
   // ---- operand offsets in a tile ----
   const int krow = mfma_row_perm(n);
+  const char* const ktile = smem + ks * C::kRing + map * P * kTile + krow * 128;
   const int kswz = tile_swz(krow);
+  const char* const vtile = smem + ks * C::kRing + C::kV;
   int tr[2][2];
   {
     const int G4 = lane >> 4, a = (lane >> 2) & 3, bq = lane & 3;
@@ -269,115 +265,130 @@ __global__ void __launch_bounds__(64 * RB * MW * KS, kMinWaves) diff_attn_kernel
       }
   }
 
-  f32x16 o[NM][kDb];
+  f32x16 o[kDb];
 #pragma unroll
-  for (int m = 0; m < NM; ++m)
-#pragma unroll
-    for (int d = 0; d < kDb; ++d) o[m][d] = f32x16{};
-  float mx[NM], sum[NM];   // maximum of the scaled scores (of lanes n and n + 32), sum over this lane's keys
-#pragma unroll
-  for (int m = 0; m < NM; ++m) {
-    mx[m] = kFloorMax;
-    sum[m] = 0.f;
-  }
+  for (int d = 0; d < kDb; ++d) o[d] = f32x16{};
+  float mx = kFloorMax, sum = 0.f;   // maximum of the scaled scores and sum of the probabilities of query n
+  f32x16 s;                          // scores of a step: element i is key 16 (i / 8) + 8 g + i % 8
+  i4 pk[2];                          // its probabilities
 
-  const auto compute = [&](int t, int slot) SIDON_INLINE {
-    const char* stage = smem + ks * C::kRing + slot * C::kStage;
-    const int k0 = t * kStep;
-    const bool masked = k0 + kStep > wave_least;
-    i4 pk[NM][2];
+  // The three parts of a step.  In round u a wavefront takes the scores of
+  // step u + 1, the softmax of step u and the product with the values of step
+  // u - 1, so that matrix and vector instructions of a round are independent.
+  const auto scores = [&](int u) SIDON_INLINE {
+    const char* tile = ktile + (u & 1) * C::kSlot;
+    f32x16 acc = {};
 #pragma unroll
-    for (int m = 0; m < NM; ++m) {
-      f32x16 s = {};
-#pragma unroll
-      for (int i = 0; i < kQ; ++i) {
-        const char* tile = stage + ((m0 + m) * P + i / 4) * kTile;
-        const i4 kop = *reinterpret_cast<const i4*>(tile + krow * 128 + (((2 * (i % 4) + g) ^ kswz) << 4));
-        s = Half<E>::mfma(kop, qop[m][i], s);
-      }
-      if (masked) {
-        const int left = lim - k0 - 8 * g;   // element i is key 16 (i / 8) + i % 8 of what this lane holds
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (16 * (i >> 3) + (i & 7) >= left) s[i] = -INFINITY;
-      }
-      const auto probs = [&](float top) SIDON_INLINE {
-        float total = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const f2 e = {fast_exp2(fmaf(s[i], p.scale, -top)), fast_exp2(fmaf(s[i + 1], p.scale, -top))};
-          total += e[0] + e[1];
-          const v2 r = __builtin_convertvector(e, v2);
-          pk[m][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, r);
-        }
-        return total;
-      };
-      float total = probs(mx[m]);
-      // A lane's 16 probabilities that sum below 2^15 are finite in fp16.
-      bool need = !(total < kSumLimit);
-      if (__builtin_amdgcn_ballot_w64(need) != 0) {
-        // Both lanes of a query raise its maximum together.
-        float top = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-        top = pair_max(top) * p.scale;
-        need = pair_max(need ? 1.f : 0.f) != 0.f;
-        const float next = need ? fmaxf(mx[m], top) : mx[m];
-        const float alpha = fast_exp2(mx[m] - next);   // 1 where nothing changed, 0 from kFloorMax
-        if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
-#pragma unroll
-          for (int d = 0; d < kDb; ++d) o[m][d] *= alpha;
-        }
-        sum[m] *= alpha;
-        mx[m] = next;
-        total = probs(next);
-      }
-      sum[m] += total;
-      __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < kQ; ++i) {
+      const i4 kop = *reinterpret_cast<const i4*>(tile + (i / 4) * kTile + (((2 * (i % 4) + g) ^ kswz) << 4));
+      acc = Half<E>::mfma(kop, qop[i], acc);
     }
+    s = acc;
+  };
+  const auto hide = [&](int u) SIDON_INLINE {
+    const int k0 = mine(u) * kStep;
+    if (k0 + kStep > wave_least) {
+      const int left = lim - k0 - 8 * g;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (16 * (i >> 3) + (i & 7) >= left) s[i] = -INFINITY;
+    }
+  };
+  const auto probs = [&](i4 (&to)[2]) SIDON_INLINE {
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const f2 e = {fast_exp2(fmaf(s[i], p.scale, -mx)), fast_exp2(fmaf(s[i + 1], p.scale, -mx))};
+      total += e[0] + e[1];
+      to[i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, __builtin_convertvector(e, v2));
+    }
+    return total;
+  };
+  const auto values = [&](int slot) SIDON_INLINE {
+    typedef int i2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
       for (int d = 0; d < kDb; ++d) {
-        const char* tile = stage + (2 * P + d / 2) * kTile + 2048 * hh;
-        const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + tr[0][d & 1]));
-        const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + tr[1][d & 1]));
-        typedef int i2 __attribute__((ext_vector_type(2)));
-        const i2 l2 = __builtin_bit_cast(i2, lo), u2 = __builtin_bit_cast(i2, hi);
-        const i4 vop = {l2[0], l2[1], u2[0], u2[1]};
-#pragma unroll
-        for (int m = 0; m < NM; ++m) o[m][d] = Half<E>::mfma(vop, pk[m][hh], o[m][d]);
-        if (d % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // few operands at a time: the registers are full
+        const char* tile = vtile + slot * C::kSlot + (d / 2) * kTile + 2048 * hh;
+        const i2 lo = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + tr[0][d & 1])));
+        const i2 hi = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + tr[1][d & 1])));
+        o[d] = Half<E>::mfma(i4{lo[0], lo[1], hi[0], hi[1]}, pk[hh], o[d]);
       }
   };
-
-  // ---- key steps ----
-  int slot = 0;
-  for (int u = 0; u < count; ++u) {
-    // Step u has landed; behind the barrier it has for every wavefront of the
-    // ring, and nobody reads slot u - 1 any more, which is filled again.
-    wait_copies<C::kCopies>(min(ST - 2, own - 1 - u));
-    if constexpr (C::kRingWaves > 1) {
-      lds_barrier();
-    } else {
-      wait_lgkm0();
-    }
-    if (u + ST - 1 < own) copy(mine(u + ST - 1), slot == 0 ? ST - 1 : slot - 1);
-    const int t = mine(u);
-    if (t < t1 && t * kStep < wave_most) compute(t, slot);
-    slot = slot == ST - 1 ? 0 : slot + 1;
-  }
+  // Raises the running maximum of the queries whose probabilities do not all
+  // fit, with what they have so far.  (The condition is a lane's, not the
+  // wavefront's: behind a branch of the wavefront the compiler keeps the
+  // accumulators in two places.)
+  const auto settle = [&](i4 (&to)[2], float total) SIDON_INLINE {
+    // 32 probabilities that sum below 2^15 are finite in fp16.
+    total = pair_sum(total);
+    if (!(total < kSumLimit)) {
+      float top = s[0];
 #pragma unroll
-  for (int m = 0; m < NM; ++m) sum[m] = pair_sum(sum[m]);
-
-  // A wavefront's partial result in LDS, lane by lane: kO values, then (maximum, sum) per map.
-  float* const mem = reinterpret_cast<float*>(smem) + lane * 4;
-  const auto put = [&](float* at, int m, int d, int i) SIDON_INLINE {
-    *reinterpret_cast<f4*>(at + ((m * kDb + d) * 4 + i) * 256) =
-        f4{o[m][d][4 * i], o[m][d][4 * i + 1], o[m][d][4 * i + 2], o[m][d][4 * i + 3]};
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+      top = fmaxf(mx, pair_max(top) * p.scale);
+      const float alpha = fast_exp2(mx - top);   // 0 from kFloorMax
+#pragma unroll
+      for (int d = 0; d < kDb; ++d) o[d] *= alpha;
+      sum *= alpha;
+      mx = top;
+      total = pair_sum(probs(to));
+    }
+    sum += total;
   };
-  const auto get = [&](const float* at, int m, int d, int i) SIDON_INLINE {
-    return *reinterpret_cast<const f4*>(at + ((m * kDb + d) * 4 + i) * 256);
+  // Behind it, what the last round copied (the keys of step u + 1, the values
+  // of step u) is there for every wavefront of the ring, and nobody reads the
+  // keys of step u or the values of step u - 2 any more: their slots are filled.
+  int vslot = 0;   // of step u + 1's values
+  const auto round = [&](int u) SIDON_INLINE {
+    wait_vmcnt<0>();
+    lds_barrier();
+    vslot = vslot == 2 ? 0 : vslot + 1;
+    copy_k(u + 2);
+    copy_v(u + 1, vslot);
+  };
+  const auto behind = [&]() SIDON_INLINE { return vslot == 2 ? 0 : vslot + 1; };   // of step u - 1: (u + 1) - 2 = + 1 mod 3
+
+  // ---- rounds -1 to `all` (the first needs the first keys alone) ----
+  int u = 0;
+  if (all > 0) {
+    if (have > 0) {
+      // The Q operands and what was copied ahead; keys 0 are the oldest.
+      wait_vmcnt<0>();
+    }
+    lds_barrier();
+    if (count > 0) scores(0);
+    round(0);
+    if (count > 0) {
+      hide(0);
+      const float total = probs(pk);
+      settle(pk, total);
+      if (count > 1) scores(1);
+    }
+    for (u = 1; u < count; ++u) {
+      round(u);
+      hide(u);
+      i4 next[2];
+      const float total = probs(next);
+      values(behind());
+      settle(next, total);
+      pk[0] = next[0];
+      pk[1] = next[1];
+      if (u + 1 < count) scores(u + 1);
+    }
+    for (; u <= all; ++u) {
+      round(u);
+      if (u == count && count > 0) values(behind());
+    }
+  }
+  // A wavefront's partial result in LDS, lane by lane: its values, then (maximum, sum).
+  float* const mem = reinterpret_cast<float*>(smem) + lane * 4;
+  const auto put = [&](float* at, int d, int i) SIDON_INLINE {
+    *reinterpret_cast<f4*>(at + (d * 4 + i) * 256) = f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+  };
+  const auto get = [&](const float* at, int d, int i) SIDON_INLINE {
+    return *reinterpret_cast<const f4*>(at + (d * 4 + i) * 256);
   };
 
   // ---- merge the key groups, half of them into the other half at a time ----
@@ -387,35 +398,29 @@ __global__ void __launch_bounds__(64 * RB * MW * KS, kMinWaves) diff_attn_kernel
       wait_vmcnt<0>();
       lds_barrier();   // the rings, or the last round's values, are done with
       float* at = mem + ((ks % half) * C::kRingWaves + wr) * (C::kPart / 4);
-      float* ml = at + NM * kDb * 4 * 256;
+      float* ml = at + kDb * 4 * 256;
       if (ks >= half && ks < 2 * half) {
 #pragma unroll
-        for (int m = 0; m < NM; ++m) {
+        for (int d = 0; d < kDb; ++d)
 #pragma unroll
-          for (int d = 0; d < kDb; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) put(at, m, d, i);
-          ml[2 * m] = mx[m];
-          ml[2 * m + 1] = sum[m];
-        }
+          for (int i = 0; i < 4; ++i) put(at, d, i);
+        ml[0] = mx;
+        ml[1] = sum;
       }
       lds_barrier();
       if (ks < half) {
+        const float top = fmaxf(mx, ml[0]);
+        const float fa = fast_exp2(mx - top), fb = fast_exp2(ml[0] - top);
+        mx = top;
+        sum = sum * fa + ml[1] * fb;
 #pragma unroll
-        for (int m = 0; m < NM; ++m) {
-          const float top = fmaxf(mx[m], ml[2 * m]);
-          const float fa = fast_exp2(mx[m] - top), fb = fast_exp2(ml[2 * m] - top);
-          mx[m] = top;
-          sum[m] = sum[m] * fa + ml[2 * m + 1] * fb;
+        for (int d = 0; d < kDb; ++d)
 #pragma unroll
-          for (int d = 0; d < kDb; ++d)
+          for (int i = 0; i < 4; ++i) {
+            const f4 v = get(at, d, i);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const f4 v = get(at, m, d, i);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[m][d][4 * i + e] = o[m][d][4 * i + e] * fa + v[e] * fb;
-            }
-        }
+            for (int e = 0; e < 4; ++e) o[d][4 * i + e] = o[d][4 * i + e] * fa + v[e] * fb;
+          }
       }
     }
     if (ks > 0) return;
@@ -425,64 +430,47 @@ __global__ void __launch_bounds__(64 * RB * MW * KS, kMinWaves) diff_attn_kernel
   if (p.splits > 1) {
     if (row >= p.R) return;
     const int64_t at = ((int64_t)bh * p.splits + split) * p.R + row;
-    float* dst = p.part_o + at * (4 * D) + 4 * g;
+    float* dst = p.part_o + at * (4 * D) + map * 2 * D + 4 * g;
+    if (g == 0) p.part_ml[at * 2 + map] = make_float2(mx, sum);
 #pragma unroll
-    for (int m = 0; m < NM; ++m) {
-      if (g == 0) p.part_ml[at * 2 + m0 + m] = make_float2(mx[m], sum[m]);
+    for (int d = 0; d < kDb; ++d)
 #pragma unroll
-      for (int d = 0; d < kDb; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<f4*>(dst + (m0 + m) * 2 * D + 32 * d + 8 * i) =
-              f4{o[m][d][4 * i], o[m][d][4 * i + 1], o[m][d][4 * i + 2], o[m][d][4 * i + 3]};
-    }
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f4*>(dst + 32 * d + 8 * i) = f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
     return;
   }
 
-  // What each map's accumulators weigh in the difference (0 where no key was seen).
-  float f[NM];
+  // What this map's accumulators weigh in the difference (0 where no key was seen).
+  float f = sum == 0.f ? 0.f : 1.f / sum;
+  float* const at = mem + rb * (C::kPart / 4);
+  lds_barrier();   // the ring, or the merge, is done with
+  if (map == 1) {
+    f *= wave_lambda<D>(p, hk, row0, rr, lane);
 #pragma unroll
-  for (int m = 0; m < NM; ++m) {
-    f[m] = sum[m] == 0.f ? 0.f : 1.f / sum[m];
-    if (m0 + m == 1) f[m] *= wave_lambda<D>(p, hk, row0, rr, lane);
-  }
-  if constexpr (MW > 1) {
-    lds_barrier();   // the ring, or the merge, is done with
-    float* at = mem + rb * (C::kPart / 4);
-    if (m0 == 1) {
+    for (int d = 0; d < kDb; ++d) {
+      o[d] *= f;
 #pragma unroll
-      for (int d = 0; d < kDb; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[0][d][4 * i] *= f[0], o[0][d][4 * i + 1] *= f[0], o[0][d][4 * i + 2] *= f[0], o[0][d][4 * i + 3] *= f[0];
-          put(at, 0, d, i);
-        }
+      for (int i = 0; i < 4; ++i) put(at, d, i);
     }
-    lds_barrier();
-    if (m0 == 1) return;
+  }
+  lds_barrier();
+  if (map == 1) return;
+  float sq = 0.f;
 #pragma unroll
-    for (int d = 0; d < kDb; ++d)
+  for (int d = 0; d < kDb; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f4 v = get(at, 0, d, i);
+    for (int i = 0; i < 4; ++i) {
+      const f4 v = get(at, d, i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[0][d][4 * i + e] = o[0][d][4 * i + e] * f[0] - v[e];
+      for (int e = 0; e < 4; ++e) {
+        const float x = o[d][4 * i + e] * f - v[e];
+        o[d][4 * i + e] = x;
+        sq = fmaf(x, x, sq);
       }
-  } else {
-#pragma unroll
-    for (int d = 0; d < kDb; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[0][d][i] = o[0][d][i] * f[0] - o[NM - 1][d][i] * f[NM - 1];
-  }
+      if (i == 3) __builtin_amdgcn_sched_barrier(0);   // (few loads at a time: the registers are full)
+    }
   float gain = 1.f;
-  if (p.norm_w != nullptr) {
-    float sq = 0.f;
-#pragma unroll
-    for (int d = 0; d < kDb; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sq = fmaf(o[0][d][i], o[0][d][i], sq);
-    gain = (1.f - p.lam_init) * rsqrtf(pair_sum(sq) * (1.f / (2 * D)) + p.eps);
-  }
+  if (p.norm_w != nullptr) gain = (1.f - p.lam_init) * rsqrtf(pair_sum(sq) * (1.f / (2 * D)) + p.eps);
   if (row >= p.R) return;
   E* dst = static_cast<E*>(p.out) + b * p.ob + (hk * p.G + row / p.L) * p.oh + (row % p.L) * p.ol + 4 * g;
 #pragma unroll
@@ -493,7 +481,7 @@ __global__ void __launch_bounds__(64 * RB * MW * KS, kMinWaves) diff_attn_kernel
       if (p.norm_w != nullptr) wv = *reinterpret_cast<const f4*>(p.norm_w + 32 * d + 8 * i + 4 * g);
       v4 r;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = (E)(o[0][d][4 * i + e] * gain * wv[e]);
+      for (int e = 0; e < 4; ++e) r[e] = (E)(o[d][4 * i + e] * gain * wv[e]);
       *reinterpret_cast<v4*>(dst + 32 * d + 8 * i) = r;
       if (i == 3) __builtin_amdgcn_sched_barrier(0);
     }
@@ -567,8 +555,8 @@ struct Plan {
 Plan plan(int B, int Hk, int R, int S, int cus) {
   Plan c;
   const int64_t heads = (int64_t)B * Hk;
-  const int64_t wide = heads * ((R + 127) / 128);
-  c.rows = R > kBlock && wide >= cus ? 128 : kBlock;
+  const int64_t wide = heads * ((R + 63) / 64);
+  c.rows = R > kBlock && wide >= cus ? 64 : kBlock;
   c.blocks = (R + c.rows - 1) / c.rows;
   c.splits = 1;
   const int64_t wgs = heads * c.blocks;
@@ -597,15 +585,15 @@ void launch(const DiffParams& p, int D, int rows, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.blocks * p.splits));
   if (D == 64) {
     if (rows == kBlock) {
-      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 1, 1, 4, 2, 1>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 1, 4, 2>), grid, dim3(512), 0, stream, p);
     } else {
-      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 4, 1, 1, 4, 2>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 2, 1, 3>), grid, dim3(256), 0, stream, p);
     }
   } else {
     if (rows == kBlock) {
-      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 1, 2, 2, 2, 1>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 1, 2, 1>), grid, dim3(256), 0, stream, p);
     } else {
-      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 4, 2, 1, 4, 2>), grid, dim3(512), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 2, 1, 2>), grid, dim3(256), 0, stream, p);
     }
   }
   if (p.splits > 1) {
