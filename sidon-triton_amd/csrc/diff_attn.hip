@@ -7,7 +7,8 @@
 //
 // with head dim D (64 or 128) per map and 2 D values, keys j < lens[b], and
 // optionally j <= lens[b] - L + i.  Grouped heads share keys and values: the
-// G heads of a group and their L queries are G L rows over one key head.
+// G heads of a group and their L queries are G L rows over one key head, a
+// query's heads side by side.
 //
 // A wavefront owns 32 rows and both maps (D = 64) or one of them (D = 128, whose
 // accumulators for both would not fit its registers): S^T = K . Q^T by
@@ -79,6 +80,9 @@ struct Half<_Float16> {
   static __device__ __forceinline__ f32x16 mfma(i4 a, i4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f4 small(i4 a, i4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  }
 };
 template <>
 struct Half<__bf16> {
@@ -87,6 +91,9 @@ struct Half<__bf16> {
   typedef b4 v4;
   static __device__ __forceinline__ f32x16 mfma(i4 a, i4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f4 small(i4 a, i4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
   }
 };
 
@@ -120,13 +127,12 @@ __device__ __forceinline__ float head_lambda(const DiffParams& p, int h, int lan
 
 // The same for a wavefront whose rows may be of several heads of its group.
 template <int D>
-__device__ __forceinline__ float wave_lambda(const DiffParams& p, int hk, int row0, int row, int lane) {
+__device__ __forceinline__ float wave_lambda(const DiffParams& p, int hk, int row, int lane) {
   if (p.lam_h == 0) return head_lambda<D>(p, 0, lane);
   float lambda = 0.f;
-  const int first = min(row0, p.R - 1) / p.L, last = min(row0 + kBlock - 1, p.R - 1) / p.L;
-  for (int j = first; j <= last; ++j) {
+  for (int j = 0; j < p.G; ++j) {
     const float l = head_lambda<D>(p, hk * p.G + j, lane);
-    if (row / p.L == j) lambda = l;
+    if (row % p.G == j) lambda = l;
   }
   return lambda;
 }
@@ -178,7 +184,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   const int blk = p.blocks - 1 - (rest - split * p.blocks);
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
   const int row0 = (blk * RB + rb) * kBlock;   // of this wavefront
-  const int row = row0 + n;                    // of this lane: head row / L of the group, query row % L
+  const int row = row0 + n;                    // of this lane: query row / G, head row % G of the group
 
   int lk = p.S;
   if (p.lens != nullptr) lk = __builtin_amdgcn_readfirstlane(min(max(p.lens[b], 0), p.S));
@@ -187,20 +193,14 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   // does, and the steps that some row of the wavefront, of the workgroup needs.
   int lim, wave_least, wave_steps, steps;
   {
-    const auto limit = [&](int r) SIDON_INLINE { return p.causal ? min(max(lk - p.L + 1 + r % p.L, 0), lk) : lk; };
-    // Over rows [a, e): a causal row's limit grows with its query and starts
-    // again at the next head.
-    const auto most = [&](int a, int e) SIDON_INLINE {
-      e = min(e, p.R);
-      if (a >= e) return 0;
-      return a / p.L != (e - 1) / p.L ? lk : limit(e - 1);
+    // (grows with the row; rows past R, never stored, see what the last one does)
+    const auto limit = [&](int r) SIDON_INLINE {
+      return p.causal ? min(max(lk - p.L + 1 + min(r, p.R - 1) / p.G, 0), lk) : lk;
     };
-    const int wave_most = most(row0, row0 + kBlock);
-    const int last = min(row0 + kBlock, p.R) - 1;
-    wave_least = row0 > last ? 0 : limit(row0 / p.L != last / p.L ? last / p.L * p.L : row0);
-    lim = row < p.R ? limit(row) : wave_most;   // (rows past R are never stored)
-    wave_steps = (wave_most + kStep - 1) / kStep;
-    steps = (most(blk * RB * kBlock, (blk + 1) * RB * kBlock) + kStep - 1) / kStep;
+    lim = limit(row);
+    wave_least = limit(row0);
+    wave_steps = row0 < p.R ? (limit(row0 + kBlock - 1) + kStep - 1) / kStep : 0;
+    steps = (limit((blk + 1) * RB * kBlock - 1) + kStep - 1) / kStep;
   }
   const int t0 = (int)((int64_t)steps * split / p.splits);
   const int t1 = (int)((int64_t)steps * (split + 1) / p.splits);
@@ -210,28 +210,45 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   const int have = until(t1);                      // of this group, in its ring
   const int count = until(min(t1, wave_steps));    // of this wavefront
 
-  // ---- copies into the ring, split over its wavefronts ----
-  const uint32_t ring = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem) + ks * C::kRing;
-  const char* const kbase = static_cast<const char*>(p.k) + 2 * (b * p.kb + hk * p.kh);
-  const char* const vbase = static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh);
-  // Rows past the valid keys read the last valid one again: their
-  // probabilities are 0, and what lies there may be anything.
-  const auto copy = [&](int t, uint32_t at, const char* base, int64_t panel0, int64_t panel, int64_t stride) SIDON_INLINE {
-    const int most = min(lk - t * kStep, kStep) - 1;
-    const char* src = base + t * (kStep * stride);
+  // ---- copies into the ring, split over its wavefronts: 1 KB copy i is rows
+  // 8 (i % 4) + [0, 8) of panel i / 4 (of the keys: dims 64 (pid % P) of map pid / P;
+  // of the values: columns 64 pid) ----
+  const uint32_t ring = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem) + ks * C::kRing + wr * C::kCopies * 1024;
+  const int pid0 = wr * C::kCopies / 4, crow = wr * C::kCopies % 4 * 8 + (lane >> 3);
+  const char* const kbase = uniform(static_cast<const char*>(p.k) + 2 * (b * p.kb + hk * p.kh + pid0 / P * p.km) +
+                                    pid0 % P * 128);
+  const char* const vbase = uniform(static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh) + pid0 * 128);
+  constexpr int kOffs = C::kCopies < 4 ? C::kCopies : 4;
+  uint32_t koff[kOffs], voff[kOffs];
 #pragma unroll
-    for (int j = 0; j < C::kCopies; ++j) {
-      const int i = wr * C::kCopies + j;
-      const int pid = i / 4, r = i % 4 * 8 + (lane >> 3);
-      const uint32_t off = (uint32_t)min(r, most) * (uint32_t)stride + 16u * ((lane & 7) ^ tile_swz(r));
-      dma_1k(at + i * 1024, uniform(src + (pid / P) * panel0 + (pid % P) * panel), off);
+  for (int j = 0; j < kOffs; ++j) {
+    const int r = crow + 8 * j;
+    koff[j] = (uint32_t)r * (uint32_t)(2 * p.kl) + 16u * ((lane & 7) ^ tile_swz(r));
+    voff[j] = (uint32_t)r * (uint32_t)(2 * p.vl) + 16u * ((lane & 7) ^ tile_swz(r));
+  }
+  const auto copy = [&](int t, uint32_t at, const char* base, int stride, const uint32_t (&off)[kOffs]) SIDON_INLINE {
+    const char* src = base + (int64_t)t * (kStep * 2 * (int64_t)stride);
+    static_assert(C::kCopies <= 4 || P == 2, "further copies are the next panel's: 128 bytes on");
+    if (lk - t * kStep >= kStep) {
+#pragma unroll
+      for (int j = 0; j < C::kCopies; ++j) dma_1k(at + j * 1024, uniform(src + j / 4 * 128), off[j % 4]);
+    } else {
+      // Rows past the valid keys read the last valid one again: their
+      // probabilities are 0, and what lies there may be anything.
+      const int most = lk - t * kStep - 1;
+#pragma unroll
+      for (int j = 0; j < C::kCopies; ++j) {
+        const int r = crow + 8 * (j % 4);
+        dma_1k(at + j * 1024, uniform(src + j / 4 * 128),
+               (uint32_t)min(r, most) * (uint32_t)(2 * stride) + 16u * ((lane & 7) ^ tile_swz(r)));
+      }
     }
   };
-  const auto copy_k = [&](int u) SIDON_INLINE {   // panel pid: dims 64 (pid % P) of map pid / P
-    if (u < have) copy(mine(u), ring + (u & 1) * C::kSlot, kbase, 2 * p.km, 128, 2 * (int64_t)p.kl);
+  const auto copy_k = [&](int u) SIDON_INLINE {
+    if (u < have) copy(mine(u), ring + (u & 1) * C::kSlot, kbase, p.kl, koff);
   };
-  const auto copy_v = [&](int u, int slot) SIDON_INLINE {   // panel pid: values 64 pid
-    if (u < have) copy(mine(u), ring + C::kV + slot * C::kSlot, vbase, 128 * P, 128, 2 * (int64_t)p.vl);
+  const auto copy_v = [&](int u, int slot) SIDON_INLINE {
+    if (u < have) copy(mine(u), ring + C::kV + slot * C::kSlot, vbase, p.vl, voff);
   };
   copy_k(0);
   copy_k(1);
@@ -241,7 +258,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   const int rr = min(row, p.R - 1);
   i4 qop[kQ];
   {
-    const E* qp = static_cast<const E*>(p.q) + b * p.qb + (hk * p.G + rr / p.L) * p.qh + (rr % p.L) * p.ql + 8 * g +
+    const E* qp = static_cast<const E*>(p.q) + b * p.qb + (hk * p.G + rr % p.G) * p.qh + (rr / p.G) * p.ql + 8 * g +
                   map * p.qm;
 #pragma unroll
     for (int s = 0; s < kQ; ++s) qop[s] = *reinterpret_cast<const i4*>(qp + 16 * s);
@@ -263,6 +280,13 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
         const int chunk = 4 * db + 2 * (G4 & 1) + (bq >> 1);
         tr[hf][db] = r * 128 + ((chunk ^ tile_swz(r)) << 4) + 8 * (bq & 1);
       }
+  }
+
+  i4 sel;
+  {
+    const E one = (((lane >> 4) ^ (lane >> 2)) & 1) == 0 ? (E)1.f : (E)0.f;
+    const int pair = __builtin_bit_cast(int, v2{one, one});
+    sel = i4{pair, pair, pair, pair};
   }
 
   f32x16 o[kDb];
@@ -294,15 +318,19 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
         if (16 * (i >> 3) + (i & 7) >= left) s[i] = -INFINITY;
     }
   };
+  // The step's probabilities, rounded, and their sum: on the matrix core, where
+  // the vector unit is the busier one.  Read as a 16x16x32 B operand, a lane's
+  // half of them holds query c + 16 (j % 2) of lane c + 16 j, keys 8 (j / 2) + [0, 8);
+  // the A operand is 1 where bit 4 of the lane equals bit 2, so that the four
+  // rows a lane receives are its own query's sum.
   const auto probs = [&](i4 (&to)[2]) SIDON_INLINE {
-    float total = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
       const f2 e = {fast_exp2(fmaf(s[i], p.scale, -mx)), fast_exp2(fmaf(s[i + 1], p.scale, -mx))};
-      total += e[0] + e[1];
       to[i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, __builtin_convertvector(e, v2));
     }
-    return total;
+    const f4 first = Half<E>::small(sel, to[0], f4{});
+    return Half<E>::small(sel, to[1], first)[0];
   };
   const auto values = [&](int slot) SIDON_INLINE {
     typedef int i2 __attribute__((ext_vector_type(2)));
@@ -321,8 +349,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   // wavefront's: behind a branch of the wavefront the compiler keeps the
   // accumulators in two places.)
   const auto settle = [&](i4 (&to)[2], float total) SIDON_INLINE {
-    // 32 probabilities that sum below 2^15 are finite in fp16.
-    total = pair_sum(total);
+    // One that left fp16 is an infinity in the sum.
     if (!(total < kSumLimit)) {
       float top = s[0];
 #pragma unroll
@@ -333,7 +360,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
       for (int d = 0; d < kDb; ++d) o[d] *= alpha;
       sum *= alpha;
       mx = top;
-      total = pair_sum(probs(to));
+      total = probs(to);
     }
     sum += total;
   };
@@ -445,7 +472,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   float* const at = mem + rb * (C::kPart / 4);
   lds_barrier();   // the ring, or the merge, is done with
   if (map == 1) {
-    f *= wave_lambda<D>(p, hk, row0, rr, lane);
+    f *= wave_lambda<D>(p, hk, rr, lane);
 #pragma unroll
     for (int d = 0; d < kDb; ++d) {
       o[d] *= f;
@@ -472,7 +499,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   float gain = 1.f;
   if (p.norm_w != nullptr) gain = (1.f - p.lam_init) * rsqrtf(pair_sum(sq) * (1.f / (2 * D)) + p.eps);
   if (row >= p.R) return;
-  E* dst = static_cast<E*>(p.out) + b * p.ob + (hk * p.G + row / p.L) * p.oh + (row % p.L) * p.ol + 4 * g;
+  E* dst = static_cast<E*>(p.out) + b * p.ob + (hk * p.G + row % p.G) * p.oh + (row / p.G) * p.ol + 4 * g;
 #pragma unroll
   for (int d = 0; d < kDb; ++d)
 #pragma unroll
@@ -499,7 +526,7 @@ __global__ void __launch_bounds__(64 * kJoinRows) diff_attn_join_kernel(const Di
   const int row = (int)(lin - bh * p.R);
   if (bh >= (int64_t)p.B * p.Hk) return;
   const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
-  const int head = hk * p.G + row / p.L;
+  const int head = hk * p.G + row % p.G;
 
   // Lane s < splits holds part s (kMaxGridSplits <= 64).
   float4 ml = make_float4(kFloorMax, 0.f, kFloorMax, 0.f);
@@ -536,7 +563,7 @@ __global__ void __launch_bounds__(64 * kJoinRows) diff_attn_join_kernel(const Di
     for (int e = 0; e < N; ++e) sq = fmaf(x[e], x[e], sq);
     gain = (1.f - p.lam_init) * rsqrtf(sidon::wave_sum(sq) * (1.f / (2 * D)) + p.eps);
   }
-  E* dst = static_cast<E*>(p.out) + b * p.ob + head * p.oh + (row % p.L) * p.ol + N * lane;
+  E* dst = static_cast<E*>(p.out) + b * p.ob + head * p.oh + (row / p.G) * p.ol + N * lane;
   typedef E en __attribute__((ext_vector_type(N)));
   en r;
 #pragma unroll
