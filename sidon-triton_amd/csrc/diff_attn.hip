@@ -112,6 +112,19 @@ __device__ __forceinline__ float pair_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// Copies of 1 KB as dma_1k's, at 2048 and 3072 beyond both addresses (dma_tile's last two).
+__device__ __forceinline__ void dma_2k(uint32_t lds_addr, const char* gbase, uint32_t v0, uint32_t v1) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %3\n\t"
+      "global_load_lds_dwordx4 %2, %3 offset:1024"
+      :: "s"(lds_addr), "v"(v0), "v"(v1), "s"(gbase) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 // The learned weight of head h, in every lane of a wavefront.
 template <int D>
 __device__ __forceinline__ float head_lambda(const DiffParams& p, int h, int lane) {
@@ -207,7 +220,6 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   const auto mine = [&](int u) SIDON_INLINE { return t0 + u * KS + ks; };   // step u of this group
   const auto until = [&](int t) SIDON_INLINE { return max(t - t0 - ks + KS - 1, 0) / KS; };   // steps u with mine(u) < t
   const int all = (t1 - t0 + KS - 1) / KS;         // most steps of a group: the workgroup's rounds
-  const int have = until(t1);                      // of this group, in its ring
   const int count = until(min(t1, wave_steps));    // of this wavefront
 
   // ---- copies into the ring, split over its wavefronts: 1 KB copy i is rows
@@ -215,44 +227,69 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   // of the values: columns 64 pid) ----
   const uint32_t ring = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem) + ks * C::kRing + wr * C::kCopies * 1024;
   const int pid0 = wr * C::kCopies / 4, crow = wr * C::kCopies % 4 * 8 + (lane >> 3);
-  const char* const kbase = uniform(static_cast<const char*>(p.k) + 2 * (b * p.kb + hk * p.kh + pid0 / P * p.km) +
-                                    pid0 % P * 128);
-  const char* const vbase = uniform(static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh) + pid0 * 128);
-  constexpr int kOffs = C::kCopies < 4 ? C::kCopies : 4;
+  const char* const kbase = static_cast<const char*>(p.k) + 2 * (b * p.kb + hk * p.kh + pid0 / P * p.km) +
+                            pid0 % P * 128 - 3072;
+  const char* const vbase = static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh) + pid0 * 128 - 3072;
+  const int whole = min(t1, lk / kStep);   // steps below it have all their rows
+  // Copy j of a set adds 1024 j to the LDS and to the global address; copies of
+  // the next panel (j >= 4) lie 128 bytes on.
+  constexpr int kOffs = C::kCopies;
+  static_assert(C::kCopies <= 4 || P == 2, "a set is within a panel, or two panels side by side");
+  const auto offset = [&](int j, int r, int stride) SIDON_INLINE {
+    return (uint32_t)r * (uint32_t)(2 * stride) + 16u * ((lane & 7) ^ tile_swz(crow + 8 * (j % 4))) + j / 4 * 128u +
+           1024u * (3 - j % 4);
+  };
   uint32_t koff[kOffs], voff[kOffs];
 #pragma unroll
   for (int j = 0; j < kOffs; ++j) {
-    const int r = crow + 8 * j;
-    koff[j] = (uint32_t)r * (uint32_t)(2 * p.kl) + 16u * ((lane & 7) ^ tile_swz(r));
-    voff[j] = (uint32_t)r * (uint32_t)(2 * p.vl) + 16u * ((lane & 7) ^ tile_swz(r));
+    koff[j] = offset(j, crow + 8 * (j % 4), p.kl);
+    voff[j] = offset(j, crow + 8 * (j % 4), p.vl);
   }
-  const auto copy = [&](int t, uint32_t at, const char* base, int stride, const uint32_t (&off)[kOffs]) SIDON_INLINE {
-    const char* src = base + (int64_t)t * (kStep * 2 * (int64_t)stride);
-    static_assert(C::kCopies <= 4 || P == 2, "further copies are the next panel's: 128 bytes on");
-    if (lk - t * kStep >= kStep) {
+  const auto issue = [&](uint32_t at, const char* src, const uint32_t (&off)[kOffs]) SIDON_INLINE {
 #pragma unroll
-      for (int j = 0; j < C::kCopies; ++j) dma_1k(at + j * 1024, uniform(src + j / 4 * 128), off[j % 4]);
-    } else {
-      // Rows past the valid keys read the last valid one again: their
-      // probabilities are 0, and what lies there may be anything.
-      const int most = lk - t * kStep - 1;
-#pragma unroll
-      for (int j = 0; j < C::kCopies; ++j) {
-        const int r = crow + 8 * (j % 4);
-        dma_1k(at + j * 1024, uniform(src + j / 4 * 128),
-               (uint32_t)min(r, most) * (uint32_t)(2 * stride) + 16u * ((lane & 7) ^ tile_swz(r)));
+    for (int j = 0; j < C::kCopies; j += 4) {
+      if constexpr (C::kCopies >= 4) {
+        dma_tile(at + j * 1024, src, off[j], off[j + 1], off[j + 2], off[j + 3]);
+      } else if constexpr (C::kCopies == 2) {
+        dma_2k(at, src, off[0], off[1]);
+      } else {
+        dma_1k(at, src, off[0]);
       }
     }
   };
-  const auto copy_k = [&](int u) SIDON_INLINE {
-    if (u < have) copy(mine(u), ring + (u & 1) * C::kSlot, kbase, p.kl, koff);
+  // Step t's copies; `src` is where its rows begin, less the 3 KB that the offsets hold.
+  const auto copy = [&](int t, uint32_t at, const char* src, int stride, const uint32_t (&off)[kOffs]) SIDON_INLINE {
+    if (t < whole) {
+      issue(at, src, off);
+    } else if (t < t1) {
+      // Rows past the valid keys read the last valid one again: their
+      // probabilities are 0, and what lies there may be anything.
+      uint32_t part[kOffs];
+#pragma unroll
+      for (int j = 0; j < kOffs; ++j) part[j] = offset(j, min(crow + 8 * (j % 4), lk - t * kStep - 1), stride);
+      issue(at, src, part);
+    }
   };
-  const auto copy_v = [&](int u, int slot) SIDON_INLINE {
-    if (u < have) copy(mine(u), ring + C::kV + slot * C::kSlot, vbase, p.vl, voff);
+  int tk = mine(0), tv = mine(0);   // the steps that are copied next
+  uint32_t kat = ring, vat = ring + C::kV;
+  const int64_t kgo = (int64_t)p.kl * (2 * kStep * KS), vgo = (int64_t)p.vl * (2 * kStep * KS);
+  const char* ksrc = kbase + (int64_t)p.kl * (2 * kStep) * tk;
+  const char* vsrc = vbase + (int64_t)p.vl * (2 * kStep) * tv;
+  const auto copy_k = [&]() SIDON_INLINE {
+    copy(tk, kat, uniform(ksrc), p.kl, koff);
+    tk += KS;
+    ksrc += kgo;
+    kat = 2 * ring + C::kSlot - kat;
   };
-  copy_k(0);
-  copy_k(1);
-  copy_v(0, 0);
+  const auto copy_v = [&]() SIDON_INLINE {
+    copy(tv, vat, uniform(vsrc), p.vl, voff);
+    tv += KS;
+    vsrc += vgo;
+    vat = vat == ring + C::kV + 2 * C::kSlot ? ring + C::kV : vat + C::kSlot;
+  };
+  copy_k();
+  copy_k();
+  copy_v();
 
   // ---- Q^T operands: lane (n, g) holds query n, dims 16 s + 8 g + [0, 8) ----
   const int rr = min(row, p.R - 1);
@@ -264,13 +301,13 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
     for (int s = 0; s < kQ; ++s) qop[s] = *reinterpret_cast<const i4*>(qp + 16 * s);
   }
 
-  // ---- operand offsets in a tile ----
-  const int krow = mfma_row_perm(n);
-  const char* const ktile = smem + ks * C::kRing + map * P * kTile + krow * 128;
-  const int kswz = tile_swz(krow);
-  const char* const vtile = smem + ks * C::kRing + C::kV;
-  int tr[2][2];
+  // ---- operand offsets from the first key and value slot ----
+  int kaddr[4], vaddr[2][2];
   {
+    const int krow = mfma_row_perm(n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      kaddr[i] = ks * C::kRing + map * P * kTile + krow * 128 + (((2 * i + g) ^ tile_swz(krow)) << 4);
     const int G4 = lane >> 4, a = (lane >> 2) & 3, bq = lane & 3;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
@@ -278,7 +315,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
       for (int db = 0; db < 2; ++db) {
         const int r = 8 * (G4 >> 1) + 4 * hf + a;
         const int chunk = 4 * db + 2 * (G4 & 1) + (bq >> 1);
-        tr[hf][db] = r * 128 + ((chunk ^ tile_swz(r)) << 4) + 8 * (bq & 1);
+        vaddr[hf][db] = ks * C::kRing + C::kV + r * 128 + ((chunk ^ tile_swz(r)) << 4) + 8 * (bq & 1);
       }
   }
 
@@ -296,59 +333,67 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   f32x16 s;                          // scores of a step: element i is key 16 (i / 8) + 8 g + i % 8
   i4 pk[2];                          // its probabilities
 
-  // The three parts of a step.  In round u a wavefront takes the scores of
-  // step u + 1, the softmax of step u and the product with the values of step
-  // u - 1, so that matrix and vector instructions of a round are independent.
-  const auto scores = [&](int u) SIDON_INLINE {
-    const char* tile = ktile + (u & 1) * C::kSlot;
+  // The three parts of a step.  In round u a wavefront takes the softmax of step
+  // u and the product with the values of step u - 1, whose vector and matrix
+  // instructions are independent, then the scores of step u + 1.
+  i4 kop[kQ];
+  uint32_t kread = 0, vread = 0;   // slots that are read next
+  const auto load_keys = [&]() SIDON_INLINE {
+#pragma unroll
+    for (int i = 0; i < kQ; ++i)
+      kop[i] = *reinterpret_cast<const i4*>(smem + (kaddr[i % 4] + kread) + i / 4 * kTile);
+    kread ^= C::kSlot;
+  };
+  const auto scores = [&]() SIDON_INLINE {
     f32x16 acc = {};
 #pragma unroll
-    for (int i = 0; i < kQ; ++i) {
-      const i4 kop = *reinterpret_cast<const i4*>(tile + (i / 4) * kTile + (((2 * (i % 4) + g) ^ kswz) << 4));
-      acc = Half<E>::mfma(kop, qop[i], acc);
-    }
+    for (int i = 0; i < kQ; ++i) acc = Half<E>::mfma(kop[i], qop[i], acc);
     s = acc;
   };
-  const auto hide = [&](int u) SIDON_INLINE {
-    const int k0 = mine(u) * kStep;
+  int k0 = mine(0) * kStep;   // first key of the step in s
+  const auto hide = [&]() SIDON_INLINE {
     if (k0 + kStep > wave_least) {
       const int left = lim - k0 - 8 * g;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (16 * (i >> 3) + (i & 7) >= left) s[i] = -INFINITY;
     }
+    k0 += KS * kStep;
+  };
+  const auto exps = [&](float (&e)[16]) SIDON_INLINE {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) e[i] = fast_exp2(fmaf(s[i], p.scale, -mx));
   };
   // The step's probabilities, rounded, and their sum: on the matrix core, where
   // the vector unit is the busier one.  Read as a 16x16x32 B operand, a lane's
   // half of them holds query c + 16 (j % 2) of lane c + 16 j, keys 8 (j / 2) + [0, 8);
   // the A operand is 1 where bit 4 of the lane equals bit 2, so that the four
   // rows a lane receives are its own query's sum.
-  const auto probs = [&](i4 (&to)[2]) SIDON_INLINE {
+  const auto round_to = [&](const float (&e)[16]) SIDON_INLINE {
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      const f2 e = {fast_exp2(fmaf(s[i], p.scale, -mx)), fast_exp2(fmaf(s[i + 1], p.scale, -mx))};
-      to[i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, __builtin_convertvector(e, v2));
-    }
-    const f4 first = Half<E>::small(sel, to[0], f4{});
-    return Half<E>::small(sel, to[1], first)[0];
+    for (int i = 0; i < 16; i += 2)
+      pk[i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, __builtin_convertvector(f2{e[i], e[i + 1]}, v2));
+    const f4 first = Half<E>::small(sel, pk[0], f4{});
+    return Half<E>::small(sel, pk[1], first)[0];
   };
-  const auto values = [&](int slot) SIDON_INLINE {
+  const auto values = [&]() SIDON_INLINE {
     typedef int i2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
       for (int d = 0; d < kDb; ++d) {
-        const char* tile = vtile + slot * C::kSlot + (d / 2) * kTile + 2048 * hh;
-        const i2 lo = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + tr[0][d & 1])));
-        const i2 hi = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + tr[1][d & 1])));
+        const char* tile = smem + vread + (d / 2) * kTile + 2048 * hh;
+        const i2 lo = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + vaddr[0][d & 1])));
+        const i2 hi = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + vaddr[1][d & 1])));
         o[d] = Half<E>::mfma(i4{lo[0], lo[1], hi[0], hi[1]}, pk[hh], o[d]);
       }
+    vread = vread == 2 * C::kSlot ? 0 : vread + C::kSlot;
   };
   // Raises the running maximum of the queries whose probabilities do not all
   // fit, with what they have so far.  (The condition is a lane's, not the
   // wavefront's: behind a branch of the wavefront the compiler keeps the
   // accumulators in two places.)
-  const auto settle = [&](i4 (&to)[2], float total) SIDON_INLINE {
+  const auto settle = [&](float total) SIDON_INLINE {
     // One that left fp16 is an infinity in the sum.
     if (!(total < kSumLimit)) {
       float top = s[0];
@@ -360,55 +405,60 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
       for (int d = 0; d < kDb; ++d) o[d] *= alpha;
       sum *= alpha;
       mx = top;
-      total = probs(to);
+      float e[16];
+      exps(e);
+      total = round_to(e);
     }
     sum += total;
   };
   // Behind it, what the last round copied (the keys of step u + 1, the values
   // of step u) is there for every wavefront of the ring, and nobody reads the
-  // keys of step u or the values of step u - 2 any more: their slots are filled.
-  int vslot = 0;   // of step u + 1's values
-  const auto round = [&](int u) SIDON_INLINE {
+  // keys of step u or the values of step u - 2 any more: their slots are filled
+  // with the keys of step u + 2 and the values of step u + 1.
+  const auto round = [&]() SIDON_INLINE {
     wait_vmcnt<0>();
     lds_barrier();
-    vslot = vslot == 2 ? 0 : vslot + 1;
-    copy_k(u + 2);
-    copy_v(u + 1, vslot);
+    copy_k();
+    copy_v();
   };
-  const auto behind = [&]() SIDON_INLINE { return vslot == 2 ? 0 : vslot + 1; };   // of step u - 1: (u + 1) - 2 = + 1 mod 3
 
   // ---- rounds -1 to `all` (the first needs the first keys alone) ----
   int u = 0;
   if (all > 0) {
-    if (have > 0) {
-      // The Q operands and what was copied ahead; keys 0 are the oldest.
-      wait_vmcnt<0>();
-    }
+    wait_vmcnt<0>();
     lds_barrier();
-    if (count > 0) scores(0);
-    round(0);
     if (count > 0) {
-      hide(0);
-      const float total = probs(pk);
-      settle(pk, total);
-      if (count > 1) scores(1);
+      load_keys();
+      scores();
+    }
+    round();
+    if (count > 0) {
+      hide();
+      float e[16];
+      exps(e);
+      settle(round_to(e));
+      if (count > 1) {
+        load_keys();
+        scores();
+      }
     }
     for (u = 1; u < count; ++u) {
-      round(u);
-      hide(u);
-      i4 next[2];
-      const float total = probs(next);
-      values(behind());
-      settle(next, total);
-      pk[0] = next[0];
-      pk[1] = next[1];
-      if (u + 1 < count) scores(u + 1);
+      round();
+      hide();
+      float e[16];
+      exps(e);
+      values();
+      const float total = round_to(e);
+      load_keys();   // (of the last round: what an earlier step left in the slot, for nothing)
+      settle(total);
+      scores();
     }
     for (; u <= all; ++u) {
-      round(u);
-      if (u == count && count > 0) values(behind());
+      round();
+      if (u == count && count > 0) values();
     }
   }
+
   // A wavefront's partial result in LDS, lane by lane: its values, then (maximum, sum).
   float* const mem = reinterpret_cast<float*>(smem) + lane * 4;
   const auto put = [&](float* at, int d, int i) SIDON_INLINE {
