@@ -65,6 +65,7 @@ struct DiffParams {
   int lam_h;
   int B, H, Hk, G, L, S, R;
   int blocks, splits;
+  int parts, parts_per_xcd;   // of a key head, of all of them on an XCD
   int causal;
   float scale;           // log2(e) / sqrt(D)
   float lam_init, eps;
@@ -187,14 +188,17 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   const int rb = wr >> 1, map = wr & 1;
   const int n = lane & 31, g = lane >> 5;
 
-  // Each XCD takes a contiguous range: key heads slowest, so that a head's keys
-  // and values stay in one L2; of a causal call the longest rows first.
-  const int lin = xcd_linear(blockIdx.x, gridDim.x);
-  const int per_head = p.splits * p.blocks;
-  const int bh = lin / per_head;
-  const int rest = lin - bh * per_head;
-  const int split = rest / p.blocks;
-  const int blk = p.blocks - 1 - (rest - split * p.blocks);
+  // Workgroups go round-robin over the 8 XCDs.  A key head's (row block, split)
+  // units are dealt into `parts` parts and the parts to the XCDs, so that each
+  // L2 holds the keys and values of few heads and every XCD gets long and short
+  // items, and causal blocks of every length; the longest come first.
+  const int xcd = blockIdx.x & 7, at_xcd = blockIdx.x >> 3;
+  const int part = at_xcd % p.parts_per_xcd * 8 + xcd;
+  const int bh = part / p.parts;
+  const int unit = at_xcd / p.parts_per_xcd * p.parts + part % p.parts;
+  if (unit >= p.blocks * p.splits) return;
+  const int split = unit / p.blocks;
+  const int blk = p.blocks - 1 - (unit - split * p.blocks);
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
   const int row0 = (blk * RB + rb) * kBlock;   // of this wavefront
   const int row = row0 + n;                    // of this lane: query row / G, head row % G of the group
@@ -215,8 +219,8 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
     wave_steps = row0 < p.R ? (limit(row0 + kBlock - 1) + kStep - 1) / kStep : 0;
     steps = (limit((blk + 1) * RB * kBlock - 1) + kStep - 1) / kStep;
   }
-  const int t0 = (int)((int64_t)steps * split / p.splits);
-  const int t1 = (int)((int64_t)steps * (split + 1) / p.splits);
+  const int t0 = (int)((uint32_t)(steps * split) / (uint32_t)p.splits);   // (steps <= 2^25, splits <= 2^6)
+  const int t1 = (int)((uint32_t)(steps * (split + 1)) / (uint32_t)p.splits);
   const auto mine = [&](int u) SIDON_INLINE { return t0 + u * KS + ks; };   // step u of this group
   const auto until = [&](int t) SIDON_INLINE { return max(t - t0 - ks + KS - 1, 0) / KS; };   // steps u with mine(u) < t
   const int all = (t1 - t0 + KS - 1) / KS;         // most steps of a group: the workgroup's rounds
@@ -325,6 +329,10 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
     const int pair = __builtin_bit_cast(int, v2{one, one});
     sel = i4{pair, pair, pair, pair};
   }
+
+  // (here, so that its loads overlap the first copies)
+  float lambda = 1.f;
+  if (p.splits == 1 && map == 1) lambda = wave_lambda<D>(p, hk, rr, lane);
 
   f32x16 o[kDb];
 #pragma unroll
@@ -522,7 +530,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   float* const at = mem + rb * (C::kPart / 4);
   lds_barrier();   // the ring, or the merge, is done with
   if (map == 1) {
-    f *= wave_lambda<D>(p, hk, rr, lane);
+    f *= lambda;
 #pragma unroll
     for (int d = 0; d < kDb; ++d) {
       o[d] *= f;
@@ -628,24 +636,34 @@ struct Plan {
   int blocks, splits;
 };
 
-// Rows per workgroup and grid splits.
-Plan plan(int B, int Hk, int R, int S, int cus) {
-  Plan c;
+// Rows per workgroup and grid splits: the least estimate of
+//
+//   8 us + rounds * (overhead + work * max(1, workgroups / CUs)) + what a split costs
+//
+// with rounds = the steps that a wavefront takes one after another (steps /
+// splits for 64 rows; a fourth of it for 32 rows, whose 4 key groups share
+// them) and, of a split, a joining launch of 4 us and its partial results
+// written and read at 4 TB/s.  Per round, measured, D = 64 | 128: 64 rows 0.3 +
+// 0.3 | 0.4 + 0.6 us, 32 rows x 4 (D = 128: 2) key groups 0.3 + 0.5 us.
+Plan plan(int B, int Hk, int R, int S, int D, int cus) {
   const int64_t heads = (int64_t)B * Hk;
-  const int64_t wide = heads * ((R + 63) / 64);
-  c.rows = R > kBlock && wide >= cus ? 64 : kBlock;
-  c.blocks = (R + c.rows - 1) / c.rows;
-  c.splits = 1;
-  const int64_t wgs = heads * c.blocks;
   const int steps = (S + kStep - 1) / kStep;
-  if (c.rows == kBlock && wgs < cus) {
-    // at least one step for each wavefront of a part
-    int64_t s = cus / wgs;
-    if (s > (steps + 3) / 4) s = (steps + 3) / 4;
-    if (s > kMaxGridSplits) s = kMaxGridSplits;
-    c.splits = s < 1 ? 1 : (int)s;
+  Plan best{};
+  double best_us = 0;
+  for (int rows = kBlock; rows <= 2 * kBlock; rows += kBlock) {
+    const int groups = rows > kBlock ? 1 : D == 64 ? 4 : 2;
+    const int blocks = (R + rows - 1) / rows;
+    const double fixed = rows > kBlock && D == 128 ? 0.4 : 0.3;
+    const double work = rows == kBlock ? 0.5 : D == 64 ? 0.3 : 0.6;
+    for (int s = 1; s <= kMaxGridSplits && (s == 1 || s * groups <= steps); ++s) {
+      const double load = (double)heads * blocks * s / cus;
+      if (s > 1 && load > 1.5) break;
+      double us = 8 + ((steps + groups * s - 1) / (groups * s)) * (fixed + work * (load > 1 ? load : 1));
+      if (s > 1) us += 4 + (double)heads * R * s * (4 * D) * 8 / 4e6;
+      if (best.rows == 0 || us < best_us) best = Plan{rows, blocks, s}, best_us = us;
+    }
   }
-  return c;
+  return best;
 }
 
 bool shape_ok(int B, int H, int Hk, int L, int S, int D) {
@@ -659,7 +677,7 @@ size_t part_bytes(int B, int Hk, int R, int D, int splits) {
 
 template <typename E>
 void launch(const DiffParams& p, int D, int rows, hipStream_t stream) {
-  const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.blocks * p.splits));
+  const dim3 grid((unsigned)(8 * p.parts_per_xcd * ((p.blocks * p.splits + p.parts - 1) / p.parts)));
   if (D == 64) {
     if (rows == kBlock) {
       hipLaunchKernelGGL((diff_attn_kernel<E, 64, 1, 4, 2>), grid, dim3(512), 0, stream, p);
@@ -689,7 +707,7 @@ void launch(const DiffParams& p, int D, int rows, hipStream_t stream) {
 SIDON_API size_t sidon_diff_attention_workspace_bytes(int B, int H, int Hk, int L, int S, int D) {
   if (!shape_ok(B, H, Hk, L, S, D)) return 0;
   const int R = H / Hk * L;
-  return part_bytes(B, Hk, R, D, plan(B, Hk, R, S, sidon::compute_units()).splits);
+  return part_bytes(B, Hk, R, D, plan(B, Hk, R, S, D, sidon::compute_units()).splits);
 }
 
 SIDON_API int sidon_diff_attention(const void* q, const void* k, const void* v, const float* lam, int lam_heads,
@@ -727,10 +745,18 @@ SIDON_API int sidon_diff_attention(const void* q, const void* k, const void* v, 
   int rc;
   if ((rc = sidon::check_device())) return rc;
   const int R = H / Hk * L;
-  const Plan c = plan(B, Hk, R, S, sidon::compute_units());
+  const Plan c = plan(B, Hk, R, S, D, sidon::compute_units());
   if (ws_bytes < part_bytes(B, Hk, R, D, c.splits) || (c.splits > 1 && ws == nullptr))
     return fail(SIDON_E_SHAPE, "ws holds %zu bytes, the call needs %zu", ws_bytes, part_bytes(B, Hk, R, D, c.splits));
-  if ((int64_t)B * Hk * c.blocks * c.splits > INT32_MAX) return fail(SIDON_E_SHAPE, "too many rows for one launch");
+  // Parts per key head (DiffParams): enough for whole heads on an XCD where
+  // possible, and all 8 where every head's keys and values fit one L2 together.
+  const int64_t heads = (int64_t)B * Hk;
+  int parts = 8;
+  while (parts > 1 && heads * (parts / 2) % 8 == 0 &&
+         (heads * S * D * 8 > (int64_t)3 << 20 || parts > c.blocks * c.splits))
+    parts /= 2;
+  if (heads * parts * (((int64_t)c.blocks * c.splits + parts - 1) / parts) > INT32_MAX / 256)
+    return fail(SIDON_E_SHAPE, "too many rows for one launch");
   DiffParams p{};
   p.q = q;
   p.k = k;
@@ -748,6 +774,7 @@ SIDON_API int sidon_diff_attention(const void* q, const void* k, const void* v, 
   p.lam_h = lam_heads == 1 ? 0 : 4 * D;
   p.B = B, p.H = H, p.Hk = Hk, p.G = H / Hk, p.L = L, p.S = S, p.R = R;
   p.blocks = c.blocks, p.splits = c.splits;
+  p.parts = parts, p.parts_per_xcd = (int)(heads * parts / 8);
   p.causal = causal != 0;
   p.scale = 1.4426950408889634f / (D == 64 ? 8.f : 11.313708498984761f);
   p.lam_init = lam_init;
