@@ -166,7 +166,8 @@ struct Shape {
   static constexpr int kPart = (kDb * 16 + 4) * 64 * 4;   // bytes of a wavefront's partial result
   static constexpr int kMerge = KS > 1 ? KS / 2 * kRingWaves * kPart : 0;
   static constexpr int kCross = RB * kPart;
-  static constexpr int kNeed = kMerge > kCross ? kMerge : kCross;
+  static constexpr int kNorm = kCross;                // the norm's weights behind it
+  static constexpr int kNeed = kMerge > kCross + 8 * D ? kMerge : kCross + 8 * D;
   static constexpr int kLds = KS * kRing > kNeed ? KS * kRing : kNeed;
   static constexpr int kCopies = kSlot / 1024 / kRingWaves;   // 1 KB copies per wavefront and slot
   static_assert(kLds <= 160 * 1024, "LDS");
@@ -469,8 +470,9 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
 
   // A wavefront's partial result in LDS, lane by lane: its values, then (maximum, sum).
   float* const mem = reinterpret_cast<float*>(smem) + lane * 4;
-  const auto put = [&](float* at, int d, int i) SIDON_INLINE {
-    *reinterpret_cast<f4*>(at + (d * 4 + i) * 256) = f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+  const auto put = [&](float* at, int d, int i, float by) SIDON_INLINE {
+    *reinterpret_cast<f4*>(at + (d * 4 + i) * 256) =
+        f4{o[d][4 * i] * by, o[d][4 * i + 1] * by, o[d][4 * i + 2] * by, o[d][4 * i + 3] * by};
   };
   const auto get = [&](const float* at, int d, int i) SIDON_INLINE {
     return *reinterpret_cast<const f4*>(at + (d * 4 + i) * 256);
@@ -484,31 +486,31 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
       lds_barrier();   // the rings, or the last round's values, are done with
       float* at = mem + ((ks % half) * C::kRingWaves + wr) * (C::kPart / 4);
       float* ml = at + kDb * 4 * 256;
-      if (ks >= half && ks < 2 * half) {
+      if (ks >= half) {
 #pragma unroll
         for (int d = 0; d < kDb; ++d)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) put(at, d, i);
+          for (int i = 0; i < 4; ++i) put(at, d, i, 1.f);
         ml[0] = mx;
         ml[1] = sum;
       }
       lds_barrier();
-      if (ks < half) {
-        const float top = fmaxf(mx, ml[0]);
-        const float fa = fast_exp2(mx - top), fb = fast_exp2(ml[0] - top);
-        mx = top;
-        sum = sum * fa + ml[1] * fb;
+      if (ks >= half) return;
+      const float top = fmaxf(mx, ml[0]);
+      const float fa = fast_exp2(mx - top), fb = fast_exp2(ml[0] - top);
+      mx = top;
+      sum = sum * fa + ml[1] * fb;
 #pragma unroll
-        for (int d = 0; d < kDb; ++d)
+      for (int d = 0; d < kDb; ++d) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const f4 v = get(at, d, i);
+        for (int i = 0; i < 4; ++i) {
+          const f4 v = get(at, d, i);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[d][4 * i + e] = o[d][4 * i + e] * fa + v[e] * fb;
-          }
+          for (int e = 0; e < 4; ++e) o[d][4 * i + e] = o[d][4 * i + e] * fa + v[e] * fb;
+        }
+        if (d % 2 == 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (ks > 0) return;
   }
 
   // Lane (n, g) holds of row n the values 32 d + 8 i + 4 g + [0, 4).
@@ -528,15 +530,27 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   // What this map's accumulators weigh in the difference (0 where no key was seen).
   float f = sum == 0.f ? 0.f : 1.f / sum;
   float* const at = mem + rb * (C::kPart / 4);
+  // The norm's weights through LDS: a lane needs 2 D / 2 of them, whose loads from
+  // memory would wait for each other (the registers are full).
+  float* const nw = reinterpret_cast<float*>(smem + C::kNorm);
+  constexpr int kThreads = 64 * C::kRingWaves, kNw = (2 * D + kThreads - 1) / kThreads;
+  float mine_w[kNw];
+  const int tid = wr * 64 + lane;
+#pragma unroll
+  for (int i = 0; i < kNw; ++i) {
+    const int c = tid + i * kThreads;
+    mine_w[i] = p.norm_w != nullptr && c < 2 * D ? p.norm_w[c] : 1.f;
+  }
   lds_barrier();   // the ring, or the merge, is done with
+#pragma unroll
+  for (int i = 0; i < kNw; ++i)
+    if (tid + i * kThreads < 2 * D) nw[tid + i * kThreads] = mine_w[i];
   if (map == 1) {
     f *= lambda;
 #pragma unroll
-    for (int d = 0; d < kDb; ++d) {
-      o[d] *= f;
+    for (int d = 0; d < kDb; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) put(at, d, i);
-    }
+      for (int i = 0; i < 4; ++i) put(at, d, i, f);
   }
   lds_barrier();
   if (map == 1) return;
@@ -562,8 +576,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   for (int d = 0; d < kDb; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f4 wv = {1.f, 1.f, 1.f, 1.f};
-      if (p.norm_w != nullptr) wv = *reinterpret_cast<const f4*>(p.norm_w + 32 * d + 8 * i + 4 * g);
+      const f4 wv = *reinterpret_cast<const f4*>(nw + 32 * d + 8 * i + 4 * g);
       v4 r;
 #pragma unroll
       for (int e = 0; e < 4; ++e) r[e] = (E)(o[d][4 * i + e] * gain * wv[e]);
@@ -572,23 +585,27 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
     }
 }
 
-// Join the grid splits of a row: one wavefront per row, 2 D / 64 values a lane.
-constexpr int kJoinRows = 4;
+// Join the grid splits of a row: a workgroup per row, whose wavefronts take every
+// fourth part; a lane has 2 D / 64 of the values.
+constexpr int kJoinWaves = 4;
 template <typename E, int D>
-__global__ void __launch_bounds__(64 * kJoinRows) diff_attn_join_kernel(const DiffParams p) {
+__global__ void __launch_bounds__(64 * kJoinWaves) diff_attn_join_kernel(const DiffParams p) {
   constexpr int N = 2 * D / 64;
   typedef float fn __attribute__((ext_vector_type(N)));
+  __shared__ fn part[kJoinWaves][64];
   const int lane = threadIdx.x & 63;
-  const int64_t lin = (int64_t)blockIdx.x * kJoinRows + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t bh = lin / p.R;
-  const int row = (int)(lin - bh * p.R);
-  if (bh >= (int64_t)p.B * p.Hk) return;
-  const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int bh = blockIdx.x / p.R;
+  const int row = blockIdx.x - bh * p.R;
+  const int b = bh / p.Hk, hk = bh - b * p.Hk;
   const int head = hk * p.G + row % p.G;
 
-  // Lane s < splits holds part s (kMaxGridSplits <= 64).
+  // Lane s < splits holds the statistics of part s (kMaxGridSplits <= 64).
   float4 ml = make_float4(kFloorMax, 0.f, kFloorMax, 0.f);
-  if (lane < p.splits) ml = *reinterpret_cast<const float4*>(p.part_ml + ((bh * p.splits + lane) * p.R + row) * 2);
+  if (lane < p.splits)
+    ml = *reinterpret_cast<const float4*>(p.part_ml + (((int64_t)bh * p.splits + lane) * p.R + row) * 2);
+  const float* src = p.part_o + ((int64_t)bh * p.splits * p.R + row) * (4 * D) + N * lane;
+  const float lambda = head_lambda<D>(p, head, lane);
   float m1 = ml.x, m2 = ml.z;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -597,23 +614,28 @@ __global__ void __launch_bounds__(64 * kJoinRows) diff_attn_join_kernel(const Di
   }
   const float f1 = fast_exp2(ml.x - m1), f2 = fast_exp2(ml.z - m2);
   const float s1 = sidon::wave_sum(ml.y * f1), s2 = sidon::wave_sum(ml.w * f2);
-  const float lambda = head_lambda<D>(p, head, lane);
-  const float i1 = s1 == 0.f ? 0.f : 1.f / s1;
-  const float i2 = s2 == 0.f ? 0.f : lambda / s2;
   // What each part weighs in the difference.
-  const float w1 = f1 * i1, w2 = f2 * i2;
+  const float w1 = s1 == 0.f ? 0.f : f1 / s1, w2 = s2 == 0.f ? 0.f : f2 / s2 * lambda;
   const uint64_t used = __builtin_amdgcn_ballot_w64(ml.y != 0.f || ml.w != 0.f);
   fn x = {};
-  const float* src = p.part_o + (bh * p.splits * p.R + row) * (4 * D) + N * lane;
 #pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
-    if (!(used >> s & 1)) continue;
-    const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w1), s));
-    const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w2), s));
-    const float* at = src + (int64_t)s * p.R * (4 * D);
-    const fn u = *reinterpret_cast<const fn*>(at), v = *reinterpret_cast<const fn*>(at + 2 * D);
-    x += u * a - v * c;
+  for (int s = w; s < p.splits; s += kJoinWaves) {
+    if ((used >> s & 1) != 0) {
+      const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w1), s));
+      const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w2), s));
+      const float* at = src + (int64_t)s * p.R * (4 * D);
+      const fn u = *reinterpret_cast<const fn*>(at), v = *reinterpret_cast<const fn*>(at + 2 * D);
+      x += u * a - v * c;
+    }
   }
+  part[w][lane] = x;
+  __syncthreads();
+  if (w != 0) return;
+#pragma unroll
+  for (int i = 1; i < kJoinWaves; ++i) x += part[i][lane];
+  fn nw;
+#pragma unroll
+  for (int e = 0; e < N; ++e) nw[e] = p.norm_w != nullptr ? p.norm_w[N * lane + e] : 1.f;
   float gain = 1.f;
   if (p.norm_w != nullptr) {
     float sq = 0.f;
@@ -625,7 +647,7 @@ __global__ void __launch_bounds__(64 * kJoinRows) diff_attn_join_kernel(const Di
   typedef E en __attribute__((ext_vector_type(N)));
   en r;
 #pragma unroll
-  for (int e = 0; e < N; ++e) r[e] = (E)(x[e] * gain * (p.norm_w != nullptr ? p.norm_w[N * lane + e] : 1.f));
+  for (int e = 0; e < N; ++e) r[e] = (E)(x[e] * gain * nw[e]);
   *reinterpret_cast<en*>(dst) = r;
 }
 
@@ -638,29 +660,35 @@ struct Plan {
 
 // Rows per workgroup and grid splits: the least estimate of
 //
-//   8 us + rounds * (overhead + work * max(1, workgroups / CUs)) + what a split costs
+//   3 us + turns * (ends + rounds * (alone + more * running)) + what a split costs
 //
-// with rounds = the steps that a wavefront takes one after another (steps /
-// splits for 64 rows; a fourth of it for 32 rows, whose 4 key groups share
-// them) and, of a split, a joining launch of 4 us and its partial results
-// written and read at 4 TB/s.  Per round, measured, D = 64 | 128: 64 rows 0.3 +
-// 0.3 | 0.4 + 0.6 us, 32 rows x 4 (D = 128: 2) key groups 0.3 + 0.5 us.
+// where a CU runs up to `fit` workgroups at once and takes `turns` turns, a
+// workgroup's rounds are its steps over its key groups, and a split adds the
+// joining launch of 4 us and its partial results, written and read at 4 TB/s.
+// Constants from timings of 1 to 1200 workgroups and 1 to 150 rounds.
 Plan plan(int B, int Hk, int R, int S, int D, int cus) {
+  static const struct {
+    int dim, rows, groups, fit;
+    double ends, alone, more;
+  } kinds[] = {{64, 32, 2, 2, 3.2, 0.37, 0.2},
+               {64, 64, 1, 3, 3.2, 0.25, 0.28},
+               {128, 32, 2, 1, 5.0, 0.0, 1.1},
+               {128, 64, 1, 2, 5.0, 1.1, 0.12}};
   const int64_t heads = (int64_t)B * Hk;
   const int steps = (S + kStep - 1) / kStep;
   Plan best{};
   double best_us = 0;
-  for (int rows = kBlock; rows <= 2 * kBlock; rows += kBlock) {
-    const int groups = rows > kBlock ? 1 : D == 64 ? 4 : 2;
-    const int blocks = (R + rows - 1) / rows;
-    const double fixed = rows > kBlock && D == 128 ? 0.4 : 0.3;
-    const double work = rows == kBlock ? 0.5 : D == 64 ? 0.3 : 0.6;
-    for (int s = 1; s <= kMaxGridSplits && (s == 1 || s * groups <= steps); ++s) {
-      const double load = (double)heads * blocks * s / cus;
-      if (s > 1 && load > 1.5) break;
-      double us = 8 + ((steps + groups * s - 1) / (groups * s)) * (fixed + work * (load > 1 ? load : 1));
+  for (const auto& k : kinds) {
+    if (k.dim != D) continue;
+    const int blocks = (R + k.rows - 1) / k.rows;
+    for (int s = 1; s <= kMaxGridSplits && (s == 1 || s * k.groups <= steps); ++s) {
+      const int64_t load = (heads * blocks * s + cus - 1) / cus;   // workgroups of the busiest CU
+      if (s > 1 && load > 2 * k.fit) break;
+      const double turns = (double)((load + k.fit - 1) / k.fit), running = (double)(load < k.fit ? load : k.fit);
+      const int rounds = (steps + k.groups * s - 1) / (k.groups * s);
+      double us = 3 + turns * (k.ends + rounds * (k.alone + k.more * running));
       if (s > 1) us += 4 + (double)heads * R * s * (4 * D) * 8 / 4e6;
-      if (best.rows == 0 || us < best_us) best = Plan{rows, blocks, s}, best_us = us;
+      if (best.rows == 0 || us < best_us) best = Plan{k.rows, blocks, s}, best_us = us;
     }
   }
   return best;
@@ -680,7 +708,7 @@ void launch(const DiffParams& p, int D, int rows, hipStream_t stream) {
   const dim3 grid((unsigned)(8 * p.parts_per_xcd * ((p.blocks * p.splits + p.parts - 1) / p.parts)));
   if (D == 64) {
     if (rows == kBlock) {
-      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 1, 4, 2>), grid, dim3(512), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 1, 2, 2>), grid, dim3(256), 0, stream, p);
     } else {
       hipLaunchKernelGGL((diff_attn_kernel<E, 64, 2, 1, 3>), grid, dim3(256), 0, stream, p);
     }
@@ -692,12 +720,11 @@ void launch(const DiffParams& p, int D, int rows, hipStream_t stream) {
     }
   }
   if (p.splits > 1) {
-    const int64_t all = (int64_t)p.B * p.Hk * p.R;
-    const dim3 join((unsigned)((all + kJoinRows - 1) / kJoinRows));
+    const dim3 join((unsigned)((int64_t)p.B * p.Hk * p.R));
     if (D == 64) {
-      hipLaunchKernelGGL((diff_attn_join_kernel<E, 64>), join, dim3(64 * kJoinRows), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_join_kernel<E, 64>), join, dim3(64 * kJoinWaves), 0, stream, p);
     } else {
-      hipLaunchKernelGGL((diff_attn_join_kernel<E, 128>), join, dim3(64 * kJoinRows), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_join_kernel<E, 128>), join, dim3(64 * kJoinWaves), 0, stream, p);
     }
   }
 }
@@ -755,7 +782,8 @@ SIDON_API int sidon_diff_attention(const void* q, const void* k, const void* v, 
   while (parts > 1 && heads * (parts / 2) % 8 == 0 &&
          (heads * S * D * 8 > (int64_t)3 << 20 || parts > c.blocks * c.splits))
     parts /= 2;
-  if (heads * parts * (((int64_t)c.blocks * c.splits + parts - 1) / parts) > INT32_MAX / 256)
+  if (heads * parts * (((int64_t)c.blocks * c.splits + parts - 1) / parts) > INT32_MAX / 256 ||
+      (c.splits > 1 && heads * R > INT32_MAX / 256))
     return fail(SIDON_E_SHAPE, "too many rows for one launch");
   DiffParams p{};
   p.q = q;
