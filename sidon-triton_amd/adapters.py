@@ -67,25 +67,28 @@ def stack_adapters(pairs):
 
 def _operands(x, w, a, b, scale, ids):
     device = x.device
+    _check_device_tensor("x", x, device)
     for name, t in (("x", x), ("w", w), ("a", a), ("b", b)):
-        _check_device_tensor(name, t, device)
+        if t.device != device:
+            _check_device_tensor(name, t, device)
         if t.dtype not in _TYPES or t.dtype != x.dtype:
             raise TypeError(f"{name} must be float16 or bfloat16, of x's type (got {t.dtype})")
-    for name, t in (("x", x), ("w", w)):
-        if t.dim() != 2 or t.stride(1) != 1:
-            raise ValueError(f"{name} must be a [rows, K] tensor with K contiguous")
+    if x.dim() != 2 or x.stride(1) != 1 or w.dim() != 2 or w.stride(1) != 1:
+        raise ValueError("x and w must be [rows, K] tensors with K contiguous")
     rows, k = x.shape
     n = w.shape[0]
     if w.shape[1] != k:
         raise ValueError(f"x has {k} columns, w {w.shape[1]}")
     if a.dim() != 3 or a.shape[2] != k or not a.is_contiguous():
         raise ValueError(f"a must be a contiguous [E, R, {k}] tensor")
-    if tuple(b.shape) != (a.shape[0], n, a.shape[1]) or not b.is_contiguous():
+    if b.shape != (a.shape[0], n, a.shape[1]) or not b.is_contiguous():
         raise ValueError(f"b must be a contiguous [{a.shape[0]}, {n}, {a.shape[1]}] tensor")
-    _check_device_tensor("scale", scale, device)
-    if scale.dtype != torch.float32 or tuple(scale.shape) != (a.shape[0],) or not scale.is_contiguous():
+    if scale.device != device:
+        _check_device_tensor("scale", scale, device)
+    if scale.dtype != torch.float32 or scale.shape != (a.shape[0],) or not scale.is_contiguous():
         raise ValueError(f"scale must be a contiguous float32 [{a.shape[0]}] tensor")
-    _check_device_tensor("ids", ids, device)
+    if ids.device != device:
+        _check_device_tensor("ids", ids, device)
     if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous() or ids.numel() < 1:
         raise ValueError("ids must be a contiguous int32 [items] tensor")
     if rows < 1 or rows % ids.numel():
@@ -118,18 +121,19 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, 
     rows, n, k = _operands(x, w, a, b, scale, ids)
     device = x.device
     if bias is not None:
-        _check_device_tensor("bias", bias, device)
-        if bias.dtype != x.dtype or tuple(bias.shape) != (n,) or not bias.is_contiguous():
+        if bias.device != device:
+            _check_device_tensor("bias", bias, device)
+        if bias.dtype != x.dtype or bias.shape != (n,) or not bias.is_contiguous():
             raise ValueError(f"bias must be a contiguous {x.dtype} [{n}] tensor")
     if act not in (None, "silu"):
         raise ValueError(f"act must be None or 'silu' (got {act!r})")
-    if not plain(*(t for t in (x, w, bias, a, b, scale) if t is not None)):
+    if not (plain(x, w, a, b, scale) if bias is None else plain(x, w, a, b, scale, bias)):
         raise ValueError("adapter_linear has no backward: call it under torch.no_grad()")
     if out is None:
         out = torch.empty(rows, n, device=device, dtype=x.dtype)
     else:
         _check_device_tensor("out", out, device)
-        if out.dtype != x.dtype or tuple(out.shape) != (rows, n) or out.stride(1) != 1:
+        if out.dtype != x.dtype or out.shape != (rows, n) or out.stride(1) != 1:
             raise ValueError(f"out must be a {x.dtype} [{rows}, {n}] tensor with rows contiguous")
     workspace = _workspace(workspace, workspace_bytes(rows, a.shape[1], False, x.dtype), device)
     lib = _lib.load()
@@ -139,7 +143,8 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, 
             a.data_ptr(), b.data_ptr(), scale.data_ptr(), ids.data_ptr(), out.data_ptr(), _row_stride(out),
             workspace.data_ptr(), workspace.numel(), rows, n, k, a.shape[1], a.shape[0], ids.numel(),
             _lib.ACTIVATIONS[act], _lib.DTYPES[x.dtype], _stream_handle(device))
-    _lib.check("sidon_adapter_linear", rc)
+    if rc:
+        _lib.check("sidon_adapter_linear", rc)
     return out
 
 
@@ -154,7 +159,7 @@ def adapter_residual(y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, a: torch
     out = y if out is None else out
     for name, t in (("y", y), ("out", out)):
         _check_device_tensor(name, t, device)
-        if t.dtype != torch.float32 or tuple(t.shape) != (rows, n) or t.stride(1) != 1:
+        if t.dtype != torch.float32 or t.shape != (rows, n) or t.stride(1) != 1:
             raise ValueError(f"{name} must be a float32 [{rows}, {n}] tensor with rows contiguous")
     if not plain(y, x, w, a, b, scale):
         raise ValueError("adapter_residual has no backward: call it under torch.no_grad()")
@@ -166,5 +171,6 @@ def adapter_residual(y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, a: torch
             ids.data_ptr(), y.data_ptr(), _row_stride(y), out.data_ptr(), _row_stride(out), workspace.data_ptr(),
             workspace.numel(), rows, n, k, a.shape[1], a.shape[0], ids.numel(), _lib.DTYPES[x.dtype],
             _stream_handle(device))
-    _lib.check("sidon_adapter_residual", rc)
+    if rc:
+        _lib.check("sidon_adapter_residual", rc)
     return out

@@ -148,12 +148,14 @@ def group_norm_act(x: torch.Tensor, batch: int, groups: int, w: torch.Tensor, b:
     if act not in _lib.ACTIVATIONS:
         raise ValueError(f"act must be one of {list(_lib.ACTIVATIONS)} (got {act!r})")
     for name, t in (("w", w), ("b", b)):
-        _check_device_tensor(name, t, device)
-        if t.dtype != torch.float32 or tuple(t.shape) != (c,) or not t.is_contiguous():
+        if t.device != device:
+            _check_device_tensor(name, t, device)
+        if t.dtype != torch.float32 or t.shape != (c,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous float32 [{c}] tensor")
     if lens is not None:
-        _check_device_tensor("lens", lens, device)
-        if lens.dtype != torch.int32 or tuple(lens.shape) != (batch,) or not lens.is_contiguous():
+        if lens.device != device:
+            _check_device_tensor("lens", lens, device)
+        if lens.dtype != torch.int32 or lens.shape != (batch,) or not lens.is_contiguous():
             raise ValueError("lens must be a contiguous int32 tensor of shape [B]")
     if not plain(x, w, b):
         raise ValueError("group_norm_act has no backward: call it under torch.no_grad()")
@@ -161,22 +163,25 @@ def group_norm_act(x: torch.Tensor, batch: int, groups: int, w: torch.Tensor, b:
         out = torch.empty(rows, c, device=device, dtype=x.dtype)
     else:
         _check_device_tensor("out", out, device)
-        if out.dtype != x.dtype or tuple(out.shape) != (rows, c) or out.stride(1) != 1:
+        if out.dtype != x.dtype or out.shape != (rows, c) or out.stride(1) != 1:
             raise ValueError(f"out must be a {x.dtype} [{rows}, {c}] tensor with channels contiguous")
     lib = _lib.load()
-    need = group_norm_workspace(batch, rows // batch, c, groups, x.dtype)
+    dtype = _lib.DTYPES[x.dtype]
     if workspace is None:
+        need = lib.sidon_group_norm_workspace_bytes(batch, rows // batch, c, groups, dtype)
         workspace = torch.empty(max(need, 8), device=device, dtype=torch.uint8)
     else:
         _check_device_tensor("workspace", workspace, device)
+        need = lib.sidon_group_norm_workspace_bytes(batch, rows // batch, c, groups, dtype)
         if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
             raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
     with _on_device(device):
         rc = lib.sidon_group_norm_act(x.data_ptr(), _row_stride(x), None if lens is None else lens.data_ptr(),
-                                      w.data_ptr(), b.data_ptr(), ctypes.c_float(float(eps)), out.data_ptr(),
+                                      w.data_ptr(), b.data_ptr(), eps, out.data_ptr(),
                                       _row_stride(out), workspace.data_ptr(), workspace.numel(), batch, rows // batch,
-                                      c, groups, _lib.DTYPES[x.dtype], _lib.ACTIVATIONS[act], _stream_handle(device))
-    _lib.check("sidon_group_norm_act", rc)
+                                      c, groups, dtype, _lib.ACTIVATIONS[act], _stream_handle(device))
+    if rc:
+        _lib.check("sidon_group_norm_act", rc)
     return out
 
 
@@ -273,10 +278,13 @@ def plain(*tensors: torch.Tensor) -> bool:
     """Whether a kernel may stand in for a torch call with ``out=`` on these:
     no subclass of its own behaviour, and nothing that autograd, in reverse or
     forward mode, would follow (torch refuses ``out=`` there)."""
-    if any(type(t) not in (torch.Tensor, torch.nn.Parameter) for t in tensors):
-        return False
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        return False
+    for t in tensors:
+        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return False
     return (getattr(forward_ad, "_current_level", 0) < 0
             or all(forward_ad.unpack_dual(t).tangent is None for t in tensors))
 

@@ -666,7 +666,7 @@ struct Plan {
 // workgroup's rounds are its steps over its key groups, and a split adds the
 // joining launch of 4 us and its partial results, written and read at 4 TB/s.
 // Constants from timings of 1 to 1200 workgroups and 1 to 150 rounds.
-Plan plan(int B, int Hk, int R, int S, int D, int cus) {
+Plan search(int B, int Hk, int R, int S, int D, int cus) {
   static const struct {
     int dim, rows, groups, fit;
     double ends, alone, more;
@@ -692,6 +692,22 @@ Plan plan(int B, int Hk, int R, int S, int D, int cus) {
     }
   }
   return best;
+}
+
+// The search (a few microseconds) once per shape: one table per thread, the
+// newest shape kept.
+Plan plan(int B, int Hk, int R, int S, int D, int cus) {
+  struct Entry {
+    int B, Hk, R, S, D, cus;
+    Plan plan;
+  };
+  constexpr unsigned kEntries = 16;
+  static thread_local Entry table[kEntries] = {};
+  const unsigned hash = ((unsigned)S * 2654435761u ^ (unsigned)R * 40503u ^ (unsigned)B * 97u) >> 9;
+  Entry& e = table[hash % kEntries];
+  if (e.B != B || e.Hk != Hk || e.R != R || e.S != S || e.D != D || e.cus != cus)
+    e = Entry{B, Hk, R, S, D, cus, search(B, Hk, R, S, D, cus)};
+  return e.plan;
 }
 
 bool shape_ok(int B, int H, int Hk, int L, int S, int D) {

@@ -14,6 +14,7 @@ reference.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -30,11 +31,19 @@ def workspace_bytes(batch: int, heads: int, kv_heads: int, length: int, keys: in
         return int(_lib.load().sidon_diff_attention_workspace_bytes(batch, heads, kv_heads, length, keys, dim))
 
 
+@functools.lru_cache(maxsize=256)
+def _int64s(values: tuple) -> ctypes.Array:
+    """The C array of these numbers (only ever read)."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
 def _strides(t: torch.Tensor) -> ctypes.Array:
     """Strides in front of the last dimension; that of a dimension of size 1
     means nothing and is given as 0."""
-    st = [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
-    return (ctypes.c_int64 * len(st))(*st)
+    st = t.stride()[:-1]
+    if 1 in t.shape[:-1]:
+        st = tuple([0 if n == 1 else s for n, s in zip(t.shape, st)])
+    return _int64s(st)
 
 
 def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, lam_init: float,
@@ -63,31 +72,36 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
         raise ValueError(f"q must be [B, H, 2, L, {HEAD_DIMS}] (got {tuple(q.shape)})")
     if min(q.shape) < 1 or min(k.shape) < 1:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must not be empty")
-    if tuple(k.shape) != (batch, kv_heads, 2, keys, dim) or tuple(v.shape) != (batch, kv_heads, keys, 2 * dim):
+    if k.shape != (batch, kv_heads, 2, keys, dim) or v.shape != (batch, kv_heads, keys, 2 * dim):
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
     if heads % kv_heads:
         raise ValueError(f"{heads} heads do not share {kv_heads} key heads")
     device = q.device
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"q must be float16 or bfloat16 (got {q.dtype})")
+    _check_device_tensor("q", q, device)
     for name, t in (("q", q), ("k", k), ("v", v)):
-        _check_device_tensor(name, t, device)
+        if t.device != device:
+            _check_device_tensor(name, t, device)
         if t.dtype != q.dtype:
             raise TypeError(f"{name} is {t.dtype}, q is {q.dtype}")
         if t.stride(-1) != 1:
             raise ValueError(f"{name} must have a contiguous last dimension")
-    _check_device_tensor("lam", lam, device)
-    if lam.dtype != torch.float32 or not lam.is_contiguous() or tuple(lam.shape) not in ((4, dim), (heads, 4, dim)):
+    if lam.device != device:
+        _check_device_tensor("lam", lam, device)
+    if lam.dtype != torch.float32 or not lam.is_contiguous() or lam.shape not in ((4, dim), (heads, 4, dim)):
         raise ValueError(f"lam must be a contiguous float32 [4, {dim}] or [{heads}, 4, {dim}] tensor")
     if lens is not None:
-        _check_device_tensor("lens", lens, device)
-        if lens.dtype != torch.int32 or tuple(lens.shape) != (batch,) or not lens.is_contiguous():
+        if lens.device != device:
+            _check_device_tensor("lens", lens, device)
+        if lens.dtype != torch.int32 or lens.shape != (batch,) or not lens.is_contiguous():
             raise ValueError("lens must be a contiguous int32 tensor of shape [B]")
     if norm_w is not None:
-        _check_device_tensor("norm_w", norm_w, device)
-        if norm_w.dtype != torch.float32 or tuple(norm_w.shape) != (2 * dim,) or not norm_w.is_contiguous():
+        if norm_w.device != device:
+            _check_device_tensor("norm_w", norm_w, device)
+        if norm_w.dtype != torch.float32 or norm_w.shape != (2 * dim,) or not norm_w.is_contiguous():
             raise ValueError(f"norm_w must be a contiguous float32 [{2 * dim}] tensor")
-    if not plain(*(t for t in (q, k, v, lam, norm_w) if t is not None)):
+    if not (plain(q, k, v, lam) if norm_w is None else plain(q, k, v, lam, norm_w)):
         raise ValueError("diff_attention has no backward: call it under torch.no_grad()")
     shape = (batch, heads, length, 2 * dim)
     if out is None:
@@ -96,21 +110,22 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
         _check_device_tensor("out", out, device)
         if out.dtype != q.dtype or tuple(out.shape) != shape or out.stride(-1) != 1:
             raise ValueError(f"out must be a {q.dtype} {shape} tensor with a contiguous last dimension")
-    need = workspace_bytes(batch, heads, kv_heads, length, keys, dim, device)
-    if workspace is None:
-        workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
-    else:
-        _check_device_tensor("workspace", workspace, device)
-        if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
-            raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
     lib = _lib.load()
     with _on_device(device):
+        need = lib.sidon_diff_attention_workspace_bytes(batch, heads, kv_heads, length, keys, dim)
+        if workspace is None:
+            workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
+        else:
+            _check_device_tensor("workspace", workspace, device)
+            if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+                raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
         rc = lib.sidon_diff_attention(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), 1 if lam.dim() == 2 else heads,
-            ctypes.c_float(float(lam_init)), None if lens is None else lens.data_ptr(),
-            None if norm_w is None else norm_w.data_ptr(), ctypes.c_float(float(eps)), out.data_ptr(),
-            None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(),
-            batch, heads, kv_heads, length, keys, dim, int(bool(causal)), _lib.DTYPES[q.dtype],
-            _strides(q), _strides(k), _strides(v), _strides(out), _stream_handle(device))
-    _lib.check("sidon_diff_attention", rc)
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), 1 if lam.dim() == 2 else heads, lam_init,
+            None if lens is None else lens.data_ptr(), None if norm_w is None else norm_w.data_ptr(), eps,
+            out.data_ptr(), None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel(), batch, heads, kv_heads, length, keys, dim,
+            1 if causal else 0, _lib.DTYPES[q.dtype], _strides(q), _strides(k), _strides(v), _strides(out),
+            _stream_handle(device))
+    if rc:
+        _lib.check("sidon_diff_attention", rc)
     return out
