@@ -24,7 +24,6 @@ using namespace sidon_gemm;
 using sidon::fail;
 
 constexpr int kMaxRank = 128;
-constexpr int kShrinkWaves = 8;     // K ranges of a row block
 constexpr int kShrinkRows = 16;     // rows of a matrix product
 
 struct ShrinkParams {
@@ -38,66 +37,97 @@ struct ShrinkParams {
   int rows;                  // per workgroup, <= 16
 };
 
-// RB blocks of 16 ranks.  A workgroup owns `rows` rows; its wavefronts take
-// every kShrinkWaves-th 32 columns of K and are summed through LDS in order.
-// Products are 16 ranks x 16 rows: a lane's accumulators are 4 ranks of one
-// row, so of several adapters among the rows each costs a pass over K whose
-// other rows' results are dropped.
-template <typename E, int RB>
-__global__ void __launch_bounds__(64 * kShrinkWaves) shrink_kernel(const ShrinkParams p) {
+// RB blocks of 16 ranks, W wavefronts.  A workgroup owns `rows` rows; its
+// wavefronts take 64 columns of K in turn, copied global -> LDS as 128-byte rows
+// into two slots of their own (16-byte chunk c of row r at c ^ ((r >> 1) & 7)), and
+// are summed through LDS in order.  Products are 16 ranks x 16 rows: a lane's
+// accumulators are 4 ranks of one row, so of several adapters among the rows each
+// costs a pass over K whose other rows' results are dropped.
+// (Operands read from memory by the lanes that multiply them cost a cache access
+// per lane, its neighbours holding other rows: 17.2 us instead of SHRINK_NOW at 4800 rows, K
+// 1024, rank 64.)
+template <typename E, int RB, int W>
+__global__ void __launch_bounds__(64 * W) shrink_kernel(const ShrinkParams p) {
   typedef typename Elem<E>::e8 e8;
-  __shared__ f4 part[kShrinkWaves][RB][64];
+  constexpr int kSlot = (1 + RB) * 2048;
+  constexpr int kPer = 2 * (1 + RB);            // copies per slice
+  static_assert(2 * W * kSlot <= 160 * 1024 && W * RB * 1024 <= 2 * W * kSlot, "LDS");
+  __shared__ __attribute__((aligned(16))) char smem[2 * W * kSlot];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, lg = lane >> 4;
   const int row0 = blockIdx.x * p.rows;
-  const int row = min(row0 + min(ln, p.rows - 1), p.M - 1);
-  int id = p.ids[row / p.rows_per_id];
+  const auto row_of = [&](int i) SIDON_INLINE { return min(row0 + min(i, p.rows - 1), p.M - 1); };
+  int id = p.ids[row_of(ln) / p.rows_per_id];
   if (id < 0 || id >= p.adapters) id = -1;
-  const E* x = static_cast<const E*>(p.x) + (int64_t)row * p.ldx + 8 * lg;
+
+  // Copy i of a slice: rows 8 i + lane / 8 of x's 16, then of the adapter's 16 RB.
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + w * 2 * kSlot;
+  const auto chunk = [&](int r) SIDON_INLINE { return 16u * ((lane & 7) ^ ((r >> 1) & 7)); };
+  uint32_t xoff[2], aoff[2 * RB];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 8 * i + (lane >> 3);
+    xoff[i] = (uint32_t)(row_of(r) - row0) * (uint32_t)(2 * p.ldx) + chunk(r);
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * RB; ++i) {
+    const int r = 8 * i + (lane >> 3);
+    aoff[i] = (uint32_t)min(r, p.R - 1) * (uint32_t)(2 * p.K) + chunk(r);
+  }
+  const char* const xbase = static_cast<const char*>(p.x) + 2 * ((int64_t)row0 * p.ldx);
+  const int slices = p.K / 64, mine = slices > w ? (slices - w + W - 1) / W : 0;
+  const char* const ops = smem + w * 2 * kSlot + ln * 128;
+  const int swz = (ln >> 1) & 7;
+
   // (the same for every wavefront: they hold the same rows)
   uint64_t todo = __builtin_amdgcn_ballot_w64(id >= 0);
   while (todo != 0) {
     const int e = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
     todo &= ~__builtin_amdgcn_ballot_w64(id == e);
-    const E* a[RB];
+    const float scale = p.scale[e];
+    const char* const abase = static_cast<const char*>(p.a) + 2 * ((int64_t)e * p.R * p.K);
+    const auto copy = [&](int t) SIDON_INLINE {
+      const uint32_t at = lds + (t & 1) * kSlot;
+      const int64_t col = 128 * (int64_t)(w + t * W);
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-      a[b] = static_cast<const E*>(p.a) + ((int64_t)e * p.R + min(16 * b + ln, p.R - 1)) * p.K + 8 * lg;
+      for (int i = 0; i < 2; ++i) copy_1k(at + i * 1024, xbase + col, xoff[i]);
+#pragma unroll
+      for (int i = 0; i < 2 * RB; ++i) copy_1k(at + (2 + i) * 1024, abase + col, aoff[i]);
+    };
     f4 acc[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) acc[b] = f4{};
-    constexpr int kUnroll = RB <= 2 ? 4 : 2;
-    for (int k0 = 32 * w; k0 < p.K; k0 += 32 * kShrinkWaves * kUnroll) {
-      e8 xv[kUnroll], av[kUnroll][RB];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int k = k0 + 32 * kShrinkWaves * u;
-        xv[u] = e8{};
-        if (k < p.K) xv[u] = *reinterpret_cast<const e8*>(x + k);
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          av[u][b] = e8{};
-          if (k < p.K) av[u][b] = *reinterpret_cast<const e8*>(a[b] + k);
-        }
+    if (mine > 0) copy(0);
+    for (int t = 0; t < mine; ++t) {
+      if (t + 1 < mine) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot's reads have retired
+        copy(t + 1);
+        wait_vmcnt<kPer>();
+      } else {
+        wait_vmcnt<0>();
       }
+      const char* at = ops + (t & 1) * kSlot;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
+      for (int s = 0; s < 2; ++s) {
+        const int c = ((4 * s + lg) ^ swz) << 4;
+        const e8 xv = *reinterpret_cast<const e8*>(at + c);
 #pragma unroll
-        for (int b = 0; b < RB; ++b) acc[b] = mma(av[u][b], xv[u], acc[b]);
+        for (int b = 0; b < RB; ++b) acc[b] = mma(*reinterpret_cast<const e8*>(at + (1 + b) * 2048 + c), xv, acc[b]);
+      }
     }
+    lds_barrier();   // everyone is done with the slots, which the sums reuse
+    f4* const part = reinterpret_cast<f4*>(smem);
 #pragma unroll
-    for (int b = 0; b < RB; ++b) part[w][b][lane] = acc[b];
-    __syncthreads();
-    const float scale = p.scale[e];
-    for (int t = threadIdx.x; t < RB * 64; t += 64 * kShrinkWaves) {
-      const int b = t >> 6, l = t & 63;
-      const int n = l & 15, r = 16 * b + 4 * (l >> 4);
-      f4 s = part[0][b][l];
+    for (int b = 0; b < RB; ++b) part[(w * RB + b) * 64 + lane] = acc[b];
+    lds_barrier();
+    // A lane's sums are of the row it holds.
+    for (int b = w; b < RB; b += W) {
+      const int r = 16 * b + 4 * lg, m = row0 + ln;
+      f4 s = part[b * 64 + lane];
 #pragma unroll
-      for (int i = 1; i < kShrinkWaves; ++i) s += part[i][b][l];
-      const int m = row0 + n;
-      if (n < p.rows && m < p.M && r < p.R && p.ids[m / p.rows_per_id] == e) {
+      for (int i = 1; i < W; ++i) s += part[(i * RB + b) * 64 + lane];
+      if (ln < p.rows && m < p.M && r < p.R && id == e) {
         E* dst = static_cast<E*>(p.low) + (int64_t)m * p.R + r;
         for (int plane = 0; plane < p.planes; ++plane) {
           typename Elem<E>::e4 v;
@@ -111,7 +141,7 @@ __global__ void __launch_bounds__(64 * kShrinkWaves) shrink_kernel(const ShrinkP
         }
       }
     }
-    if (todo != 0) __syncthreads();
+    if (todo != 0) lds_barrier();
   }
 }
 
@@ -138,7 +168,7 @@ struct ExpandKernel {
 const ExpandKernel kExpand[] = {
     SIDON_BOTH(32, 64, 2, 2, 16, 6),   SIDON_BOTH(64, 64, 2, 2, 16, 4),   SIDON_BOTH(64, 128, 2, 4, 16, 4),
     SIDON_BOTH(128, 128, 2, 4, 16, 4), SIDON_BOTH(192, 128, 2, 4, 16, 3), SIDON_HALF(128, 256, 2, 4, 16, 3),
-    SIDON_HALF(256, 256, 2, 4, 16, 2),
+    SIDON_HALF(160, 256, 1, 4, 32, 3),
 };
 
 struct Call {
@@ -176,8 +206,9 @@ int check_and_launch(Call& c, sidon_stream_t stream) {
       (c.residual && (p.ldadd < p.N || p.ldadd % step != 0)))
     return fail(SIDON_E_STRIDE, "row strides ldx=%d ldw=%d (multiples of 8, >= K) ldy=%d ldadd=%d (multiples of %d, >= N)",
                 p.ldx, p.ldw, p.ldy, p.ldadd, step);
-  if ((int64_t)p.M * p.ldx * 2 >= (int64_t(1) << 32) || (int64_t)p.N * p.ldw * 2 >= (int64_t(1) << 32))
-    return fail(SIDON_E_SHAPE, "x and w must each span less than 4 GiB");
+  if ((int64_t)p.M * p.ldx * 2 >= (int64_t(1) << 32) || (int64_t)p.N * p.ldw * 2 >= (int64_t(1) << 32) ||
+      (int64_t)p.rank * p.K * 2 >= (int64_t(1) << 32))
+    return fail(SIDON_E_SHAPE, "x, w and an adapter's a must each span less than 4 GiB");
   if (!sidon::aligned16(p.x) || !sidon::aligned16(p.w) || !sidon::aligned16(c.a) || !sidon::aligned16(p.up) ||
       !sidon::aligned16(p.y) || !sidon::aligned16(c.ws) || (c.residual && !sidon::aligned16(p.add)) ||
       (reinterpret_cast<uintptr_t>(p.bias) & 7u) != 0 || (reinterpret_cast<uintptr_t>(p.ids) & 3u) != 0 ||
@@ -218,17 +249,17 @@ int check_and_launch(Call& c, sidon_stream_t stream) {
   s.rows = (p.M + cus - 1) / cus;
   if (s.rows > kShrinkRows) s.rows = kShrinkRows;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)((p.M + s.rows - 1) / s.rows)), block(64 * kShrinkWaves);
+  const dim3 grid((unsigned)((p.M + s.rows - 1) / s.rows));
   const auto shrink = [&](auto zero) {
     typedef decltype(zero) E;
     if (s.R <= 16) {
-      hipLaunchKernelGGL((shrink_kernel<E, 1>), grid, block, 0, st, s);
+      hipLaunchKernelGGL((shrink_kernel<E, 1, 8>), grid, dim3(512), 0, st, s);
     } else if (s.R <= 32) {
-      hipLaunchKernelGGL((shrink_kernel<E, 2>), grid, block, 0, st, s);
+      hipLaunchKernelGGL((shrink_kernel<E, 2, 8>), grid, dim3(512), 0, st, s);
     } else if (s.R <= 64) {
-      hipLaunchKernelGGL((shrink_kernel<E, 4>), grid, block, 0, st, s);
+      hipLaunchKernelGGL((shrink_kernel<E, 4, 4>), grid, dim3(256), 0, st, s);
     } else {
-      hipLaunchKernelGGL((shrink_kernel<E, 8>), grid, block, 0, st, s);
+      hipLaunchKernelGGL((shrink_kernel<E, 8, 4>), grid, dim3(256), 0, st, s);
     }
   };
   if (c.dtype == SIDON_FP16) {

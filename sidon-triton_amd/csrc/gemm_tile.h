@@ -149,8 +149,10 @@ __device__ __forceinline__ E to_elem(float y) {
   return (E)y;
 }
 
-// Up to this many adapters among a block's rows, a matrix product each.
-constexpr int kFewKinds = 4;
+// A tile of up to this many items takes its low-rank term's operands through LDS,
+// one adapter at a time; of more, straight from memory: up to kFewKinds adapters
+// among a block's rows a matrix product each, past them every lane its own row.
+constexpr int kFewItems = 4, kFewKinds = 4;
 
 template <int BM, int BN, int WM, int WN, int MF, int ST, int kMode>
 struct Tile {
@@ -249,6 +251,14 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
   const int swz = (ln >> 1) & 7;  // rows MF b + ln share the swizzle of row ln
   const char* xrow = smem + (TM * wm + ln) * 128;
   const char* wrow = smem + (BM + TN * wn + ln) * 128;
+
+  // The adapters of this lane's rows: read here, a memory latency before their use.
+  constexpr bool kLow = IsLow<Params>::value;
+  int id[kLow ? IM : 1];
+  if constexpr (kLow) {
+#pragma unroll
+    for (int i = 0; i < IM; ++i) id[i] = p.ids[min(m0 + TM * wm + MF * i + ln, p.M - 1) / p.rows_per_id];
+  }
 
   acc_t acc[IM][IN];
 #pragma unroll
@@ -359,52 +369,119 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
     for (int t = 0; t < kOld; ++t)
       old[t] = *reinterpret_cast<const f4*>(yb + min(m0 + TM * wm + kFRows * t + lane / kFLanes, p.M - 1) * ld);
   }
-  body(kt, No{}, No{}, No{});
-  if constexpr (IsLow<Params>::value) {
-    // The low-rank term.  A lane's row of block i is MF i + ln, as its
-    // accumulators' row, so rows of different adapters in a block cost one
-    // product per adapter and a selection; up's rows come straight from global
-    // memory (each is used once by a workgroup).
-    const int col0 = tn * BN + TN * wn;
-    const E* const lowb = static_cast<const E*>(p.low);
-    const E* const upb = static_cast<const E*>(p.up);
-    constexpr int kW = 8 * NG;   // ranks per product
-    int id[IM];
-    int e0 = -1;
-    bool same = true;
-#pragma unroll
-    for (int i = 0; i < IM; ++i) {
-      const int e = p.ids[min(m0 + TM * wm + MF * i + ln, p.M - 1) / p.rows_per_id];
-      id[i] = e >= 0 && e < p.adapters ? e : -1;
-      if (i == 0) e0 = __builtin_amdgcn_readfirstlane(id[0]);
-      same = same && id[i] == e0;
+  // The low-rank term of a tile with few items: the tile's rows of `low`, and of
+  // `up` for one adapter after another, each one contiguous block, are copied into
+  // a free ring slot, the first under the last slice.  (Read from memory by the lanes
+  // that multiply them, whose neighbours hold other rows, they cost a cache access
+  // each: 128 x 256 tiles of rank 64, 4 us a tile.)
+  constexpr int kW = 8 * NG;   // ranks per product
+  const int spare = (slot == 0 ? ST - 1 : slot - 1) * T::kStage;   // (slot: of the last slice)
+  int item = 0, items_end = 0, low_bytes = 0;   // low_bytes: of a plane
+  bool staged = false;
+  const auto adapter_of = [&](int i) SIDON_INLINE {
+    if constexpr (kLow) {
+      const int e = p.ids[i];
+      return e >= 0 && e < p.adapters ? e : -1;
     }
-    const auto low_at = [&](int i, int plane, int r) SIDON_INLINE {
-      const E* at = lowb + plane * p.plane + (int64_t)min(m0 + TM * wm + MF * i + ln, p.M - 1) * p.rank + r;
-      return r < p.rank ? *reinterpret_cast<const h8*>(at) : h8{};
-    };
-    const auto up_at = [&](int e, int col, int r) SIDON_INLINE {
-      const E* at = upb + ((int64_t)e * p.N + col0 + col) * p.rank + r;
-      return r < p.rank ? *reinterpret_cast<const h8*>(at) : h8{};
-    };
-    if (__builtin_amdgcn_ballot_w64(!same) == 0) {
-      if (e0 >= 0) {
-        for (int r0 = 0; r0 < p.rank; r0 += kW) {
-          const int r = r0 + 8 * lg;
-          h8 u[IN];
+    return -1;
+  };
+  // The first item from i on whose adapter no earlier item of the tile has.
+  const auto next_item = [&](int first, int i) SIDON_INLINE {
+    for (; i < items_end; ++i) {
+      const int e = adapter_of(i);
+      bool fresh = e >= 0;
+      for (int k = first; k < i; ++k) fresh = fresh && adapter_of(k) != e;
+      if (fresh) break;
+    }
+    return i;
+  };
+  // Rows of `rank` values from `src`, `count` of them, as 1 KB copies; what lies past
+  // them is read again from their end.
+  const auto stage = [&](int at, const char* src, int bytes, int count) SIDON_INLINE {
+    if constexpr (kLow) {
+      const int most = count * p.rank * 2 - 16;
+      for (int i = w; i < bytes >> 10; i += NW)
+        copy_1k(lds0 + (uint32_t)(at + i * 1024), src, (uint32_t)min(1024 * i + 16 * lane, most));
+    }
+  };
+  const auto stage_up = [&](int e) SIDON_INLINE {
+    if constexpr (kLow)
+      stage(spare + p.planes * low_bytes, static_cast<const char*>(p.up) + 2 * ((int64_t)e * p.N + tn * BN) * p.rank,
+            (BN * p.rank * 2 + 1023) & ~1023, BN);
+  };
+  int first_item = 0;
+  if constexpr (kLow) {
+    first_item = m0 / p.rows_per_id;
+    items_end = min(m0 + BM - 1, p.M - 1) / p.rows_per_id + 1;
+    low_bytes = (BM * p.rank * 2 + 1023) & ~1023;
+    staged = items_end - first_item <= kFewItems &&
+             p.planes * low_bytes + ((BN * p.rank * 2 + 1023) & ~1023) <= T::kStage;
+    if (staged) {
+      item = next_item(first_item, first_item);
+      if (item < items_end) {
+        for (int plane = 0; plane < p.planes; ++plane)
+          stage(spare + plane * low_bytes, static_cast<const char*>(p.low) + 2 * (plane * p.plane + (int64_t)m0 * p.rank),
+                low_bytes, min(BM, p.M - m0));
+        stage_up(adapter_of(item));
+      }
+    }
+  }
+  body(kt, No{}, No{}, No{});
+  if constexpr (kLow) {
+    // A lane's row of block i is MF i + ln, as its accumulators' row.  A product is
+    // taken for a block's rows together, apart from acc, and added to those rows
+    // that have its adapter: what another one holds, infinities among it, never
+    // meets a row's sum.
 #pragma unroll
-          for (int j = 0; j < IN; ++j) u[j] = up_at(e0, MF * j + ln, r);
-          for (int plane = 0; plane < p.planes; ++plane) {
+    for (int i = 0; i < IM; ++i) id[i] = id[i] >= 0 && id[i] < p.adapters ? id[i] : -1;
+    if (staged) {
+      const char* const lows = smem + spare + (TM * wm + ln) * p.rank * 2;
+      const char* const ups = smem + spare + p.planes * low_bytes + (TN * wn + ln) * p.rank * 2;
+      while (item < items_end) {
+        const int e = adapter_of(item);
+        wait_vmcnt<0>();
+        lds_barrier();
 #pragma unroll
-            for (int i = 0; i < IM; ++i) {
-              const h8 v = low_at(i, plane, r);
+        for (int i = 0; i < IM; ++i) {
+          if (__builtin_amdgcn_ballot_w64(id[i] == e) == 0) continue;
+          acc_t t[IN];
 #pragma unroll
-              for (int j = 0; j < IN; ++j) acc[i][j] = mma(u[j], v, acc[i][j]);
+          for (int j = 0; j < IN; ++j) t[j] = acc_t{};
+          for (int r0 = 0; r0 < p.rank; r0 += kW) {
+            const int r = r0 + 8 * lg;
+            h8 u[IN];
+#pragma unroll
+            for (int j = 0; j < IN; ++j)
+              u[j] = r < p.rank ? *reinterpret_cast<const h8*>(ups + (MF * j * p.rank + r) * 2) : h8{};
+            for (int plane = 0; plane < p.planes; ++plane) {
+              const h8 v = r < p.rank ? *reinterpret_cast<const h8*>(lows + plane * low_bytes + (MF * i * p.rank + r) * 2)
+                                      : h8{};
+#pragma unroll
+              for (int j = 0; j < IN; ++j) t[j] = mma(u[j], v, t[j]);
             }
           }
+#pragma unroll
+          for (int j = 0; j < IN; ++j)
+#pragma unroll
+            for (int a = 0; a < AR; ++a) acc[i][j][a] += id[i] == e ? t[j][a] : 0.f;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        item = next_item(first_item, item + 1);
+        if (item < items_end) {
+          lds_barrier();   // everyone has read this adapter's rows
+          stage_up(adapter_of(item));
         }
       }
     } else {
+      const auto low_at = [&](int i, int plane, int r) SIDON_INLINE {
+        const E* at = static_cast<const E*>(p.low) + plane * p.plane +
+                      (int64_t)min(m0 + TM * wm + MF * i + ln, p.M - 1) * p.rank + r;
+        return r < p.rank ? *reinterpret_cast<const h8*>(at) : h8{};
+      };
+      const auto up_at = [&](int e, int col, int r) SIDON_INLINE {
+        const E* at = static_cast<const E*>(p.up) + ((int64_t)e * p.N + tn * BN + TN * wn + col) * p.rank + r;
+        return r < p.rank ? *reinterpret_cast<const h8*>(at) : h8{};
+      };
 #pragma unroll
       for (int i = 0; i < IM; ++i) {
         uint64_t todo = __builtin_amdgcn_ballot_w64(id[i] >= 0);
@@ -415,19 +492,25 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
           while (todo != 0) {
             const int e = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(todo));
             todo &= ~__builtin_amdgcn_ballot_w64(id[i] == e);
+            acc_t t[IN];
 #pragma unroll
-            for (int j = 0; j < IN; ++j) {
-              // (apart from acc, so that what another adapter holds, infinities
-              // among it, never meets this row's sum)
-              acc_t t = {};
-              for (int r0 = 0; r0 < p.rank; r0 += kW) {
-                const int r = r0 + 8 * lg;
-                const h8 u = up_at(e, MF * j + ln, r);
-                for (int plane = 0; plane < p.planes; ++plane) t = mma(u, low_at(i, plane, r), t);
+            for (int j = 0; j < IN; ++j) t[j] = acc_t{};
+#pragma unroll 2
+            for (int r0 = 0; r0 < p.rank; r0 += kW) {
+              const int r = r0 + 8 * lg;
+              h8 u[IN];
+#pragma unroll
+              for (int j = 0; j < IN; ++j) u[j] = up_at(e, MF * j + ln, r);
+              for (int plane = 0; plane < p.planes; ++plane) {
+                const h8 v = low_at(i, plane, r);
+#pragma unroll
+                for (int j = 0; j < IN; ++j) t[j] = mma(u[j], v, t[j]);
               }
-#pragma unroll
-              for (int a = 0; a < AR; ++a) acc[i][j][a] += id[i] == e ? t[a] : 0.f;
             }
+#pragma unroll
+            for (int j = 0; j < IN; ++j)
+#pragma unroll
+              for (int a = 0; a < AR; ++a) acc[i][j][a] += id[i] == e ? t[j][a] : 0.f;
           }
         } else if (id[i] >= 0) {
           // Nearly every row has an adapter of its own: each lane takes its
