@@ -150,16 +150,17 @@ __global__ void __launch_bounds__(64 * W) shrink_kernel(const ShrinkParams p) {
 typedef void (*ExpandFn)(LowParams);
 struct ExpandKernel {
   int bm, bn, threads;
+  bool direct;         // takes rows of any adapters (kDirectTile)
   ExpandFn fn[2][2];   // [fp16, bf16][half out, fp32 add]
 };
 
 #define SIDON_LOW(BM, BN, WM, WN, MF, ST, MODE, E) gemm_tile_kernel<BM, BN, WM, WN, MF, ST, MODE, E, LowParams>
 #define SIDON_BOTH(BM, BN, WM, WN, MF, ST)                                              \
-  {BM, BN, 64 * WM * WN,                                                                \
+  {BM, BN, 64 * WM * WN, kDirectTile<BM, BN, WM, WN>,                                   \
    {{SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, _Float16), SIDON_LOW(BM, BN, WM, WN, MF, ST, kAdd, _Float16)}, \
     {SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, __bf16), SIDON_LOW(BM, BN, WM, WN, MF, ST, kAdd, __bf16)}}}
 #define SIDON_HALF(BM, BN, WM, WN, MF, ST)                                              \
-  {BM, BN, 64 * WM * WN,                                                                \
+  {BM, BN, 64 * WM * WN, kDirectTile<BM, BN, WM, WN>,                                   \
    {{SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, _Float16), nullptr},                      \
     {SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, __bf16), nullptr}}}
 
@@ -168,7 +169,7 @@ struct ExpandKernel {
 const ExpandKernel kExpand[] = {
     SIDON_BOTH(32, 64, 2, 2, 16, 6),   SIDON_BOTH(64, 64, 2, 2, 16, 4),   SIDON_BOTH(64, 128, 2, 4, 16, 4),
     SIDON_BOTH(128, 128, 2, 4, 16, 4), SIDON_BOTH(192, 128, 2, 4, 16, 3), SIDON_HALF(128, 256, 2, 4, 16, 3),
-    SIDON_HALF(160, 256, 1, 4, 32, 3),
+    SIDON_HALF(160, 256, 1, 4, 32, 3), SIDON_HALF(192, 256, 2, 4, 16, 2),
 };
 
 struct Call {
@@ -272,6 +273,7 @@ int check_and_launch(Call& c, sidon_stream_t stream) {
   double best_us = 0;
   for (const ExpandKernel& t : kExpand) {
     if (t.fn[0][c.residual] == nullptr || p.N % t.bn != 0) continue;
+    if (!t.direct && !low_staged(t.bm, t.bn, p.rows_per_id, p.rank)) continue;
     const double us = tile_us(t.bm, t.bn, p.M, p.N, p.K, 1, !c.residual, cus);
     if (best == nullptr || us < best_us) best = &t, best_us = us;
   }

@@ -153,6 +153,15 @@ __device__ __forceinline__ E to_elem(float y) {
 // one adapter at a time; of more, straight from memory: up to kFewKinds adapters
 // among a block's rows a matrix product each, past them every lane its own row.
 constexpr int kFewItems = 4, kFewKinds = 4;
+// The tiles that have the second way too: where it fits the registers beside the
+// accumulators.  The others only run calls all of whose tiles take the first.
+template <int BM, int BN, int WM, int WN>
+inline constexpr bool kDirectTile = BM * BN <= 192 * 128 && BM / WM * (BN / WN) <= 96 * 64;
+// Whether every BM x BN tile takes the low-rank term through LDS.
+inline bool low_staged(int bm, int bn, int rows_per_id, int rank) {
+  return (bm - 2) / rows_per_id + 2 <= kFewItems &&
+         ((bm * rank * 2 + 1023) & ~1023) + ((bn * rank * 2 + 1023) & ~1023) <= (bm + bn) * 128;
+}
 
 template <int BM, int BN, int WM, int WN, int MF, int ST, int kMode>
 struct Tile {
@@ -337,6 +346,74 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
         if (kt < ST - 1 || j < kFirst) copy(kt, kt, j);
     }
   }
+
+  // The low-rank term of a tile with few items: the tile's rows of `low`, and of
+  // `up` for one adapter after another, each one contiguous block, are copied into
+  // a free ring slot, the first under the last slice.  (Read from memory by the lanes
+  // that multiply them, whose neighbours hold other rows, they cost a cache access
+  // each: 128 x 256 tiles of rank 64, 4 us a tile.)  `fit` planes of low at a time.
+  constexpr int kW = 8 * NG;   // ranks per product
+  int first_item = 0, item = 0, items_end = 0, adapter = -1, low_bytes = 0, up_bytes = 0, fit = 1;
+  constexpr bool kDirect = kLow && kDirectTile<BM, BN, WM, WN>;
+  bool staged = false;
+  const auto adapter_of = [&](int i) SIDON_INLINE {
+    if constexpr (kLow) {
+      const int e = p.ids[i];
+      return e >= 0 && e < p.adapters ? e : -1;
+    }
+    return -1;
+  };
+  // The first item from `item` on whose adapter no earlier item of the tile has.
+  const auto next_item = [&]() SIDON_INLINE {
+    for (; item < items_end; ++item) {
+      adapter = adapter_of(item);
+      bool fresh = adapter >= 0;
+      for (int k = first_item; k < item; ++k) fresh = fresh && adapter_of(k) != adapter;
+      if (fresh) break;
+    }
+  };
+  // Rows of `rank` values from `src`, `count` of them, as 1 KB copies; what lies past
+  // them is read again from their end.  Of a power of two of 16-byte chunks per
+  // row, chunk c of row r sits at c ^ ((r >> mix) & mask), so that the 16 rows
+  // of an operand read are on distinct banks (other counts spread by themselves).
+  int chunks = 1, mix = 0, mask = 0;
+  const auto stage = [&](int at, const char* src, int bytes, int count) SIDON_INLINE {
+    const int most = count * chunks - 1;
+    for (int i = w; i < bytes >> 10; i += NW) {
+      int q = min(64 * i + lane, most);
+      if (mask != 0) q ^= (q >> (31 - __builtin_clz(chunks)) >> mix) & mask;
+      copy_1k(lds0 + (uint32_t)(at + i * 1024), src, (uint32_t)q * 16u);
+    }
+  };
+  const auto stage_low = [&](int at, int plane) SIDON_INLINE {
+    if constexpr (kLow) {
+      for (int k = 0; k < min(fit, p.planes - plane); ++k)
+        stage(at + k * low_bytes,
+              static_cast<const char*>(p.low) + 2 * ((plane + k) * p.plane + (int64_t)m0 * p.rank), low_bytes,
+              min(BM, p.M - m0));
+    }
+  };
+  const auto stage_up = [&](int at, int e) SIDON_INLINE {
+    if constexpr (kLow)
+      stage(at + fit * low_bytes, static_cast<const char*>(p.up) + 2 * ((int64_t)e * p.N + tn * BN) * p.rank, up_bytes,
+            BN);
+  };
+  if constexpr (kLow) {
+    chunks = p.rank >> 3;
+    if ((chunks & (chunks - 1)) == 0) {
+      mask = chunks - 1;
+      mix = 4 - (31 - __builtin_clz(chunks));
+    }
+    first_item = m0 / p.rows_per_id;
+    items_end = min(m0 + BM - 1, p.M - 1) / p.rows_per_id + 1;
+    low_bytes = (BM * p.rank * 2 + 1023) & ~1023;
+    up_bytes = (BN * p.rank * 2 + 1023) & ~1023;
+    fit = p.planes * low_bytes + up_bytes <= T::kStage ? p.planes : 1;
+    staged = !kDirect || (items_end - first_item <= kFewItems && fit * low_bytes + up_bytes <= T::kStage);
+    item = first_item;
+    if (staged) next_item();
+  }
+
   if (nk >= ST) {
     wait_vmcnt<kPer * (ST - 2) + kFirst>();
   } else {
@@ -369,61 +446,12 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
     for (int t = 0; t < kOld; ++t)
       old[t] = *reinterpret_cast<const f4*>(yb + min(m0 + TM * wm + kFRows * t + lane / kFLanes, p.M - 1) * ld);
   }
-  // The low-rank term of a tile with few items: the tile's rows of `low`, and of
-  // `up` for one adapter after another, each one contiguous block, are copied into
-  // a free ring slot, the first under the last slice.  (Read from memory by the lanes
-  // that multiply them, whose neighbours hold other rows, they cost a cache access
-  // each: 128 x 256 tiles of rank 64, 4 us a tile.)
-  constexpr int kW = 8 * NG;   // ranks per product
-  const int spare = (slot == 0 ? ST - 1 : slot - 1) * T::kStage;   // (slot: of the last slice)
-  int item = 0, items_end = 0, low_bytes = 0;   // low_bytes: of a plane
-  bool staged = false;
-  const auto adapter_of = [&](int i) SIDON_INLINE {
-    if constexpr (kLow) {
-      const int e = p.ids[i];
-      return e >= 0 && e < p.adapters ? e : -1;
-    }
-    return -1;
-  };
-  // The first item from i on whose adapter no earlier item of the tile has.
-  const auto next_item = [&](int first, int i) SIDON_INLINE {
-    for (; i < items_end; ++i) {
-      const int e = adapter_of(i);
-      bool fresh = e >= 0;
-      for (int k = first; k < i; ++k) fresh = fresh && adapter_of(k) != e;
-      if (fresh) break;
-    }
-    return i;
-  };
-  // Rows of `rank` values from `src`, `count` of them, as 1 KB copies; what lies past
-  // them is read again from their end.
-  const auto stage = [&](int at, const char* src, int bytes, int count) SIDON_INLINE {
-    if constexpr (kLow) {
-      const int most = count * p.rank * 2 - 16;
-      for (int i = w; i < bytes >> 10; i += NW)
-        copy_1k(lds0 + (uint32_t)(at + i * 1024), src, (uint32_t)min(1024 * i + 16 * lane, most));
-    }
-  };
-  const auto stage_up = [&](int e) SIDON_INLINE {
-    if constexpr (kLow)
-      stage(spare + p.planes * low_bytes, static_cast<const char*>(p.up) + 2 * ((int64_t)e * p.N + tn * BN) * p.rank,
-            (BN * p.rank * 2 + 1023) & ~1023, BN);
-  };
-  int first_item = 0;
+  // (slot: of the last slice)
+  const int spare = (slot == 0 ? ST - 1 : slot - 1) * T::kStage;
   if constexpr (kLow) {
-    first_item = m0 / p.rows_per_id;
-    items_end = min(m0 + BM - 1, p.M - 1) / p.rows_per_id + 1;
-    low_bytes = (BM * p.rank * 2 + 1023) & ~1023;
-    staged = items_end - first_item <= kFewItems &&
-             p.planes * low_bytes + ((BN * p.rank * 2 + 1023) & ~1023) <= T::kStage;
-    if (staged) {
-      item = next_item(first_item, first_item);
-      if (item < items_end) {
-        for (int plane = 0; plane < p.planes; ++plane)
-          stage(spare + plane * low_bytes, static_cast<const char*>(p.low) + 2 * (plane * p.plane + (int64_t)m0 * p.rank),
-                low_bytes, min(BM, p.M - m0));
-        stage_up(adapter_of(item));
-      }
+    if (staged && item < items_end) {
+      stage_low(spare, 0);
+      stage_up(spare, adapter);
     }
   }
   body(kt, No{}, No{}, No{});
@@ -436,43 +464,55 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
     for (int i = 0; i < IM; ++i) id[i] = id[i] >= 0 && id[i] < p.adapters ? id[i] : -1;
     if (staged) {
       const char* const lows = smem + spare + (TM * wm + ln) * p.rank * 2;
-      const char* const ups = smem + spare + p.planes * low_bytes + (TN * wn + ln) * p.rank * 2;
-      while (item < items_end) {
-        const int e = adapter_of(item);
+      const char* const ups = smem + spare + fit * low_bytes + (TN * wn + ln) * p.rank * 2;
+      const int mixed = (ln >> mix) & mask;   // (blocks are multiples of 16 rows)
+      int plane = 0;
+      bool more = item < items_end;
+      while (more) {
         wait_vmcnt<0>();
         lds_barrier();
+        const int now = kMode == kHalf ? 1 : min(fit, p.planes - plane);   // (16-bit outputs: one plane)
 #pragma unroll
         for (int i = 0; i < IM; ++i) {
-          if (__builtin_amdgcn_ballot_w64(id[i] == e) == 0) continue;
           acc_t t[IN];
 #pragma unroll
           for (int j = 0; j < IN; ++j) t[j] = acc_t{};
+#pragma unroll 2
           for (int r0 = 0; r0 < p.rank; r0 += kW) {
-            const int r = r0 + 8 * lg;
+            const int c = (r0 >> 3) + lg, at = (c ^ mixed) << 4;
             h8 u[IN];
 #pragma unroll
             for (int j = 0; j < IN; ++j)
-              u[j] = r < p.rank ? *reinterpret_cast<const h8*>(ups + (MF * j * p.rank + r) * 2) : h8{};
-            for (int plane = 0; plane < p.planes; ++plane) {
-              const h8 v = r < p.rank ? *reinterpret_cast<const h8*>(lows + plane * low_bytes + (MF * i * p.rank + r) * 2)
-                                      : h8{};
+              u[j] = c < chunks ? *reinterpret_cast<const h8*>(ups + MF * j * p.rank * 2 + at) : h8{};
+            for (int k = 0; k < now; ++k) {
+              const h8 v = c < chunks ? *reinterpret_cast<const h8*>(lows + k * low_bytes + MF * i * p.rank * 2 + at) : h8{};
 #pragma unroll
               for (int j = 0; j < IN; ++j) t[j] = mma(u[j], v, t[j]);
             }
           }
+          const bool mine = id[i] == adapter;
 #pragma unroll
           for (int j = 0; j < IN; ++j)
 #pragma unroll
-            for (int a = 0; a < AR; ++a) acc[i][j][a] += id[i] == e ? t[j][a] : 0.f;
+            for (int a = 0; a < AR; ++a) acc[i][j][a] += mine ? t[j][a] : 0.f;
           __builtin_amdgcn_sched_barrier(0);
         }
-        item = next_item(first_item, item + 1);
-        if (item < items_end) {
-          lds_barrier();   // everyone has read this adapter's rows
-          stage_up(adapter_of(item));
+        // The next planes of this adapter, or the first of the next one.
+        plane += now;
+        const bool done = plane == p.planes;
+        if (done) {
+          plane = 0;
+          ++item;
+          next_item();
+          more = item < items_end;
+        }
+        if (more) {
+          lds_barrier();   // everyone has read what the copies replace
+          if (done) stage_up(spare, adapter);
+          if (fit < p.planes) stage_low(spare, plane);
         }
       }
-    } else {
+    } else if constexpr (kDirect) {
       const auto low_at = [&](int i, int plane, int r) SIDON_INLINE {
         const E* at = static_cast<const E*>(p.low) + plane * p.plane +
                       (int64_t)min(m0 + TM * wm + MF * i + ln, p.M - 1) * p.rank + r;
@@ -515,9 +555,11 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
         } else if (id[i] >= 0) {
           // Nearly every row has an adapter of its own: each lane takes its
           // row's products itself, from whole rows of up.
-          for (int r = 0; r < p.rank; r += 8) {
-            float v[8] = {};
-            for (int plane = 0; plane < p.planes; ++plane) {
+          const auto own = [&](int r, h8 first, auto up) SIDON_INLINE {
+            float v[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] = (float)first[c];
+            for (int plane = 1; plane < p.planes; ++plane) {
               const h8 part = low_at(i, plane, r);
 #pragma unroll
               for (int c = 0; c < 8; ++c) v[c] += (float)part[c];
@@ -526,13 +568,18 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
             for (int j = 0; j < IN; ++j)
 #pragma unroll
               for (int a = 0; a < AR; ++a) {
-                const h8 u = up_at(id[i], MF * j + 8 * (a >> 2) + 4 * lg + (a & 3), r);
+                const h8 u = up(j, a);
                 float t = acc[i][j][a];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) t = fmaf(v[c], (float)u[c], t);
                 acc[i][j][a] = t;
               }
-          }
+          };
+#pragma unroll 2
+          for (int r = 0; r < p.rank; r += 8)
+            own(r, low_at(i, 0, r), [&](int j, int a) SIDON_INLINE {
+              return up_at(id[i], MF * j + 8 * (a >> 2) + 4 * lg + (a & 3), r);
+            });
         }
       }
     }
