@@ -44,8 +44,8 @@ struct ShrinkParams {
 // accumulators are 4 ranks of one row, so of several adapters among the rows each
 // costs a pass over K whose other rows' results are dropped.
 // (Operands read from memory by the lanes that multiply them cost a cache access
-// per lane, its neighbours holding other rows: 17.2 us instead of SHRINK_NOW at 4800 rows, K
-// 1024, rank 64.)
+// per lane, its neighbours holding other rows: 17.2 us instead of 8.3 at 4800 rows, K 1024,
+// rank 64.)
 template <typename E, int RB, int W>
 __global__ void __launch_bounds__(64 * W) shrink_kernel(const ShrinkParams p) {
   typedef typename Elem<E>::e8 e8;
@@ -156,20 +156,25 @@ struct ExpandKernel {
 
 #define SIDON_LOW(BM, BN, WM, WN, MF, ST, MODE, E) gemm_tile_kernel<BM, BN, WM, WN, MF, ST, MODE, E, LowParams>
 #define SIDON_BOTH(BM, BN, WM, WN, MF, ST)                                              \
-  {BM, BN, 64 * WM * WN, kDirectTile<BM, BN, WM, WN>,                                   \
+  {BM, BN, 64 * WM * WN, kDirectTile<BM, BN>,                                           \
    {{SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, _Float16), SIDON_LOW(BM, BN, WM, WN, MF, ST, kAdd, _Float16)}, \
     {SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, __bf16), SIDON_LOW(BM, BN, WM, WN, MF, ST, kAdd, __bf16)}}}
 #define SIDON_HALF(BM, BN, WM, WN, MF, ST)                                              \
-  {BM, BN, 64 * WM * WN, kDirectTile<BM, BN, WM, WN>,                                   \
+  {BM, BN, 64 * WM * WN, kDirectTile<BM, BN>,                                           \
    {{SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, _Float16), nullptr},                      \
     {SIDON_LOW(BM, BN, WM, WN, MF, ST, kHalf, __bf16), nullptr}}}
 
-// gemm.hip's shapes, a third of them: what the rest would gain is small next
-// to the low-rank term.
+// gemm.hip's shapes, half of them: what the rest would gain is small next to the
+// low-rank term.  us, of it the shrink launch, and the shared projection alone
+// (conformer.linear_silu_lt, residual_gemm): 1 x 1024 x 1024 rank 16 9.7 (2.4) | 5.8,
+// 48 rows of 48 adapters x 4096 x 1024 rank 16 12.7 (3.3) | 6.0, 4 x 400 x 2048 x 1024
+// rank 32 21 (4.8) | 12.3, 8 x 600 x 4096 x 1024 rank 64 64 (8.3) | 51-57, rank 16 56 |
+// 51, residual 3 x 1463 x 1024 x 4096 rank 16 58 (11) | 40.
 const ExpandKernel kExpand[] = {
     SIDON_BOTH(32, 64, 2, 2, 16, 6),   SIDON_BOTH(64, 64, 2, 2, 16, 4),   SIDON_BOTH(64, 128, 2, 4, 16, 4),
     SIDON_BOTH(128, 128, 2, 4, 16, 4), SIDON_BOTH(192, 128, 2, 4, 16, 3), SIDON_HALF(128, 256, 2, 4, 16, 3),
     SIDON_HALF(160, 256, 1, 4, 32, 3), SIDON_HALF(192, 256, 2, 4, 16, 2),
+    SIDON_HALF(320, 256, 2, 4, 32, 2),
 };
 
 struct Call {

@@ -155,8 +155,8 @@ __device__ __forceinline__ E to_elem(float y) {
 constexpr int kFewItems = 4, kFewKinds = 4;
 // The tiles that have the second way too: where it fits the registers beside the
 // accumulators.  The others only run calls all of whose tiles take the first.
-template <int BM, int BN, int WM, int WN>
-inline constexpr bool kDirectTile = BM * BN <= 192 * 128 && BM / WM * (BN / WN) <= 96 * 64;
+template <int BM, int BN>
+inline constexpr bool kDirectTile = BM * BN <= 128 * 128;
 // Whether every BM x BN tile takes the low-rank term through LDS.
 inline bool low_staged(int bm, int bn, int rows_per_id, int rank) {
   return (bm - 2) / rows_per_id + 2 <= kFewItems &&
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
   // each: 128 x 256 tiles of rank 64, 4 us a tile.)  `fit` planes of low at a time.
   constexpr int kW = 8 * NG;   // ranks per product
   int first_item = 0, item = 0, items_end = 0, adapter = -1, low_bytes = 0, up_bytes = 0, fit = 1;
-  constexpr bool kDirect = kLow && kDirectTile<BM, BN, WM, WN>;
+  constexpr bool kDirect = kLow && kDirectTile<BM, BN>;
   bool staged = false;
   const auto adapter_of = [&](int i) SIDON_INLINE {
     if constexpr (kLow) {
@@ -490,11 +490,12 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
               for (int j = 0; j < IN; ++j) t[j] = mma(u[j], v, t[j]);
             }
           }
-          const bool mine = id[i] == adapter;
+          // (A lane's own condition: behind one of the wavefront, or a selection, the
+          // compiler keeps the accumulators in two places.)
+          if (id[i] == adapter) {
 #pragma unroll
-          for (int j = 0; j < IN; ++j)
-#pragma unroll
-            for (int a = 0; a < AR; ++a) acc[i][j][a] += mine ? t[j][a] : 0.f;
+            for (int j = 0; j < IN; ++j) acc[i][j] += t[j];
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
         // The next planes of this adapter, or the first of the next one.
@@ -547,10 +548,10 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
                 for (int j = 0; j < IN; ++j) t[j] = mma(u[j], v, t[j]);
               }
             }
+            if (id[i] == e) {
 #pragma unroll
-            for (int j = 0; j < IN; ++j)
-#pragma unroll
-              for (int a = 0; a < AR; ++a) acc[i][j][a] += id[i] == e ? t[j][a] : 0.f;
+              for (int j = 0; j < IN; ++j) acc[i][j] += t[j];
+            }
           }
         } else if (id[i] >= 0) {
           // Nearly every row has an adapter of its own: each lane takes its
