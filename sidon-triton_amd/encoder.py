@@ -14,7 +14,11 @@ Mirrors src/sidon_triton/triton_encoder.py:
   * ``save_encoder`` / ``load_encoder`` (:514-525): here a safetensors file
     with the scalars in its metadata, loaded without unpickling anything;
     ``load_encoder`` also reads the reference's own ``encoder_triton.pt``
-    (with ``torch.load(weights_only=True)``).
+    (with ``torch.load(weights_only=True)``);
+  * ``pack_adapters`` and the call's ``adapters`` / ``ids``: low-rank adapters of
+    the projections, one per item of a batch (``adapters.adapter_linear``), where
+    the reference merges a single one into the weights
+    (tools/convert_torchscript.py:179-205).
 
 Per layer the work is: res_norm (HIP); the projections, on this library's tiled
 GEMM kernel (csrc/gemm.hip) with the bias, the SiLU or the GLU in its epilogue,
@@ -34,6 +38,7 @@ from pathlib import Path
 
 import torch
 
+from . import adapters as low_rank
 from .blas import gemm_nt
 from .conformer import (causal_dw_norm, glu_causal_dw_norm, linear, linear_glu, linear_glu_fits, linear_silu,
                         linear_silu_lt, linear_silu_preferred, partial_values, residual_gemm, residual_partials,
@@ -45,6 +50,11 @@ from .flexrel import HEAD_DIM, LEFT, NUM_POS, RIGHT
 ENCODER_FILE = "encoder_mi355x.safetensors"
 _FORMAT = "sidon-mi355x-encoder"
 _NORMS = ("ffn1_ln", "attn_ln", "conv_ln", "dw_ln", "ffn2_ln", "final_ln")
+# Projections that take adapters, by packed name: the model's parts of each (fused
+# along their outputs) and the factor that the packed weights carry.
+_ADAPTED = {"ffn1_w1": (("ffn1_w1",), 1.0), "ffn1_w2": (("ffn1_w2",), 0.5), "qkv_w": (("q_w", "k_w", "v_w"), 1.0),
+            "out_w": (("out_w",), 1.0), "pw2_w": (("pw2_w",), 1.0), "ffn2_w1": (("ffn2_w1",), 1.0),
+            "ffn2_w2": (("ffn2_w2",), 0.5)}
 _LAYER_TENSORS = ("ffn1_w1", "ffn1_b1", "ffn1_w2", "qkv_w", "qkv_b", "rel", "out_w", "pw1_w", "dwt", "pw2_w",
                   "ffn2_w1", "ffn2_b1", "ffn2_w2")
 
@@ -139,6 +149,47 @@ def pack_encoder(model) -> dict:
     return pack_weights(model_weights(model))
 
 
+def pack_adapters(packed: dict, adapters, device=None) -> list[dict]:
+    """Fine-tuned variants of the encoder as one set of adapters for
+    ``HipEncoder``'s calls.
+
+    packed: the shared weights (``pack_encoder`` / ``pack_weights``).  adapters: one
+    (scale, layers) per variant, layers a dict per encoder layer of {name: (A [r,
+    in], B [out, r])} with the model's names (``model_weights``): ffn1_w1, ffn1_w2,
+    q_w, k_w, v_w, out_w, pw2_w, ffn2_w1, ffn2_w2; a variant computes with W + scale
+    B A.  What a variant leaves out stays shared.  -> per layer {packed name: (a,
+    b, scale)}, only of projections that some variant adapts."""
+    adapters = [(float(scale), list(layers)) for scale, layers in adapters]
+    names = {name for parts, _ in _ADAPTED.values() for name in parts}
+    for _, layers in adapters:
+        if len(layers) != len(packed["layers"]):
+            raise ValueError(f"adapters of {len(layers)} layers, the encoder has {len(packed['layers'])}")
+        for layer in layers:
+            if set(layer) - names:
+                raise ValueError(f"no adapters for {sorted(set(layer) - names)}: {sorted(names)} take them")
+    out = []
+    for i, weights in enumerate(packed["layers"]):
+        layer = {}
+        for name, (parts, factor) in _ADAPTED.items():
+            if not any(part in layers[i] for _, layers in adapters for part in parts):
+                continue
+            n, k = weights[name].shape[0] // len(parts), weights[name].shape[1]
+            none = (torch.zeros(1, k), torch.zeros(n, 1))
+            pairs = []
+            for _, layers in adapters:
+                mine = [layers[i].get(part, none) for part in parts]
+                for part, (a, b) in zip(parts, mine):
+                    if a.shape[1] != k or b.shape[0] != n or a.shape[0] != b.shape[1]:
+                        raise ValueError(f"{part}'s adapter must be A [r, {k}] and B [{n}, r] "
+                                         f"(got {tuple(a.shape)} and {tuple(b.shape)})")
+                pairs.append(low_rank.stack_adapters([(a.detach().float().cpu(), b.detach().float().cpu())
+                                                      for a, b in mine]))
+            layer[name] = low_rank.pack_adapters(pairs, [scale * factor for scale, _ in adapters],
+                                                 device=weights[name].device if device is None else device)
+        out.append(layer)
+    return out
+
+
 def _to(value, device):
     if isinstance(value, torch.Tensor):
         return value.to(device)
@@ -180,31 +231,45 @@ class HipEncoder:
         self.fused_ffn = fused_ffn
         self.own_residual = own_residual
 
-    def workspace(self, rows: int) -> dict:
+    def workspace(self, rows: int, rank: int = 0) -> dict:
         """Buffers for calls of up to ``rows`` = B*L rows (graph capture
         reuses them): normalized features, the normed stream, one fp16 buffer
         for the FFN intermediate / fused QKV / GLU output (their lifetimes do
         not overlap), the attention context / conv output, and the partial
-        sums of the residual projections of short chunks."""
+        sums of the residual projections of short chunks; with ``rank``, the
+        low-rank products of adapters of up to that rank."""
         wide = max(self.inter, 3 * self.hidden)
         f16 = dict(device=self.device, dtype=torch.float16)
-        return {"rows": rows, "fn": torch.empty(rows * self.features, device=self.device),
-                "xn": torch.empty(rows * self.hidden, **f16), "wide": torch.empty(rows * wide, **f16),
-                "ctx": torch.empty(rows * self.hidden, **f16),
-                "part": torch.empty(partial_values(rows, self.hidden), device=self.device)}
+        ws = {"rows": rows, "fn": torch.empty(rows * self.features, device=self.device),
+              "xn": torch.empty(rows * self.hidden, **f16), "wide": torch.empty(rows * wide, **f16),
+              "ctx": torch.empty(rows * self.hidden, **f16),
+              "part": torch.empty(partial_values(rows, self.hidden), device=self.device)}
+        if rank:
+            ws["low"] = torch.empty(low_rank.workspace_bytes(rows, rank, residual=True), dtype=torch.uint8,
+                                    device=self.device)
+        return ws
 
     @torch.no_grad()
     def __call__(self, features: torch.Tensor, frames: torch.Tensor | None = None,
-                 out: torch.Tensor | None = None, workspace: dict | None = None) -> torch.Tensor:
+                 out: torch.Tensor | None = None, workspace: dict | None = None, adapters: list[dict] | None = None,
+                 ids: torch.Tensor | None = None) -> torch.Tensor:
         """out: optional fp32 [B, L, C] buffer the residual stream (and so the
         result) lives in.  frames: int32 [B] valid frames on the device (None:
         all L).  Rows past an item's valid frames hold finite values nobody
-        should read."""
+        should read.  adapters: a set from ``pack_adapters`` on this device, with
+        ids int32 [B] on the device, each item's variant (none where it is
+        outside the set): an adapted projection runs on ``adapters.adapter_linear``
+        / ``adapter_residual``, the others as without."""
         batch, length, nfeat = features.shape
         if nfeat != self.features:
             raise ValueError(f"features must have {self.features} channels (got {nfeat})")
         rows = batch * length
         device = self.device
+        if (adapters is None) != (ids is None):
+            raise ValueError("adapters and ids go together")
+        if adapters is not None and (len(adapters) != len(self.layers) or tuple(ids.shape) != (batch,)):
+            raise ValueError(f"adapters must be of {len(self.layers)} layers and ids [{batch}] "
+                             f"(got {len(adapters)} and {tuple(ids.shape)})")
         if frames is None:
             lens = torch.full((batch,), length, dtype=torch.int32, device=device)
         else:
@@ -220,6 +285,7 @@ class HipEncoder:
         h_buf = wide[:rows * self.inter].view(rows, self.inter)
         qkv_buf = wide[:rows * 3 * hid].view(rows, 3 * hid)
         part_buf = ws.get("part")
+        low_buf = ws.get("low")
 
         feats = features.reshape(rows, nfeat)
         if feats.dtype != torch.float32 or not feats.is_contiguous():
@@ -234,7 +300,9 @@ class HipEncoder:
         if fused is None:
             fused = True if linear_silu_preferred(rows, self.inter, hid, device) else "lt"
 
-        def ffn_in(w, b):
+        def ffn_in(w, b, low):
+            if low is not None:
+                return low_rank.adapter_linear(xn, w, b, *low, ids, act="silu", out=h_buf, workspace=low_buf)
             if fused == "lt":
                 return linear_silu_lt(xn, w, b, out=h_buf)
             if fused:
@@ -249,8 +317,11 @@ class HipEncoder:
         else:
             split = dict.fromkeys((hid, self.inter), int(self.own_residual))
 
-        def res(a, w, bias, norm1=None, norm2=None):
+        def res(a, w, bias, norm1=None, norm2=None, low=None):
             to = xn_buf if norm2 is not None else None
+            if low is not None:
+                low_rank.adapter_residual(x, a, w, *low, ids, workspace=low_buf)
+                return res_norm(x, bias=bias, norm1=norm1, write_x=norm1 is not None, norm2=norm2, xn=to)
             n = split[a.shape[1]]
             if self.own_residual is None and not (tile_operand(a) and tile_operand(w)):
                 n = 0
@@ -273,16 +344,21 @@ class HipEncoder:
         for i, p in enumerate(layers):
             b1, b2, b4 = p["cum_bias"]
             last = i + 1 == len(layers)
-            h = ffn_in(p["ffn1_w1"], p["ffn1_b1"])
-            xn = res(h, p["ffn1_w2"], b1, norm2=p["attn_ln"])
-            qkv = linear(xn, p["qkv_w"], p["qkv_b"], qkv_buf)
+            low = {} if adapters is None else adapters[i]
+            h = ffn_in(p["ffn1_w1"], p["ffn1_b1"], low.get("ffn1_w1"))
+            xn = res(h, p["ffn1_w2"], b1, norm2=p["attn_ln"], low=low.get("ffn1_w2"))
+            if "qkv_w" in low:
+                qkv = low_rank.adapter_linear(xn, p["qkv_w"], p["qkv_b"], *low["qkv_w"], ids, out=qkv_buf,
+                                              workspace=low_buf)
+            else:
+                qkv = linear(xn, p["qkv_w"], p["qkv_b"], qkv_buf)
             c = flexrel_attention(qkv, batch, self.heads, p["rel"], lens, out=ctx)
-            xn = res(c, p["out_w"], b2, norm2=p["conv_ln"])
+            xn = res(c, p["out_w"], b2, norm2=p["conv_ln"], low=low.get("out_w"))
             s = conv_in(p)
-            xn = res(s, p["pw2_w"], b2, norm2=p["ffn2_ln"])
-            h = ffn_in(p["ffn2_w1"], p["ffn2_b1"])
+            xn = res(s, p["pw2_w"], b2, norm2=p["ffn2_ln"], low=low.get("pw2_w"))
+            h = ffn_in(p["ffn2_w1"], p["ffn2_b1"], low.get("ffn2_w1"))
             xn = res(h, p["ffn2_w2"], b4, norm1=p["final_ln"],
-                     norm2=None if last else layers[i + 1]["ffn1_ln"])
+                     norm2=None if last else layers[i + 1]["ffn1_ln"], low=low.get("ffn2_w2"))
         return x.view(batch, length, hid)
 
 
