@@ -104,7 +104,9 @@ int sidon_adapter_residual(const void* x, int ldx, const void* w, int ldw, const
  * lam_heads 1 or H.  norm_w fp32 [2 D].  out must not overlap an input.
  *
  * Scores, softmax statistics, sums and the norm in fp32, probabilities rounded to
- * `dtype` in front of the product with v, one rounding at the end.  ws:
+ * `dtype` in front of the product with v (with few rows what the rounding left is
+ * multiplied too), one rounding at the end.  What a key within LK but past a
+ * query's own position holds must be finite (its weight is 0).  ws:
  * sidon_diff_attention_workspace_bytes bytes for these sizes on the current
  * device (0: ws may be NULL), 16-byte aligned, contents irrelevant.
  */

@@ -10,21 +10,36 @@
 // G heads of a group and their L queries are G L rows over one key head, a
 // query's heads side by side.
 //
-// A wavefront owns 32 rows and both maps (D = 64) or one of them (D = 128, whose
-// accumulators for both would not fit its registers): S^T = K . Q^T by
-// v_mfma_f32_32x32x16, an online softmax per map with the running maximum
-// raised only when a step's probabilities would leave the fp16 range,
-// O^T += V^T . P^T, for both maps from one read of the values.  Key rows enter
-// the A operand with bits 2 and 3 of their index swapped, which makes the
-// accumulator, rounded to 16 bits, the B operand of the second product.
+// A wavefront owns 32 rows of one map (the accumulators of both would not fit its
+// registers beside the operands): S^T = K . Q^T by v_mfma_f32_32x32x16, an online
+// softmax with the running maximum raised only when a step's probabilities would
+// leave the fp16 range, O^T += V^T . P^T.  Key rows enter the A operand with bits 2
+// and 3 of their index swapped, which makes the accumulator, rounded to 16 bits,
+// the B operand of the second product; the sums of the rounded probabilities, which
+// the result is divided by, come from the matrix core too.  In a round a wavefront
+// takes the softmax of one step and the values of the step before, whose vector
+// and matrix instructions do not wait for each other.
 //
-// Keys go by steps of 32: a step's keys and values (8 D x 32 bytes) are copied
-// global -> LDS by global_load_lds_dwordx4 into a ring, as tiles of 32 rows x
-// 128 bytes with swizzled 16-byte chunks; keys are read with ds_read_b128,
-// values transposed with ds_read_b64_tr_b16.  RB wavefronts (row blocks)
-// share a ring; KS such groups take every KS-th step and are merged through
-// LDS; and over the grid a row block's steps can be split again, each part
-// leaving (max, sum, O) of both maps in fp32 for a joining launch.
+// Keys go by steps of 32: a step's keys of both maps and its values (8 D x 32
+// bytes) are copied global -> LDS by global_load_lds_dwordx4, as tiles of 32 rows
+// x 128 bytes with swizzled 16-byte chunks; keys are read with ds_read_b128,
+// values transposed with ds_read_b64_tr_b16.  The two maps of RB row blocks share a
+// ring of two key and three value slots, so the values are read once for both maps;
+// KS such groups take every KS-th step and are merged through LDS; over the grid a
+// row block's steps can be split again, each part leaving (max, sum, O) of both maps
+// in fp32 for a joining launch.
+//
+// Two forms: 64 rows on one ring for prompts, 32 rows on two rings for few rows.
+// Measured (D 64, fp16 or bf16, whole calls in a graph):
+//   1 x 8 heads x 4800 x 4800        167 us, 846 TFLOP/s (a large matrix product: 1330)
+//   3 x 16 heads (4 key heads) x 1037, causal   43 us
+//   32 x 16 heads (4 key heads) x 1 x 6000, ragged   42 us, 4.7 TB/s (a large copy: 5.0)
+//   1 x 8 heads x 1 x 4800           12 us, two launches
+// Prompts are bound by the vector unit's exponentials and roundings beside the
+// matrix core (16 exponentials per two 32x32x16 score products and four value
+// products), and by whole workgroups: 600 on 256 CUs are three on the busiest.
+// Single tokens are bound by memory once the cache is large, by launches and the
+// first copies' latency where it is small.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -115,7 +130,7 @@ __device__ __forceinline__ float pair_sum(float x) {
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-// Copies of 1 KB as dma_1k's, at 2048 and 3072 beyond both addresses (dma_tile's last two).
+// Two copies as dma_1k's, the second 1024 beyond both addresses.
 __device__ __forceinline__ void dma_2k(uint32_t lds_addr, const char* gbase, uint32_t v0, uint32_t v1) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
@@ -174,7 +189,13 @@ struct Shape {
   static_assert(kSlot / 1024 % kRingWaves == 0, "an even split of the copies");
 };
 
-template <typename E, int D, int RB, int KS, int kMinWaves>
+// kFine: probabilities as two summands of the type, the rounded value and what the
+// rounding left, so that only the output is rounded.  For few rows, where memory and
+// latency leave the matrix cores idle (32 x 1 against 6000 42.4 us, of single
+// probabilities 41.0; 1 x 1 against 4800 12.0 and 11.4).  Prompts round once, as
+// flexrel's do: each probability off by half a step of itself, in sum about what
+// rounding the output costs; a second summand would be two thirds more matrix work.
+template <typename E, int D, int RB, int KS, bool kFine, int kMinWaves>
 __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(const DiffParams p) {
   using C = Shape<D, RB, KS>;
   typedef typename Half<E>::v2 v2;
@@ -220,8 +241,8 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
     wave_steps = row0 < p.R ? (limit(row0 + kBlock - 1) + kStep - 1) / kStep : 0;
     steps = (limit((blk + 1) * RB * kBlock - 1) + kStep - 1) / kStep;
   }
-  const int t0 = (int)((uint32_t)(steps * split) / (uint32_t)p.splits);   // (steps <= 2^25, splits <= 2^6)
-  const int t1 = (int)((uint32_t)(steps * (split + 1)) / (uint32_t)p.splits);
+  const int t0 = (int)((uint32_t)steps * (uint32_t)split / (uint32_t)p.splits);   // (steps <= 2^25, splits <= 2^6)
+  const int t1 = (int)((uint32_t)steps * (uint32_t)(split + 1) / (uint32_t)p.splits);
   const auto mine = [&](int u) SIDON_INLINE { return t0 + u * KS + ks; };   // step u of this group
   const auto until = [&](int t) SIDON_INLINE { return max(t - t0 - ks + KS - 1, 0) / KS; };   // steps u with mine(u) < t
   const int all = (t1 - t0 + KS - 1) / KS;         // most steps of a group: the workgroup's rounds
@@ -255,10 +276,9 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
     for (int j = 0; j < C::kCopies; j += 4) {
       if constexpr (C::kCopies >= 4) {
         dma_tile(at + j * 1024, src, off[j], off[j + 1], off[j + 2], off[j + 3]);
-      } else if constexpr (C::kCopies == 2) {
-        dma_2k(at, src, off[0], off[1]);
       } else {
-        dma_1k(at, src, off[0]);
+        static_assert(C::kCopies == 2 || C::kCopies % 4 == 0, "copies go by two or four");
+        dma_2k(at, src, off[0], off[1]);
       }
     }
   };
@@ -340,7 +360,8 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   for (int d = 0; d < kDb; ++d) o[d] = f32x16{};
   float mx = kFloorMax, sum = 0.f;   // maximum of the scaled scores and sum of the probabilities of query n
   f32x16 s;                          // scores of a step: element i is key 16 (i / 8) + 8 g + i % 8
-  i4 pk[2];                          // its probabilities
+  constexpr int kTerms = kFine ? 2 : 1;
+  i4 pk[kTerms][2];                  // its probabilities
 
   // The three parts of a step.  In round u a wavefront takes the softmax of step
   // u and the product with the values of step u - 1, whose vector and matrix
@@ -380,10 +401,21 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   // rows a lane receives are its own query's sum.
   const auto round_to = [&](const float (&e)[16]) SIDON_INLINE {
 #pragma unroll
-    for (int i = 0; i < 16; i += 2)
-      pk[i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, __builtin_convertvector(f2{e[i], e[i + 1]}, v2));
-    const f4 first = Half<E>::small(sel, pk[0], f4{});
-    return Half<E>::small(sel, pk[1], first)[0];
+    for (int i = 0; i < 16; i += 2) {
+      const v2 hi = __builtin_convertvector(f2{e[i], e[i + 1]}, v2);
+      pk[0][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, hi);
+      if constexpr (kFine) {
+        const f2 left = {e[i] - (float)hi[0], e[i + 1] - (float)hi[1]};
+        pk[kTerms - 1][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, __builtin_convertvector(left, v2));
+      }
+    }
+    f4 total = {};
+#pragma unroll
+    for (int k = 0; k < kTerms; ++k) {
+      total = Half<E>::small(sel, pk[k][0], total);
+      total = Half<E>::small(sel, pk[k][1], total);
+    }
+    return total[0];
   };
   const auto values = [&]() SIDON_INLINE {
     typedef int i2 __attribute__((ext_vector_type(2)));
@@ -394,7 +426,8 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
         const char* tile = smem + vread + (d / 2) * kTile + 2048 * hh;
         const i2 lo = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + vaddr[0][d & 1])));
         const i2 hi = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + vaddr[1][d & 1])));
-        o[d] = Half<E>::mfma(i4{lo[0], lo[1], hi[0], hi[1]}, pk[hh], o[d]);
+#pragma unroll
+        for (int k = 0; k < kTerms; ++k) o[d] = Half<E>::mfma(i4{lo[0], lo[1], hi[0], hi[1]}, pk[k][hh], o[d]);
       }
     vread = vread == 2 * C::kSlot ? 0 : vread + C::kSlot;
   };
@@ -724,15 +757,15 @@ void launch(const DiffParams& p, int D, int rows, hipStream_t stream) {
   const dim3 grid((unsigned)(8 * p.parts_per_xcd * ((p.blocks * p.splits + p.parts - 1) / p.parts)));
   if (D == 64) {
     if (rows == kBlock) {
-      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 1, 2, 2>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 1, 2, true, 2>), grid, dim3(256), 0, stream, p);
     } else {
-      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 2, 1, 3>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_kernel<E, 64, 2, 1, false, 3>), grid, dim3(256), 0, stream, p);
     }
   } else {
     if (rows == kBlock) {
-      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 1, 2, 1>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 1, 2, true, 1>), grid, dim3(256), 0, stream, p);
     } else {
-      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 2, 1, 2>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 2, 1, false, 2>), grid, dim3(256), 0, stream, p);
     }
   }
   if (p.splits > 1) {
