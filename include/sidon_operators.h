@@ -101,7 +101,9 @@ int sidon_adapter_residual(const void* x, int ldx, const void* w, int ldw, const
  * strides int64 arrays in elements ((batch, head, map, row) for q and k, (batch,
  * head, row) for v and out), multiples of 8 from 0 to 2^40, rows of k and v less
  * than 2^25 apart; D 64 or 128.  lam fp32 [lam_heads, 4, D]: lq1, lk1, lq2, lk2,
- * lam_heads 1 or H.  norm_w fp32 [2 D].  out must not overlap an input.
+ * lam_heads 1 or H.  norm_w fp32 [2 D], eps > 0 with it.  out's rows must not overlap one
+ * another, and the memory from its first to its last element must hold nothing of
+ * q, k and v.
  *
  * Scores, softmax statistics, sums and the norm in fp32, probabilities rounded to
  * `dtype` in front of the product with v (with few rows what the rounding left is

@@ -22,6 +22,7 @@ namespace {
 
 using namespace sidon_gemm;
 using sidon::fail;
+using sidon::ranges_meet;
 
 constexpr int kMaxRank = 128;
 constexpr int kShrinkRows = 16;     // rows of a matrix product
@@ -188,11 +189,6 @@ struct Call {
 };
 
 int planes_of(bool residual, int dtype) { return !residual ? 1 : dtype == SIDON_FP16 ? 2 : 3; }
-
-bool ranges_meet(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-  const uintptr_t ab = reinterpret_cast<uintptr_t>(a), bb = reinterpret_cast<uintptr_t>(b);
-  return ab < bb + (uintptr_t)b_bytes && bb < ab + (uintptr_t)a_bytes;
-}
 
 int check_and_launch(Call& c, sidon_stream_t stream) {
   LowParams& p = c.p;

@@ -42,6 +42,7 @@
 // first copies' latency where it is small.
 #include <hip/hip_runtime.h>
 
+#include <float.h>
 #include <stdint.h>
 
 #include "flexrel_device.h"
@@ -752,6 +753,30 @@ size_t part_bytes(int B, int Hk, int R, int D, int splits) {
   return splits > 1 ? (size_t)B * Hk * R * splits * (16 + (size_t)D * 16) : 0;
 }
 
+// Elements from the first to past the last of sizes n and strides st, with `last` contiguous ones.
+__int128 span(const int* n, const int64_t* st, int dims, int last) {
+  __int128 e = last;
+  for (int i = 0; i < dims; ++i) e += (__int128)(n[i] - 1) * st[i];
+  return e;
+}
+
+// Whether rows of `last` elements lie apart: in the order of their strides, every
+// dimension steps past all that the ones before it cover.
+bool apart(const int* n, const int64_t* st, int dims, int last) {
+  __int128 covered = last;
+  bool used[3] = {};
+  for (int k = 0; k < dims; ++k) {
+    int at = -1;
+    for (int i = 0; i < dims; ++i)
+      if (!used[i] && (at < 0 || st[i] < st[at])) at = i;
+    used[at] = true;
+    if (n[at] == 1) continue;
+    if (st[at] < covered) return false;
+    covered += (__int128)(n[at] - 1) * st[at];
+  }
+  return true;
+}
+
 template <typename E>
 void launch(const DiffParams& p, int D, int rows, hipStream_t stream) {
   const dim3 grid((unsigned)(8 * p.parts_per_xcd * ((p.blocks * p.splits + p.parts - 1) / p.parts)));
@@ -818,6 +843,22 @@ SIDON_API int sidon_diff_attention(const void* q, const void* k, const void* v, 
       (norm_w && !sidon::aligned16(norm_w)) || (reinterpret_cast<uintptr_t>(lam) & 3u) != 0 ||
       (reinterpret_cast<uintptr_t>(lens) & 3u) != 0 || !sidon::aligned16(ws))
     return fail(SIDON_E_ALIGN, "q, k, v, out, norm_w and ws must be 16-byte aligned, lam and lens 4-byte aligned");
+  if (norm_w && !(eps >= FLT_MIN)) return fail(SIDON_E_SHAPE, "eps=%g must be positive (a query without keys has no mean square)", eps);
+  // Workgroups read q, k and v while others already write out.
+  {
+    const int qn[] = {B, H, 2, L}, kn[] = {B, Hk, 2, S}, vn[] = {B, Hk, S}, on[] = {B, H, L};
+    if (!apart(on, o_strides, 3, 2 * D)) return fail(SIDON_E_STRIDE, "rows of out overlap one another");
+    const __int128 most = (__int128)1 << 61, o_span = span(on, o_strides, 3, 2 * D) * 2;
+    const struct {
+      const void* at;
+      __int128 bytes;
+    } in[] = {{q, span(qn, q_strides, 4, D) * 2}, {k, span(kn, k_strides, 4, D) * 2}, {v, span(vn, v_strides, 3, 2 * D) * 2}};
+    for (const auto& t : in) {
+      if (o_span > most || t.bytes > most) return fail(SIDON_E_STRIDE, "a tensor spans more than the address space");
+      if (sidon::ranges_meet(out, (int64_t)o_span, t.at, (int64_t)t.bytes))
+        return fail(SIDON_E_SHAPE, "out must lie apart from q, k and v");
+    }
+  }
   int rc;
   if ((rc = sidon::check_device())) return rc;
   const int R = H / Hk * L;

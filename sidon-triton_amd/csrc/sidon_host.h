@@ -30,4 +30,10 @@ int gemm_half(const void* x, int ldx, const void* w, int ldw, const void* bias, 
 
 inline bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
+// Whether two ranges of bytes share memory.
+inline bool ranges_meet(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t ab = reinterpret_cast<uintptr_t>(a), bb = reinterpret_cast<uintptr_t>(b);
+  return ab < bb + (uintptr_t)b_bytes && bb < ab + (uintptr_t)a_bytes;
+}
+
 }  // namespace sidon

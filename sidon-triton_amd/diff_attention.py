@@ -60,8 +60,9 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     past them is not read.  causal: the L queries are the last L of an item's
     valid positions, query i sees the keys up to its own.  A query without keys
     gives zeros.  norm_w fp32 [2D]: each head's output is divided by its root
-    mean square and multiplied by (1 - lam_init) norm_w; None: left as it is.
-    out: optional [B, H, L, 2D], apart from the inputs.  workspace: a contiguous
+    mean square (with eps > 0 under the root) and multiplied by (1 - lam_init)
+    norm_w; None: left as it is.  out: optional [B, H, L, 2D], in memory apart from
+    q, k and v.  workspace: a contiguous
     uint8 tensor of ``workspace_bytes``; allocated per call when None.  A single
     query against a long cache splits the keys over the chip.  Forward only."""
     if q.dim() != 5 or k.dim() != 5 or v.dim() != 4:

@@ -46,12 +46,12 @@ def test_group_norm_rejects_host_tensors(sidon):
 
 def _attention(lib, **over):
     i64 = ctypes.c_int64
-    a = dict(q=16, k=16, v=16, lam=16, lam_heads=1, lens=None, norm_w=16, out=16, ws=None, wsb=0, B=2, H=4, Hk=2, L=10,
+    a = dict(q=16, k=16, v=16, lam=16, lam_heads=1, eps=1e-5, lens=None, norm_w=16, out=16, ws=None, wsb=0, B=2, H=4, Hk=2, L=10,
              S=100, D=64, causal=0, dtype=1, qs=(512, 128, 64, 1024), ks=(8192, 128, 64, 256), vs=(8192, 128, 256),
              os=(8192, 128, 512))
     a.update(over)
     st = [None if a[n] is None else (i64 * len(a[n]))(*a[n]) for n in ("qs", "ks", "vs", "os")]
-    return lib.sidon_diff_attention(a["q"], a["k"], a["v"], a["lam"], a["lam_heads"], 0.5, a["lens"], a["norm_w"], 1e-5,
+    return lib.sidon_diff_attention(a["q"], a["k"], a["v"], a["lam"], a["lam_heads"], 0.5, a["lens"], a["norm_w"], a["eps"],
                                     a["out"], a["ws"], a["wsb"], a["B"], a["H"], a["Hk"], a["L"], a["S"], a["D"],
                                     a["causal"], a["dtype"], *st, None)
 
@@ -68,6 +68,20 @@ def _attention(lib, **over):
 def test_diff_attention_refuses(sidon, over, code):
     lib = sidon._lib.load()
     assert _attention(lib, **over) == code
+    assert lib.sidon_last_error().decode()
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(os=(8192, 128, 0)), -3), (dict(os=(0, 128, 512)), -3), (dict(os=(8192, 64, 512)), -3),
+    (dict(os=(8192, 128, 504)), -3), (dict(os=(2048, 128, 512)), -3), (dict(os=(128, 256, 64)), -3),
+    (dict(out=1 << 30), -2), (dict(out=(1 << 30) + 2 * (512 + 3 * 128 + 9 * 1024)), -2), (dict(out=(1 << 31) + 4096), -2),
+    (dict(out=(1 << 32) - 4096), -2), (dict(eps=0.0), -2), (dict(eps=-1e-5), -2), (dict(eps=float("nan")), -2),
+    (dict(ks=(1 << 40, 1 << 40, 1 << 40, 0), L=1, Hk=4, B=1 << 22), -3),
+])
+def test_diff_attention_refuses_overlaps(sidon, over, code):
+    """Rows of out that share memory, out across an input, and a norm without eps."""
+    lib = sidon._lib.load()
+    assert _attention(lib, **{**dict(q=1 << 30, k=1 << 31, v=1 << 32, out=1 << 33), **over}) == code
     assert lib.sidon_last_error().decode()
 
 
