@@ -40,7 +40,7 @@ extern "C" {
  *
  * x [B*T, C] and y [B*T, C] of `dtype`, rows ldx / ldy elements apart (>= C);
  * w and bias fp32 [C].  y may be x itself (same stride); any other overlap is
- * refused.  1 <= C <= 8192, C % G == 0.  Statistics and arithmetic in fp32,
+ * refused.  B <= 65535, T <= 2^30, 1 <= C <= 8192, C % G == 0.  Statistics and arithmetic in fp32,
  * one rounding at the end.  ws: sidon_group_norm_workspace_bytes bytes, 8-byte
  * aligned, contents irrelevant before and after.
  */

@@ -495,7 +495,7 @@ int element_size(int dtype) { return dtype == SIDON_FP32 ? 4 : 2; }
 // enough workgroups to fill the chip, a few rows per thread at least, at most
 // kMaxChunks for the second pass to join.  (With all columns in a block and 128
 // chunks, joining 128 x 32 groups in every workgroup of the second pass took
-// as long as its rows: 1 x 4800 x 1024 fp16 21 us against 13.)
+// as long as its rows: 1 x 4800 x 1024 fp16 21 us against 16.)
 void plan_passes(Params& p, int vec) {
   const int cg = p.C / p.G;
   int step = 1;   // groups whose channels are whole vectors
@@ -568,7 +568,7 @@ void run(Params& p, bool vector, hipStream_t stream) {
   // 1463 x 32 21.0 | 22.7, 8 x 1500 x 32 25.6 | 34.5.
   const double slab_kb = vecs * 16.0 / 1024, all_mb = slab_kb * p.B * p.G / 1024;
   if (vector && cg % V == 0 && vecs <= kSlabVecs * kSlabThreads && slab_kb <= 80 + 6 * all_mb &&
-      (int64_t)p.B * p.G <= INT32_MAX) {
+      (int64_t)p.B * p.G <= INT32_MAX / kSlabThreads) {   // (a launch holds less than 2^32 threads)
     slab<T>(p, vecs, stream);
   } else if (vector) {
     plan_passes(p, V);
@@ -581,7 +581,7 @@ void run(Params& p, bool vector, hipStream_t stream) {
 
 bool shape_ok(int B, int T, int C, int G, int dtype) {
   return B >= 1 && T >= 1 && C >= 1 && C <= kMaxC && G >= 1 && C % G == 0 && dtype >= SIDON_FP32 && dtype <= SIDON_BF16 &&
-         B <= 65535;
+         B <= 65535 && T <= (1 << 30);
 }
 
 // Whether x and y, as rows of C elements ld apart, share memory in any way
@@ -616,7 +616,7 @@ SIDON_API int sidon_group_norm_act(const void* x, int64_t ldx, const int32_t* le
   if (dtype < SIDON_FP32 || dtype > SIDON_BF16) return fail(SIDON_E_SHAPE, "dtype=%d is no SIDON_FP32 / FP16 / BF16", dtype);
   if (act < SIDON_ACT_NONE || act > SIDON_ACT_RELU) return fail(SIDON_E_SHAPE, "act=%d is no SIDON_ACT_*", act);
   if (!shape_ok(B, T, C, G, dtype))
-    return fail(SIDON_E_SHAPE, "B=%d T=%d C=%d G=%d: need B in [1, 65535], T >= 1, C in [1, %d], C a multiple of G", B,
+    return fail(SIDON_E_SHAPE, "B=%d T=%d C=%d G=%d: need B in [1, 65535], T in [1, 2^30], C in [1, %d], C a multiple of G", B,
                 T, C, G, kMaxC);
   const int size = element_size(dtype);
   const int64_t rows = (int64_t)B * T;

@@ -18,7 +18,7 @@ def _norm(lib, **over):
 
 @pytest.mark.parametrize("over,code", [
     (dict(x=None), -1), (dict(w=None), -1), (dict(b=None), -1), (dict(y=None), -1), (dict(ws=None), -1),
-    (dict(dtype=3), -2), (dict(dtype=-1), -2), (dict(act=4), -2), (dict(B=0), -2), (dict(T=0), -2), (dict(C=0), -2),
+    (dict(dtype=3), -2), (dict(dtype=-1), -2), (dict(act=4), -2), (dict(B=0), -2), (dict(T=0), -2), (dict(T=(1 << 30) + 1), -2), (dict(C=0), -2),
     (dict(G=0), -2), (dict(G=5), -2), (dict(C=8256, ldx=8256, ldy=8256, G=1), -2), (dict(B=65536), -2),
     (dict(wsb=0), -2), (dict(ldx=63), -3), (dict(ldy=0), -3), (dict(ldx=-64), -3), (dict(x=(1 << 20) + 1), -4),
     (dict(w=18), -4), (dict(lens=6), -4), (dict(ws=20), -4),
