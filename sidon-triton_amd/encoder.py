@@ -157,7 +157,8 @@ def pack_adapters(packed: dict, adapters, device=None) -> list[dict]:
     (scale, layers) per variant, layers a dict per encoder layer of {name: (A [r,
     in], B [out, r])} with the model's names (``model_weights``): ffn1_w1, ffn1_w2,
     q_w, k_w, v_w, out_w, pw2_w, ffn2_w1, ffn2_w2; a variant computes with W + scale
-    B A.  What a variant leaves out stays shared.  -> per layer {packed name: (a,
+    B A.  What a variant leaves out stays shared.  Ranks up to 128, of q_w, k_w and v_w
+    together.  -> per layer {packed name: (a,
     b, scale)}, only of projections that some variant adapts."""
     adapters = [(float(scale), list(layers)) for scale, layers in adapters]
     names = {name for parts, _ in _ADAPTED.values() for name in parts}
@@ -174,7 +175,7 @@ def pack_adapters(packed: dict, adapters, device=None) -> list[dict]:
             if not any(part in layers[i] for _, layers in adapters for part in parts):
                 continue
             n, k = weights[name].shape[0] // len(parts), weights[name].shape[1]
-            none = (torch.zeros(1, k), torch.zeros(n, 1))
+            none = (torch.zeros(0, k), torch.zeros(n, 0))
             pairs = []
             for _, layers in adapters:
                 mine = [layers[i].get(part, none) for part in parts]
@@ -182,8 +183,10 @@ def pack_adapters(packed: dict, adapters, device=None) -> list[dict]:
                     if a.shape[1] != k or b.shape[0] != n or a.shape[0] != b.shape[1]:
                         raise ValueError(f"{part}'s adapter must be A [r, {k}] and B [{n}, r] "
                                          f"(got {tuple(a.shape)} and {tuple(b.shape)})")
-                pairs.append(low_rank.stack_adapters([(a.detach().float().cpu(), b.detach().float().cpu())
-                                                      for a, b in mine]))
+                a, b = low_rank.stack_adapters([(a.detach().float().cpu(), b.detach().float().cpu()) for a, b in mine])
+                if a.shape[0] == 0:   # a variant that leaves this projection shared
+                    a, b = torch.zeros(1, k), torch.zeros(b.shape[0], 1)
+                pairs.append((a, b))
             layer[name] = low_rank.pack_adapters(pairs, [scale * factor for scale, _ in adapters],
                                                  device=weights[name].device if device is None else device)
         out.append(layer)

@@ -171,3 +171,15 @@ def test_adapter_linear_rejects_wrong_tensors(sidon):
     a, b = torch.zeros(1, 8, 64, dtype=torch.float16), torch.zeros(1, 64, 8, dtype=torch.float16)
     with pytest.raises(ValueError, match="HIP device"):
         sidon.adapters.adapter_linear(x, w, None, a, b, torch.ones(1), torch.zeros(1, dtype=torch.int32))
+
+
+def test_encoder_adapters_of_the_largest_rank(sidon):
+    """A part that a variant leaves out takes none of the rank that its fused
+    projection has."""
+    packed = {"layers": [{"qkv_w": torch.zeros(192, 64), "out_w": torch.zeros(64, 64)}]}
+    pair = (torch.ones(128, 64), torch.ones(64, 128))
+    packed_set = sidon.encoder.pack_adapters(packed, [(1.0, [{"k_w": pair}]), (2.0, [{"out_w": pair}])])
+    a, b, scale = packed_set[0]["qkv_w"]
+    assert tuple(a.shape) == (2, 128, 64) and tuple(b.shape) == (2, 192, 128) and scale.tolist() == [1.0, 2.0]
+    assert (a[0] == 1).all() and (b[0, 64:128] == 1).all() and b[0].sum() == 64 * 128 and not b[1].any()
+    assert not packed_set[0]["out_w"][1][0].any()
