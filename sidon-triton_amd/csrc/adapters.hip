@@ -222,13 +222,13 @@ int check_and_launch(Call& c, sidon_stream_t stream) {
   const int64_t ysize = c.residual ? 4 : 2;
   const int64_t ybytes = ((int64_t)(p.M - 1) * p.ldy + p.N) * ysize;
   const int64_t up_bytes = (int64_t)p.adapters * p.N * p.rank * 2, a_bytes = (int64_t)p.adapters * p.rank * p.K * 2;
-  if (ranges_meet(p.y, ybytes, p.x, ((int64_t)(p.M - 1) * p.ldx + p.K) * 2) ||
+  if (sidon::rows_meet(p.y, p.ldy * ysize, p.N * ysize, p.x, (int64_t)p.ldx * 2, (int64_t)p.K * 2, p.M) ||
       ranges_meet(p.y, ybytes, p.w, ((int64_t)(p.N - 1) * p.ldw + p.K) * 2) || ranges_meet(p.y, ybytes, p.up, up_bytes) ||
       ranges_meet(p.y, ybytes, c.a, a_bytes) || ranges_meet(p.y, ybytes, c.ws, (int64_t)need) ||
       (p.bias != nullptr && ranges_meet(p.y, ybytes, p.bias, (int64_t)p.N * 2)))
     return fail(SIDON_E_SHAPE, "y must not overlap an input or ws");
   if (c.residual && !(p.add == p.y && p.ldadd == p.ldy) &&
-      ranges_meet(p.y, ybytes, p.add, ((int64_t)(p.M - 1) * p.ldadd + p.N) * 4))
+      sidon::rows_meet(p.y, p.ldy * ysize, p.N * ysize, p.add, (int64_t)p.ldadd * 4, (int64_t)p.N * 4, p.M))
     return fail(SIDON_E_SHAPE, "y may be add itself but must not overlap it otherwise");
   int rc;
   if ((rc = sidon::check_device())) return rc;

@@ -584,21 +584,6 @@ bool shape_ok(int B, int T, int C, int G, int dtype) {
          B <= 65535 && T <= (1 << 30);
 }
 
-// Whether x and y, as rows of C elements ld apart, share memory in any way
-// other than being the same tensor.
-bool overlap(const void* x, int64_t ldx, const void* y, int64_t ldy, int64_t rows, int C, int size) {
-  const uintptr_t xb = reinterpret_cast<uintptr_t>(x), yb = reinterpret_cast<uintptr_t>(y);
-  const uintptr_t xe = xb + (uintptr_t)(((rows - 1) * ldx + C) * size);
-  const uintptr_t ye = yb + (uintptr_t)(((rows - 1) * ldy + C) * size);
-  if (xb >= ye || yb >= xe || (xb == yb && ldx == ldy)) return false;
-  if (ldx == ldy) {   // column blocks of one wider tensor
-    const uintptr_t row = (uintptr_t)ldx * size, width = (uintptr_t)C * size;
-    const uintptr_t d = xb < yb ? (yb - xb) % row : (row - (xb - yb) % row) % row;
-    if (d >= width && row - d >= width) return false;
-  }
-  return true;
-}
-
 }  // namespace
 
 SIDON_API size_t sidon_group_norm_workspace_bytes(int B, int T, int C, int G, int dtype) {
@@ -630,7 +615,8 @@ SIDON_API int sidon_group_norm_act(const void* x, int64_t ldx, const int32_t* le
   if (ws_bytes < sidon_group_norm_workspace_bytes(B, T, C, G, dtype))
     return fail(SIDON_E_SHAPE, "ws holds %zu bytes, the call needs %zu", ws_bytes,
                 sidon_group_norm_workspace_bytes(B, T, C, G, dtype));
-  if (overlap(x, ldx, y, ldy, rows, C, size)) return fail(SIDON_E_SHAPE, "y may be x itself but must not overlap it otherwise");
+  if (!(x == y && ldx == ldy) && sidon::rows_meet(x, ldx * size, C * size, y, ldy * size, C * size, rows))
+    return fail(SIDON_E_SHAPE, "y may be x itself but must not overlap it otherwise");
   int rc;
   if ((rc = sidon::check_device())) return rc;
   Params p{};

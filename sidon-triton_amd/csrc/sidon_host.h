@@ -35,5 +35,15 @@ inline bool ranges_meet(const void* a, int64_t a_bytes, const void* b, int64_t b
   const uintptr_t ab = reinterpret_cast<uintptr_t>(a), bb = reinterpret_cast<uintptr_t>(b);
   return ab < bb + (uintptr_t)b_bytes && bb < ab + (uintptr_t)a_bytes;
 }
+// Whether `rows` rows of a_width and b_width bytes, a_pitch and b_pitch apart, share
+// memory.  Column blocks of one wider tensor do not, though their ranges meet.
+inline bool rows_meet(const void* a, int64_t a_pitch, int64_t a_width, const void* b, int64_t b_pitch, int64_t b_width,
+                      int64_t rows) {
+  if (!ranges_meet(a, (rows - 1) * a_pitch + a_width, b, (rows - 1) * b_pitch + b_width)) return false;
+  if (a_pitch != b_pitch) return true;
+  const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a)) % a_pitch;
+  const int64_t on = d < 0 ? d + a_pitch : d;   // from a's column to b's
+  return on < a_width || a_pitch - on < b_width;
+}
 
 }  // namespace sidon

@@ -150,6 +150,27 @@ def test_adapter_calls_refuse_their_own(sidon):
     assert _adapter(lib, True, add=96 * (1 << 20), ldadd=260) == -2   # the same memory, other rows
 
 
+def test_column_blocks_of_one_tensor(sidon):
+    """Rows side by side in a wider tensor are apart, a column of both is not:
+    here the call gets as far as asking for a device (-6) or is refused (-2)."""
+    lib = sidon._lib.load()
+    mb = 1 << 20
+    wide = dict(ldx=512, ldy=512)   # x 128 columns, y 256, of 512
+    if torch.cuda.is_available():
+        pytest.skip("fake addresses: only where no device would take the launch")
+    assert _adapter(lib, False, y=16 * mb + 2 * 128, **wide) == -6
+    assert _adapter(lib, False, y=16 * mb + 2 * 256, **wide) == -6
+    assert _adapter(lib, False, x=96 * mb + 2 * 256, **wide) == -6
+    assert _adapter(lib, False, y=16 * mb + 2 * 120, **wide) == -2
+    assert _adapter(lib, False, y=16 * mb + 2 * 264, **wide) == -2
+    assert _adapter(lib, False, y=16 * mb + 2 * 128, ldx=512, ldy=520) == -2
+    assert _adapter(lib, True, add=96 * mb + 4 * 256, ldadd=512, ldy=512) == -6
+    assert _adapter(lib, True, add=96 * mb + 4 * 252, ldadd=512, ldy=512) == -2
+    assert _norm(lib, y=(1 << 20) + 128, ldx=128, ldy=128) == -6
+    assert _norm(lib, y=(1 << 20) + 126, ldx=128, ldy=128) == -2
+    assert _norm(lib, x=1 << 22, ldx=128, y=(1 << 22) - 256 * 3 + 128, ldy=128) == -6
+
+
 def test_adapter_workspace_and_packing(sidon):
     ws = sidon.adapters.workspace_bytes
     assert ws(100, 16) == 3200 and ws(100, 16, True) == 6400 and ws(100, 16, True, torch.bfloat16) == 9600
