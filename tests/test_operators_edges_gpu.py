@@ -1,11 +1,17 @@
 """The language-model operators at the ends of their ranges (needs an MI355X):
-offsets past 32 bits, launches of many workgroups, two calls at once, captured
-calls that share a workspace.  Values are held against the same call on an
-ordinary layout, which the operators' own tests hold against float64."""
+offsets past 32 bits, launches of many workgroups, every tile of the adapters,
+two calls at once, captured calls that share a workspace.  Values are held against
+float64, with the tolerances of the operators' own tests, or against the same call
+on an ordinary layout, which those tests hold against float64."""
 
 from __future__ import annotations
 
+import threading
+
 import pytest
+import test_adapters_gpu as adapters_test
+import test_diff_attention_gpu as attention_test
+import test_group_norm_gpu as norm_test
 import torch
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +34,173 @@ def test_group_norm_of_many_groups(sidon):
     # one fp16 rounding; fp32 arithmetic on values below 8
     assert ((got[some].double() - want).abs() <= want.abs() * 2.0 ** -11 + 2.0 ** -18).all()
     assert torch.isfinite(got).all()
+
+
+# (items, rows, N, K, R, adapters): every tile of the adapters' second launch, one output type or both (of 16-bit
+# outputs 32 x 64, 64 x 64, 64 x 128, 128 x 128, 192 x 128, 128 x 256, 160 x 256, 192 x 256, 320 x 256), with ranks
+# that are a power of two and not, items shorter and longer than a tile, and as many as a tile holds
+TILES = [(2, 90, 256, 64, 16, 2), (2, 1037, 256, 64, 40, 3), (3, 1037, 512, 64, 16, 2), (3, 1037, 1024, 64, 24, 3),
+         (5, 1037, 1024, 64, 64, 2), (13, 90, 4096, 64, 16, 3), (3, 1037, 2048, 64, 40, 2), (2, 1037, 4096, 64, 16, 2),
+         (5, 1037, 2048, 64, 64, 6), (8, 600, 4096, 128, 48, 3), (37, 130, 4096, 64, 32, 3), (40, 96, 1024, 64, 128, 5),
+         (24, 64, 2048, 128, 64, 2), (9, 333, 2048, 192, 104, 4)]
+
+
+@pytest.mark.parametrize("kind", adapters_test.KINDS, ids=str)
+@pytest.mark.parametrize("shape", TILES, ids=str)
+def test_adapter_tiles(sidon, shape, kind):
+    s = adapters_test.inputs(*shape, kind, sum(shape))
+    # what another adapter's rows would drag in, and rows without one whose low-rank products are left as they are
+    ws = torch.full((sidon.adapters.workspace_bytes(s["x"].shape[0], shape[4], True, kind),), 255, dtype=torch.uint8,
+                    device=DEV)
+    adapters_test.check(adapters_test.linear(sidon, s, workspace=ws), *adapters_test.reference(s, False))
+    ws.fill_(255)
+    want, tol = adapters_test.reference(s, True)
+    adapters_test.check(adapters_test.residual(sidon, s, workspace=ws), want, tol)
+
+
+def test_adapters_past_32_bits(sidon):
+    """Adapters, outputs and the stream at offsets of more than 4 GiB."""
+    s = adapters_test.inputs(7, 30, 1024, 1024, 64, 3, torch.float16, 5)
+    want, tol = adapters_test.reference(s, False)
+    res, res_tol = adapters_test.reference(s, True)
+    many = 40000
+    a = torch.empty(many, 64, 1024, dtype=torch.float16, device=DEV)
+    b = torch.empty(many, 1024, 64, dtype=torch.float16, device=DEV)
+    scale = torch.zeros(many, device=DEV)
+    a[-3:], b[-3:], scale[-3:] = s["a"], s["b"], s["scale"]
+    s.update(a=a, b=b, scale=scale, ids=torch.where(s["ids"] < 0, -1, s["ids"] + many - 3).int())
+    adapters_test.check(adapters_test.linear(sidon, s), want, tol)
+    del a, b
+    s.update(a=s["a"][-3:].clone(), b=s["b"][-3:].clone(), scale=scale[-3:].clone(),
+             ids=torch.where(s["ids"] < 0, -1, s["ids"] - many + 3).int())
+    out = torch.empty(210, 1 << 24, dtype=torch.float16, device=DEV)[:, :1024]
+    adapters_test.check(adapters_test.linear(sidon, s, out=out), want, tol)
+    del out
+    stream = torch.empty(210, 1 << 23, device=DEV)[:, 64:1088]
+    stream.copy_(s["y"])
+    s["y"] = stream
+    adapters_test.check(adapters_test.residual(sidon, s), res, res_tol)
+
+
+def test_attention_past_32_bits(sidon):
+    """Queries, a cache and an output whose rows, heads and items lie gibibytes apart."""
+    q, k, v, lam, norm_w = attention_test.inputs(2, 2, 1, 40, 33, 64, torch.bfloat16, 4)
+    lens = torch.tensor([33, 20], dtype=torch.int32, device=DEV)
+    for length in (40, 1):
+        want = sidon.diff_attention.diff_attention(q[:, :, :, :length], k, v, lam, 0.3, lens=lens, norm_w=norm_w)
+        row = (1 << 25) - 8
+        cache = torch.empty(35 * row + (1 << 31), dtype=torch.bfloat16, device=DEV)
+        far_k = cache.as_strided(k.shape, (1 << 31, 0, row // 2 // 8 * 8, row, 1), 64)
+        far_v = cache.as_strided(v.shape, (1 << 31, 0, row, 1), 4096)
+        far_k.copy_(k)
+        far_v.copy_(v)
+        q_row = 1 << 26
+        far_q = torch.empty(41 * q_row, dtype=torch.bfloat16, device=DEV).as_strided(
+            (2, 2, 2, length, 64), (256, 1 << 25, 128, q_row, 1))
+        far_q.copy_(q[:, :, :, :length])
+        out = torch.empty(41 * q_row, dtype=torch.bfloat16, device=DEV).as_strided(
+            (2, 2, length, 128), (q_row // 4, q_row // 2, q_row, 1))
+        sidon.diff_attention.diff_attention(far_q, far_k, far_v, lam, 0.3, lens=lens, norm_w=norm_w, out=out)
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 1, 1, 131072, 64), (2, 2, 2, 1, 40000, 128), (1, 1, 1, 9000, 9001, 64)],
+                         ids=str)
+def test_attention_of_long_caches(sidon, shape):
+    b, h, hk, l, s, d = shape
+    q, k, v, lam, norm_w = attention_test.inputs(b, h, hk, l, s, d, torch.bfloat16, 9)
+    lens = [s, s - 4321][:b]
+    attention_test.poison(k, v, lens)
+    got = sidon.diff_attention.diff_attention(q, k, v, lam, 0.3, lens=torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                              causal=True, norm_w=norm_w)
+    attention_test.check(got, *attention_test.reference(q, k, v, lam, 0.3, lens, True, norm_w, 1e-5))
+
+
+def test_group_norm_past_32_bits(sidon):
+    x, w, b = norm_test.inputs(60, 256, torch.float16, 6)
+    lens = torch.tensor([30, 17], dtype=torch.int32, device=DEV)
+    for groups in (8, 2, 64):
+        want = sidon.conformer.group_norm_act(x, 2, groups, w, b, lens=lens)
+        far = torch.empty(60, 1 << 26, dtype=torch.float16, device=DEV)
+        far[:, 512:768] = x
+        got = sidon.conformer.group_norm_act(far[:, 512:768], 2, groups, w, b, lens=lens, out=far[:, 1024:1280])
+        assert torch.equal(got, want)
+        sidon.conformer.group_norm_act(far[:, 512:768], 2, groups, w, b, lens=lens, out=far[:, 512:768])
+        assert torch.equal(far[:, 512:768], want)
+
+
+def calls(sidon, seed):
+    """One call of each operator with its workspace -> [(call, workspace bytes)]; call(workspace) -> the output."""
+    x, w, b = norm_test.inputs(4000, 512, torch.float16, seed)
+    s = adapters_test.inputs(6, 200, 1024, 512, 32, 4, torch.float16, seed)
+    one = adapters_test.inputs(40, 1, 1024, 512, 16, 30, torch.bfloat16, seed)
+    att = attention_test.inputs(2, 8, 4, 1, 3000, 64, torch.float16, seed)
+    pro = attention_test.inputs(2, 4, 4, 300, 300, 128, torch.bfloat16, seed)
+    d = sidon.diff_attention
+    return [
+        (lambda ws: sidon.conformer.group_norm_act(x, 2, 4, w, b, workspace=ws),
+         sidon.conformer.group_norm_workspace(2, 2000, 512, 4, torch.float16)),
+        (lambda ws: adapters_test.linear(sidon, s, act="silu", workspace=ws), sidon.adapters.workspace_bytes(1200, 32)),
+        (lambda ws: adapters_test.residual(sidon, one, out=torch.empty_like(one["y"]), workspace=ws),
+         sidon.adapters.workspace_bytes(40, 16, True, torch.bfloat16)),
+        (lambda ws: d.diff_attention(*att[:4], 0.3, norm_w=att[4], workspace=ws),
+         d.workspace_bytes(2, 8, 4, 1, 3000, 64, DEV)),
+        (lambda ws: d.diff_attention(*pro[:4], 0.3, causal=True, workspace=ws),
+         d.workspace_bytes(2, 4, 4, 300, 300, 128, DEV)),
+    ]
+
+
+def buffer(size):
+    return torch.empty(max(size, 16), dtype=torch.uint8, device=DEV)
+
+
+def test_graphs_that_share_a_workspace(sidon):
+    """Captured calls of every operator over one buffer, replayed in turn with
+    eager calls over the same buffer between them."""
+    todo = calls(sidon, 3)
+    ws = buffer(max(size for _, size in todo))
+    wants = [call(None).clone() for call, _ in todo]
+    torch.cuda.synchronize()
+    graphs = []
+    for call, size in todo:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(ws)
+        graphs.append((graph, out))
+    for turn in range(3):
+        for i, (graph, out) in enumerate(graphs):
+            out.zero_()
+            ws.fill_(255)
+            graph.replay()
+            other, _ = todo[(i + turn) % len(todo)]
+            assert torch.equal(other(ws), wants[(i + turn) % len(todo)])
+        torch.cuda.synchronize()
+        for (_, out), want in zip(graphs, wants):
+            assert torch.equal(out, want)
+
+
+def test_two_streams_and_threads_at_once(sidon):
+    """Calls side by side, each stream and thread with its own workspaces."""
+    todo = calls(sidon, 5)
+    wants = [call(None).clone() for call, _ in todo]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(first):
+        stream = torch.cuda.Stream()
+        spaces = [buffer(size) for _, size in todo]
+        with torch.cuda.stream(stream):
+            for turn in range(12):
+                i = (first + turn) % len(todo)
+                out = todo[i][0](spaces[i])
+                stream.synchronize()
+                if not torch.equal(out, wants[i]):
+                    wrong.append(i)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
