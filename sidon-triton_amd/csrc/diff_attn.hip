@@ -32,7 +32,7 @@
 // Two forms: 64 rows on one ring for prompts, 32 rows on two rings for few rows.
 // Measured (D 64, fp16 or bf16, whole calls in a graph):
 //   1 x 8 heads x 4800 x 4800        167 us, 846 TFLOP/s (a large matrix product: 1330)
-//   3 x 16 heads (4 key heads) x 1037, causal   43 us
+//   3 x 8 heads (2 key heads) x 1037, D 128, ragged, causal   43 us
 //   32 x 16 heads (4 key heads) x 1 x 6000, ragged   42 us, 4.7 TB/s (a large copy: 5.0)
 //   1 x 8 heads x 1 x 4800           12 us, two launches
 // Prompts are bound by the vector unit's exponentials and roundings beside the
@@ -650,16 +650,26 @@ __global__ void __launch_bounds__(64 * kJoinWaves) diff_attn_join_kernel(const D
   const float s1 = sidon::wave_sum(ml.y * f1), s2 = sidon::wave_sum(ml.w * f2);
   // What each part weighs in the difference.
   const float w1 = s1 == 0.f ? 0.f : f1 / s1, w2 = s2 == 0.f ? 0.f : f2 / s2 * lambda;
-  const uint64_t used = __builtin_amdgcn_ballot_w64(ml.y != 0.f || ml.w != 0.f);
+  // Four parts of a wavefront at a time, their loads together.  (A part without keys
+  // holds zeros and weighs nothing.)
+  constexpr int kAtOnce = 4;
   fn x = {};
-#pragma unroll 4
-  for (int s = w; s < p.splits; s += kJoinWaves) {
-    if ((used >> s & 1) != 0) {
-      const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w1), s));
-      const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w2), s));
-      const float* at = src + (int64_t)s * p.R * (4 * D);
-      const fn u = *reinterpret_cast<const fn*>(at), v = *reinterpret_cast<const fn*>(at + 2 * D);
-      x += u * a - v * c;
+  for (int s0 = w; s0 < p.splits; s0 += kAtOnce * kJoinWaves) {
+    fn u[kAtOnce], v[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float* at = src + (int64_t)min(s0 + i * kJoinWaves, p.splits - 1) * p.R * (4 * D);
+      u[i] = *reinterpret_cast<const fn*>(at);
+      v[i] = *reinterpret_cast<const fn*>(at + 2 * D);
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int s = s0 + i * kJoinWaves;
+      if (s < p.splits) {
+        const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w1), s));
+        const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w2), s));
+        x += u[i] * a - v[i] * c;
+      }
     }
   }
   part[w][lane] = x;
@@ -692,22 +702,27 @@ struct Plan {
   int blocks, splits;
 };
 
-// Rows per workgroup and grid splits: the least estimate of
+// Rows per workgroup and grid splits: the least estimate (us) of
 //
-//   3 us + turns * (ends + rounds * (alone + more * running)) + what a split costs
+//   turns (ends + rounds (alone + more running)) + what a split costs
 //
-// where a CU runs up to `fit` workgroups at once and takes `turns` turns, a
-// workgroup's rounds are its steps over its key groups, and a split adds the
-// joining launch of 4 us and its partial results, written and read at 4 TB/s.
-// Constants from timings of 1 to 1200 workgroups and 1 to 150 rounds.
+// where a CU runs up to `fit` workgroups at once, so that its share of them takes
+// full turns and one with the rest, `running` is what a turn holds, and a workgroup's
+// rounds are its steps over its key groups.  A split adds the joining launch, its walk
+// over the parts, and the partial results, written and read.  (A launch's own
+// share is the same for every choice.)  Constants fitted to 4700 shapes of 1 to
+// 32 items, 1 to 5000 queries and 32 to 8000 keys, each timed in every choice: on
+// average 1.0% (D 64) and 1.8% (D 128) over the best choice, 24% at most; causal
+// calls, whose blocks differ, 1.2% and 1.9%.  (Counting every turn as full, and
+// splits at half their cost, it was 7.5% and 5.7%, twice the best at worst.)
 Plan search(int B, int Hk, int R, int S, int D, int cus) {
   static const struct {
     int dim, rows, groups, fit;
-    double ends, alone, more;
-  } kinds[] = {{64, 32, 2, 2, 3.2, 0.37, 0.2},
-               {64, 64, 1, 3, 3.2, 0.25, 0.28},
-               {128, 32, 2, 1, 5.0, 0.0, 1.1},
-               {128, 64, 1, 2, 5.0, 1.1, 0.12}};
+    double ends, alone, more, join, part, bytes;   // bytes: per us of the partial results' traffic
+  } kinds[] = {{64, 32, 2, 2, 2.7, 0.2, 0.47, 2.0, 0.05, 2.64e6},
+               {64, 64, 1, 3, 2.4, 0.275, 0.15, 2.0, 0.05, 2.64e6},
+               {128, 32, 2, 1, 4.15, 0.33, 1.17, 1.5, 0.04, 3.5e6},
+               {128, 64, 1, 2, 4.0, 0.65, 0.4, 1.5, 0.04, 3.5e6}};
   const int64_t heads = (int64_t)B * Hk;
   const int steps = (S + kStep - 1) / kStep;
   Plan best{};
@@ -715,13 +730,14 @@ Plan search(int B, int Hk, int R, int S, int D, int cus) {
   for (const auto& k : kinds) {
     if (k.dim != D) continue;
     const int blocks = (R + k.rows - 1) / k.rows;
-    for (int s = 1; s <= kMaxGridSplits && (s == 1 || s * k.groups <= steps); ++s) {
+    for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, kMaxGridSplits}) {
       const int64_t load = (heads * blocks * s + cus - 1) / cus;   // workgroups of the busiest CU
-      if (s > 1 && load > 2 * k.fit) break;
-      const double turns = (double)((load + k.fit - 1) / k.fit), running = (double)(load < k.fit ? load : k.fit);
+      if (s > 1 && (s * k.groups > steps || load > 6)) break;
       const int rounds = (steps + k.groups * s - 1) / (k.groups * s);
-      double us = 3 + turns * (k.ends + rounds * (k.alone + k.more * running));
-      if (s > 1) us += 4 + (double)heads * R * s * (4 * D) * 8 / 4e6;
+      const int64_t full = load / k.fit, rest = load % k.fit;
+      double us = (double)full * (k.ends + rounds * (k.alone + k.more * k.fit));
+      if (rest > 0) us += k.ends + rounds * (k.alone + k.more * (double)rest);
+      if (s > 1) us += k.join + k.part * s + (double)heads * R * s * (4 * D) * 8 / k.bytes;
       if (best.rows == 0 || us < best_us) best = Plan{k.rows, blocks, s}, best_us = us;
     }
   }
