@@ -29,12 +29,13 @@
 // row block's steps can be split again, each part leaving (max, sum, O) of both maps
 // in fp32 for a joining launch.
 //
-// Two forms: 64 rows on one ring for prompts, 32 rows on two rings for few rows.
+// Two forms: 64 rows on one ring, and 32 rows for few (D 64: on two rings of every
+// other step, which one workgroup's latency hides; D 128: on one, two workgroups a CU).
 // Measured (D 64, fp16 or bf16, whole calls in a graph):
 //   1 x 8 heads x 4800 x 4800        167 us, 846 TFLOP/s (a large matrix product: 1330)
 //   3 x 8 heads (2 key heads) x 1037, D 128, ragged, causal   43 us
-//   32 x 16 heads (4 key heads) x 1 x 6000, ragged   42 us, 4.7 TB/s (a large copy: 5.0)
-//   1 x 8 heads x 1 x 4800           12 us, two launches
+//   32 x 16 heads (4 key heads) x 1 x 6000, ragged   42 us, 4.8 TB/s (a large copy: 5.0)
+//   1 x 8 heads x 1 x 4800           10.6 us, two launches
 // Prompts are bound by the vector unit's exponentials and roundings beside the
 // matrix core (16 exponentials per two 32x32x16 score products and four value
 // products), and by whole workgroups: 600 on 256 CUs are three on the busiest.
@@ -192,8 +193,8 @@ struct Shape {
 
 // kFine: probabilities as two summands of the type, the rounded value and what the
 // rounding left, so that only the output is rounded.  For few rows, where memory and
-// latency leave the matrix cores idle (32 x 1 against 6000 42.4 us, of single
-// probabilities 41.0; 1 x 1 against 4800 12.0 and 11.4).  Prompts round once, as
+// latency leave the matrix cores idle (32 x 1 against 6000 41.9 us, with single
+// probabilities 40.3; 1 x 1 against 4800 11.0 and 10.4).  Prompts round once, as
 // flexrel's do: each probability off by half a step of itself, in sum about what
 // rounding the output costs; a second summand would be two thirds more matrix work.
 template <typename E, int D, int RB, int KS, bool kFine, int kMinWaves>
@@ -710,25 +711,26 @@ struct Plan {
 // full turns and one with the rest, `running` is what a turn holds, and a workgroup's
 // rounds are its steps over its key groups.  A split adds the joining launch, its walk
 // over the parts, and the partial results, written and read.  (A launch's own
-// share is the same for every choice.)  Constants fitted to 4700 shapes of 1 to
-// 32 items, 1 to 5000 queries and 32 to 8000 keys, each timed in every choice: on
-// average 1.0% (D 64) and 1.8% (D 128) over the best choice, 24% at most; causal
-// calls, whose blocks differ, 1.2% and 1.9%.  (Counting every turn as full, and
-// splits at half their cost, it was 7.5% and 5.7%, twice the best at worst.)
+// share is the same for every choice.)  Constants fitted to 7700 shapes of 1 to
+// 32 items, 1 to 5000 queries and 32 to 8000 keys, each timed in every choice, causal
+// ones too, whose blocks differ: on average within 1% of the best choice, 24% at
+// most.  (Counting every turn as full, and splits at half their cost, it was 7%,
+// twice the best at worst.)  A single block of rows takes the 32-row form, whose
+// probabilities keep two summands: 2 to 4% over the other's time at its best.
 Plan search(int B, int Hk, int R, int S, int D, int cus) {
   static const struct {
     int dim, rows, groups, fit;
     double ends, alone, more, join, part, bytes;   // bytes: per us of the partial results' traffic
   } kinds[] = {{64, 32, 2, 2, 2.7, 0.2, 0.47, 2.0, 0.05, 2.64e6},
                {64, 64, 1, 3, 2.4, 0.275, 0.15, 2.0, 0.05, 2.64e6},
-               {128, 32, 2, 1, 4.15, 0.33, 1.17, 1.5, 0.04, 3.5e6},
-               {128, 64, 1, 2, 4.0, 0.65, 0.4, 1.5, 0.04, 3.5e6}};
+               {128, 32, 1, 2, 4.05, 0.32, 0.83, 1.75, 0.04, 4.6e6},
+               {128, 64, 1, 2, 6.5, 0.57, 0.24, 1.75, 0.04, 4.6e6}};
   const int64_t heads = (int64_t)B * Hk;
   const int steps = (S + kStep - 1) / kStep;
   Plan best{};
   double best_us = 0;
   for (const auto& k : kinds) {
-    if (k.dim != D) continue;
+    if (k.dim != D || (R <= kBlock && k.rows != kBlock)) continue;
     const int blocks = (R + k.rows - 1) / k.rows;
     for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, kMaxGridSplits}) {
       const int64_t load = (heads * blocks * s + cus - 1) / cus;   // workgroups of the busiest CU
@@ -804,7 +806,7 @@ void launch(const DiffParams& p, int D, int rows, hipStream_t stream) {
     }
   } else {
     if (rows == kBlock) {
-      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 1, 2, true, 1>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((diff_attn_kernel<E, 128, 1, 1, true, 1>), grid, dim3(128), 0, stream, p);
     } else {
       hipLaunchKernelGGL((diff_attn_kernel<E, 128, 2, 1, false, 2>), grid, dim3(256), 0, stream, p);
     }
