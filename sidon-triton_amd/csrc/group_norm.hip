@@ -560,14 +560,20 @@ void run(Params& p, bool vector, hipStream_t stream) {
   constexpr int V = 16 / sizeof(T);
   const int cg = p.C / p.G;
   const int64_t vecs = (int64_t)p.T * (cg / V);
-  // A workgroup takes about 3.5 us + 0.085 us/KB for its slab (fp16, SiLU; the
-  // CU's own rate), the two passes 10.5 us + 0.6 us/MB for the whole tensor, so
-  // a large slab pays only where many of them run at once.  us, slab | passes:
-  // 1 x 500 x 32 channels a group 6.0 | 11.5, 1 x 1463 x 32 10.7 | 11.7, 1 x 1463 x
+  // A workgroup takes about 3.5 us + 0.085 us/KB for its slab (fp16, SiLU: the CU's
+  // own arithmetic; less without an activation, more with GELU and where a group's
+  // row is one vector of a cache line), the two passes 10.5 us + 0.6 us/MB for the whole
+  // tensor, so a large slab pays only where many of them run at once.  us, slab |
+  // passes: 1 x 500 x 32 channels a group 6.0 | 11.5, 1 x 1463 x 32 10.7 | 11.7, 1 x 1463 x
   // 64 18.5 | 12.0, 8 x 1500 x 64 21.5 | 25.8, fp32 1 x 1463 x 32 18.0 | 12.5, 4 x
-  // 1463 x 32 21.0 | 22.7, 8 x 1500 x 32 25.6 | 34.5.
+  // 1463 x 32 21.0 | 22.7, 8 x 1500 x 32 25.6 | 34.5; fp32 4 x 13 x 2048 without
+  // activation 7.4 | 11.9, fp16 GELU 8 x 7985 x 8 23.5 | 14.5.  Fitted to 13000
+  // shapes in both ways: 0.1% over the better one on average (without the
+  // weights 0.6%).
   const double slab_kb = vecs * 16.0 / 1024, all_mb = slab_kb * p.B * p.G / 1024;
-  if (vector && cg % V == 0 && vecs <= kSlabVecs * kSlabThreads && slab_kb <= 80 + 6 * all_mb &&
+  const bool plain = p.act == SIDON_ACT_NONE || p.act == SIDON_ACT_RELU;
+  const double weight = (plain ? (sizeof(T) == 4 ? 0.65 : 0.8) : p.act == SIDON_ACT_GELU ? 1.33 : 1.0) * (cg == V ? 1.25 : 1.0);
+  if (vector && cg % V == 0 && vecs <= kSlabVecs * kSlabThreads && slab_kb * weight <= 85 + 4.2 * all_mb &&
       (int64_t)p.B * p.G <= INT32_MAX / kSlabThreads) {   // (a launch holds less than 2^32 threads)
     slab<T>(p, vecs, stream);
   } else if (vector) {
