@@ -477,7 +477,6 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
           acc_t t[IN];
 #pragma unroll
           for (int j = 0; j < IN; ++j) t[j] = acc_t{};
-#pragma unroll 2
           for (int r0 = 0; r0 < p.rank; r0 += kW) {
             const int c = (r0 >> 3) + lg, at = (c ^ mixed) << 4;
             h8 u[IN];
@@ -536,7 +535,6 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
             acc_t t[IN];
 #pragma unroll
             for (int j = 0; j < IN; ++j) t[j] = acc_t{};
-#pragma unroll 2
             for (int r0 = 0; r0 < p.rank; r0 += kW) {
               const int r = r0 + 8 * lg;
               h8 u[IN];
