@@ -106,6 +106,21 @@ ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "relu": 3}
 _lib = None
 
 
+class Layouts(dict):
+    """What a call's checks found for operands of one layout (their shapes,
+    strides, types and devices, which the key holds all of, and nothing of what
+    they contain): the next call of the same layout skips them, half of a small
+    call's time on the host.  Emptied when full."""
+
+    MOST = 1024
+
+    def keep(self, key: tuple, found: tuple) -> tuple:
+        if len(self) >= self.MOST:
+            self.clear()
+        self[key] = found
+        return found
+
+
 class SidonError(RuntimeError):
     """A nonzero return code of the C ABI."""
 

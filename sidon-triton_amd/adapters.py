@@ -65,7 +65,20 @@ def stack_adapters(pairs):
     return torch.cat([a for a, _ in pairs]), torch.block_diag(*[b for _, b in pairs])
 
 
-def _operands(x, w, a, b, scale, ids):
+_layouts = _lib.Layouts()
+
+
+def _operands(x, w, a, b, scale, ids, bias, residual: bool) -> tuple:
+    """-> (rows, n, strides of x and w, the sizes behind them in a call, type code,
+    workspace bytes) of operands that fit."""
+    key = (x.shape, x.stride(), x.dtype, x.device, w.shape, w.stride(), w.dtype, w.device, a.shape, a.stride(), a.dtype,
+           a.device, b.shape, b.stride(), b.dtype, b.device, scale.shape, scale.stride(), scale.dtype, scale.device,
+           ids.shape, ids.stride(), ids.dtype, ids.device,
+           None if bias is None else (bias.shape, bias.stride(), bias.dtype, bias.device), residual)
+    return _layouts.get(key) or _layouts.keep(key, _check(x, w, a, b, scale, ids, bias, residual))
+
+
+def _check(x, w, a, b, scale, ids, bias, residual):
     device = x.device
     _check_device_tensor("x", x, device)
     for name, t in (("x", x), ("w", w), ("a", a), ("b", b)):
@@ -93,7 +106,13 @@ def _operands(x, w, a, b, scale, ids):
         raise ValueError("ids must be a contiguous int32 [items] tensor")
     if rows < 1 or rows % ids.numel():
         raise ValueError(f"{rows} rows do not split into {ids.numel()} items")
-    return rows, n, k
+    if bias is not None:
+        if bias.device != device:
+            _check_device_tensor("bias", bias, device)
+        if bias.dtype != x.dtype or bias.shape != (n,) or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous {x.dtype} [{n}] tensor")
+    return (rows, n, _row_stride(x), _row_stride(w), (rows, n, k, a.shape[1], a.shape[0], ids.numel()),
+            _lib.DTYPES[x.dtype], workspace_bytes(rows, a.shape[1], residual, x.dtype))
 
 
 def _workspace(workspace, need, device):
@@ -118,31 +137,27 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, 
     64, R of 8 up to 128.  Sums in fp32, scale (x A_e^T) rounded to x's type.  Rows of x, w and out
     may be strided.  workspace: a contiguous uint8 tensor of ``workspace_bytes``.
     Forward only."""
-    rows, n, k = _operands(x, w, a, b, scale, ids)
+    rows, n, ldx, ldw, sizes, dtype, need = _operands(x, w, a, b, scale, ids, bias, False)
     device = x.device
-    if bias is not None:
-        if bias.device != device:
-            _check_device_tensor("bias", bias, device)
-        if bias.dtype != x.dtype or bias.shape != (n,) or not bias.is_contiguous():
-            raise ValueError(f"bias must be a contiguous {x.dtype} [{n}] tensor")
     if act not in (None, "silu"):
         raise ValueError(f"act must be None or 'silu' (got {act!r})")
     if not (plain(x, w, a, b, scale) if bias is None else plain(x, w, a, b, scale, bias)):
         raise ValueError("adapter_linear has no backward: call it under torch.no_grad()")
     if out is None:
         out = torch.empty(rows, n, device=device, dtype=x.dtype)
+        ldy = n
     else:
         _check_device_tensor("out", out, device)
         if out.dtype != x.dtype or out.shape != (rows, n) or out.stride(1) != 1:
             raise ValueError(f"out must be a {x.dtype} [{rows}, {n}] tensor with rows contiguous")
-    workspace = _workspace(workspace, workspace_bytes(rows, a.shape[1], False, x.dtype), device)
+        ldy = _row_stride(out)
+    workspace = _workspace(workspace, need, device)
     lib = _lib.load()
     with _on_device(device):
         rc = lib.sidon_adapter_linear(
-            x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), None if bias is None else bias.data_ptr(),
-            a.data_ptr(), b.data_ptr(), scale.data_ptr(), ids.data_ptr(), out.data_ptr(), _row_stride(out),
-            workspace.data_ptr(), workspace.numel(), rows, n, k, a.shape[1], a.shape[0], ids.numel(),
-            _lib.ACTIVATIONS[act], _lib.DTYPES[x.dtype], _stream_handle(device))
+            x.data_ptr(), ldx, w.data_ptr(), ldw, None if bias is None else bias.data_ptr(), a.data_ptr(), b.data_ptr(),
+            scale.data_ptr(), ids.data_ptr(), out.data_ptr(), ldy, workspace.data_ptr(), workspace.numel(), *sizes,
+            _lib.ACTIVATIONS[act], dtype, _stream_handle(device))
     if rc:
         _lib.check("sidon_adapter_linear", rc)
     return out
@@ -154,7 +169,7 @@ def adapter_residual(y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, a: torch
     """y + x W^T + scale_e (x A_e^T) B_e^T into the fp32 stream y [M, N], in place
     or, with ``out`` fp32 [M, N], beside it; the other arguments as for
     ``adapter_linear``.  The low-rank term keeps fp32 accuracy."""
-    rows, n, k = _operands(x, w, a, b, scale, ids)
+    rows, n, ldx, ldw, sizes, dtype, need = _operands(x, w, a, b, scale, ids, None, True)
     device = x.device
     out = y if out is None else out
     for name, t in (("y", y), ("out", out)):
@@ -163,14 +178,13 @@ def adapter_residual(y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, a: torch
             raise ValueError(f"{name} must be a float32 [{rows}, {n}] tensor with rows contiguous")
     if not plain(y, x, w, a, b, scale):
         raise ValueError("adapter_residual has no backward: call it under torch.no_grad()")
-    workspace = _workspace(workspace, workspace_bytes(rows, a.shape[1], True, x.dtype), device)
+    workspace = _workspace(workspace, need, device)
     lib = _lib.load()
     with _on_device(device):
         rc = lib.sidon_adapter_residual(
-            x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w), a.data_ptr(), b.data_ptr(), scale.data_ptr(),
-            ids.data_ptr(), y.data_ptr(), _row_stride(y), out.data_ptr(), _row_stride(out), workspace.data_ptr(),
-            workspace.numel(), rows, n, k, a.shape[1], a.shape[0], ids.numel(), _lib.DTYPES[x.dtype],
-            _stream_handle(device))
+            x.data_ptr(), ldx, w.data_ptr(), ldw, a.data_ptr(), b.data_ptr(), scale.data_ptr(), ids.data_ptr(),
+            y.data_ptr(), _row_stride(y), out.data_ptr(), _row_stride(out), workspace.data_ptr(), workspace.numel(),
+            *sizes, dtype, _stream_handle(device))
     if rc:
         _lib.check("sidon_adapter_residual", rc)
     return out

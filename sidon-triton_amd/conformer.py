@@ -123,6 +123,34 @@ def glu_causal_dw_norm(h: torch.Tensor, batch: int, dwt: torch.Tensor, ln_w: tor
     return _dw(h, True, batch, dwt, ln_w, ln_b, eps, out)
 
 
+_norm_layouts = _lib.Layouts()
+
+
+def _check_group_norm(x, batch, groups, w, b, lens) -> tuple:
+    """-> (rows, channels, row stride, type code, workspace bytes) of operands that fit."""
+    device = x.device
+    _check_device_tensor("x", x, device)
+    if x.dtype not in _lib.DTYPES or x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError("x must be a float16, bfloat16 or float32 [R, C] tensor with channels contiguous")
+    rows, c = x.shape
+    if batch < 1 or rows < 1 or rows % batch:
+        raise ValueError(f"{rows} rows do not split into {batch} items")
+    if groups < 1 or c % groups:
+        raise ValueError(f"{c} channels do not split into {groups} groups")
+    for name, t in (("w", w), ("b", b)):
+        if t.device != device:
+            _check_device_tensor(name, t, device)
+        if t.dtype != torch.float32 or t.shape != (c,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 [{c}] tensor")
+    if lens is not None:
+        if lens.device != device:
+            _check_device_tensor("lens", lens, device)
+        if lens.dtype != torch.int32 or lens.shape != (batch,) or not lens.is_contiguous():
+            raise ValueError("lens must be a contiguous int32 tensor of shape [B]")
+    return (rows, c, _row_stride(x), _lib.DTYPES[x.dtype],
+            max(group_norm_workspace(batch, rows // batch, c, groups, x.dtype), 8))
+
+
 def group_norm_act(x: torch.Tensor, batch: int, groups: int, w: torch.Tensor, b: torch.Tensor, eps: float = 1e-5,
                    lens: torch.Tensor | None = None, act: str | None = "silu", out: torch.Tensor | None = None,
                    workspace: torch.Tensor | None = None) -> torch.Tensor:
@@ -136,50 +164,35 @@ def group_norm_act(x: torch.Tensor, batch: int, groups: int, w: torch.Tensor, b:
     they hold, and come back as zeros.  act: None, "silu", "gelu" (the erf form)
     or "relu".  out may be x itself.  workspace: a contiguous uint8 tensor of
     ``group_norm_workspace`` bytes; allocated per call when None.  Forward only."""
+    key = (x.shape, x.stride(), x.dtype, x.device, w.shape, w.stride(), w.dtype, w.device, b.shape, b.stride(), b.dtype,
+           b.device, None if lens is None else (lens.shape, lens.stride(), lens.dtype, lens.device), batch, groups)
+    rows, c, ldx, dtype, need = (
+        _norm_layouts.get(key) or _norm_layouts.keep(key, _check_group_norm(x, batch, groups, w, b, lens)))
     device = x.device
-    _check_device_tensor("x", x, device)
-    if x.dtype not in _lib.DTYPES or x.dim() != 2 or x.stride(1) != 1:
-        raise ValueError("x must be a float16, bfloat16 or float32 [R, C] tensor with channels contiguous")
-    rows, c = x.shape
-    if batch < 1 or rows < 1 or rows % batch:
-        raise ValueError(f"{rows} rows do not split into {batch} items")
-    if groups < 1 or c % groups:
-        raise ValueError(f"{c} channels do not split into {groups} groups")
     if act not in _lib.ACTIVATIONS:
         raise ValueError(f"act must be one of {list(_lib.ACTIVATIONS)} (got {act!r})")
-    for name, t in (("w", w), ("b", b)):
-        if t.device != device:
-            _check_device_tensor(name, t, device)
-        if t.dtype != torch.float32 or t.shape != (c,) or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous float32 [{c}] tensor")
-    if lens is not None:
-        if lens.device != device:
-            _check_device_tensor("lens", lens, device)
-        if lens.dtype != torch.int32 or lens.shape != (batch,) or not lens.is_contiguous():
-            raise ValueError("lens must be a contiguous int32 tensor of shape [B]")
     if not plain(x, w, b):
         raise ValueError("group_norm_act has no backward: call it under torch.no_grad()")
     if out is None:
         out = torch.empty(rows, c, device=device, dtype=x.dtype)
+        ldy = c
     else:
         _check_device_tensor("out", out, device)
         if out.dtype != x.dtype or out.shape != (rows, c) or out.stride(1) != 1:
             raise ValueError(f"out must be a {x.dtype} [{rows}, {c}] tensor with channels contiguous")
-    lib = _lib.load()
-    dtype = _lib.DTYPES[x.dtype]
+        ldy = _row_stride(out)
     if workspace is None:
-        need = lib.sidon_group_norm_workspace_bytes(batch, rows // batch, c, groups, dtype)
-        workspace = torch.empty(max(need, 8), device=device, dtype=torch.uint8)
+        workspace = torch.empty(need, device=device, dtype=torch.uint8)
     else:
         _check_device_tensor("workspace", workspace, device)
-        need = lib.sidon_group_norm_workspace_bytes(batch, rows // batch, c, groups, dtype)
         if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
             raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
+    lib = _lib.load()
     with _on_device(device):
-        rc = lib.sidon_group_norm_act(x.data_ptr(), _row_stride(x), None if lens is None else lens.data_ptr(),
-                                      w.data_ptr(), b.data_ptr(), eps, out.data_ptr(),
-                                      _row_stride(out), workspace.data_ptr(), workspace.numel(), batch, rows // batch,
-                                      c, groups, dtype, _lib.ACTIVATIONS[act], _stream_handle(device))
+        rc = lib.sidon_group_norm_act(x.data_ptr(), ldx, None if lens is None else lens.data_ptr(), w.data_ptr(),
+                                      b.data_ptr(), eps, out.data_ptr(), ldy, workspace.data_ptr(), workspace.numel(),
+                                      batch, rows // batch, c, groups, dtype, _lib.ACTIVATIONS[act],
+                                      _stream_handle(device))
     if rc:
         _lib.check("sidon_group_norm_act", rc)
     return out

@@ -46,25 +46,12 @@ def _strides(t: torch.Tensor) -> ctypes.Array:
     return _int64s(st)
 
 
-def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, lam_init: float,
-                   lens: torch.Tensor | None = None, causal: bool = False, norm_w: torch.Tensor | None = None,
-                   eps: float = 1e-5, out: torch.Tensor | None = None,
-                   workspace: torch.Tensor | None = None) -> torch.Tensor:
-    """q [B, H, 2, L, D], k [B, Hk, 2, S, D], v [B, Hk, S, 2D] fp16 or bf16 ->
-    [B, H, L, 2D] of their type.
+_layouts = _lib.Layouts()
 
-    Any strides that are multiples of 8 elements with the last dimension
-    contiguous (views of fused projections or of a cache), D 64 or 128.  H / Hk
-    neighbouring heads share a key head.  lam fp32 [4, D] (lq1, lk1, lq2, lk2) or
-    [H, 4, D].  lens: int32 [B] valid keys on the device (None: all S); what lies
-    past them is not read.  causal: the L queries are the last L of an item's
-    valid positions, query i sees the keys up to its own.  A query without keys
-    gives zeros.  norm_w fp32 [2D]: each head's output is divided by its root
-    mean square (with eps > 0 under the root) and multiplied by (1 - lam_init)
-    norm_w; None: left as it is.  out: optional [B, H, L, 2D], in memory apart from
-    q, k and v.  workspace: a contiguous
-    uint8 tensor of ``workspace_bytes``; allocated per call when None.  A single
-    query against a long cache splits the keys over the chip.  Forward only."""
+
+def _check(q, k, v, lam, lens, norm_w) -> tuple:
+    """-> (sizes, the output's shape, workspace bytes, heads of lam, type code,
+    strides of q, k and v, strides of a contiguous output) of operands that fit."""
     if q.dim() != 5 or k.dim() != 5 or v.dim() != 4:
         raise ValueError("q and k must be [B, heads, 2, length, D], v [B, heads, length, 2D]")
     batch, heads, two, length, dim = q.shape
@@ -102,18 +89,49 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
             _check_device_tensor("norm_w", norm_w, device)
         if norm_w.dtype != torch.float32 or norm_w.shape != (2 * dim,) or not norm_w.is_contiguous():
             raise ValueError(f"norm_w must be a contiguous float32 [{2 * dim}] tensor")
+    sizes, shape = (batch, heads, kv_heads, length, keys, dim), (batch, heads, length, 2 * dim)
+    o_strides = _strides(torch.empty(shape, device="meta"))
+    return (sizes, shape, workspace_bytes(*sizes, device), 1 if lam.dim() == 2 else heads, _lib.DTYPES[q.dtype],
+            (_strides(q), _strides(k), _strides(v)), o_strides)
+
+
+def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, lam_init: float,
+                   lens: torch.Tensor | None = None, causal: bool = False, norm_w: torch.Tensor | None = None,
+                   eps: float = 1e-5, out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """q [B, H, 2, L, D], k [B, Hk, 2, S, D], v [B, Hk, S, 2D] fp16 or bf16 ->
+    [B, H, L, 2D] of their type.
+
+    Any strides that are multiples of 8 elements with the last dimension
+    contiguous (views of fused projections or of a cache), D 64 or 128.  H / Hk
+    neighbouring heads share a key head.  lam fp32 [4, D] (lq1, lk1, lq2, lk2) or
+    [H, 4, D].  lens: int32 [B] valid keys on the device (None: all S); what lies
+    past them is not read.  causal: the L queries are the last L of an item's
+    valid positions, query i sees the keys up to its own.  A query without keys
+    gives zeros.  norm_w fp32 [2D]: each head's output is divided by its root
+    mean square (with eps > 0 under the root) and multiplied by (1 - lam_init)
+    norm_w; None: left as it is.  out: optional [B, H, L, 2D], in memory apart from
+    q, k and v.  workspace: a contiguous
+    uint8 tensor of ``workspace_bytes``; allocated per call when None.  A single
+    query against a long cache splits the keys over the chip.  Forward only."""
+    key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype,
+           v.device, lam.shape, lam.stride(), lam.dtype, lam.device,
+           None if lens is None else (lens.shape, lens.stride(), lens.dtype, lens.device),
+           None if norm_w is None else (norm_w.shape, norm_w.stride(), norm_w.dtype, norm_w.device))
+    sizes, shape, need, lam_heads, dtype, strides, o_strides = (
+        _layouts.get(key) or _layouts.keep(key, _check(q, k, v, lam, lens, norm_w)))
+    device = q.device
     if not (plain(q, k, v, lam) if norm_w is None else plain(q, k, v, lam, norm_w)):
         raise ValueError("diff_attention has no backward: call it under torch.no_grad()")
-    shape = (batch, heads, length, 2 * dim)
     if out is None:
         out = torch.empty(shape, device=device, dtype=q.dtype)
     else:
         _check_device_tensor("out", out, device)
         if out.dtype != q.dtype or tuple(out.shape) != shape or out.stride(-1) != 1:
             raise ValueError(f"out must be a {q.dtype} {shape} tensor with a contiguous last dimension")
+        o_strides = _strides(out)
     lib = _lib.load()
     with _on_device(device):
-        need = lib.sidon_diff_attention_workspace_bytes(batch, heads, kv_heads, length, keys, dim)
         if workspace is None:
             workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
         else:
@@ -121,11 +139,10 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
             if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
                 raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
         rc = lib.sidon_diff_attention(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), 1 if lam.dim() == 2 else heads, lam_init,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), lam_heads, lam_init,
             None if lens is None else lens.data_ptr(), None if norm_w is None else norm_w.data_ptr(), eps,
             out.data_ptr(), None if workspace is None else workspace.data_ptr(),
-            0 if workspace is None else workspace.numel(), batch, heads, kv_heads, length, keys, dim,
-            1 if causal else 0, _lib.DTYPES[q.dtype], _strides(q), _strides(k), _strides(v), _strides(out),
+            0 if workspace is None else workspace.numel(), *sizes, 1 if causal else 0, dtype, *strides, o_strides,
             _stream_handle(device))
     if rc:
         _lib.check("sidon_diff_attention", rc)

@@ -204,3 +204,48 @@ def test_two_streams_and_threads_at_once(sidon):
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_calls_of_other_layouts_are_checked_again(sidon):
+    """What one call's checks found serves only calls of the same shapes,
+    strides, types and devices."""
+    x, w, b = norm_test.inputs(64, 128, torch.float16, 2)
+    lens = torch.tensor([20, 32], dtype=torch.int32, device=DEV)
+    norm = sidon.conformer.group_norm_act
+    want = norm(x, 2, 4, w, b, lens=lens)
+    wide = torch.zeros(64, 192, dtype=torch.float16, device=DEV)
+    wide[:, 32:160] = x
+    assert torch.equal(norm(wide[:, 32:160], 2, 4, w, b, lens=lens), want)
+    for bad in (lens.long(), lens[:1], lens.cpu(), torch.stack([lens, lens], 1)[:, 0]):
+        with pytest.raises(ValueError):
+            norm(x, 2, 4, w, b, lens=bad)
+    for bad in (w.half(), w[:64], w.cpu(), torch.stack([w, w], 1)[:, 0]):
+        with pytest.raises(ValueError):
+            norm(x, 2, 4, bad, b, lens=lens)
+    with pytest.raises(ValueError):
+        norm(x, 2, 5, w, b, lens=lens)
+    with pytest.raises(ValueError):
+        norm(x.t(), 2, 4, w, b, lens=lens)
+    assert torch.equal(norm(x, 2, 4, w, b, lens=lens), want)
+
+    s = adapters_test.inputs(6, 3, 128, 64, 8, 2, torch.float16, 3)
+    want = adapters_test.linear(sidon, s)
+    for name, bad in (("x", s["x"].float()), ("w", s["w"].bfloat16()), ("scale", s["scale"].double()),
+                      ("ids", s["ids"].long()), ("a", s["a"].transpose(1, 2)), ("bias", s["bias"][:64]),
+                      ("ids", s["ids"][:4]), ("b", s["b"][:1]), ("w", s["w"].cpu())):
+        with pytest.raises((ValueError, TypeError)):
+            adapters_test.linear(sidon, {**s, name: bad})
+    assert torch.equal(adapters_test.linear(sidon, s), want)
+
+    q, k, v, lam, norm_w = attention_test.inputs(2, 4, 2, 3, 50, 64, torch.float16, 7)
+    call = sidon.diff_attention.diff_attention
+    want = call(q, k, v, lam, 0.3, norm_w=norm_w)
+    assert torch.equal(call(q.contiguous(), k, v.contiguous(), lam, 0.3, norm_w=norm_w), want)
+    out = torch.zeros(2, 3, 4, 128, dtype=torch.float16, device=DEV)
+    assert torch.equal(call(q, k, v, lam, 0.3, norm_w=norm_w, out=out.transpose(1, 2)), want)
+    assert torch.equal(call(q, k, v, lam, 0.3, norm_w=norm_w), want)
+    for bad in (dict(q=q.float()), dict(k=k[..., :32]), dict(v=v[:1]), dict(lam=lam.half()), dict(lam=lam[:3]),
+                dict(norm_w=norm_w[:64]), dict(k=k.cpu()), dict(v=v.bfloat16())):
+        a = {"q": q, "k": k, "v": v, "lam": lam, "lam_init": 0.3, "norm_w": norm_w, **bad}
+        with pytest.raises((ValueError, TypeError)):
+            call(**a)

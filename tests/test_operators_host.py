@@ -204,3 +204,11 @@ def test_encoder_adapters_of_the_largest_rank(sidon):
     assert tuple(a.shape) == (2, 128, 64) and tuple(b.shape) == (2, 192, 128) and scale.tolist() == [1.0, 2.0]
     assert (a[0] == 1).all() and (b[0, 64:128] == 1).all() and b[0].sum() == 64 * 128 and not b[1].any()
     assert not packed_set[0]["out_w"][1][0].any()
+
+
+def test_layouts_are_bounded(sidon):
+    kept = sidon._lib.Layouts()
+    for i in range(3 * kept.MOST + 5):
+        assert kept.keep((i,), (i, "found")) == (i, "found") and kept.get((i,)) == (i, "found")
+        assert len(kept) <= kept.MOST
+    assert kept.get((0,)) is None
