@@ -11,6 +11,8 @@
 //
 // Rows of different adapters share tiles: the shared product does not see
 // them, and the low-rank terms cost a product per adapter among a block's rows.
+// Few rows are bound by the two launches' latencies, many by the shared product
+// (4800 x 4096 x 1024 0.74 PFLOP/s with the low-rank term, rank 64).
 #include "gemm_tile.h"
 
 #include "sidon_host.h"
@@ -167,10 +169,11 @@ struct ExpandKernel {
 
 // gemm.hip's shapes, half of them: what the rest would gain is small next to the
 // low-rank term.  us, of it the shrink launch, and the shared projection alone
-// (conformer.linear_silu_lt, residual_gemm): 1 x 1024 x 1024 rank 16 9.7 (2.4) | 5.8,
-// 48 rows of 48 adapters x 4096 x 1024 rank 16 12.7 (3.3) | 6.0, 4 x 400 x 2048 x 1024
-// rank 32 21 (4.8) | 12.3, 8 x 600 x 4096 x 1024 rank 64 64 (8.3) | 51-57, rank 16 56 |
-// 51, residual 3 x 1463 x 1024 x 4096 rank 16 58 (11) | 40.
+// (conformer.linear_silu_lt, residual_gemm): 1 x 1024 x 1024 rank 16 9.3 (2.5) | 5.8,
+// 48 rows of 43 adapters x 4096 x 1024 rank 16 12.6 (3.3) | 6.0, 4 x 400 x 2048 x 1024
+// rank 32 18.8 (4.7) | 12.3, 8 x 600 x 4096 x 1024 rank 64 59 (8.5) | 51-57, rank 16 56 |
+// 51, residual 3 x 1463 x 1024 x 4096 rank 16 56 (11) | 40.  The shared projection's
+// cost picks the tile: on 5000 calls, each timed with every tile, 1% over the best on average.
 const ExpandKernel kExpand[] = {
     SIDON_BOTH(32, 64, 2, 2, 16, 6),   SIDON_BOTH(64, 64, 2, 2, 16, 4),   SIDON_BOTH(64, 128, 2, 4, 16, 4),
     SIDON_BOTH(128, 128, 2, 4, 16, 4), SIDON_BOTH(192, 128, 2, 4, 16, 3), SIDON_HALF(128, 256, 2, 4, 16, 3),

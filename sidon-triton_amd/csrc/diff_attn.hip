@@ -65,6 +65,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 constexpr int kBlock = 32;          // rows per wavefront
 constexpr float kFloorMax = -1e30f; // a running maximum that no key has raised yet (finite: -inf - -inf is NaN)
 constexpr int kMaxGridSplits = 64;
+constexpr int kBack = 3 * 1024;     // bytes that the copies' offsets hold beyond their rows (dma_tile's last copy adds none)
 
 struct DiffParams {
   const void* q;
@@ -256,8 +257,8 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   const uint32_t ring = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem) + ks * C::kRing + wr * C::kCopies * 1024;
   const int pid0 = wr * C::kCopies / 4, crow = wr * C::kCopies % 4 * 8 + (lane >> 3);
   const char* const kbase = static_cast<const char*>(p.k) + 2 * (b * p.kb + hk * p.kh + pid0 / P * p.km) +
-                            pid0 % P * 128 - 3072;
-  const char* const vbase = static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh) + pid0 * 128 - 3072;
+                            pid0 % P * 128 - kBack;
+  const char* const vbase = static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh) + pid0 * 128 - kBack;
   const int whole = min(t1, lk / kStep);   // steps below it have all their rows
   // Copy j of a set adds 1024 j to the LDS and to the global address; copies of
   // the next panel (j >= 4) lie 128 bytes on.
