@@ -48,6 +48,11 @@ size_t sidon_group_norm_workspace_bytes(int B, int T, int C, int G, int dtype);
 int sidon_group_norm_act(const void* x, int64_t ldx, const int32_t* lens, const float* w, const float* bias, float eps,
                          void* y, int64_t ldy, void* ws, size_t ws_bytes, int B, int T, int C, int G, int dtype,
                          int act, sidon_stream_t stream);
+/* How the two-launch way cuts these sizes, with vectors of `vec` elements (16 bytes, or 1 where the tensors do
+ * not lie on them): groups per column block (the last block may have fewer), row chunks per item, and the LDS
+ * bytes of a workgroup of the first launch.  No GPU needed. */
+int sidon_group_norm_passes(int B, int T, int C, int G, int dtype, int vec, int* block_groups, int* chunks,
+                            int* lds_bytes);
 
 /*
  * A shared projection with a low-rank adapter per request.  For row m of

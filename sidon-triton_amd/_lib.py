@@ -82,6 +82,7 @@ SIGNATURES = {
     "sidon_stage_items": (ctypes.c_int, [_VP, ctypes.c_int64, _VP, ctypes.c_int64, _I64P, _VP, _IP, _VP, _IP,
                                          ctypes.c_int, _VP]),
     "sidon_group_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 5),
+    "sidon_group_norm_passes": (ctypes.c_int, [*[ctypes.c_int] * 6, _IP, _IP, _IP]),
     "sidon_group_norm_act": (ctypes.c_int, [_VP, ctypes.c_int64, _VP, _VP, _VP, ctypes.c_float, _VP, ctypes.c_int64,
                                             _VP, ctypes.c_size_t, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                             ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP]),

@@ -525,6 +525,19 @@ void plan_passes(Params& p, int vec) {
   p.apply_rows = split(kApplyWgs, 4, 65535);
 }
 
+// LDS of the statistics launch: the units of every thread that has a vector, in
+// the full column blocks or in a last, narrower one, which leaves the threads more
+// row lanes (33 vectors: 7 lanes, 231 threads; 3 vectors: 85 lanes, 255).
+size_t unit_bytes(const Params& p, int vec) {
+  const int cg = p.C / p.G;
+  const auto vectors = [&](int groups) {
+    const int nv = groups * cg / vec;
+    return nv < kThreads ? kThreads / nv * nv : nv;
+  };
+  const int full = vectors(p.block_groups), last = vectors(p.G - (p.G - 1) / p.block_groups * p.block_groups);
+  return (size_t)(full > last ? full : last) * (cg % vec == 0 ? 1 : vec) * sizeof(float2);
+}
+
 template <typename T, int NV, int TH>
 void slab_launch(const Params& p, hipStream_t stream) {
   hipLaunchKernelGGL((gn_slab_kernel<T, NV, TH>), dim3((unsigned)(p.B * p.G)), dim3(TH), 0, stream, p);
@@ -546,15 +559,13 @@ void slab(const Params& p, int64_t vecs, hipStream_t stream) {
 template <typename T, int V>
 void passes(const Params& p, hipStream_t stream) {
   const bool wide = (p.C / p.G) % V == 0;
-  const int nv = p.block_groups * (p.C / p.G) / V;
-  const int threads_used = nv < kThreads ? (kThreads / nv) * nv : nv;
-  const size_t unit_bytes = (size_t)threads_used * (wide ? 1 : V) * sizeof(float2);
+  const size_t units = unit_bytes(p, V);
   const unsigned blocks = (unsigned)((p.G + p.block_groups - 1) / p.block_groups);
   const dim3 grid((unsigned)p.chunks, (unsigned)p.B, blocks);
   if (wide) {
-    hipLaunchKernelGGL((gn_stat_kernel<T, V, true>), grid, dim3(kThreads), unit_bytes, stream, p);
+    hipLaunchKernelGGL((gn_stat_kernel<T, V, true>), grid, dim3(kThreads), units, stream, p);
   } else {
-    hipLaunchKernelGGL((gn_stat_kernel<T, V, false>), grid, dim3(kThreads), unit_bytes, stream, p);
+    hipLaunchKernelGGL((gn_stat_kernel<T, V, false>), grid, dim3(kThreads), units, stream, p);
   }
   hipLaunchKernelGGL((gn_apply_kernel<T, V>), 
                      dim3((unsigned)((p.T + p.apply_rows - 1) / p.apply_rows), (unsigned)p.B, blocks), dim3(kThreads),
@@ -602,6 +613,22 @@ SIDON_API size_t sidon_group_norm_workspace_bytes(int B, int T, int C, int G, in
   if (!shape_ok(B, T, C, G, dtype)) return 0;
   const int64_t chunks = T < kMaxChunks ? T : kMaxChunks;
   return (size_t)B * (size_t)chunks * (size_t)G * sizeof(float2);
+}
+
+SIDON_API int sidon_group_norm_passes(int B, int T, int C, int G, int dtype, int vec, int* block_groups, int* chunks,
+                                      int* lds_bytes) {
+  sidon::clear_error();
+  if (!block_groups || !chunks || !lds_bytes) return sidon::fail(SIDON_E_NULL, "the results must be non-NULL");
+  if (!shape_ok(B, T, C, G, dtype) || (vec != 1 && (vec != 16 / element_size(dtype) || C % vec != 0)))
+    return sidon::fail(SIDON_E_SHAPE, "B=%d T=%d C=%d G=%d dtype=%d vec=%d is no shape of sidon_group_norm_act", B, T, C,
+                       G, dtype, vec);
+  Params p{};
+  p.B = B, p.T = T, p.C = C, p.G = G;
+  plan_passes(p, vec);
+  *block_groups = p.block_groups;
+  *chunks = p.chunks;
+  *lds_bytes = (int)unit_bytes(p, vec);
+  return SIDON_OK;
 }
 
 SIDON_API int sidon_group_norm_act(const void* x, int64_t ldx, const int32_t* lens, const float* w, const float* bias,

@@ -87,6 +87,24 @@ def test_against_float64(sidon, shape, kind):
     check(y, want, scale, kind)
 
 
+# (items, frames, channels, groups, types): vectors that lie in two groups, and a last column block of fewer groups
+# than the others, whose threads have more row lanes than the full blocks' (the statistics' LDS has to hold them)
+NARROW_LAST = [(2, 1500, 352, 8, KINDS[1:]), (3, 1700, 416, 8, KINDS[1:]), (8, 4800, 480, 8, KINDS[1:]),
+               (1, 1463, 648, 6, KINDS[1:]), (1, 4800, 320, 32, KINDS[1:]), (2, 1500, 176, 8, KINDS[:1]),
+               (3, 1001, 208, 8, KINDS[:1]), (1, 1463, 240, 8, KINDS[:1]), (2, 700, 36, 12, KINDS)]
+
+
+@pytest.mark.parametrize("shape,kind", [(s[:4], k) for s in NARROW_LAST for k in s[4]], ids=str)
+def test_narrower_last_block(sidon, shape, kind):
+    batch, t, c, groups = shape
+    x, w, b = inputs(batch * t, c, kind, t + c)
+    lens = [(t, t - t // 3, 1, 17)[i % 4] for i in range(batch)]
+    x.view(batch, t, c)[torch.arange(t, device=DEV).view(1, t) >= torch.tensor(lens, device=DEV).view(batch, 1)] = float("nan")
+    y = sidon.conformer.group_norm_act(x, batch, groups, w, b, 1e-5, lens=torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                       act="silu")
+    check(y, *reference(x, batch, groups, w, b, 1e-5, lens, "silu"), kind)
+
+
 @pytest.mark.parametrize("act", [None, "silu", "gelu", "relu"])
 @pytest.mark.parametrize("kind", KINDS, ids=str)
 def test_activations(sidon, act, kind):

@@ -38,6 +38,34 @@ def test_group_norm_workspace(sidon):
         assert 0 < ws(*shape, torch.float32) <= 8 * shape[0] * shape[3] * min(128, shape[1])
 
 
+@pytest.mark.parametrize("dtype,vec", [(0, 4), (1, 8), (2, 8), (0, 1), (1, 1)])
+def test_group_norm_statistics_fit_their_lds(sidon, dtype, vec):
+    """Every column block's units, the last and narrower one's too, whose fewer
+    columns leave a workgroup of 256 threads more row lanes."""
+    lib = sidon._lib.load()
+    block, chunks, lds = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
+    short = 0
+    for c in sorted({*range(vec, 1400, vec), *range(2048, 8193, 8 * vec), 8184, 8192}):
+        for groups in range(1, min(c, 700) + 1):
+            if c % groups:
+                continue
+            assert lib.sidon_group_norm_passes(2, 1500, c, groups, dtype, vec, *map(ctypes.byref, (block, chunks, lds))) == 0
+            cg = c // groups
+            assert 1 <= block.value <= groups and 1 <= chunks.value <= 64 and lds.value <= 64 << 10
+            last = groups - (groups - 1) // block.value * block.value
+            short += last < block.value
+            for n in {block.value, last}:
+                assert n * cg % vec == 0
+                nv = n * cg // vec
+                lanes = 256 // nv if nv < 256 else 1
+                # a (mean, M2) of 8 bytes per vector, or per channel where a vector lies in two groups
+                assert lanes * nv * (1 if cg % vec == 0 else vec) * 8 <= lds.value, (c, groups, n)
+    assert short > 100
+    assert lib.sidon_group_norm_passes(2, 10, 64, 5, dtype, vec, *map(ctypes.byref, (block, chunks, lds))) == -2
+    assert lib.sidon_group_norm_passes(2, 10, 64, 4, dtype, 3, *map(ctypes.byref, (block, chunks, lds))) == -2
+    assert lib.sidon_group_norm_passes(2, 10, 64, 4, dtype, vec, None, None, None) == -1
+
+
 def test_group_norm_rejects_host_tensors(sidon):
     x = torch.zeros(4, 8)
     with pytest.raises(ValueError, match="HIP device"):
