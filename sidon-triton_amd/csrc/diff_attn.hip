@@ -397,11 +397,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
 #pragma unroll
     for (int i = 0; i < 16; ++i) e[i] = fast_exp2(fmaf(s[i], p.scale, -mx));
   };
-  // The step's probabilities, rounded, and their sum: on the matrix core, where
-  // the vector unit is the busier one.  Read as a 16x16x32 B operand, a lane's
-  // half of them holds query c + 16 (j % 2) of lane c + 16 j, keys 8 (j / 2) + [0, 8);
-  // the A operand is 1 where bit 4 of the lane equals bit 2, so that the four
-  // rows a lane receives are its own query's sum.
+  // The step's probabilities, rounded.
   const auto round_to = [&](const float (&e)[16]) SIDON_INLINE {
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
@@ -412,6 +408,14 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
         pk[kTerms - 1][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, __builtin_convertvector(left, v2));
       }
     }
+  };
+  // Their sum, on the matrix core, where the vector unit is the busier one.  Read
+  // as a 16x16x32 B operand, a lane's half of them holds query c + 16 (j % 2) of
+  // lane c + 16 j, keys 8 (j / 2) + [0, 8); the A operand is 1 where bit 4 of the
+  // lane equals bit 2, so that the four rows a lane receives are its own query's
+  // sum.  The other query of the column enters times 0: where its probabilities are
+  // infinite or NaN, so is this sum, and `settle` takes the query's own.
+  const auto matrix_sum = [&]() SIDON_INLINE {
     f4 total = {};
 #pragma unroll
     for (int k = 0; k < kTerms; ++k) {
@@ -419,6 +423,19 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
       total = Half<E>::small(sel, pk[k][1], total);
     }
     return total[0];
+  };
+  // The same from the lane pair that holds the query, nothing else.
+  const auto own_sum = [&]() SIDON_INLINE {
+    float total = 0.f;
+#pragma unroll
+    for (int k = 0; k < kTerms; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int pair = pk[k][i >> 2][i & 3];   // (a bit cast of the element itself takes the vector's first)
+        const v2 x = __builtin_bit_cast(v2, pair);
+        total += (float)x[0] + (float)x[1];
+      }
+    return pair_sum(total);
   };
   const auto values = [&]() SIDON_INLINE {
     typedef int i2 __attribute__((ext_vector_type(2)));
@@ -435,7 +452,8 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
     vread = vread == 2 * C::kSlot ? 0 : vread + C::kSlot;
   };
   // Raises the running maximum of the queries whose probabilities do not all
-  // fit, with what they have so far.  (The condition is a lane's, not the
+  // fit, with what they have so far, and takes their sums apart from the other
+  // queries'.  (The condition is a lane's, not the
   // wavefront's: behind a branch of the wavefront the compiler keeps the
   // accumulators in two places.)
   const auto settle = [&](float total) SIDON_INLINE {
@@ -452,7 +470,8 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
       mx = top;
       float e[16];
       exps(e);
-      total = round_to(e);
+      round_to(e);
+      total = own_sum();
     }
     sum += total;
   };
@@ -481,7 +500,8 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
       hide();
       float e[16];
       exps(e);
-      settle(round_to(e));
+      round_to(e);
+      settle(matrix_sum());
       if (count > 1) {
         load_keys();
         scores();
@@ -493,7 +513,8 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
       float e[16];
       exps(e);
       values();
-      const float total = round_to(e);
+      round_to(e);
+      const float total = matrix_sum();
       load_keys();   // (of the last round: what an earlier step left in the slot, for nothing)
       settle(total);
       scores();

@@ -166,6 +166,26 @@ def test_a_row_does_not_depend_on_the_others(sidon):
     assert torch.equal(a[0], c[0]) and (c[1] == 0).all()
 
 
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(1, 2, 2, 32, 200, 64), (2, 8, 2, 5, 900, 128), (9, 8, 8, 517, 517, 64),
+                                   (9, 8, 4, 300, 333, 128), (1, 8, 8, 30, 4800, 64)], ids=str)
+def test_queries_that_are_no_numbers(sidon, shape, kind):
+    """NaN and infinities in some queries (the padding of a batch, say) come back
+    as NaN and reach no other query, head or item."""
+    b, h, hk, l, s, d = shape
+    q, k, v, lam, norm_w = inputs(*shape, kind, 12)
+    want, tol = reference(q, k, v, lam, 0.3, None, False, norm_w, 1e-5)
+    bad = torch.zeros(b, h, l, dtype=torch.bool, device=DEV)
+    bad[:, :, 1::5] = True
+    bad[:, 0, 0] = True
+    q = q.clone()
+    q[:, :, 0][bad] = float("nan")
+    q[:, :, 1, 1::10] = float("inf")
+    got = sidon.diff_attention.diff_attention(q, k, v, lam, 0.3, norm_w=norm_w)
+    check(got[~bad], want[~bad], tol[~bad])
+    assert torch.isnan(got[bad]).all()
+
+
 def test_repeats_are_equal(sidon):
     for shape in ((1, 8, 8, 1, 4800, 64), (2, 8, 8, 1037, 1037, 64), (6, 8, 8, 700, 700, 128)):
         q, k, v, lam, norm_w = inputs(*shape, torch.bfloat16, 2)
