@@ -111,7 +111,9 @@ int sidon_adapter_residual(const void* x, int ldx, const void* w, int ldw, const
  * q, k and v.
  *
  * Scores, softmax statistics, sums and the norm in fp32, probabilities rounded to
- * `dtype` in front of the product with v (with few rows what the rounding left is
+ * `dtype` in front of the product with v: each off by half a step of itself, in
+ * fp16 down to 2^-23 of the row's largest, and none below 2^-34 of it (with few rows
+ * what the rounding left is
  * multiplied too), one rounding at the end.  What a key within LK but past a
  * query's own position holds must be finite (its weight is 0).  ws:
  * sidon_diff_attention_workspace_bytes bytes for these sizes on the current

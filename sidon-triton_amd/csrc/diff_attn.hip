@@ -96,6 +96,11 @@ struct Half<_Float16> {
   typedef h8 v8;
   typedef h2 v2;
   typedef h4 v4;
+  // The running maximum stands for a probability of 2^kLift, not of 1, so that
+  // probabilities keep their 11 bits down to 2^-23 of the largest and vanish below
+  // 2^-34 (with 1: 2^-14 and 2^-25, which the keys of a long cache add up to).  A
+  // step's 32 sum to 2^14 at most, under what raises the maximum.
+  static constexpr float kLift = 9.f;
   static __device__ __forceinline__ f32x16 mfma(i4 a, i4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
   }
@@ -108,6 +113,7 @@ struct Half<__bf16> {
   typedef b8 v8;
   typedef b2 v2;
   typedef b4 v4;
+  static constexpr float kLift = 0.f;   // (as many exponents as fp32)
   static __device__ __forceinline__ f32x16 mfma(i4 a, i4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
   }
@@ -361,7 +367,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
   f32x16 o[kDb];
 #pragma unroll
   for (int d = 0; d < kDb; ++d) o[d] = f32x16{};
-  float mx = kFloorMax, sum = 0.f;   // maximum of the scaled scores and sum of the probabilities of query n
+  float mx = kFloorMax, sum = 0.f;   // maximum of the scaled scores, less kLift, and sum of the probabilities of query n
   f32x16 s;                          // scores of a step: element i is key 16 (i / 8) + 8 g + i % 8
   constexpr int kTerms = kFine ? 2 : 1;
   i4 pk[kTerms][2];                  // its probabilities
@@ -462,7 +468,7 @@ __global__ void __launch_bounds__(128 * RB * KS, kMinWaves) diff_attn_kernel(con
       float top = s[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-      top = fmaxf(mx, pair_max(top) * p.scale);
+      top = fmaxf(mx, pair_max(top) * p.scale - Half<E>::kLift);
       const float alpha = fast_exp2(mx - top);   // 0 from kFloorMax
 #pragma unroll
       for (int d = 0; d < kDb; ++d) o[d] *= alpha;

@@ -129,6 +129,26 @@ def test_rising_scores(sidon, shape, kind):
     check(got, *reference(q, k, v, lam, 0.3, None, False, None, 1e-5))
 
 
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(2, 4, 2, 1, 20000, 64), (1, 2, 1, 3, 3000, 128), (6, 8, 8, 700, 1900, 64),
+                                   (6, 8, 8, 300, 1900, 128)], ids=str)
+def test_small_probabilities(sidon, shape, kind):
+    """A key with no value in every 128 that takes nearly all of the weight, and an
+    output that comes from the others: e^-15 of it each (under fp16's smallest
+    normal number), and each still rounded by half a step of itself."""
+    b, h, hk, l, s, d = shape
+    q, k, v, lam, _ = inputs(*shape, kind, 7)
+    q = torch.zeros_like(q)
+    q[..., 0] = 8.0   # (scores: k at D = 64, k / sqrt 2 at 128)
+    k = torch.zeros_like(k)
+    k[..., 0] = -15.125 if d == 64 else -21.375
+    k[:, :, :, ::128] = 0
+    v = v.abs().clone()
+    v[:, :, ::128] = 0
+    got = sidon.diff_attention.diff_attention(q, k, v, lam, 0.3)
+    check(got, *reference(q, k, v, lam, 0.3, None, False, None, 1e-5))
+
+
 @pytest.mark.parametrize("l", [1, 300])
 def test_strides_and_out(sidon, l):
     """[B, H, 2, L, D] contiguous, key rows and heads in other orders, an output
