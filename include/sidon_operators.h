@@ -76,6 +76,10 @@ int sidon_group_norm_passes(int B, int T, int C, int G, int dtype, int vec, int*
  *
  * Sums in fp32.  linear rounds scale (x . a^T) to `dtype` in front of the product
  * with b; residual, whose result is fp32, keeps all of it (two or three summands).
+ * fp16 holds them divided by a power of two of each row's own, exactly, so that
+ * products past 65504 do not overflow and small ones keep their digits, down to 2^-24
+ * of the row's largest.  A row with a product that is no
+ * finite number below 2^127 gives infinities or NaN, in that row alone.
  * ws: sidon_adapter_workspace_bytes bytes, 16-byte aligned, contents irrelevant.
  */
 size_t sidon_adapter_workspace_bytes(int M, int R, int residual, int dtype);

@@ -134,8 +134,9 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, 
     ids: int32 [items] on the device, M a multiple of items: rows in order, M /
     items per item (an utterance of a padded batch; items = M: single tokens).  An
     id outside [0, E) means no adapter.  act: None or "silu".  N and K multiples of
-    64, R of 8 up to 128.  Sums in fp32, scale (x A_e^T) rounded to x's type.  Rows of x, w and out
-    may be strided.  workspace: a contiguous uint8 tensor of ``workspace_bytes``.
+    64, R of 8 up to 128.  Sums in fp32, scale (x A_e^T) rounded to x's type (fp16: relative
+    to a power of two of its row, so that it neither overflows nor loses the digits
+    of small values).  Rows of x, w and out may be strided.  workspace: a contiguous uint8 tensor of ``workspace_bytes``.
     Forward only."""
     rows, n, ldx, ldw, sizes, dtype, need = _operands(x, w, a, b, scale, ids, bias, False)
     device = x.device

@@ -46,6 +46,10 @@ struct ShrinkParams {
 // are summed through LDS in order.  Products are 16 ranks x 16 rows: a lane's
 // accumulators are 4 ranks of one row, so of several adapters among the rows each
 // costs a pass over K whose other rows' results are dropped.
+// 16-bit outputs get the products rounded once: u of each, beside the output's own
+// u of the sum, a few per cent of the error of a projection with an adapter of the usual
+// size; a second summand would double the second launch's low-rank products and
+// the bytes between the launches.  fp16 keeps them relative to their row (LowRow).
 // (Operands read from memory by the lanes that multiply them cost a cache access
 // per lane, its neighbours holding other rows: 17.2 us instead of 8.3 at 4800 rows, K 1024,
 // rank 64.)
@@ -54,7 +58,7 @@ __global__ void __launch_bounds__(64 * W) shrink_kernel(const ShrinkParams p) {
   typedef typename Elem<E>::e8 e8;
   constexpr int kSlot = (1 + RB) * 2048;
   constexpr int kPer = 2 * (1 + RB);            // copies per slice
-  static_assert(2 * W * kSlot <= 160 * 1024 && W * RB * 1024 <= 2 * W * kSlot, "LDS");
+  static_assert(2 * W * kSlot <= 160 * 1024 && W * RB * 1024 + W * 64 <= 2 * W * kSlot, "LDS");
   __shared__ __attribute__((aligned(16))) char smem[2 * W * kSlot];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -125,21 +129,61 @@ __global__ void __launch_bounds__(64 * W) shrink_kernel(const ShrinkParams p) {
     for (int b = 0; b < RB; ++b) part[(w * RB + b) * 64 + lane] = acc[b];
     lds_barrier();
     // A lane's sums are of the row it holds.
-    for (int b = w; b < RB; b += W) {
-      const int r = 16 * b + 4 * lg, m = row0 + ln;
-      f4 s = part[b * 64 + lane];
+    constexpr int NB = (RB + W - 1) / W;
+    using Row = LowRow<E>;
+    f4 sum[NB];
+    uint32_t largest = 0;   // magnitude's bits, in whose order infinity and NaN come last
 #pragma unroll
-      for (int i = 1; i < W; ++i) s += part[(i * RB + b) * 64 + lane];
+    for (int k = 0; k < NB; ++k) {
+      const int b = w + k * W;
+      if (b >= RB) break;
+      sum[k] = part[b * 64 + lane];
+#pragma unroll
+      for (int i = 1; i < W; ++i) sum[k] += part[(i * RB + b) * 64 + lane];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        sum[k][c] *= scale;
+        const float v = sum[k][c];
+        largest = max(largest, __builtin_bit_cast(uint32_t, v) & 0x7fffffffu);
+      }
+    }
+    uint32_t power = 0;
+    if constexpr (Row::kDivided) {
+      // The row's: of the four lanes that hold it, and of all wavefronts.
+      const auto p16 = __builtin_amdgcn_permlane16_swap(largest, largest, false, false);
+      largest = max(p16[0], p16[1]);
+      const auto p32 = __builtin_amdgcn_permlane32_swap(largest, largest, false, false);
+      largest = max(p32[0], p32[1]);
+      if constexpr (RB > 1) {
+        uint32_t* const all = reinterpret_cast<uint32_t*>(smem + W * RB * 1024);   // (behind the sums)
+        if (lg == 0) all[w * 16 + ln] = largest;
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < (RB < W ? RB : W); ++i) largest = max(largest, all[i * 16 + ln]);
+      }
+      power = Row::power(largest);
+    }
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int b = w + k * W;
+      if (b >= RB) break;
+      const int r = 16 * b + 4 * lg, m = row0 + ln;
       if (ln < p.rows && m < p.M && r < p.R && id == e) {
+        f4 s = sum[k];
+        if constexpr (Row::kDivided) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[c] = Row::divided(s[c], power);
+        }
         E* dst = static_cast<E*>(p.low) + (int64_t)m * p.R + r;
         for (int plane = 0; plane < p.planes; ++plane) {
           typename Elem<E>::e4 v;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            if (plane == 0) s[c] *= scale;
             v[c] = to_elem<E>(s[c]);
             s[c] -= (float)v[c];   // exact: what the rounding left
           }
+          if constexpr (Row::kDivided)
+            v = __builtin_bit_cast(typename Elem<E>::e4, Row::packed(__builtin_bit_cast(typename Row::i2, v), power, r / 4));
           *reinterpret_cast<typename Elem<E>::e4*>(dst + plane * p.plane) = v;
         }
       }

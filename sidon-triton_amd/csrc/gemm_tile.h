@@ -86,7 +86,8 @@ struct TileParams {
 // The same with a low-rank term per row in front of the epilogue:
 //   acc[m, n] += sum_r low[m, r] . up[e, n, r],   e = ids[m / rows_per_id], none where e is outside [0, adapters)
 // low holds `planes` summands of its values (rounded values and what the
-// roundings left), each [M, rank].
+// roundings left), each [M, rank]; of fp16 a row's are divided by a power of two
+// (LowRow).
 struct LowParams : TileParams {
   const void* low;
   const void* up;            // [adapters, N, rank]
@@ -148,6 +149,53 @@ __device__ __forceinline__ E to_elem(float y) {
   asm volatile("" : "+v"(y));
   return (E)y;
 }
+
+// The low-rank values of a row as they are stored.  bf16 holds them as they are.  fp16
+// would overflow past 65504 and lose digits below 2^-14 (a small A with a large B), so
+// a row's values are divided by the power of two just above the largest of them:
+// magnitudes up to 1 leave the top exponent bit (14) of each at 0, and those bits of
+// the row's first eight values, of every plane, hold the power's biased exponent, in
+// the order that the fewest instructions read.  Exponent 255 is a row with a value
+// that is no finite number below 2^127; its products are infinite or NaN.
+template <typename E>
+struct LowRow {
+  typedef typename Elem<E>::e8 e8;
+  static constexpr bool kDivided = false;
+  static __device__ __forceinline__ e8 values(e8 v) { return v; }
+  static __device__ __forceinline__ float factor(e8) { return 1.f; }
+};
+template <>
+struct LowRow<_Float16> {
+  typedef Elem<_Float16>::e8 e8;
+  typedef int i2 __attribute__((ext_vector_type(2)));
+  typedef int i4 __attribute__((ext_vector_type(4)));
+  static constexpr bool kDivided = true;
+  static constexpr uint32_t kTop = 0x40004000u, kHigh = 0x78000000u;
+  // The power (a float's bits) from the largest magnitude's bits.
+  static __device__ __forceinline__ uint32_t power(uint32_t largest) {
+    return min((largest & 0x7f800000u) + 0x00800000u, 0x7f800000u);
+  }
+  static __device__ __forceinline__ float divided(float v, uint32_t power) {
+    return __builtin_ldexpf(v, 127 - (int)(power >> 23));
+  }
+  // Dwords 2 j and 2 j + 1 of a row (values 4 j to 4 j + 3) as they are stored.
+  static __device__ __forceinline__ i2 packed(i2 v, uint32_t power, int j) {
+    const uint32_t x = j >= 2 ? 0u : (power & kHigh) | (power >> 12 & 0x7800u);
+    return i2{(int)(((uint32_t)v[0] & ~kTop) | (x << 2 * j & kTop)), (int)(((uint32_t)v[1] & ~kTop) | (x << (2 * j + 1) & kTop))};
+  }
+  // Stored values without the exponent's bits.
+  static __device__ __forceinline__ e8 values(e8 v) {
+    return __builtin_bit_cast(e8, __builtin_bit_cast(i4, v) & (int)~kTop);
+  }
+  // What a row's values are multiplied by, from its first eight.
+  static __device__ __forceinline__ float factor(e8 first) {
+    const i4 v = __builtin_bit_cast(i4, first);
+    uint32_t x = (uint32_t)v[3];
+#pragma unroll
+    for (int c = 2; c >= 0; --c) x = ((uint32_t)v[c] & kTop) | (x >> 1 & ~kTop);
+    return __builtin_bit_cast(float, ((x & kHigh) | (x << 12 & ~kHigh)) & 0x7f800000u);
+  }
+};
 
 // A tile of up to this many items takes its low-rank term's operands through LDS,
 // one adapter at a time; of more, straight from memory: up to kFewKinds adapters
@@ -477,6 +525,7 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
           acc_t t[IN];
 #pragma unroll
           for (int j = 0; j < IN; ++j) t[j] = acc_t{};
+          const float f = LowRow<E>::factor(*reinterpret_cast<const h8*>(lows + MF * i * p.rank * 2 + (mixed << 4)));
           for (int r0 = 0; r0 < p.rank; r0 += kW) {
             const int c = (r0 >> 3) + lg, at = (c ^ mixed) << 4;
             h8 u[IN];
@@ -484,7 +533,9 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
             for (int j = 0; j < IN; ++j)
               u[j] = c < chunks ? *reinterpret_cast<const h8*>(ups + MF * j * p.rank * 2 + at) : h8{};
             for (int k = 0; k < now; ++k) {
-              const h8 v = c < chunks ? *reinterpret_cast<const h8*>(lows + k * low_bytes + MF * i * p.rank * 2 + at) : h8{};
+              h8 v = {};
+              if (c < chunks)
+                v = LowRow<E>::values(*reinterpret_cast<const h8*>(lows + k * low_bytes + MF * i * p.rank * 2 + at));
 #pragma unroll
               for (int j = 0; j < IN; ++j) t[j] = mma(u[j], v, t[j]);
             }
@@ -493,7 +544,7 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
           // compiler keeps the accumulators in two places.)
           if (id[i] == adapter) {
 #pragma unroll
-            for (int j = 0; j < IN; ++j) acc[i][j] += t[j];
+            for (int j = 0; j < IN; ++j) acc[i][j] += t[j] * f;
           }
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -518,6 +569,10 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
                       (int64_t)min(m0 + TM * wm + MF * i + ln, p.M - 1) * p.rank + r;
         return r < p.rank ? *reinterpret_cast<const h8*>(at) : h8{};
       };
+      const auto factor_of = [&](int i) SIDON_INLINE {
+        if constexpr (LowRow<E>::kDivided) return LowRow<E>::factor(low_at(i, 0, 0));
+        return 1.f;
+      };
       const auto up_at = [&](int e, int col, int r) SIDON_INLINE {
         const E* at = static_cast<const E*>(p.up) + ((int64_t)e * p.N + tn * BN + TN * wn + col) * p.rank + r;
         return r < p.rank ? *reinterpret_cast<const h8*>(at) : h8{};
@@ -535,34 +590,39 @@ __global__ void __launch_bounds__(64 * WM * WN) gemm_tile_kernel(const Params p)
             acc_t t[IN];
 #pragma unroll
             for (int j = 0; j < IN; ++j) t[j] = acc_t{};
+            const float f = factor_of(i);
             for (int r0 = 0; r0 < p.rank; r0 += kW) {
               const int r = r0 + 8 * lg;
               h8 u[IN];
 #pragma unroll
               for (int j = 0; j < IN; ++j) u[j] = up_at(e, MF * j + ln, r);
               for (int plane = 0; plane < p.planes; ++plane) {
-                const h8 v = low_at(i, plane, r);
+                const h8 v = LowRow<E>::values(low_at(i, plane, r));
 #pragma unroll
                 for (int j = 0; j < IN; ++j) t[j] = mma(u[j], v, t[j]);
               }
             }
             if (id[i] == e) {
 #pragma unroll
-              for (int j = 0; j < IN; ++j) acc[i][j] += t[j];
+              for (int j = 0; j < IN; ++j) acc[i][j] += t[j] * f;
             }
           }
         } else if (id[i] >= 0) {
           // Nearly every row has an adapter of its own: each lane takes its
           // row's products itself, from whole rows of up.
+          const float f = factor_of(i);
           const auto own = [&](int r, h8 first, auto up) SIDON_INLINE {
             float v[8];
+            first = LowRow<E>::values(first);
 #pragma unroll
             for (int c = 0; c < 8; ++c) v[c] = (float)first[c];
             for (int plane = 1; plane < p.planes; ++plane) {
-              const h8 part = low_at(i, plane, r);
+              const h8 part = LowRow<E>::values(low_at(i, plane, r));
 #pragma unroll
               for (int c = 0; c < 8; ++c) v[c] += (float)part[c];
             }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] *= f;
 #pragma unroll
             for (int j = 0; j < IN; ++j)
 #pragma unroll

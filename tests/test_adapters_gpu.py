@@ -108,6 +108,46 @@ def test_residual_against_float64(sidon, shape, kind):
     assert torch.equal(s["y"], out)
 
 
+# binary orders of x, a, w, b, scale: small products with a large b, products past fp16's largest number, small ones
+# from a and from the scale, a tiny x, a large scale
+ORDERS = [(0, -14, 0, 14, 0), (10, 2, -8, -16, 2), (0, -12, 0, 0, -12), (-6, 0, 0, 15, -8), (0, 0, 0, -10, 17)]
+PATHS = [(40, 1, 256, 256, 16, 30), (4, 100, 512, 256, 64, 3), (10, 7, 192, 320, 40, 6), (5, 1037, 1024, 64, 64, 2),
+         (9, 333, 2048, 192, 104, 4), (3, 1, 64, 64, 8, 2), (8, 600, 4096, 128, 48, 3)]
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("orders", ORDERS, ids=str)
+@pytest.mark.parametrize("shape", PATHS, ids=str)
+def test_low_rank_products_of_any_size(sidon, shape, orders, kind):
+    s = inputs(*shape, kind, sum(shape) + 3)
+    for name, p in zip(("x", "a", "w", "b", "scale"), orders):
+        s[name] = (s[name].float() * 2.0 ** p).to(s[name].dtype)
+    check(linear(sidon, s), *reference(s, False))
+    want, tol = reference(s, True)
+    check(residual(sidon, s), want, tol)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("shape", PATHS, ids=str)
+def test_rows_that_are_no_numbers(sidon, shape, kind):
+    """An infinity or a NaN in a row of x stays in that row, and a row of zeros
+    keeps what the stream holds."""
+    s = inputs(*shape, kind, sum(shape) + 4)
+    want, tol = reference(s, False)
+    res, res_tol = reference(s, True)
+    rows = torch.arange(s["x"].shape[0], device=DEV)
+    s["x"][rows % 7 == 2, 5] = float("inf")
+    s["x"][rows % 7 == 6, 9] = float("nan")
+    s["x"][0] = 0
+    clean = (rows % 7 != 2) & (rows % 7 != 6) & (rows != 0)
+    got, got_res = linear(sidon, s), residual(sidon, s, out=torch.empty_like(s["y"]))
+    check(got[clean], want[clean], tol[clean])
+    check(got_res[clean], res[clean], res_tol[clean])
+    bad = ~clean & (rows != 0)
+    assert not torch.isfinite(got[bad]).any() and not torch.isfinite(got_res[bad]).any()
+    assert torch.equal(got[0], s["bias"]) and torch.equal(got_res[0], s["y"][0])
+
+
 @pytest.mark.parametrize("items,rows", [(40, 1), (10, 7), (3, 100)])
 def test_ids_outside_and_adapters_of_others(sidon, items, rows):
     """Ids below, at and past the adapters leave the row as the shared
