@@ -153,6 +153,16 @@ def check(func: str, code: int) -> None:
         raise SidonError(func, code, msg)
 
 
+INT_MAX = 2 ** 31 - 1
+
+
+def ints(**values: int) -> None:
+    """Refuses what a C int does not hold (ctypes would pass its low 32 bits)."""
+    for name, value in values.items():
+        if not -INT_MAX <= value <= INT_MAX:
+            raise ValueError(f"{name.replace('_', ' ')} {value} must fit 32 bits")
+
+
 def strides3(st) -> ctypes.Array:
     return (ctypes.c_int64 * 3)(*[int(x) for x in st])
 

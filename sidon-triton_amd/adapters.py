@@ -29,6 +29,7 @@ _TYPES = (torch.float16, torch.bfloat16)
 
 def workspace_bytes(rows: int, rank: int, residual: bool = False, dtype: torch.dtype = torch.float16) -> int:
     """Bytes of the workspace of a call on ``rows`` rows (all items together)."""
+    _lib.ints(rows=rows, rank=rank)
     return int(_lib.load().sidon_adapter_workspace_bytes(rows, rank, int(residual), _lib.DTYPES[dtype]))
 
 
@@ -111,8 +112,16 @@ def _check(x, w, a, b, scale, ids, bias, residual):
             _check_device_tensor("bias", bias, device)
         if bias.dtype != x.dtype or bias.shape != (n,) or not bias.is_contiguous():
             raise ValueError(f"bias must be a contiguous {x.dtype} [{n}] tensor")
+    _lib.ints(outputs=n, columns=k, adapters=a.shape[0], row_stride_of_x=_row_stride(x), row_stride_of_w=_row_stride(w))
     return (rows, n, _row_stride(x), _row_stride(w), (rows, n, k, a.shape[1], a.shape[0], ids.numel()),
             _lib.DTYPES[x.dtype], workspace_bytes(rows, a.shape[1], residual, x.dtype))
+
+
+def _stride_of(name: str, t: torch.Tensor) -> int:
+    stride = _row_stride(t)
+    if stride > _lib.INT_MAX:
+        raise ValueError(f"{name}'s row stride {stride} must fit 32 bits")
+    return stride
 
 
 def _workspace(workspace, need, device):
@@ -151,7 +160,7 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, 
         _check_device_tensor("out", out, device)
         if out.dtype != x.dtype or out.shape != (rows, n) or out.stride(1) != 1:
             raise ValueError(f"out must be a {x.dtype} [{rows}, {n}] tensor with rows contiguous")
-        ldy = _row_stride(out)
+        ldy = _stride_of("out", out)
     workspace = _workspace(workspace, need, device)
     lib = _lib.load()
     with _on_device(device):
@@ -179,12 +188,13 @@ def adapter_residual(y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, a: torch
             raise ValueError(f"{name} must be a float32 [{rows}, {n}] tensor with rows contiguous")
     if not plain(y, x, w, a, b, scale):
         raise ValueError("adapter_residual has no backward: call it under torch.no_grad()")
+    ldadd, ldy = _stride_of("y", y), _stride_of("out", out)
     workspace = _workspace(workspace, need, device)
     lib = _lib.load()
     with _on_device(device):
         rc = lib.sidon_adapter_residual(
             x.data_ptr(), ldx, w.data_ptr(), ldw, a.data_ptr(), b.data_ptr(), scale.data_ptr(), ids.data_ptr(),
-            y.data_ptr(), _row_stride(y), out.data_ptr(), _row_stride(out), workspace.data_ptr(), workspace.numel(),
+            y.data_ptr(), ldadd, out.data_ptr(), ldy, workspace.data_ptr(), workspace.numel(),
             *sizes, dtype, _stream_handle(device))
     if rc:
         _lib.check("sidon_adapter_residual", rc)

@@ -205,6 +205,7 @@ def _row_stride(t: torch.Tensor) -> int:
 
 def group_norm_workspace(batch: int, length: int, channels: int, groups: int, dtype: torch.dtype) -> int:
     """Bytes of ``group_norm_act``'s workspace for [batch * length, channels]."""
+    _lib.ints(batch=batch, frames=length, channels=channels, groups=groups)
     return int(_lib.load().sidon_group_norm_workspace_bytes(batch, length, channels, groups, _lib.DTYPES[dtype]))
 
 

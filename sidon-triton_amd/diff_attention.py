@@ -27,6 +27,7 @@ HEAD_DIMS = (64, 128)
 
 def workspace_bytes(batch: int, heads: int, kv_heads: int, length: int, keys: int, dim: int, device=None) -> int:
     """Bytes of ``diff_attention``'s workspace on ``device`` (0: none needed)."""
+    _lib.ints(batch=batch, heads=heads, kv_heads=kv_heads, length=length, keys=keys, dim=dim)
     with _on_device(device):
         return int(_lib.load().sidon_diff_attention_workspace_bytes(batch, heads, kv_heads, length, keys, dim))
 

@@ -129,6 +129,35 @@ def test_group_norm_past_32_bits(sidon):
         assert torch.equal(far[:, 512:768], want)
 
 
+def test_sizes_and_strides_past_32_bits_are_refused(sidon):
+    """The ABI's ints hold 32 bits: 2^32 + n would arrive as n, and the call would
+    read or write other rows than it was given."""
+    far = 1 << 32
+    s = adapters_test.inputs(2, 1, 64, 64, 8, 2, torch.float16, 3)
+    half = torch.empty(far + 256, dtype=torch.float16, device=DEV)
+    rows = lambda t: t.as_strided((2, 64), (far + 64, 1))  # noqa: E731
+    with pytest.raises(ValueError, match="32 bits"):
+        adapters_test.linear(sidon, {**s, "x": rows(half)})
+    with pytest.raises(ValueError, match="32 bits"):
+        adapters_test.linear(sidon, {**s, "w": rows(half), "b": s["b"][:, :2].contiguous(), "bias": None})
+    with pytest.raises(ValueError, match="32 bits"):
+        adapters_test.linear(sidon, s, out=rows(half))
+    x = half[:far + 64].view(1, -1)
+    with pytest.raises(ValueError, match="32 bits"):
+        sidon.conformer.group_norm_act(x, 1, 1, torch.empty(far + 64, device=DEV), torch.empty(far + 64, device=DEV))
+    with pytest.raises(ValueError, match="32 bits"):
+        sidon.conformer.group_norm_act(x.view(-1, 1), 1, 1, torch.ones(1, device=DEV), torch.zeros(1, device=DEV))
+    del half, x
+    full = torch.empty(far + 256, device=DEV)
+    for over in (dict(out=rows(full)), dict(y=rows(full))):
+        with pytest.raises(ValueError, match="32 bits"):
+            adapters_test.residual(sidon, {**s, "y": over.pop("y", s["y"])}, **over)
+    del full
+    q, k, v, lam, _ = attention_test.inputs(1, 1, 1, 1, 1, 64, torch.float16, 1)
+    with pytest.raises(ValueError, match="32 bits"):
+        sidon.diff_attention.diff_attention(q, k.expand(1, 1, 2, far + 33, 64), v.expand(1, 1, far + 33, 128), lam, 0.3)
+
+
 def calls(sidon, seed):
     """One call of each operator with its workspace -> [(call, workspace bytes)]; call(workspace) -> the output."""
     x, w, b = norm_test.inputs(4000, 512, torch.float16, seed)

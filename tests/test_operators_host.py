@@ -234,6 +234,19 @@ def test_encoder_adapters_of_the_largest_rank(sidon):
     assert not packed_set[0]["out_w"][1][0].any()
 
 
+def test_sizes_past_32_bits_are_refused(sidon):
+    """2^32 + n must not arrive as n."""
+    far = 1 << 32
+    for call in (lambda: sidon.adapters.workspace_bytes(far + 100, 16),
+                 lambda: sidon.conformer.group_norm_workspace(1, far + 10, 64, 4, torch.float16),
+                 lambda: sidon.conformer.group_norm_workspace(1, 10, far + 64, 4, torch.float16),
+                 lambda: sidon.diff_attention.workspace_bytes(1, 8, 8, 1, far + 4800, 64),
+                 lambda: sidon._lib.ints(row_stride=1 << 31)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+    sidon._lib.ints(row_stride=(1 << 31) - 1, other=-5)
+
+
 def test_layouts_are_bounded(sidon):
     kept = sidon._lib.Layouts()
     for i in range(3 * kept.MOST + 5):
