@@ -200,7 +200,7 @@ def group_norm_act(x: torch.Tensor, batch: int, groups: int, w: torch.Tensor, b:
 
 def _row_stride(t: torch.Tensor) -> int:
     """Elements between rows; a single row's stride means nothing."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def group_norm_workspace(batch: int, length: int, channels: int, groups: int, dtype: torch.dtype) -> int:

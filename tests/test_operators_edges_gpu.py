@@ -158,6 +158,19 @@ def test_sizes_and_strides_past_32_bits_are_refused(sidon):
         sidon.diff_attention.diff_attention(q, k.expand(1, 1, 2, far + 33, 64), v.expand(1, 1, far + 33, 128), lam, 0.3)
 
 
+@pytest.mark.parametrize("stride", [67, 0, 1 << 33])
+def test_a_single_rows_stride_means_nothing(sidon, stride):
+    row = lambda t: t.as_strided((1, t.shape[1]), (stride, 1))  # noqa: E731
+    s = adapters_test.inputs(1, 1, 128, 64, 8, 2, torch.float16, 3)
+    want, res = adapters_test.linear(sidon, s), adapters_test.residual(sidon, s, out=torch.empty_like(s["y"]))
+    out, into = torch.empty_like(want), torch.empty_like(res)
+    adapters_test.linear(sidon, {**s, "x": row(s["x"])}, out=row(out))
+    adapters_test.residual(sidon, {**s, "x": row(s["x"]), "y": row(s["y"])}, out=row(into))
+    assert torch.equal(out, want) and torch.equal(into, res)
+    x, w, b = norm_test.inputs(1, 256, torch.float16, 4)
+    assert torch.equal(sidon.conformer.group_norm_act(row(x), 1, 8, w, b), sidon.conformer.group_norm_act(x, 1, 8, w, b))
+
+
 def calls(sidon, seed):
     """One call of each operator with its workspace -> [(call, workspace bytes)]; call(workspace) -> the output."""
     x, w, b = norm_test.inputs(4000, 512, torch.float16, seed)
