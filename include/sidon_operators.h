@@ -39,8 +39,8 @@ extern "C" {
  * hold, and are written as zeros.
  *
  * x [B*T, C] and y [B*T, C] of `dtype`, rows ldx / ldy elements apart (>= C);
- * w and bias fp32 [C].  y may be x itself (same stride); any other overlap is
- * refused.  B <= 65535, T <= 2^30, 1 <= C <= 8192, C % G == 0.  Statistics and arithmetic in fp32,
+ * w and bias fp32 [C].  y may be x itself (same stride); any other overlap of y, or of
+ * a workspace that the call uses, with another operand is refused.  B <= 65535, T <= 2^30, 1 <= C <= 8192, C % G == 0.  Statistics and arithmetic in fp32,
  * one rounding at the end.  ws: sidon_group_norm_workspace_bytes bytes, 8-byte
  * aligned, contents irrelevant before and after.
  */
@@ -69,7 +69,7 @@ int sidon_group_norm_passes(int B, int T, int C, int G, int dtype, int vec, int*
  * of `dtype` (SIDON_FP16 or SIDON_BF16), K contiguous, rows of x and w ldx / ldw
  * apart, a and b contiguous; scale fp32 [adapters].  linear: y [M, N] of `dtype`,
  * act SIDON_ACT_NONE or SIDON_ACT_SILU.  residual: y and add fp32 [M, N], y may be
- * add itself (same stride), any other overlap of y with an input is refused.
+ * add itself (same stride), any other overlap of y or of ws with an input is refused.
  * N and K multiples of 64, R a multiple of 8 in [8, 128], M a multiple of items;
  * strides multiples of 8 (y and add of residual: 4); x and w each under 4 GiB;
  * pointers 16-byte aligned (bias 8, ids and scale 4).
@@ -112,7 +112,7 @@ int sidon_adapter_residual(const void* x, int ldx, const void* w, int ldw, const
  * than 2^25 apart; D 64 or 128.  lam fp32 [lam_heads, 4, D]: lq1, lk1, lq2, lk2,
  * lam_heads 1 or H.  norm_w fp32 [2 D], eps > 0 with it.  out's rows must not overlap one
  * another, and the memory from its first to its last element must hold nothing of
- * q, k and v.
+ * an input; neither must ws.
  *
  * Scores, softmax statistics, sums and the norm in fp32, probabilities rounded to
  * `dtype` in front of the product with v: each off by half a step of itself, in

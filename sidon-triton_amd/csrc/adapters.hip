@@ -265,7 +265,7 @@ int check_and_launch(Call& c, sidon_stream_t stream) {
     return fail(SIDON_E_ALIGN, "x, w, a, b, y, add and ws must be 16-byte aligned, bias 8, ids and scale 4");
   const size_t need = sidon_adapter_workspace_bytes(p.M, p.rank, c.residual, c.dtype);
   if (c.ws_bytes < need) return fail(SIDON_E_SHAPE, "ws holds %zu bytes, the call needs %zu", c.ws_bytes, need);
-  // Workgroups read the inputs while others already write y.
+  // Workgroups read the inputs while others already write y, or ws.
   const int64_t ysize = c.residual ? 4 : 2;
   const int64_t ybytes = ((int64_t)(p.M - 1) * p.ldy + p.N) * ysize;
   const int64_t up_bytes = (int64_t)p.adapters * p.N * p.rank * 2, a_bytes = (int64_t)p.adapters * p.rank * p.K * 2;
@@ -274,6 +274,21 @@ int check_and_launch(Call& c, sidon_stream_t stream) {
       ranges_meet(p.y, ybytes, c.a, a_bytes) || ranges_meet(p.y, ybytes, c.ws, (int64_t)need) ||
       (p.bias != nullptr && ranges_meet(p.y, ybytes, p.bias, (int64_t)p.N * 2)))
     return fail(SIDON_E_SHAPE, "y must not overlap an input or ws");
+  const struct {
+    const void* at;
+    int64_t bytes;
+  } in[] = {{p.ids, (int64_t)c.items * 4}, {c.scale, (int64_t)p.adapters * 4}, {c.a, a_bytes}, {p.up, up_bytes},
+            {p.bias, p.bias != nullptr ? (int64_t)p.N * 2 : 0}};
+  for (int i = 0; i < 5; ++i) {
+    if (i < 2 && sidon::row_meets(p.y, p.ldy * ysize, p.N * ysize, p.M, in[i].at, in[i].bytes))
+      return fail(SIDON_E_SHAPE, "y must not overlap an input or ws");
+    if (in[i].bytes > 0 && ranges_meet(c.ws, (int64_t)need, in[i].at, in[i].bytes))
+      return fail(SIDON_E_SHAPE, "ws must not overlap an input");
+  }
+  if (sidon::row_meets(p.x, (int64_t)p.ldx * 2, (int64_t)p.K * 2, p.M, c.ws, (int64_t)need) ||
+      sidon::row_meets(p.w, (int64_t)p.ldw * 2, (int64_t)p.K * 2, p.N, c.ws, (int64_t)need) ||
+      (c.residual && sidon::row_meets(p.add, (int64_t)p.ldadd * 4, (int64_t)p.N * 4, p.M, c.ws, (int64_t)need)))
+    return fail(SIDON_E_SHAPE, "ws must not overlap an input");
   if (c.residual && !(p.add == p.y && p.ldadd == p.ldy) &&
       sidon::rows_meet(p.y, p.ldy * ysize, p.N * ysize, p.add, (int64_t)p.ldadd * 4, (int64_t)p.N * 4, p.M))
     return fail(SIDON_E_SHAPE, "y may be add itself but must not overlap it otherwise");

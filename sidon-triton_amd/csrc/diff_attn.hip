@@ -890,19 +890,29 @@ SIDON_API int sidon_diff_attention(const void* q, const void* k, const void* v, 
       (reinterpret_cast<uintptr_t>(lens) & 3u) != 0 || !sidon::aligned16(ws))
     return fail(SIDON_E_ALIGN, "q, k, v, out, norm_w and ws must be 16-byte aligned, lam and lens 4-byte aligned");
   if (norm_w && !(eps >= FLT_MIN)) return fail(SIDON_E_SHAPE, "eps=%g must be positive (a query without keys has no mean square)", eps);
-  // Workgroups read q, k and v while others already write out.
+  // Workgroups read the inputs while others already write out, or ws.
+  struct Range {
+    const void* at;
+    __int128 bytes;
+    const char* name;
+  };
+  Range in[7];
   {
     const int qn[] = {B, H, 2, L}, kn[] = {B, Hk, 2, S}, vn[] = {B, Hk, S}, on[] = {B, H, L};
     if (!apart(on, o_strides, 3, 2 * D)) return fail(SIDON_E_STRIDE, "rows of out overlap one another");
     const __int128 most = (__int128)1 << 61, o_span = span(on, o_strides, 3, 2 * D) * 2;
-    const struct {
-      const void* at;
-      __int128 bytes;
-    } in[] = {{q, span(qn, q_strides, 4, D) * 2}, {k, span(kn, k_strides, 4, D) * 2}, {v, span(vn, v_strides, 3, 2 * D) * 2}};
-    for (const auto& t : in) {
-      if (o_span > most || t.bytes > most) return fail(SIDON_E_STRIDE, "a tensor spans more than the address space");
-      if (sidon::ranges_meet(out, (int64_t)o_span, t.at, (int64_t)t.bytes))
-        return fail(SIDON_E_SHAPE, "out must lie apart from q, k and v");
+    in[0] = Range{q, span(qn, q_strides, 4, D) * 2, "q"};
+    in[1] = Range{k, span(kn, k_strides, 4, D) * 2, "k"};
+    in[2] = Range{v, span(vn, v_strides, 3, 2 * D) * 2, "v"};
+    in[3] = Range{lam, (__int128)lam_heads * D * 16, "lam"};
+    in[4] = Range{norm_w, norm_w ? D * 8 : 0, "norm_w"};
+    in[5] = Range{lens, lens ? (__int128)B * 4 : 0, "lens"};
+    in[6] = Range{out, o_span, "out"};
+    for (const Range& t : in)
+      if (t.bytes > most) return fail(SIDON_E_STRIDE, "a tensor spans more than the address space");
+    for (const Range& t : in) {
+      if (&t != &in[6] && t.bytes > 0 && sidon::ranges_meet(out, (int64_t)o_span, t.at, (int64_t)t.bytes))
+        return fail(SIDON_E_SHAPE, "out must lie apart from %s", t.name);
     }
   }
   int rc;
@@ -911,6 +921,11 @@ SIDON_API int sidon_diff_attention(const void* q, const void* k, const void* v, 
   const Plan c = plan(B, Hk, R, S, D, sidon::compute_units());
   if (ws_bytes < part_bytes(B, Hk, R, D, c.splits) || (c.splits > 1 && ws == nullptr))
     return fail(SIDON_E_SHAPE, "ws holds %zu bytes, the call needs %zu", ws_bytes, part_bytes(B, Hk, R, D, c.splits));
+  if (c.splits > 1) {
+    for (const Range& t : in)
+      if (t.bytes > 0 && sidon::ranges_meet(ws, (int64_t)part_bytes(B, Hk, R, D, c.splits), t.at, (int64_t)t.bytes))
+        return fail(SIDON_E_SHAPE, "ws must lie apart from %s", t.name);
+  }
   // Parts per key head (DiffParams): enough for whole heads on an XCD where
   // possible, and all 8 where every head's keys and values fit one L2 together.
   const int64_t heads = (int64_t)B * Hk;

@@ -572,11 +572,11 @@ void passes(const Params& p, hipStream_t stream) {
                      (size_t)p.block_groups * sizeof(float2), stream, p);
 }
 
-template <typename T>
-void run(Params& p, bool vector, hipStream_t stream) {
-  constexpr int V = 16 / sizeof(T);
-  const int cg = p.C / p.G;
-  const int64_t vecs = (int64_t)p.T * (cg / V);
+// Whether the slab way is taken, for elements of `size` bytes; `vector`: the tensors
+// lie on 16 bytes.
+bool slab_way(const Params& p, int size, bool vector) {
+  const int v = 16 / size, cg = p.C / p.G;
+  const int64_t vecs = (int64_t)p.T * (cg / v);
   // A workgroup takes about 3.5 us + 0.085 us/KB for its slab (fp16, SiLU: the CU's
   // own arithmetic; less without an activation, more with GELU and where a group's
   // row is one vector of a cache line), the two passes 10.5 us + 0.6 us/MB for the whole
@@ -589,10 +589,16 @@ void run(Params& p, bool vector, hipStream_t stream) {
   // weights 0.6%).
   const double slab_kb = vecs * 16.0 / 1024, all_mb = slab_kb * p.B * p.G / 1024;
   const bool plain = p.act == SIDON_ACT_NONE || p.act == SIDON_ACT_RELU;
-  const double weight = (plain ? (sizeof(T) == 4 ? 0.65 : 0.8) : p.act == SIDON_ACT_GELU ? 1.33 : 1.0) * (cg == V ? 1.25 : 1.0);
-  if (vector && cg % V == 0 && vecs <= kSlabVecs * kSlabThreads && slab_kb * weight <= 85 + 4.2 * all_mb &&
-      (int64_t)p.B * p.G <= INT32_MAX / kSlabThreads) {   // (a launch holds less than 2^32 threads)
-    slab<T>(p, vecs, stream);
+  const double weight = (plain ? (size == 4 ? 0.65 : 0.8) : p.act == SIDON_ACT_GELU ? 1.33 : 1.0) * (cg == v ? 1.25 : 1.0);
+  return vector && cg % v == 0 && vecs <= kSlabVecs * kSlabThreads && slab_kb * weight <= 85 + 4.2 * all_mb &&
+         (int64_t)p.B * p.G <= INT32_MAX / kSlabThreads;   // (a launch holds less than 2^32 threads)
+}
+
+template <typename T>
+void run(Params& p, bool vector, hipStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  if (slab_way(p, sizeof(T), vector)) {
+    slab<T>(p, (int64_t)p.T * (p.C / p.G / V), stream);
   } else if (vector) {
     plan_passes(p, V);
     passes<T, V>(p, stream);
@@ -656,8 +662,6 @@ SIDON_API int sidon_group_norm_act(const void* x, int64_t ldx, const int32_t* le
                 sidon_group_norm_workspace_bytes(B, T, C, G, dtype));
   if (!(x == y && ldx == ldy) && sidon::rows_meet(x, ldx * size, C * size, y, ldy * size, C * size, rows))
     return fail(SIDON_E_SHAPE, "y may be x itself but must not overlap it otherwise");
-  int rc;
-  if ((rc = sidon::check_device())) return rc;
   Params p{};
   p.x = x;
   p.lens = lens;
@@ -676,6 +680,26 @@ SIDON_API int sidon_group_norm_act(const void* x, int64_t ldx, const int32_t* le
   const int v = 16 / size;
   const bool vector = C % v == 0 && ldx % v == 0 && ldy % v == 0 && sidon::aligned16(x) && sidon::aligned16(y) &&
                       sidon::aligned16(w) && sidon::aligned16(bias);
+  // Workgroups read w, bias and lens while others already write y; ws is written beside
+  // all of them, where the call takes two launches.
+  const struct {
+    const void* at;
+    int64_t bytes;
+  } in[] = {{w, (int64_t)C * 4}, {bias, (int64_t)C * 4}, {lens, lens ? (int64_t)B * 4 : 0}};
+  const bool ws_used = !slab_way(p, size, vector);
+  const int64_t ws_need = (int64_t)sidon_group_norm_workspace_bytes(B, T, C, G, dtype);
+  for (const auto& t : in) {
+    if (t.bytes == 0) continue;
+    if (sidon::row_meets(y, ldy * size, (int64_t)C * size, rows, t.at, t.bytes))
+      return fail(SIDON_E_SHAPE, "y must not overlap w, bias or lens");
+    if (ws_used && sidon::ranges_meet(ws, ws_need, t.at, t.bytes))
+      return fail(SIDON_E_SHAPE, "ws must not overlap w, bias or lens");
+  }
+  if (ws_used && (sidon::row_meets(x, ldx * size, (int64_t)C * size, rows, ws, ws_need) ||
+                  sidon::row_meets(y, ldy * size, (int64_t)C * size, rows, ws, ws_need)))
+    return fail(SIDON_E_SHAPE, "ws must not overlap x or y");
+  int rc;
+  if ((rc = sidon::check_device())) return rc;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == SIDON_FP32) {
     run<float>(p, vector, s);

@@ -35,6 +35,13 @@ inline bool ranges_meet(const void* a, int64_t a_bytes, const void* b, int64_t b
   const uintptr_t ab = reinterpret_cast<uintptr_t>(a), bb = reinterpret_cast<uintptr_t>(b);
   return ab < bb + (uintptr_t)b_bytes && bb < ab + (uintptr_t)a_bytes;
 }
+// Whether `rows` rows of `width` bytes, `pitch` apart, share memory with a range: one
+// between two rows does not.
+inline bool row_meets(const void* a, int64_t pitch, int64_t width, int64_t rows, const void* b, int64_t bytes) {
+  if (!ranges_meet(a, (rows - 1) * pitch + width, b, bytes)) return false;
+  const int64_t on = (int64_t)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));
+  return on < 0 || on % pitch < width || on % pitch + bytes > pitch;
+}
 // Whether `rows` rows of a_width and b_width bytes, a_pitch and b_pitch apart, share
 // memory.  Column blocks of one wider tensor do not, though their ranges meet.
 inline bool rows_meet(const void* a, int64_t a_pitch, int64_t a_width, const void* b, int64_t b_pitch, int64_t b_width,

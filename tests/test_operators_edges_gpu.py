@@ -171,6 +171,29 @@ def test_a_single_rows_stride_means_nothing(sidon, stride):
     assert torch.equal(sidon.conformer.group_norm_act(row(x), 1, 8, w, b), sidon.conformer.group_norm_act(x, 1, 8, w, b))
 
 
+def test_attention_refuses_a_workspace_over_its_operands(sidon):
+    """(On a device: the workspace that a call needs depends on it.)"""
+    q, k, v, lam, norm_w = attention_test.inputs(1, 8, 8, 1, 4800, 64, torch.float16, 3)
+    need = sidon.diff_attention.workspace_bytes(1, 8, 8, 1, 4800, 64, DEV)
+    out = torch.empty(1, 8, 1, 128, dtype=torch.float16, device=DEV)
+    lens = torch.tensor([4800], dtype=torch.int32, device=DEV)
+    assert need > 0
+    for t in (q, k, v, lam, norm_w, lens, out):
+        ws = torch.as_strided(t, (1,), (1,)).view(torch.uint8).untyped_storage()
+        if ws.nbytes() < need:   # the workspace begins at the operand and goes on behind it
+            buf = torch.empty(need + 4096, dtype=torch.uint8, device=DEV)
+            n = t.numel() * t.element_size()
+            moved = buf[:n].view(t.dtype).view(t.shape).copy_(t)
+            ws = buf
+        else:
+            moved, ws = t, torch.empty(0, dtype=torch.uint8, device=DEV).set_(ws)
+        a = {"q": q, "k": k, "v": v, "lam": lam, "norm_w": norm_w, "lens": lens, "out": out}
+        name = next(n for n, x in a.items() if x is t)
+        a[name] = moved
+        with pytest.raises(RuntimeError, match="apart"):
+            sidon.diff_attention.diff_attention(**a, lam_init=0.3, workspace=ws)
+
+
 def calls(sidon, seed):
     """One call of each operator with its workspace -> [(call, workspace bytes)]; call(workspace) -> the output."""
     x, w, b = norm_test.inputs(4000, 512, torch.float16, seed)

@@ -199,6 +199,45 @@ def test_column_blocks_of_one_tensor(sidon):
     assert _norm(lib, x=1 << 22, ldx=128, y=(1 << 22) - 256 * 3 + 128, ldy=128) == -6
 
 
+MB = 1 << 20
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("over", [
+    dict(ids=96 * MB), dict(ids=96 * MB + 1024), dict(scale=96 * MB + 2048), dict(scale=96 * MB - 4),
+    *[dict(ws=n * MB + 64) for n in (16, 32, 64, 80)], dict(ws=16 * MB - 16), dict(ids=128 * MB + 16),
+    dict(scale=128 * MB + 4),
+], ids=str)
+def test_adapter_calls_refuse_overlaps(sidon, residual, over):
+    """y over what other workgroups still read, ws over an input."""
+    lib = sidon._lib.load()
+    assert _adapter(lib, residual, **over) == -2
+    assert "overlap" in lib.sidon_last_error().decode()
+
+
+def test_workspaces_and_outputs_refuse_overlaps(sidon):
+    lib = sidon._lib.load()
+    assert _adapter(lib, False, ws=48 * MB) == -2 and _adapter(lib, True, ws=112 * MB) == -2
+    one = dict(w=8 * MB, b=9 * MB, ws=10 * MB)
+    for over in (dict(w=1 << 22), dict(b=(1 << 22) + 16), dict(lens=(1 << 22) + 4)):
+        assert _norm(lib, **{**one, **over}) == -2
+    two = dict(x=16 * MB, y=64 * MB, T=100000, lens=11 * MB, **one)   # two launches
+    for ws in (8 * MB, 9 * MB, 11 * MB, 16 * MB + 64, 64 * MB):
+        assert _norm(lib, **{**two, "ws": ws}) == -2
+        assert "overlap" in lib.sidon_last_error().decode()
+    apart = dict(q=1 << 30, k=1 << 31, v=1 << 32, out=1 << 33, lam=16, norm_w=4096, lens=8192)
+    for over in (dict(lam=(1 << 33) + 64), dict(norm_w=(1 << 33) + 64), dict(lens=(1 << 33) + 64)):
+        assert _attention(lib, **{**apart, **over}) == -2
+        assert "apart" in lib.sidon_last_error().decode()
+    if torch.cuda.is_available():
+        return   # (fake addresses: below, only where no device would take the launch)
+    # between the rows of a wider tensor, and a workspace that the call does not use
+    assert _adapter(lib, False, ldy=512, ids=96 * MB + 512, scale=96 * MB + 1024 + 512) == -6
+    assert _adapter(lib, False, ldx=1 << 16, ws=16 * MB + 1024) == -6
+    assert _norm(lib, **two) == -6 and _norm(lib, ws=1 << 20) == -6
+    assert _attention(lib, **apart) == -6
+
+
 def test_adapter_workspace_and_packing(sidon):
     ws = sidon.adapters.workspace_bytes
     assert ws(100, 16) == 3200 and ws(100, 16, True) == 6400 and ws(100, 16, True, torch.bfloat16) == 9600
