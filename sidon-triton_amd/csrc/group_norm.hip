@@ -22,7 +22,9 @@
 //
 // Statistics never form a difference of large sums: every thread takes the
 // mean of what it holds and the squares around that mean, and partial results
-// (n, mean, M2) are joined by  M2 = sum M2_i + n_i (mean_i - mean)^2, in fp32.
+// (n, mean, M2) are joined by  M2 = sum M2_i + n_i (mean_i - mean)^2, in fp32, the
+// count multiplied in before the square: one of 0 leaves 0 also where the square
+// of a mean past 2^63 would be infinite.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(kThreads) gn_stat_kernel(const Params p) {
         }
         const float delta = m - mean[u];
         mean[u] = fmaf(delta, frac, mean[u]);
-        m2[u] += q + delta * delta * (have * frac);
+        m2[u] += q + delta * (delta * (have * frac));
       }
       have += more;
     }
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(kThreads) gn_stat_kernel(const Params p) {
       const int i = u / cols;
       const float2 v = unit[i * stride + g * cols + u - i * cols];
       const float d = v.x - mean;
-      q += fmaf(d * d, count(i), v.y);
+      q += fmaf(d, d * count(i), v.y);
     }
     const float m2 = team_sum(q, team);
     if (tl == 0) out[g] = make_float2(mean, m2);
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kThreads) gn_apply_kernel(const Params p) {
         const float cnt = (float)(min(p.rows_per_chunk, n - c * p.rows_per_chunk)) * (float)cg;
         const float2 v = part[(int64_t)c * p.G + g];
         const float d = v.x - mean;
-        q += fmaf(d * d, cnt, v.y);
+        q += fmaf(d, d * cnt, v.y);
       }
       const float var = team_sum(q, team) * inv_n;
       if (tl == 0) stat[g] = make_float2(mean, rsqrtf(var + p.eps));

@@ -127,6 +127,22 @@ def test_large_mean(sidon, shape):
     check(y, want, scale, torch.float32)
 
 
+@pytest.mark.parametrize("shape", [(2, 40, 64, 4), (2, 3000, 512, 2), (1, 1463, 100, 25), (3, 1500, 36, 4)], ids=str)
+def test_far_from_zero(sidon, shape):
+    """Values whose squares leave fp32, whose variance does not."""
+    batch, t, c, groups = shape
+    gen = torch.Generator().manual_seed(2)
+    x = (torch.randn(batch * t, c, generator=gen) * 1e16 + 3e20).to(DEV)
+    w, b = torch.ones(c, device=DEV), torch.zeros(c, device=DEV)
+    lens = [max(1, t - 37 * i) for i in range(batch)]
+    y = sidon.conformer.group_norm_act(x, batch, groups, w, b, lens=torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                       act=None)
+    want, _ = reference(x, batch, groups, w, b, 1e-5, lens, None)
+    assert torch.isfinite(y).all()
+    # the fp32 chain's share of the module's bound, 2^-19 of (|x| + |mean|) rstd (about 6e4)
+    assert ((y.double() - want).abs() <= 2.0 ** -19 * 6.2e4).all()
+
+
 @pytest.mark.parametrize("c,groups", [(256, 8), (256, 1)])
 def test_views(sidon, c, groups):
     """Rows of a wider tensor, unaligned columns, the output beside the input,
