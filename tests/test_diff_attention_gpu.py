@@ -149,6 +149,32 @@ def test_small_probabilities(sidon, shape, kind):
     check(got, *reference(q, k, v, lam, 0.3, None, False, None, 1e-5))
 
 
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(64, 1, 1, 1, 8, 64), (16, 8, 2, 5, 7, 128), (16, 2, 2, 32, 8, 64), (20, 3, 1, 9, 33, 64)],
+                         ids=str)
+def test_few_rows_keep_two_summands(sidon, shape, kind):
+    """Up to 32 rows of a key head: two maps that nearly cancel, so that what the
+    probabilities lose is far more than the output's rounding.  Two summands of a
+    type keep u^2 of each.  Scores of products below 1 (D of them, over sqrt D, to
+    2^-24 each) and exp2 move a probability by less than 2^-15 of itself.  (One
+    summand would be 7 times over this bound in fp16, 30 times in bf16.)"""
+    b, h, hk, l, s, d = shape
+    q, k, v, lam, _ = inputs(*shape, kind, 21)
+    q, k = (0.5 * q.float()).to(kind), (0.5 * k.float()).to(kind)
+    gen = torch.Generator().manual_seed(22)
+    q[:, :, 1], k[:, :, 1] = q[:, :, 0], k[:, :, 0] + (0.01 * torch.randn(b, hk, s, d, generator=gen)).to(kind).to(DEV)
+    lam = torch.zeros_like(lam)
+    got = sidon.diff_attention.diff_attention(q, k, v, lam, 1.0).double()
+    u = torch.finfo(kind).eps / 2
+    maps = torch.softmax(torch.matmul(q.double(), k.double().repeat_interleave(h // hk, 1).transpose(-1, -2).contiguous())
+                         / math.sqrt(d), -1)
+    vals = v.double().repeat_interleave(h // hk, 1)
+    want = torch.matmul(maps[:, :, 0] - maps[:, :, 1], vals)
+    size = torch.matmul(maps[:, :, 0] + maps[:, :, 1], vals.abs())
+    tiny = 2.0 ** -24 if kind == torch.float16 else 2.0 ** -100
+    assert ((got - want).abs() <= (u * u + 2.0 ** -15) * size + u * want.abs() + tiny).all()
+
+
 @pytest.mark.parametrize("l", [1, 300])
 def test_strides_and_out(sidon, l):
     """[B, H, 2, L, D] contiguous, key rows and heads in other orders, an output

@@ -221,6 +221,40 @@ def test_adapted_encoder_against_merged_weights(sidon):
             assert torch.equal(out[b, :n], want[b, :n])
 
 
+def test_adapted_encoder_at_its_own_width(sidon):
+    """Hidden 1024 (16 heads), feed-forward 4096, one layer, where the projections
+    take the wide tiles, with a captured call on the encoder's own workspace."""
+    weights = encoder_weights(16, 1, seed=6, inter_mult=4)
+    packed = sidon.encoder.pack_weights(weights)
+    enc = sidon.encoder.HipEncoder(packed, DEV)
+    gen = torch.Generator().manual_seed(5)
+    low = {n: (torch.randn(8, w.shape[1], generator=gen) * w.shape[1] ** -0.5, torch.randn(w.shape[0], 8, generator=gen) * 0.2)
+           for n in ("ffn1_w1", "ffn1_w2", "q_w", "k_w", "v_w", "out_w", "pw2_w", "ffn2_w1", "ffn2_w2")
+           for w in (weights["layers"][0][n],)}
+    tuned = (0.5, [low])
+    adapters = sidon.encoder.pack_adapters(packed, [(1.0, [{}]), tuned], device=DEV)
+    lens, ids = [400, 333, 150], [1, -1, 1]
+    feats = encoder_features(3, 400, 9).float().to(DEV)
+    frames = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    which = torch.tensor(ids, dtype=torch.int32, device=DEV)
+    ws = enc.workspace(3 * 400, rank=24)
+    got = enc(feats, frames, workspace=ws, adapters=adapters, ids=which).clone()
+    for b, (n, e) in enumerate(zip(lens, ids)):
+        want = encoder_reference(feats[b:b + 1].double().cpu(), weights if e < 0 else merged(weights, tuned), [n],
+                                 dtype=torch.float64)[0, :n]
+        assert snr(want, got[b, :n]) > 60, b
+    out = torch.empty_like(got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        enc(feats, frames, out=out, workspace=ws, adapters=adapters, ids=which)
+    for _ in range(3):
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for b, n in enumerate(lens):
+            assert torch.equal(out[b, :n], got[b, :n])
+
+
 def test_adapted_encoder_refusals(sidon):
     weights = encoder_weights(2, 2, seed=4)
     packed = sidon.encoder.pack_weights(weights)
