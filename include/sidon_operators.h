@@ -114,12 +114,16 @@ int sidon_adapter_residual(const void* x, int ldx, const void* w, int ldw, const
  * another, and the memory from its first to its last element must hold nothing of
  * an input; neither must ws.
  *
- * Scores, softmax statistics, sums and the norm in fp32, probabilities rounded to
- * `dtype` in front of the product with v: each off by half a step of itself, in
- * fp16 down to 2^-23 of the row's largest, and none below 2^-34 of it (with few rows
- * what the rounding left is
- * multiplied too), one rounding at the end.  What a key within LK but past a
- * query's own position holds must be finite (its weight is 0).  ws:
+ * Scores, softmax statistics, sums and the norm in fp32; scores |q . k| / sqrt D up to
+ * 2^24 (their fp32 steps past it are more than the softmax takes).  Probabilities are
+ * rounded to `dtype` in front of the product with v: each off by half a step of itself,
+ * in fp16 down to 2^-23 of the row's largest, and none below 2^-34 of it.  With H / Hk * L
+ * <= 32 what the rounding left is multiplied too, and the result is off by its own
+ * rounding; with more it may be or not, as the kernel that is fastest for B, L, S and the
+ * device has it, so the same prompt can be rounded differently in another batch.  One
+ * rounding at the end.  A query that is no number (or whose scores are none) gives NaN
+ * and reaches no other.  What a key within LK but past a query's own position holds must
+ * be finite (its weight is 0).  ws:
  * sidon_diff_attention_workspace_bytes bytes for these sizes on the current
  * device (0: ws may be NULL), 16-byte aligned, contents irrelevant.
  */

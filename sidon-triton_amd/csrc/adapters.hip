@@ -12,7 +12,8 @@
 // Rows of different adapters share tiles: the shared product does not see
 // them, and the low-rank terms cost a product per adapter among a block's rows.
 // Few rows are bound by the two launches' latencies, many by the shared product
-// (4800 x 4096 x 1024 0.74 PFLOP/s with the low-rank term, rank 64).
+// (4800 x 4096 x 1024 0.74 PFLOP/s with the low-rank term, rank 64), many items of a
+// few rows by the lanes' own reads of b (300 x 1 x 4096 x 1024: rank 8 17 us, 64 73, 128 142).
 #include "gemm_tile.h"
 
 #include "sidon_host.h"
@@ -213,10 +214,10 @@ struct ExpandKernel {
 
 // gemm.hip's shapes, half of them: what the rest would gain is small next to the
 // low-rank term.  us, of it the shrink launch, and the shared projection alone
-// (conformer.linear_silu_lt, residual_gemm): 1 x 1024 x 1024 rank 16 9.3 (2.5) | 5.8,
-// 48 rows of 43 adapters x 4096 x 1024 rank 16 12.6 (3.3) | 6.0, 4 x 400 x 2048 x 1024
-// rank 32 18.8 (4.7) | 12.3, 8 x 600 x 4096 x 1024 rank 64 59 (8.5) | 51-57, rank 16 56 |
-// 51, residual 3 x 1463 x 1024 x 4096 rank 16 56 (11) | 40.  The shared projection's
+// (conformer.linear_silu_lt, residual_gemm): 1 x 1024 x 1024 rank 16 9.0 (2.6) | 5.8,
+// 48 rows of 43 adapters x 4096 x 1024 rank 16 12.2 (3.3) | 6.0, 4 x 400 x 2048 x 1024
+// rank 32 20.3 (5.0; bf16 19.0) | 12.3, 8 x 600 x 4096 x 1024 rank 64 59 (9.0; fp16 64) |
+// 51-57, rank 16 56 | 51, residual 3 x 1463 x 1024 x 4096 rank 16 57.5 (11.3) | 40.  The shared projection's
 // cost picks the tile: on 5000 calls, each timed with every tile, 1% over the best on average.
 const ExpandKernel kExpand[] = {
     SIDON_BOTH(32, 64, 2, 2, 16, 6),   SIDON_BOTH(64, 64, 2, 2, 16, 4),   SIDON_BOTH(64, 128, 2, 4, 16, 4),

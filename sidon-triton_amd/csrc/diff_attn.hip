@@ -31,16 +31,19 @@
 //
 // Two forms: 64 rows on one ring, and 32 rows for few (D 64: on two rings of every
 // other step, which one workgroup's latency hides; D 128: on one, two workgroups a CU).
-// Measured (D 64, fp16 or bf16, whole calls in a graph):
-//   1 x 8 heads x 4800 x 4800        167 us, 846 TFLOP/s (a large matrix product: 1330)
-//   3 x 8 heads (2 key heads) x 1037, D 128, ragged, causal   43 us
-//   32 x 16 heads (4 key heads) x 1 x 6000, ragged   42 us, 4.8 TB/s (a large copy: 5.0)
-//   1 x 8 heads x 1 x 4800           10.6 us, two launches
+// Measured (D 64, fp16 or bf16, whole calls in a graph, on the same operands again and
+// again | on others each time, past the 256 MB of the Infinity Cache):
+//   1 x 8 heads x 4800 x 4800        170 | 172 us, 834 TFLOP/s (a large matrix product: 1330)
+//   3 x 8 heads (2 key heads) x 1037, D 128, ragged, causal   42 | 43 us
+//   32 x 16 heads (4 key heads) x 1 x 6000, ragged   42 | 56 us: 3.6 TB/s from memory (a large copy: 5.0)
+//   1 x 8 heads x 1 x 4800           10.2 | 14.3 us, two launches
 // Prompts are bound by the vector unit's exponentials and roundings beside the
 // matrix core (16 exponentials per two 32x32x16 score products and four value
 // products), and by whole workgroups: 600 on 256 CUs are three on the busiest.
-// Single tokens are bound by memory once the cache is large, by launches and the
-// first copies' latency where it is small.
+// The 64-row form at D 128 has more values than its 256 registers hold (88 bytes of
+// scratch a lane) and one wavefront on most SIMDs: its rounds wait for one another.
+// Single tokens against a large cache wait for memory, whose copies drain at every
+// round; against a small one for launches and the first copies' latency.
 #include <hip/hip_runtime.h>
 
 #include <float.h>

@@ -17,8 +17,8 @@
 // Measured, whole calls in a graph: 1 x 150 x 1024 fp16 in 32 groups 4.4 us (slab: one
 // launch, a few memory latencies), 3 x 1463 x 1024 bf16 in 16 groups with GELU 14 us
 // (passes: two launches, the second's arithmetic), 8 x 4800 x 1024 fp32 in 32 groups
-// 83-86 us (passes: x and y once at 3.7 TB/s; half of x's second reading comes from
-// the caches; a copy of x takes 60).
+// 83-87 us on the same x again and again, which the Infinity Cache holds half of, 106-108
+// on another x each time (passes: x twice and y once at 4.4 TB/s; a copy of x takes 63).
 //
 // Statistics never form a difference of large sums: every thread takes the
 // mean of what it holds and the squares around that mean, and partial results

@@ -112,9 +112,13 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     gives zeros.  norm_w fp32 [2D]: each head's output is divided by its root
     mean square (with eps > 0 under the root) and multiplied by (1 - lam_init)
     norm_w; None: left as it is.  out: optional [B, H, L, 2D], in memory apart from
-    q, k and v.  workspace: a contiguous
-    uint8 tensor of ``workspace_bytes``; allocated per call when None.  A single
-    query against a long cache splits the keys over the chip.  Forward only."""
+    the inputs.  workspace: a contiguous uint8 tensor of ``workspace_bytes``, apart
+    from all of them; allocated per call when None.  A single query against a long
+    cache splits the keys over the chip.  Valid keys and values must be finite, also
+    those that causal hides from some queries.  Probabilities are rounded to the
+    inputs' type in front of v, but with H / Hk * L <= 32 (single tokens), where the
+    output's rounding is the only one; with more that depends on all sizes.  Forward
+    only."""
     key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype,
            v.device, lam.shape, lam.stride(), lam.dtype, lam.device,
            None if lens is None else (lens.shape, lens.stride(), lens.dtype, lens.device),
