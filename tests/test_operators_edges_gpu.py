@@ -116,6 +116,20 @@ def test_attention_of_long_caches(sidon, shape):
     attention_test.check(got, *attention_test.reference(q, k, v, lam, 0.3, lens, True, norm_w, 1e-5))
 
 
+@pytest.mark.parametrize("shape", [(1, 2, 1, 1, 262144, 64), (2, 2, 2, 1, 40000, 128), (1, 1, 1, 70, 120000, 64)], ids=str)
+def test_attention_of_long_fp16_caches(sidon, shape):
+    """Scores of a few standard deviations more than the others' in some keys: what
+    the rest is worth lies below fp16's smallest normal number relative to them."""
+    b, h, hk, l, s, d = shape
+    q, k, v, lam, norm_w = attention_test.inputs(b, h, hk, l, s, d, torch.float16, 9)
+    k[:, :, :, ::911] *= 3
+    lens = [s, s - 4321][:b]
+    attention_test.poison(k, v, lens)
+    got = sidon.diff_attention.diff_attention(q, k, v, lam, 0.3, lens=torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                              causal=True, norm_w=norm_w)
+    attention_test.check(got, *attention_test.reference(q, k, v, lam, 0.3, lens, True, norm_w, 1e-5))
+
+
 def test_group_norm_past_32_bits(sidon):
     x, w, b = norm_test.inputs(60, 256, torch.float16, 6)
     lens = torch.tensor([30, 17], dtype=torch.int32, device=DEV)
