@@ -49,6 +49,7 @@
 #include <float.h>
 #include <stdint.h>
 
+#include "attn_device.h"
 #include "flexrel_device.h"
 #include "sidon_host.h"
 #include "sidon_operators.h"
@@ -59,16 +60,10 @@
 
 namespace {
 
-using namespace sidon_flexrel;
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-typedef int i4 __attribute__((ext_vector_type(4)));
+using namespace sidon_attn;
 
 constexpr int kBlock = 32;          // rows per wavefront
-constexpr float kFloorMax = -1e30f; // a running maximum that no key has raised yet (finite: -inf - -inf is NaN)
 constexpr int kMaxGridSplits = 64;
-constexpr int kBack = 3 * 1024;     // bytes that the copies' offsets hold beyond their rows (dma_tile's last copy adds none)
 
 struct DiffParams {
   const void* q;
@@ -91,67 +86,6 @@ struct DiffParams {
   float scale;           // log2(e) / sqrt(D)
   float lam_init, eps;
 };
-
-template <typename E>
-struct Half;
-template <>
-struct Half<_Float16> {
-  typedef h8 v8;
-  typedef h2 v2;
-  typedef h4 v4;
-  // The running maximum stands for a probability of 2^kLift, not of 1, so that
-  // probabilities keep their 11 bits down to 2^-23 of the largest and vanish below
-  // 2^-34 (with 1: 2^-14 and 2^-25, which the keys of a long cache add up to).  A
-  // step's 32 sum to 2^14 at most, under what raises the maximum.
-  static constexpr float kLift = 9.f;
-  static __device__ __forceinline__ f32x16 mfma(i4 a, i4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f4 small(i4 a, i4 b, f4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-  }
-};
-template <>
-struct Half<__bf16> {
-  typedef b8 v8;
-  typedef b2 v2;
-  typedef b4 v4;
-  static constexpr float kLift = 0.f;   // (as many exponents as fp32)
-  static __device__ __forceinline__ f32x16 mfma(i4 a, i4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f4 small(i4 a, i4 b, f4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-  }
-};
-
-// A pointer that is the same in every lane, in scalar registers (the copies
-// take it there, and under pressure the compiler forms it in vector ones).
-__device__ __forceinline__ const char* uniform(const char* x) {
-  const uint64_t u = reinterpret_cast<uint64_t>(x);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)u);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
-  return reinterpret_cast<const char*>((uint64_t)hi << 32 | lo);
-}
-
-// x of lane l plus x of lane l ^ 32.
-__device__ __forceinline__ float pair_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-// Two copies as dma_1k's, the second 1024 beyond both addresses.
-__device__ __forceinline__ void dma_2k(uint32_t lds_addr, const char* gbase, uint32_t v0, uint32_t v1) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %3\n\t"
-      "global_load_lds_dwordx4 %2, %3 offset:1024"
-      :: "s"(lds_addr), "v"(v0), "v"(v1), "s"(gbase) : "memory", "m0");
-}
-#pragma clang diagnostic pop
 
 // The learned weight of head h, in every lane of a wavefront.
 template <int D>
@@ -802,30 +736,6 @@ size_t part_bytes(int B, int Hk, int R, int D, int splits) {
   return splits > 1 ? (size_t)B * Hk * R * splits * (16 + (size_t)D * 16) : 0;
 }
 
-// Elements from the first to past the last of sizes n and strides st, with `last` contiguous ones.
-__int128 span(const int* n, const int64_t* st, int dims, int last) {
-  __int128 e = last;
-  for (int i = 0; i < dims; ++i) e += (__int128)(n[i] - 1) * st[i];
-  return e;
-}
-
-// Whether rows of `last` elements lie apart: in the order of their strides, every
-// dimension steps past all that the ones before it cover.
-bool apart(const int* n, const int64_t* st, int dims, int last) {
-  __int128 covered = last;
-  bool used[3] = {};
-  for (int k = 0; k < dims; ++k) {
-    int at = -1;
-    for (int i = 0; i < dims; ++i)
-      if (!used[i] && (at < 0 || st[i] < st[at])) at = i;
-    used[at] = true;
-    if (n[at] == 1) continue;
-    if (st[at] < covered) return false;
-    covered += (__int128)(n[at] - 1) * st[at];
-  }
-  return true;
-}
-
 template <typename E>
 void launch(const DiffParams& p, int D, int rows, hipStream_t stream) {
   const dim3 grid((unsigned)(8 * p.parts_per_xcd * ((p.blocks * p.splits + p.parts - 1) / p.parts)));
@@ -902,11 +812,11 @@ SIDON_API int sidon_diff_attention(const void* q, const void* k, const void* v, 
   Range in[7];
   {
     const int qn[] = {B, H, 2, L}, kn[] = {B, Hk, 2, S}, vn[] = {B, Hk, S}, on[] = {B, H, L};
-    if (!apart(on, o_strides, 3, 2 * D)) return fail(SIDON_E_STRIDE, "rows of out overlap one another");
-    const __int128 most = (__int128)1 << 61, o_span = span(on, o_strides, 3, 2 * D) * 2;
-    in[0] = Range{q, span(qn, q_strides, 4, D) * 2, "q"};
-    in[1] = Range{k, span(kn, k_strides, 4, D) * 2, "k"};
-    in[2] = Range{v, span(vn, v_strides, 3, 2 * D) * 2, "v"};
+    if (!sidon::apart(on, o_strides, 3, 2 * D)) return fail(SIDON_E_STRIDE, "rows of out overlap one another");
+    const __int128 most = (__int128)1 << 61, o_span = sidon::span(on, o_strides, 3, 2 * D) * 2;
+    in[0] = Range{q, sidon::span(qn, q_strides, 4, D) * 2, "q"};
+    in[1] = Range{k, sidon::span(kn, k_strides, 4, D) * 2, "k"};
+    in[2] = Range{v, sidon::span(vn, v_strides, 3, 2 * D) * 2, "v"};
     in[3] = Range{lam, (__int128)lam_heads * D * 16, "lam"};
     in[4] = Range{norm_w, norm_w ? D * 8 : 0, "norm_w"};
     in[5] = Range{lens, lens ? (__int128)B * 4 : 0, "lens"};

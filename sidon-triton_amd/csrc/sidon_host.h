@@ -53,4 +53,60 @@ inline bool rows_meet(const void* a, int64_t a_pitch, int64_t a_width, const voi
   return on < a_width || a_pitch - on < b_width;
 }
 
+// Elements from the first to past the last of sizes n and strides st, with `last` contiguous ones.
+inline __int128 span(const int* n, const int64_t* st, int dims, int last) {
+  __int128 e = last;
+  for (int i = 0; i < dims; ++i) e += (__int128)(n[i] - 1) * st[i];
+  return e;
+}
+
+// Whether rows of `last` elements lie apart: in the order of their strides, every
+// dimension steps past all that the ones before it cover.
+inline bool apart(const int* n, const int64_t* st, int dims, int last) {
+  __int128 covered = last;
+  bool used[3] = {};
+  for (int k = 0; k < dims; ++k) {
+    int at = -1;
+    for (int i = 0; i < dims; ++i)
+      if (!used[i] && (at < 0 || st[i] < st[at])) at = i;
+    used[at] = true;
+    if (n[at] == 1) continue;
+    if (st[at] < covered) return false;
+    covered += (__int128)(n[at] - 1) * st[at];
+  }
+  return true;
+}
+
+// Rows of `last` elements of `size` bytes over (batch, head, row), with element strides.
+struct Rows {
+  const void* at;
+  int n[3];
+  int64_t st[3];
+  int last, size;
+  __int128 bytes() const { return span(n, st, 3, last) * size; }
+};
+// Whether two such tensors may share memory.  Column blocks of one wider tensor do
+// not, though their ranges meet: where every (batch, row) step of both is a multiple
+// of the smallest one, the heads of each stay within it, and so do their columns.
+inline bool tensors_meet(const Rows& a, const Rows& b) {
+  if (!ranges_meet(a.at, (int64_t)a.bytes(), b.at, (int64_t)b.bytes())) return false;
+  int64_t pitch = 0;
+  for (const Rows* t : {&a, &b})
+    for (const int d : {0, 2})
+      if (t->n[d] > 1 && t->st[d] > 0 && (pitch == 0 || t->st[d] * t->size < pitch)) pitch = t->st[d] * t->size;
+  if (pitch == 0) return true;
+  int64_t width[2];
+  int i = 0;
+  for (const Rows* t : {&a, &b}) {
+    for (const int d : {0, 2})
+      if (t->n[d] > 1 && t->st[d] * t->size % pitch != 0) return true;
+    const __int128 w = ((__int128)(t->n[1] - 1) * t->st[1] + t->last) * t->size;
+    if (w > pitch) return true;
+    width[i++] = (int64_t)w;
+  }
+  const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(b.at) - reinterpret_cast<uintptr_t>(a.at)) % pitch;
+  const int64_t on = d < 0 ? d + pitch : d;   // from a's column to b's
+  return on < width[0] || pitch - on < width[1];
+}
+
 }  // namespace sidon
