@@ -134,6 +134,124 @@ int sidon_diff_attention(const void* q, const void* k, const void* v, const floa
                          const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
                          sidon_stream_t stream);
 
+/*
+ * The norm of queries and keys for each head, with the position rotation in the
+ * same pass.  For a row x of D values (a head of one token) at place p:
+ *
+ *   y = R_p (w * x / sqrt(mean(x^2) + eps))
+ *
+ * R_p turns pairs of the first `rot` values by the angle of row p of the tables cos
+ * and sin (fp32 [places, rot / 2]): pair j is (j, j + rot / 2), or with interleaved
+ * != 0 (2 j, 2 j + 1), and becomes (a cos - b sin, a sin + b cos).  rot == 0: no
+ * rotation, tables may be NULL.  The place of token l of item b is pos[b * L + l]
+ * (int32 on the device; NULL: l, at most `places` tokens).  A token at a negative
+ * place is padding: whatever it holds, its rows become zeros and it has no part in
+ * any gradient.  One at a place past the tables gives NaN in what is rotated.
+ *
+ * q [B, H, L, D] and k [B, Hk, S, D] (Hk == 0: no k) of `dtype` with q_out and k_out
+ * of the same shapes; strides int64 arrays (batch, head, row) in elements, multiples
+ * of 16 bytes from 0 to 2^40, the last dimension contiguous.  D a multiple of 16 in
+ * [16, 256], rot one in [0, D]; q_w and k_w fp32 [D]; eps > 0.  q_out may be q itself
+ * (same strides) and k_out k, as column blocks of one tensor too; any other memory
+ * that an output shares with another operand is refused, as are outputs whose rows
+ * overlap.  Arithmetic in fp32, one rounding at the end; rows whose squares leave fp32
+ * are scaled by a power of two.
+ *
+ * sidon_qk_norm_rotary_bwd: from the gradients dq_out, dk_out of the outputs (any
+ * strides as above, 0 too) and the inputs q, k (not the outputs), the gradients dq, dk of
+ * `dtype` and dq_w, dk_w fp32 [D], which are written, not added to, and summed in the
+ * same order every time.  dq may be dq_out or q itself, dk dk_out or k.  ws:
+ * sidon_qk_norm_rotary_workspace_bytes bytes, 16-byte aligned, contents irrelevant.
+ */
+int sidon_qk_norm_rotary(const void* q, const void* k, void* q_out, void* k_out, const float* q_w, const float* k_w,
+                         const float* cos, const float* sin, int places, int rot, int interleaved,
+                         const int32_t* q_pos, const int32_t* k_pos, float eps, int B, int H, int Hk, int L, int S, int D,
+                         int dtype, const int64_t* q_strides, const int64_t* k_strides, const int64_t* q_out_strides,
+                         const int64_t* k_out_strides, sidon_stream_t stream);
+size_t sidon_qk_norm_rotary_workspace_bytes(int B, int H, int Hk, int L, int S, int D);
+int sidon_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void* q, const void* k, void* dq, void* dk,
+                             float* dq_w, float* dk_w, const float* q_w, const float* k_w, const float* cos,
+                             const float* sin, int places, int rot, int interleaved, const int32_t* q_pos,
+                             const int32_t* k_pos, float eps, void* ws, size_t ws_bytes, int B, int H, int Hk, int L,
+                             int S, int D, int dtype, const int64_t* dq_out_strides, const int64_t* dk_out_strides,
+                             const int64_t* q_strides, const int64_t* k_strides, const int64_t* dq_strides,
+                             const int64_t* dk_strides, sidon_stream_t stream);
+
+/*
+ * Attention over states of another length (a decoder's tokens over the encoder's
+ * frames).  For batch b, head h and query i < LQ = q_lens[b]:
+ *
+ *   out = sum_j softmax_j(scale q . k_j) v_j,    lse = log(sum_j exp(scale q . k_j))
+ *
+ * over the keys j < LK = lens[b] (both int32 [B] on the device, clamped to [0, S] and
+ * [0, L]; NULL = S, L).  A query that sees no key, and those from LQ on, whatever they
+ * hold, give zeros and an lse of -infinity.  Keys and values past LK are not read.
+ * Heads h / (H / Hk) share keys and values.
+ *
+ * q [B, H, L, D], k and v [B, Hk, S, D], out [B, H, L, D] of `dtype` (SIDON_FP16 or
+ * SIDON_BF16), the last dimension contiguous, the other strides int64 arrays (batch,
+ * head, row) in elements, multiples of 8 from 0 to 2^40, rows of k and v less than 2^25
+ * apart; D 64 or 128; 0 < scale <= 2^100.  lse fp32 [B, H, L] contiguous, or NULL.  out's
+ * rows must not overlap one another, and out, lse and ws hold nothing of another operand
+ * (out may be a column block of one tensor with q).
+ *
+ * Scores, softmax statistics and sums in fp32; |scale q . k| up to 2^24.  Probabilities
+ * are rounded to `dtype` in front of the product with v: each off by half a step of
+ * itself, in fp16 down to 2^-23 of the row's largest, and none below 2^-34 of it.  With
+ * H / Hk * L <= 32 what the rounding left is multiplied too, and the result is off by
+ * its own rounding; with more it may be or not, as the kernel that is fastest for the
+ * sizes and the device has it.  One rounding at the end.  lse sums what was not rounded.
+ * A query that is no number gives NaN and reaches no other.  ws:
+ * sidon_cross_attention_workspace_bytes bytes for these sizes on the current device
+ * (0: ws may be NULL), 16-byte aligned, contents irrelevant.
+ *
+ * sidon_cross_attention_bwd: the gradients dq [B, H, L, D], dk and dv [B, Hk, S, D] of
+ * `dtype` from the output's, dout, and the forward call's q, k, v, out and lse under the
+ * same lens, q_lens and scale; written, not added to; zeros past LQ and LK.  Rows of
+ * dout and q less than 2^25 apart, S <= 2^24, B * H <= 2^20, the rest as above; an output
+ * may be a column block of one tensor with another operand, and shares no memory
+ * otherwise.  What dout holds past LQ does not matter.  Products in
+ * `dtype` with fp32 sums: probabilities and dS are rounded once in front of them (fp16
+ * scales both by powers of two, so that neither leaves its range whatever the size of
+ * dout).  The same bits every time.  ws: sidon_cross_attention_bwd_workspace_bytes bytes.
+ */
+size_t sidon_cross_attention_workspace_bytes(int B, int H, int Hk, int L, int S, int D);
+int sidon_cross_attention(const void* q, const void* k, const void* v, const int32_t* lens, const int32_t* q_lens,
+                          float scale, void* out, float* lse, void* ws, size_t ws_bytes, int B, int H, int Hk, int L,
+                          int S, int D, int dtype, const int64_t* q_strides, const int64_t* k_strides,
+                          const int64_t* v_strides, const int64_t* o_strides, sidon_stream_t stream);
+size_t sidon_cross_attention_bwd_workspace_bytes(int B, int H, int Hk, int L, int S, int D, int dtype);
+int sidon_cross_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                              const float* lse, const int32_t* lens, const int32_t* q_lens, float scale, void* dq,
+                              void* dk, void* dv, void* ws, size_t ws_bytes, int B, int H, int Hk, int L, int S, int D,
+                              int dtype, const int64_t* g_strides, const int64_t* q_strides, const int64_t* k_strides,
+                              const int64_t* v_strides, const int64_t* o_strides, const int64_t* dq_strides,
+                              const int64_t* dk_strides, const int64_t* dv_strides, sidon_stream_t stream);
+
+/*
+ * A projection with 4-bit weights and group scales, for few rows:
+ *
+ *   y[m, n] = act(bias[n] + sum_g s[n, g] sum_{k in g} x[m, k] (w[n, k] - z[n, g]))
+ *
+ * x [M, K], bias [N] (or NULL) and y [M, N] of `dtype` (SIDON_FP16 or SIDON_BF16), rows
+ * ldx (a multiple of 8) and ldy elements apart; x 16-byte aligned, bias and y 2-byte.  act
+ * SIDON_ACT_NONE or SIDON_ACT_SILU.  group 32, 64 or 128, K a multiple of it; M <= 2^21,
+ * N <= 2^24, K <= 2^20.  y shares no memory with an operand (it may be a column block
+ * of one tensor with x).  Sums in fp32, one rounding at the end; a row's sums of |x|
+ * over a group times 143 must be fp32 numbers.
+ *
+ * The weights w (0 to 15) and (s, z) as they are laid out once, for N and K rounded up
+ * to 16 and 128 with zeros, 16-byte aligned:
+ *   words   [N / 16][K / 128][4 q][16 r][4 i] of 32 bits: rows n = 16 t + r, and the inputs
+ *           k = 128 b + 32 i + 8 q + (0 2 4 6 1 3 5 7), a nibble each from the lowest
+ *   scales  [N / 16][K / 128][128 / group][16 r] of 32 bits: s of `dtype` in the low half, in the
+ *           high half what goes off the weight as the kernel has it, of `dtype`: z - 8 in
+ *           fp16 (with zeros == 0 taken as 0: z = 8 throughout), 128 + z in bf16
+ */
+int sidon_int4_linear(const void* x, int64_t ldx, const void* words, const void* scales, const void* bias, void* y,
+                      int64_t ldy, int M, int N, int K, int group, int zeros, int act, int dtype,
+                      sidon_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

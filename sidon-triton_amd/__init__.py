@@ -33,14 +33,20 @@ include/sidon_operators.h beside them:
     projection with a low-rank adapter per request;
   * ``diff_attention.diff_attention`` -- differential attention, prompts and
     single tokens against a cache;
-  * ``conformer.group_norm_act`` -- group norm with an activation, channels last.
+  * ``conformer.group_norm_act`` -- group norm with an activation, channels last;
+and those of a decoder that reads the encoder's states:
+  * ``head_norm.qk_norm_rotary`` -- the norm of queries and keys for each head with
+    the position rotation, and its gradients;
+  * ``cross_attention.cross_attention`` -- attention over states of another length,
+    prompts and single tokens, and its gradients;
+  * ``int4.int4_linear`` -- projections with 4-bit weights and group scales.
 
 The package directory name is not a Python identifier; the repository's
 entry scripts load it under the module name ``sidon_triton_amd``.
 """
 
-from . import (_lib, adapters, blas, conformer, diff_attention, encoder, encoder_attention, encoder_block, flexrel,
-               frontend, graphs, modeling, runtime)
+from . import (_lib, adapters, blas, conformer, cross_attention, diff_attention, encoder, encoder_attention,
+               encoder_block, flexrel, frontend, graphs, head_norm, int4, modeling, runtime)
 from .flexrel import HEAD_DIM, LEFT, NUM_POS, RIGHT, flexrel_attention
 
 __all__ = [
@@ -51,6 +57,7 @@ __all__ = [
     "adapters",
     "blas",
     "conformer",
+    "cross_attention",
     "diff_attention",
     "encoder",
     "encoder_attention",
@@ -59,6 +66,8 @@ __all__ = [
     "flexrel_attention",
     "frontend",
     "graphs",
+    "head_norm",
+    "int4",
     "modeling",
     "runtime",
     "_lib",

@@ -96,6 +96,19 @@ SIGNATURES = {
     "sidon_diff_attention": (ctypes.c_int, [_VP, _VP, _VP, _VP, ctypes.c_int, ctypes.c_float, _VP, _VP, ctypes.c_float,
                                             _VP, _VP, ctypes.c_size_t, *[ctypes.c_int] * 8, _I64P, _I64P, _I64P, _I64P,
                                             _VP]),
+    "sidon_qk_norm_rotary": (ctypes.c_int, [*[_VP] * 8, *[ctypes.c_int] * 3, _VP, _VP, ctypes.c_float,
+                                            *[ctypes.c_int] * 7, *[_I64P] * 4, _VP]),
+    "sidon_qk_norm_rotary_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
+    "sidon_qk_norm_rotary_bwd": (ctypes.c_int, [*[_VP] * 12, *[ctypes.c_int] * 3, _VP, _VP, ctypes.c_float, _VP,
+                                                ctypes.c_size_t, *[ctypes.c_int] * 7, *[_I64P] * 6, _VP]),
+    "sidon_cross_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
+    "sidon_cross_attention": (ctypes.c_int, [*[_VP] * 5, ctypes.c_float, _VP, _VP, _VP, ctypes.c_size_t,
+                                             *[ctypes.c_int] * 7, *[_I64P] * 4, _VP]),
+    "sidon_cross_attention_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 7),
+    "sidon_cross_attention_bwd": (ctypes.c_int, [*[_VP] * 8, ctypes.c_float, *[_VP] * 4, ctypes.c_size_t,
+                                                 *[ctypes.c_int] * 7, *[_I64P] * 8, _VP]),
+    "sidon_int4_linear": (ctypes.c_int, [_VP, ctypes.c_int64, _VP, _VP, _VP, _VP, ctypes.c_int64, *[ctypes.c_int] * 7,
+                                         _VP]),
     "sidon_last_error": (ctypes.c_char_p, []),
     "sidon_version": (ctypes.c_char_p, []),
 }

@@ -1,0 +1,589 @@
+// cross_attn_bwd.hip -- gradients of the attention over states of another length
+// (MI355X / gfx950).  With P_ij = exp(scale q_i . k_j - lse_i) from the forward
+// call's lse, and delta_i = dout_i . out_i (= sum_j P_ij dP_ij):
+//
+//   dv_j = sum_i P_ij dout_i          dP_ij = dout_i . v_j
+//   dS_ij = P_ij (dP_ij - delta_i)    dq_i = scale sum_j dS_ij k_j    dk_j = scale sum_i dS_ij q_i
+//
+// Three launches.  The first takes delta and lse row by row.  In the second a
+// wavefront owns 32 keys, whose k and v stay in its registers as B operands, and goes
+// over the queries of the heads that share them: S = Q . K^T and dP = dO . V^T by
+// v_mfma_f32_32x32x16, whose accumulators, rounded, are the B operands of
+// dV^T += dO^T . P and dK^T += Q^T . dS.  In the third a wavefront owns 32 queries and
+// goes over the keys: S^T = K . Q^T, dP^T = V . dO^T, dQ^T += K^T . dS^T.  (Seven
+// products where one pass would do with five and add dq up across workgroups: no
+// atomics, so the same bits every time.)  The tiles of 32 rows that the wavefronts of
+// a workgroup share are copied global -> LDS by global_load_lds_dwordx4 one step
+// ahead, and read as they are and transposed.
+//
+// fp16 holds P times 2^15, and dS times a power of two that keeps it below 2^15: the
+// bound |dS_ij| <= 2 |dout_i| |v_j| needs the longest v, and for dk the longest dout,
+// of a key head, which the first launch leaves.  bf16 has fp32's exponents.
+#include <hip/hip_runtime.h>
+
+#include <float.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "attn_device.h"
+#include "sidon_host.h"
+#include "sidon_operators.h"
+#include "sidon_wave.h"
+
+#define SIDON_API extern "C" __attribute__((visibility("default")))
+#define SIDON_INLINE __attribute__((always_inline))
+
+namespace {
+
+using namespace sidon_attn;
+
+constexpr int kBlock = 32;          // rows of a tile, rows or keys of a wavefront
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct BwdParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* out;
+  const void* dout;
+  const float* lse;      // [B, H, L]
+  void* dq;
+  void* dk;
+  void* dv;
+  const int32_t* lens;
+  const int32_t* q_lens;
+  float* stat;           // [B, H, tiles, 2, 32]: lse in powers of two (infinite: no such row), delta
+  float* length;         // [B, H, tiles, 32]: |dout_i|
+  float* longest;        // [B, H, tiles]: of a tile
+  float* longest_v;      // [B, Hk, key tiles]: |v_j|
+  int64_t qb, qh, kb, kh, vb, vh, ob, oh, gb, gh;           // strides (elements): batch, head
+  int64_t dqb, dqh, dql, dkb, dkh, dkl, dvb, dvh, dvl, ol;
+  int ql, kl, vl, gl;    // row strides (< 2^25)
+  int B, H, Hk, G, L, S;
+  int tiles, key_tiles;  // of 32 queries, of 32 keys
+  Deal deal;
+  float scale;
+};
+
+template <typename E>
+struct Range;   // P and dS are held times 2^kLift and a power of two
+template <>
+struct Range<_Float16> {
+  static constexpr bool kScaled = true;
+  static constexpr float kLift = 15.f;
+};
+template <>
+struct Range<__bf16> {
+  static constexpr bool kScaled = false;
+  static constexpr float kLift = 0.f;
+};
+
+// The power of two that keeps numbers up to 2 a b below 1 (1 where there is none).
+__device__ __forceinline__ float below_one(float a, float b) {
+  const float bound = 2.f * a * b;
+  if (!(bound > 0.f && bound < FLT_MAX)) return 1.f;
+  return __uint_as_float((253u - (__float_as_uint(bound) >> 23)) << 23);   // 2^-(exponent + 1)
+}
+
+__device__ __forceinline__ int valid(const int32_t* lens, int b, int most) {
+  return lens == nullptr ? most : __builtin_amdgcn_readfirstlane(min(max(lens[b], 0), most));
+}
+
+// ---- the first launch: a workgroup per 32 queries of a head, or (fp16) 32 keys of a key head ----
+template <typename E, int D>
+__global__ void __launch_bounds__(4 * D) cross_bwd_rows_kernel(const BwdParams p) {
+  typedef typename Half<E>::v8 v8;
+  constexpr int kTeam = D / 8;   // lanes of a row
+  __shared__ float most[D / 16];
+  const int tid = threadIdx.x, i = tid % kTeam, r = tid / kTeam;
+  const int groups = p.B * p.H * p.tiles;
+  const bool keys = (int)blockIdx.x >= groups;
+  int block = keys ? blockIdx.x - groups : blockIdx.x;
+  const int per = keys ? p.key_tiles : p.tiles, heads = keys ? p.Hk : p.H;
+  const int tile = block % per, bh = block / per, b = bh / heads, h = bh - b * heads;
+  const int row = tile * kBlock + r;
+  const int rows = keys ? valid(p.lens, b, p.S) : valid(p.q_lens, b, p.L);
+  float dot = 0.f, sq = 0.f;
+  if (row < rows) {
+    if (keys) {
+      const v8 x = *reinterpret_cast<const v8*>(static_cast<const E*>(p.v) + b * p.vb + h * p.vh + (int64_t)row * p.vl + 8 * i);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sq = fmaf((float)x[k], (float)x[k], sq);
+    } else {
+      const v8 x = *reinterpret_cast<const v8*>(static_cast<const E*>(p.dout) + b * p.gb + h * p.gh + (int64_t)row * p.gl + 8 * i);
+      const v8 y = *reinterpret_cast<const v8*>(static_cast<const E*>(p.out) + b * p.ob + h * p.oh + row * p.ol + 8 * i);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        dot = fmaf((float)x[k], (float)y[k], dot);
+        sq = fmaf((float)x[k], (float)x[k], sq);
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < kTeam; d <<= 1) {
+    dot += __shfl_xor(dot, d);
+    sq += __shfl_xor(sq, d);
+  }
+  if (!keys && i == 0) {
+    float lse = INFINITY;   // no such row, or one that sees no key: P = 0
+    if (row < rows) {
+      lse = p.lse[(int64_t)bh * p.L + row];
+      lse = lse == -INFINITY ? INFINITY : lse * kLog2e;
+    }
+    float* at = p.stat + ((int64_t)bh * p.tiles + tile) * (2 * kBlock) + r;
+    at[0] = lse;
+    at[kBlock] = dot;
+  }
+  if constexpr (Range<E>::kScaled) {
+    const float length = sqrtf(sq);
+    if (!keys && i == 0) p.length[((int64_t)bh * p.tiles + tile) * kBlock + r] = length;
+    float top = length;
+#pragma unroll
+    for (int d = kTeam; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (tid % 64 == 0) most[tid / 64] = top;
+    __syncthreads();
+    if (tid == 0) {
+      for (int k = 1; k < D / 16; ++k) top = fmaxf(top, most[k]);
+      (keys ? p.longest_v : p.longest)[(int64_t)bh * per + tile] = top;
+    }
+  }
+}
+
+// The largest of `count` numbers, by a wavefront.
+__device__ __forceinline__ float largest(const float* at, int count, int lane) {
+  float top = 0.f;
+  for (int i = lane; i < count; i += 64) top = fmaxf(top, at[i]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  return top;
+}
+
+// Copies of tiles of 32 rows x D into LDS, 1 KB copies split over W wavefronts: copy i
+// is rows 8 (i % 4) + [0, 8) of panel i / 4 (dims 64 (i / 4)).
+template <int D, int W>
+struct Copies {
+  static constexpr int kBytes = D / 64 * kTile;      // of a tile
+  static constexpr int kCount = kBytes / 1024 / W;   // per wavefront
+  static_assert(kBytes / 1024 % W == 0 && (kCount == 1 || kCount == 2), "an even split of the copies");
+  uint32_t off[kCount];
+  int crow, lane, stride;
+  uint32_t at;   // this wavefront's share of a tile in LDS
+  int panel;
+
+  __device__ __forceinline__ uint32_t offset(int j, int r) const {
+    return (uint32_t)r * (uint32_t)(2 * stride) + 16u * ((lane & 7) ^ tile_swz(crow + 8 * j)) + 1024u * (3 - j);
+  }
+  __device__ __forceinline__ void init(int w, int lane_, int stride_) {
+    lane = lane_, stride = stride_;
+    panel = w * kCount / 4;
+    crow = w * kCount % 4 * 8 + (lane >> 3);
+    at = w * kCount * 1024;
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) off[j] = offset(j, crow + 8 * j);
+  }
+  // Rows of `src` (the tile's first row) into the tile at LDS address lds; rows from
+  // `rows` on read the last one again.
+  __device__ __forceinline__ void copy(uint32_t lds, const char* src, int rows) const {
+    const char* const base = uniform(src + panel * 128 - kBack);
+    uint32_t o[kCount];
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) o[j] = rows >= kBlock ? off[j] : offset(j, min(crow + 8 * j, rows - 1));
+    if constexpr (kCount == 2) {
+      dma_2k(lds + at, base, o[0], o[1]);
+    } else {
+      dma_1k(lds + at, base, o[0]);
+    }
+  }
+};
+
+// Where a lane reads a tile: rows with bits 2 and 3 swapped as an A operand, and
+// transposed (rows 16 hh + 8 (lane / 32) + [0, 8) of dims 32 d + ...) as one.
+struct Reads {
+  int row[4], turned[2][2];
+  __device__ __forceinline__ void init(int lane) {
+    const int krow = mfma_row_perm(lane & 31), g = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) row[i] = krow * 128 + (((2 * i + g) ^ tile_swz(krow)) << 4);
+    const int G4 = lane >> 4, a = (lane >> 2) & 3, bq = lane & 3;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        const int r = 8 * (G4 >> 1) + 4 * hf + a;
+        const int chunk = 4 * db + 2 * (G4 & 1) + (bq >> 1);
+        turned[hf][db] = r * 128 + ((chunk ^ tile_swz(r)) << 4) + 8 * (bq & 1);
+      }
+  }
+  __device__ __forceinline__ i4 rows(const char* tile, int i) const {
+    return *reinterpret_cast<const i4*>(tile + row[i % 4] + i / 4 * kTile);
+  }
+  __device__ __forceinline__ i4 columns(const char* tile, int hh, int d) const {
+    typedef int i2 __attribute__((ext_vector_type(2)));
+    const char* at = tile + (d / 2) * kTile + 2048 * hh;
+    const i2 lo = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, at + turned[0][d & 1])));
+    const i2 hi = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, at + turned[1][d & 1])));
+    return i4{lo[0], lo[1], hi[0], hi[1]};
+  }
+};
+
+// An accumulator, rounded: the B operands of two products.
+template <typename E>
+__device__ __forceinline__ void round_to(const f32x16& x, i4 (&r)[2]) {
+  typedef typename Half<E>::v2 v2;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2)
+    r[i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, __builtin_convertvector(f2{x[i], x[i + 1]}, v2));
+}
+
+// Stores of an accumulator set: lane (n, g) holds of its row the values 32 d + 8 i + 4 g + [0, 4).
+template <typename E, int N>
+__device__ __forceinline__ void store(E* dst, const f32x16 (&x)[N], float by, bool there) {
+  typedef typename Half<E>::v4 v4;
+#pragma unroll
+  for (int d = 0; d < N; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = there ? (E)(x[d][4 * i + e] * by) : (E)0.f;
+      *reinterpret_cast<v4*>(dst + 32 * d + 8 * i) = r;
+    }
+}
+
+// ---- dk and dv: W wavefronts of 32 keys each ----
+template <typename E, int D, int W, int kMinWaves>
+__global__ void __launch_bounds__(64 * W, kMinWaves) cross_bwd_keys_kernel(const BwdParams p) {
+  using C = Copies<D, W>;
+  constexpr int kQ = D / 16, kDb = D / 32;
+  constexpr int kStat = 2 * kBlock * 4, kSlot = 2 * C::kBytes + kStat;   // a step's q, dout, statistics
+  __shared__ __attribute__((aligned(16))) char smem[2 * kSlot];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, g = lane >> 5;
+  int bh;
+  const int unit = dealt(p.deal, blockIdx.x, bh);
+  if (unit >= p.deal.units) return;
+  const int b = bh / p.Hk, hk = bh - b * p.Hk;
+  const int key = (unit * W + w) * kBlock + n;
+  const int lk = valid(p.lens, b, p.S), lq = valid(p.q_lens, b, p.L);
+  const int tiles = unit * W * kBlock < lk ? (lq + kBlock - 1) / kBlock : 0;   // of a head
+  const int steps = tiles * p.G;
+
+  C cq, cg;
+  cq.init(w, lane, p.ql);
+  cg.init(w, lane, p.gl);
+  const uint32_t lds = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem);
+  const char* const q0 = static_cast<const char*>(p.q) + 2 * (b * p.qb + (int64_t)hk * p.G * p.qh);
+  const char* const g0 = static_cast<const char*>(p.dout) + 2 * (b * p.gb + (int64_t)hk * p.G * p.gh);
+  int ch = 0, ct = 0;   // head of the group and tile that are copied next
+  const auto copy = [&](int slot) SIDON_INLINE {
+    if (ch < p.G) {
+      const int rows = lq - ct * kBlock;
+      const uint32_t at = lds + slot * kSlot;
+      cq.copy(at, q0 + 2 * (ch * p.qh + (int64_t)ct * kBlock * p.ql), rows);
+      cg.copy(at + C::kBytes, g0 + 2 * (ch * p.gh + (int64_t)ct * kBlock * p.gl), rows);
+      if (w == 0)
+        dma_256(at + 2 * C::kBytes,
+                uniform(reinterpret_cast<const char*>(p.stat + (((int64_t)b * p.H + hk * p.G + ch) * p.tiles + ct) * (2 * kBlock))),
+                4 * lane);
+      if (++ct == tiles) ct = 0, ++ch;
+    }
+  };
+  if (steps > 0) copy(0);
+
+  Reads at;
+  at.init(lane);
+  i4 kop[kQ], vop[kQ];
+  {
+    const int kk = max(min(key, lk - 1), 0);
+    const E* kp = static_cast<const E*>(p.k) + b * p.kb + hk * p.kh + (int64_t)kk * p.kl + 8 * g;
+    const E* vp = static_cast<const E*>(p.v) + b * p.vb + hk * p.vh + (int64_t)kk * p.vl + 8 * g;
+#pragma unroll
+    for (int s = 0; s < kQ; ++s) {
+      kop[s] = *reinterpret_cast<const i4*>(kp + 16 * s);
+      vop[s] = *reinterpret_cast<const i4*>(vp + 16 * s);
+    }
+  }
+  constexpr float kLift = Range<E>::kLift;
+  float c = 1.f;
+  if constexpr (Range<E>::kScaled)
+    c = below_one(largest(p.longest + ((int64_t)b * p.H + hk * p.G) * p.tiles, p.G * p.tiles, lane),
+                  largest(p.longest_v + (int64_t)bh * p.key_tiles, p.key_tiles, lane));
+  const float scale2 = p.scale * kLog2e;
+
+  f32x16 dk[kDb], dv[kDb];
+#pragma unroll
+  for (int d = 0; d < kDb; ++d) dk[d] = f32x16{}, dv[d] = f32x16{};
+  for (int u = 0; u < steps; ++u) {
+    wait_vmcnt<0>();
+    lds_barrier();   // step u is there, and step u - 1 is read
+    copy((u + 1) & 1);
+    const char* const tq = smem + (u & 1) * kSlot;
+    const char* const tg = tq + C::kBytes;
+    // element i of an accumulator is row 16 (i / 8) + 8 g + i % 8
+    const float* const st = reinterpret_cast<const float*>(tq + 2 * C::kBytes) + 8 * g;
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) s = Half<E>::mfma(at.rows(tq, i), kop[i], s);
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) dp = Half<E>::mfma(at.rows(tg, i), vop[i], dp);
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const f4 lse = *reinterpret_cast<const f4*>(st + 16 * (i >> 3) + (i & 7));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i + e] = fast_exp2(fmaf(s[i + e], scale2, kLift - lse[e]));
+    }
+    i4 pk[2];
+    round_to<E>(s, pk);
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int d = 0; d < kDb; ++d) dv[d] = Half<E>::mfma(at.columns(tg, hh, d), pk[hh], dv[d]);
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const f4 delta = *reinterpret_cast<const f4*>(st + kBlock + 16 * (i >> 3) + (i & 7));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i + e] *= (dp[i + e] - delta[e]) * c;
+    }
+    round_to<E>(s, pk);
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int d = 0; d < kDb; ++d) dk[d] = Half<E>::mfma(at.columns(tq, hh, d), pk[hh], dk[d]);
+  }
+  if (key >= p.S) return;
+  const bool there = key < lk;
+  const float down = fast_exp2(-kLift);
+  store<E>(static_cast<E*>(p.dk) + b * p.dkb + hk * p.dkh + key * p.dkl + 4 * g, dk, p.scale * down / c, there);
+  store<E>(static_cast<E*>(p.dv) + b * p.dvb + hk * p.dvh + key * p.dvl + 4 * g, dv, down, there);
+}
+
+// ---- dq: W wavefronts of 32 queries each ----
+template <typename E, int D, int W, int kMinWaves>
+__global__ void __launch_bounds__(64 * W, kMinWaves) cross_bwd_queries_kernel(const BwdParams p) {
+  using C = Copies<D, W>;
+  constexpr int kQ = D / 16, kDb = D / 32;
+  constexpr int kSlot = 2 * C::kBytes;   // a step's k and v
+  __shared__ __attribute__((aligned(16))) char smem[2 * kSlot];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, g = lane >> 5;
+  int bh;   // of a key head
+  const int unit = dealt(p.deal, blockIdx.x, bh);
+  if (unit >= p.deal.units) return;
+  const int b = bh / p.Hk, hk = bh - b * p.Hk;
+  const int head = hk * p.G + unit % p.G, row = (unit / p.G * W + w) * kBlock + n;
+  const int lk = valid(p.lens, b, p.S), lq = valid(p.q_lens, b, p.L);
+  const int steps = unit / p.G * W * kBlock < lq ? (lk + kBlock - 1) / kBlock : 0;
+
+  C ck, cv;
+  ck.init(w, lane, p.kl);
+  cv.init(w, lane, p.vl);
+  const uint32_t lds = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem);
+  const char* const k0 = static_cast<const char*>(p.k) + 2 * (b * p.kb + hk * p.kh);
+  const char* const v0 = static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh);
+  const auto copy = [&](int t) SIDON_INLINE {
+    if (t < steps) {
+      const uint32_t at = lds + (t & 1) * kSlot;
+      ck.copy(at, k0 + (int64_t)t * kBlock * p.kl * 2, lk - t * kBlock);
+      cv.copy(at + C::kBytes, v0 + (int64_t)t * kBlock * p.vl * 2, lk - t * kBlock);
+    }
+  };
+  copy(0);
+
+  Reads at;
+  at.init(lane);
+  i4 qop[kQ], gop[kQ];
+  const int rr = max(min(row, lq - 1), 0);
+  {
+    const E* qp = static_cast<const E*>(p.q) + b * p.qb + head * p.qh + (int64_t)rr * p.ql + 8 * g;
+    const E* gp = static_cast<const E*>(p.dout) + b * p.gb + head * p.gh + (int64_t)rr * p.gl + 8 * g;
+#pragma unroll
+    for (int s = 0; s < kQ; ++s) {
+      qop[s] = *reinterpret_cast<const i4*>(qp + 16 * s);
+      gop[s] = *reinterpret_cast<const i4*>(gp + 16 * s);
+    }
+  }
+  constexpr float kLift = Range<E>::kLift;
+  const int64_t tile = ((int64_t)b * p.H + head) * p.tiles + rr / kBlock;
+  const float lse = p.stat[tile * (2 * kBlock) + rr % kBlock] - kLift, delta = p.stat[tile * (2 * kBlock) + kBlock + rr % kBlock];
+  float c = 1.f;
+  if constexpr (Range<E>::kScaled)
+    c = below_one(p.length[tile * kBlock + rr % kBlock], largest(p.longest_v + (int64_t)bh * p.key_tiles, p.key_tiles, lane));
+  const float scale2 = p.scale * kLog2e;
+
+  f32x16 dq[kDb];
+#pragma unroll
+  for (int d = 0; d < kDb; ++d) dq[d] = f32x16{};
+  for (int u = 0; u < steps; ++u) {
+    wait_vmcnt<0>();
+    lds_barrier();
+    copy(u + 1);
+    const char* const tk = smem + (u & 1) * kSlot;
+    const char* const tv = tk + C::kBytes;
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) s = Half<E>::mfma(at.rows(tk, i), qop[i], s);
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) dp = Half<E>::mfma(at.rows(tv, i), gop[i], dp);
+    if ((u + 1) * kBlock > lk) {
+      const int left = lk - u * kBlock - 8 * g;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (16 * (i >> 3) + (i & 7) >= left) s[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], scale2, -lse)) * ((dp[i] - delta) * c);
+    i4 pk[2];
+    round_to<E>(s, pk);
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int d = 0; d < kDb; ++d) dq[d] = Half<E>::mfma(at.columns(tk, hh, d), pk[hh], dq[d]);
+  }
+  if (row >= p.L) return;
+  store<E>(static_cast<E*>(p.dq) + b * p.dqb + head * p.dqh + row * p.dql + 4 * g, dq, p.scale * fast_exp2(-kLift) / c,
+           row < lq && lk > 0);
+}
+
+// ---- host -------------------------------------------------------------------------
+
+bool shape_ok(int B, int H, int Hk, int L, int S, int D) {
+  return B >= 1 && H >= 1 && Hk >= 1 && H % Hk == 0 && L >= 1 && S >= 1 && (D == 64 || D == 128) &&
+         S <= (1 << 24) && (int64_t)(H / Hk) * L <= (1 << 24) && (int64_t)B * H <= (1 << 20);
+}
+
+int tiles_of(int rows) { return (rows + kBlock - 1) / kBlock; }
+
+// In floats: statistics, lengths, the longest of a tile and of a key tile.
+struct Workspace {
+  size_t stat, length, longest, longest_v;
+  size_t bytes() const { return 4 * (stat + length + longest + longest_v); }
+};
+Workspace workspace(int B, int H, int Hk, int L, int S, int dtype) {
+  const size_t tiles = (size_t)B * H * tiles_of(L);
+  if (dtype == SIDON_BF16) return Workspace{tiles * 2 * kBlock, 0, 0, 0};
+  return Workspace{tiles * 2 * kBlock, tiles * kBlock, tiles, (size_t)B * Hk * tiles_of(S)};
+}
+
+template <typename E, int D>
+void launch(BwdParams& p, hipStream_t stream) {
+  constexpr int W = 4;
+  unsigned rows = (unsigned)p.B * p.H * p.tiles;
+  if (Range<E>::kScaled) rows += (unsigned)p.B * p.Hk * p.key_tiles;
+  hipLaunchKernelGGL((cross_bwd_rows_kernel<E, D>), dim3(rows), dim3(4 * D), 0, stream, p);
+  const int64_t heads = (int64_t)p.B * p.Hk;
+  p.deal = deal(heads, (p.S + W * kBlock - 1) / (W * kBlock), (int64_t)p.G * p.L * D * 4);
+  hipLaunchKernelGGL((cross_bwd_keys_kernel<E, D, W, 2>), dim3(p.deal.groups()), dim3(64 * W), 0, stream, p);
+  p.deal = deal(heads, (int64_t)p.G * ((p.L + W * kBlock - 1) / (W * kBlock)), (int64_t)p.S * D * 4);
+  hipLaunchKernelGGL((cross_bwd_queries_kernel<E, D, W, 2>), dim3(p.deal.groups()), dim3(64 * W), 0, stream, p);
+}
+
+}  // namespace
+
+SIDON_API size_t sidon_cross_attention_bwd_workspace_bytes(int B, int H, int Hk, int L, int S, int D, int dtype) {
+  if (!shape_ok(B, H, Hk, L, S, D) || (dtype != SIDON_FP16 && dtype != SIDON_BF16)) return 0;
+  return workspace(B, H, Hk, L, S, dtype).bytes();
+}
+
+SIDON_API int sidon_cross_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                                        const float* lse, const int32_t* lens, const int32_t* q_lens, float scale,
+                                        void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, int B, int H, int Hk,
+                                        int L, int S, int D, int dtype, const int64_t* g_strides,
+                                        const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                        const int64_t* o_strides, const int64_t* dq_strides, const int64_t* dk_strides,
+                                        const int64_t* dv_strides, sidon_stream_t stream) {
+  using sidon::fail;
+  using sidon::Rows;
+  sidon::clear_error();
+  if (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv || !ws || !g_strides || !q_strides || !k_strides ||
+      !v_strides || !o_strides || !dq_strides || !dk_strides || !dv_strides)
+    return fail(SIDON_E_NULL, "dout, q, k, v, out, lse, dq, dk, dv, ws and the strides must be non-NULL");
+  if (dtype != SIDON_FP16 && dtype != SIDON_BF16) return fail(SIDON_E_SHAPE, "dtype=%d is neither SIDON_FP16 nor SIDON_BF16", dtype);
+  if (!shape_ok(B, H, Hk, L, S, D))
+    return fail(SIDON_E_SHAPE, "B=%d H=%d Hk=%d L=%d S=%d D=%d: need sizes >= 1, H a multiple of Hk, D 64 or 128, H / Hk * L and S <= 2^24, B * H <= 2^20",
+                B, H, Hk, L, S, D);
+  if (!(scale >= FLT_MIN && scale <= 0x1p100f)) return fail(SIDON_E_SHAPE, "scale=%g must be positive and at most 2^100", scale);
+  const int64_t far = int64_t(1) << 40, near = (int64_t(1) << 25) - 1;
+  const struct {
+    const char* name;
+    const void* at;
+    const int64_t* s;
+    int heads, len;
+    int64_t row_most;
+  } all[] = {{"dout", dout, g_strides, H, L, near}, {"q", q, q_strides, H, L, near}, {"k", k, k_strides, Hk, S, near},
+             {"v", v, v_strides, Hk, S, near},      {"out", out, o_strides, H, L, far}, {"dq", dq, dq_strides, H, L, far},
+             {"dk", dk, dk_strides, Hk, S, far},    {"dv", dv, dv_strides, Hk, S, far}};
+  constexpr int kTensors = 8, kRead = 5;
+  Rows rows[kTensors];
+  const __int128 most = (__int128)1 << 61;
+  for (int t = 0; t < kTensors; ++t) {
+    for (int i = 0; i < 3; ++i)
+      if (all[t].s[i] < 0 || all[t].s[i] % 8 != 0 || all[t].s[i] > (i == 2 ? all[t].row_most : far))
+        return fail(SIDON_E_STRIDE, "%s stride %lld (number %d) must be a multiple of 8 in [0, %s]", all[t].name,
+                    (long long)all[t].s[i], i, i == 2 && all[t].row_most < far ? "2^25)" : "2^40]");
+    if (!sidon::aligned16(all[t].at)) return fail(SIDON_E_ALIGN, "%s must be 16-byte aligned", all[t].name);
+    rows[t] = Rows{all[t].at, {B, all[t].heads, all[t].len}, {all[t].s[0], all[t].s[1], all[t].s[2]}, D, 2};
+    if (rows[t].bytes() > most) return fail(SIDON_E_STRIDE, "%s spans more than the address space", all[t].name);
+    if (t >= kRead && !sidon::apart(rows[t].n, rows[t].st, 3, D)) return fail(SIDON_E_STRIDE, "rows of %s overlap one another", all[t].name);
+  }
+  if (((reinterpret_cast<uintptr_t>(lens) | reinterpret_cast<uintptr_t>(q_lens) | reinterpret_cast<uintptr_t>(lse)) & 3u) != 0 ||
+      !sidon::aligned16(ws))
+    return fail(SIDON_E_ALIGN, "lens, q_lens and lse must be 4-byte aligned, ws 16-byte aligned");
+  const Workspace need = workspace(B, H, Hk, L, S, dtype);
+  if (ws_bytes < need.bytes()) return fail(SIDON_E_SHAPE, "ws holds %zu bytes, the call needs %zu", ws_bytes, need.bytes());
+  for (int t = kRead; t < kTensors; ++t)
+    for (int o = 0; o < t; ++o)
+      if (sidon::tensors_meet(rows[o], rows[t])) return fail(SIDON_E_SHAPE, "%s must lie apart from %s", all[t].name, all[o].name);
+  const struct {
+    const char* name;
+    const void* at;
+    int64_t bytes;
+  } flat[] = {{"ws", ws, (int64_t)need.bytes()},
+              {"lse", lse, (int64_t)4 * B * H * L},
+              {"lens", lens, lens ? (int64_t)4 * B : 0},
+              {"q_lens", q_lens, q_lens ? (int64_t)4 * B : 0}};
+  for (int i = 0; i < 4; ++i) {
+    if (flat[i].bytes == 0) continue;
+    for (int t = i == 0 ? 0 : kRead; t < kTensors; ++t)
+      if (sidon::ranges_meet(flat[i].at, flat[i].bytes, rows[t].at, (int64_t)rows[t].bytes()))
+        return fail(SIDON_E_SHAPE, "%s must lie apart from %s", flat[i].name, all[t].name);
+    if (i > 0 && sidon::ranges_meet(ws, flat[0].bytes, flat[i].at, flat[i].bytes))
+      return fail(SIDON_E_SHAPE, "ws must lie apart from %s", flat[i].name);
+  }
+  const int64_t heads = (int64_t)B * Hk;
+  if ((int64_t)B * H * tiles_of(L) + heads * tiles_of(S) > INT32_MAX / 256 || !deal_fits(heads, tiles_of(S)) ||
+      !deal_fits(heads, (int64_t)(H / Hk) * tiles_of(L)))
+    return fail(SIDON_E_SHAPE, "too many rows for one launch");
+  const int rc = sidon::check_device();
+  if (rc) return rc;
+  BwdParams p{};
+  p.q = q, p.k = k, p.v = v, p.out = out, p.dout = dout, p.lse = lse, p.dq = dq, p.dk = dk, p.dv = dv;
+  p.lens = lens, p.q_lens = q_lens;
+  p.stat = static_cast<float*>(ws);
+  p.length = p.stat + need.stat;
+  p.longest = p.length + need.length;
+  p.longest_v = p.longest + need.longest;
+  p.gb = g_strides[0], p.gh = g_strides[1], p.gl = (int)g_strides[2];
+  p.qb = q_strides[0], p.qh = q_strides[1], p.ql = (int)q_strides[2];
+  p.kb = k_strides[0], p.kh = k_strides[1], p.kl = (int)k_strides[2];
+  p.vb = v_strides[0], p.vh = v_strides[1], p.vl = (int)v_strides[2];
+  p.ob = o_strides[0], p.oh = o_strides[1], p.ol = o_strides[2];
+  p.dqb = dq_strides[0], p.dqh = dq_strides[1], p.dql = dq_strides[2];
+  p.dkb = dk_strides[0], p.dkh = dk_strides[1], p.dkl = dk_strides[2];
+  p.dvb = dv_strides[0], p.dvh = dv_strides[1], p.dvl = dv_strides[2];
+  p.B = B, p.H = H, p.Hk = Hk, p.G = H / Hk, p.L = L, p.S = S;
+  p.tiles = tiles_of(L), p.key_tiles = tiles_of(S);
+  p.scale = scale;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == SIDON_FP16) {
+    if (D == 64) launch<_Float16, 64>(p, s);
+    else launch<_Float16, 128>(p, s);
+  } else {
+    if (D == 64) launch<__bf16, 64>(p, s);
+    else launch<__bf16, 128>(p, s);
+  }
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return fail(SIDON_E_LAUNCH, "cross attention gradient launch failed: %s", hipGetErrorString(err));
+  return SIDON_OK;
+}

@@ -1,0 +1,263 @@
+// int4_linear.hip -- projections with 4-bit weights and group scales for few rows
+// (MI355X / gfx950):
+//
+//   y[m, n] = act(bias[n] + sum_g s[n, g] sum_{k in g} x[m, k] (w[n, k] - z[n, g]))
+//
+// Few rows read every weight once, so the weights' bytes bound it.  They are laid out
+// when they are loaded (include/sidon_operators.h), 16 outputs x 128 inputs as the 1 KB
+// that a wavefront loads with 16 bytes a lane, in the order in which its lanes hold
+// the B operands of four v_mfma_f32_16x16x32.  A nibble becomes an operand by its bits
+// alone: q | 0x6400 is the fp16 1024 + q (less 1032, exactly, q - 8), q | 0x4300 the
+// bf16 128 + q.  What that adds, and the zero point, times the sum of the group's
+// inputs, which a product with ones gives in the accumulator's own layout, is taken
+// off in fp32 with the group's scale.
+//
+// A wavefront has 16 NT outputs of 16 MT rows and every WK-th block of 128 inputs;
+// the WK wavefronts of a workgroup are summed through LDS.
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "attn_device.h"
+#include "sidon_host.h"
+#include "sidon_operators.h"
+
+#define SIDON_API extern "C" __attribute__((visibility("default")))
+
+namespace {
+
+using namespace sidon_attn;
+
+constexpr int kTileN = 16, kTileK = 128;
+
+struct Int4Params {
+  const void* x;
+  const void* words;        // [N / 16, K / 128, 64 lanes] of 16 bytes
+  const uint32_t* scales;   // [N / 16, K / 128, 128 / group, 16]: scale, and in the high half what goes off the weights
+  const void* bias;
+  void* y;
+  int64_t ldx, ldy;
+  int M, N, K;
+  int tiles, blocks;        // of N by 16, of K by 128
+  int act;
+};
+
+// Eight nibbles of a word (in the order 0 2 4 6 1 3 5 7 from the lowest) as an operand.
+template <typename E>
+__device__ __forceinline__ i4 operand(uint32_t word) {
+  i4 r;
+  if constexpr (__is_same(E, _Float16)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const h2 v = __builtin_bit_cast(h2, ((word >> (4 * i)) & 0x000f000fu) | 0x64006400u);
+      r[i] = __builtin_bit_cast(int, v - h2{(_Float16)1032.f, (_Float16)1032.f});
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (int)(((word >> (4 * i)) & 0x000f000fu) | 0x43004300u);
+  }
+  return r;
+}
+
+// SPG: steps of 32 inputs per group within a block.  kOff: something goes off the weights.
+template <typename E, int MT, int NT, int WK, int SPG, bool kOff>
+__global__ void __launch_bounds__(64 * WK) int4_linear_kernel(const Int4Params p) {
+  constexpr int kGroups = 4 / SPG;
+  __shared__ f4 part[WK][MT * NT][64];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int tile0 = blockIdx.x * NT, row0 = blockIdx.y * (16 * MT);
+
+  const i4* wp[NT];
+  const uint32_t* sp[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t tile = min(tile0 + j, p.tiles - 1);   // (tiles past the last are not stored)
+    wp[j] = static_cast<const i4*>(p.words) + tile * p.blocks * 64 + lane;
+    sp[j] = p.scales + tile * p.blocks * (kGroups * 16) + c;
+  }
+  const E* xp[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xp[m] = static_cast<const E*>(p.x) + (row0 + 16 * m + c) * p.ldx + 8 * g;
+
+  f4 total[MT][NT] = {};
+  const int one2 = __is_same(E, _Float16) ? 0x3c003c00 : 0x3f803f80;
+  const i4 ones = {one2, one2, one2, one2};
+#pragma unroll 2
+  for (int b = w; b < p.blocks; b += WK) {
+    i4 words[NT];
+    uint32_t scale[NT][kGroups];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      words[j] = wp[j][(int64_t)b * 64];
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) scale[j][k] = sp[j][(int64_t)b * (kGroups * 16) + k * 16];
+    }
+    i4 xop[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        xop[m][i] = i4{};
+        if (row0 + 16 * m + c < p.M && b * kTileK + 32 * i < p.K)
+          xop[m][i] = *reinterpret_cast<const i4*>(xp[m] + b * kTileK + 32 * i);
+      }
+    f4 sums[MT][kGroups] = {};
+    if constexpr (kOff) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[m][i / SPG] = Half<E>::small(xop[m][i], ones, sums[m][i / SPG]);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        f4 acc[MT] = {};
+#pragma unroll
+        for (int i = k * SPG; i < (k + 1) * SPG; ++i) {
+          const i4 op = operand<E>((uint32_t)words[j][i]);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[m] = Half<E>::small(xop[m][i], op, acc[m]);
+        }
+        typedef E e2 __attribute__((ext_vector_type(2)));
+        const e2 so = __builtin_bit_cast(e2, scale[j][k]);
+        const float s = (float)so[0], off = -(float)so[1];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float a = acc[m][e];
+            if constexpr (kOff) a = fmaf(off, sums[m][k][e], a);
+            total[m][j][e] = fmaf(s, a, total[m][j][e]);
+          }
+      }
+  }
+
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) part[w][m * NT + j][lane] = total[m][j];
+  __syncthreads();
+  for (int t = w; t < MT * NT; t += WK) {
+    f4 sum = part[0][t][lane];
+#pragma unroll
+    for (int k = 1; k < WK; ++k) sum += part[k][t][lane];
+    const int n = (tile0 + t % NT) * kTileN + c, row = row0 + t / NT * 16 + 4 * g;
+    if (n >= p.N) continue;
+    const float bias = p.bias != nullptr ? (float)static_cast<const E*>(p.bias)[n] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (row + e >= p.M) break;
+      float v = sum[e] + bias;
+      if (p.act == SIDON_ACT_SILU) v = v / (1.f + __expf(-v));
+      static_cast<E*>(p.y)[(int64_t)(row + e) * p.ldy + n] = (E)v;
+    }
+  }
+}
+
+// ---- host -------------------------------------------------------------------------
+
+struct Shape {
+  int mt, nt, wk;
+};
+
+// Rows of a workgroup by what M needs; outputs of a wavefront and wavefronts along K so
+// that the launch has at least a workgroup per CU.
+Shape shape(int M, int N, int cus) {
+  const int mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  const int64_t tiles = (N + kTileN - 1) / kTileN, rows = (M + 16 * mt - 1) / (16 * mt);
+  if (tiles * rows >= 8 * (int64_t)cus) return Shape{mt, 4, 4};
+  return Shape{mt, 1, 8};
+}
+
+template <typename E, int MT, int NT, int WK>
+void launch_groups(const Int4Params& p, int group, bool off, dim3 grid, hipStream_t s) {
+#define SIDON_INT4(SPG)                                                                                      \
+  if (off)                                                                                                   \
+    hipLaunchKernelGGL((int4_linear_kernel<E, MT, NT, WK, SPG, true>), grid, dim3(64 * WK), 0, s, p);        \
+  else if constexpr (__is_same(E, _Float16))                                                                 \
+    hipLaunchKernelGGL((int4_linear_kernel<E, MT, NT, WK, SPG, false>), grid, dim3(64 * WK), 0, s, p);
+  if (group == 32) {
+    SIDON_INT4(1)
+  } else if (group == 64) {
+    SIDON_INT4(2)
+  } else {
+    SIDON_INT4(4)
+  }
+#undef SIDON_INT4
+}
+
+template <typename E, int MT>
+void launch_shape(const Int4Params& p, const Shape& c, int group, bool off, hipStream_t s) {
+  const dim3 grid((p.tiles + c.nt - 1) / c.nt, (p.M + 16 * MT - 1) / (16 * MT));
+  if (c.nt == 4)
+    launch_groups<E, MT, 4, 4>(p, group, off, grid, s);
+  else
+    launch_groups<E, MT, 1, 8>(p, group, off, grid, s);
+}
+
+template <typename E>
+void launch(const Int4Params& p, const Shape& c, int group, bool off, hipStream_t s) {
+  if (c.mt == 1)
+    launch_shape<E, 1>(p, c, group, off, s);
+  else if (c.mt == 2)
+    launch_shape<E, 2>(p, c, group, off, s);
+  else
+    launch_shape<E, 4>(p, c, group, off, s);
+}
+
+}  // namespace
+
+SIDON_API int sidon_int4_linear(const void* x, int64_t ldx, const void* words, const void* scales, const void* bias,
+                                void* y, int64_t ldy, int M, int N, int K, int group, int zeros, int act, int dtype,
+                                sidon_stream_t stream) {
+  using sidon::fail;
+  using sidon::Rows;
+  sidon::clear_error();
+  if (!x || !words || !scales || !y) return fail(SIDON_E_NULL, "x, words, scales and y must be non-NULL");
+  if (dtype != SIDON_FP16 && dtype != SIDON_BF16) return fail(SIDON_E_SHAPE, "dtype=%d is neither SIDON_FP16 nor SIDON_BF16", dtype);
+  if (act != SIDON_ACT_NONE && act != SIDON_ACT_SILU) return fail(SIDON_E_SHAPE, "act=%d is neither SIDON_ACT_NONE nor SIDON_ACT_SILU", act);
+  if (M < 1 || N < 1 || K < 1 || M > (1 << 21) || N > (1 << 24) || K > (1 << 20))
+    return fail(SIDON_E_SHAPE, "M=%d N=%d K=%d: need 1 <= M <= 2^21, N <= 2^24, K <= 2^20", M, N, K);
+  if ((group != 32 && group != 64 && group != 128) || K % group != 0)
+    return fail(SIDON_E_SHAPE, "group=%d K=%d: need group 32, 64 or 128 and K a multiple of it", group, K);
+  if (ldx < K || ldx % 8 != 0 || ldx > (int64_t)1 << 40 || ldy < N || ldy > (int64_t)1 << 40)
+    return fail(SIDON_E_STRIDE, "ldx=%lld must be a multiple of 8 from K=%d, ldy=%lld at least N=%d, both at most 2^40",
+                (long long)ldx, K, (long long)ldy, N);
+  if (!sidon::aligned16(x) || !sidon::aligned16(words) || !sidon::aligned16(scales) ||
+      ((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(y)) & 1u) != 0)
+    return fail(SIDON_E_ALIGN, "x, words and scales must be 16-byte aligned, bias and y 2-byte aligned");
+  Int4Params p{};
+  p.tiles = (N + kTileN - 1) / kTileN, p.blocks = (K + kTileK - 1) / kTileK;
+  {
+    const Rows out{y, {1, 1, M}, {0, 0, ldy}, N, 2};
+    if (sidon::tensors_meet(out, Rows{x, {1, 1, M}, {0, 0, ldx}, K, 2})) return fail(SIDON_E_SHAPE, "y must lie apart from x");
+    const struct {
+      const char* name;
+      const void* at;
+      int64_t bytes;
+    } flat[] = {{"words", words, (int64_t)p.tiles * p.blocks * 1024},
+                {"scales", scales, (int64_t)p.tiles * p.blocks * (kTileK / group) * 64},
+                {"bias", bias, bias ? (int64_t)2 * N : 0}};
+    for (const auto& f : flat)
+      if (f.bytes > 0 && sidon::ranges_meet(y, (int64_t)out.bytes(), f.at, f.bytes))
+        return fail(SIDON_E_SHAPE, "y must lie apart from %s", f.name);
+  }
+  const int rc = sidon::check_device();
+  if (rc) return rc;
+  p.x = x, p.words = words, p.scales = static_cast<const uint32_t*>(scales), p.bias = bias, p.y = y;
+  p.ldx = ldx, p.ldy = ldy;
+  p.M = M, p.N = N, p.K = K, p.act = act;
+  const Shape c = shape(M, N, sidon::compute_units());
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  // (fp16's operands are off by 8 already, bf16's by -128)
+  if (dtype == SIDON_FP16)
+    launch<_Float16>(p, c, group, zeros != 0, s);
+  else
+    launch<__bf16>(p, c, group, true, s);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return fail(SIDON_E_LAUNCH, "4-bit projection launch failed: %s", hipGetErrorString(err));
+  return SIDON_OK;
+}
