@@ -90,6 +90,14 @@ __device__ __forceinline__ void dma_256(uint32_t lds_addr, const char* gbase, ui
 }
 #pragma clang diagnostic pop
 
+// Waits for the loads of x here.  Left to its first use, within a loop, the compiler's
+// wait would come round with every turn and take the loop's own copies with it.
+template <int N>
+__device__ __forceinline__ void arrived(i4 (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
+}
+
 // How a launch's workgroups go over the heads.  They are dispatched round-robin over
 // the 8 XCDs; a head's `units` of work are dealt into `parts` parts and the parts to
 // the XCDs, so that each L2 holds the keys and values of few heads and every XCD gets

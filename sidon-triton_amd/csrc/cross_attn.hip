@@ -63,9 +63,9 @@ struct CrossParams {
   float scale;           // log2(e) times the caller's
 };
 
-// A workgroup: RB row blocks x KS key groups, a wavefront each.  The wavefronts of a
+// A workgroup: RB wavefronts of NB row blocks each x KS key groups.  The wavefronts of a
 // key group share a ring of two key slots and three value slots, a step of 32 keys each.
-template <int D, int RB, int KS>
+template <int D, int NB, int RB, int KS>
 struct Shape {
   static constexpr int kWaves = RB * KS;
   static constexpr int kP = D / 64;                   // 128-byte panels
@@ -73,7 +73,7 @@ struct Shape {
   static constexpr int kV = 2 * kSlot;                // value slots behind the key slots
   static constexpr int kRing = 5 * kSlot;
   static constexpr int kDb = D / 32;                  // 32-wide blocks of the values
-  static constexpr int kPart = (kDb * 16 + 4) * 64 * 4;   // bytes of a wavefront's partial result
+  static constexpr int kPart = NB * (kDb * 16 + 4) * 64 * 4;   // bytes of a wavefront's partial result
   static constexpr int kMerge = KS > 1 ? KS / 2 * RB * kPart : 0;
   static constexpr int kLds = KS * kRing > kMerge ? KS * kRing : kMerge;
   static constexpr int kCopies = kSlot / 1024 / RB;   // 1 KB copies per wavefront and slot
@@ -84,9 +84,12 @@ struct Shape {
 // kFine: probabilities as two summands of the type, the rounded value and what the
 // rounding left, so that only the output is rounded.  For few rows, where memory and
 // latency leave the matrix cores idle.
-template <typename E, int D, int RB, int KS, bool kFine, int kMinWaves>
+// kLse: the sums of probabilities before their rounding are wanted, and the rounded ones'
+// do not stand for them (kFine's do).
+template <typename E, int D, int NB, int RB, int KS, bool kFine, bool kLse, int kMinWaves>
 __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(const CrossParams p) {
-  using C = Shape<D, RB, KS>;
+  using C = Shape<D, NB, RB, KS>;
+  static_assert(!(kFine && kLse), "the sums of two summands are as good");
   typedef typename Half<E>::v2 v2;
   typedef typename Half<E>::v4 v4;
   constexpr int P = C::kP, kDb = C::kDb;
@@ -104,14 +107,14 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
   const int split = unit / p.blocks;
   const int blk = unit - split * p.blocks;
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
-  const int row0 = (blk * RB + rb) * kBlock;   // of this wavefront
-  const int row = row0 + n;                    // of this lane: query row / G, head row % G of the group
+  const int row0 = (blk * RB + rb) * (NB * kBlock);   // of this wavefront
+  // Lane n holds the rows row0 + 32 j + n, j < NB: query row / G, head row % G of the group.
 
   int lk = p.S, rows = p.R;                    // valid keys, rows of valid queries
   if (p.lens != nullptr) lk = __builtin_amdgcn_readfirstlane(min(max(p.lens[b], 0), p.S));
   if (p.q_lens != nullptr) rows = p.G * __builtin_amdgcn_readfirstlane(min(max(p.q_lens[b], 0), p.L));
 
-  const int steps = blk * RB * kBlock < rows ? (lk + kStep - 1) / kStep : 0;   // of the workgroup
+  const int steps = blk * RB * NB * kBlock < rows ? (lk + kStep - 1) / kStep : 0;   // of the workgroup
   const int t0 = (int)((uint32_t)steps * (uint32_t)split / (uint32_t)p.splits);   // (steps <= 2^25, splits <= 2^6)
   const int t1 = (int)((uint32_t)steps * (uint32_t)(split + 1) / (uint32_t)p.splits);
   const auto mine = [&](int u) SIDON_INLINE { return t0 + u * KS + ks; };   // step u of this group
@@ -185,13 +188,16 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
 
   // ---- Q^T operands: lane (n, g) holds query n, dims 16 s + 8 g + [0, 8); rows past
   // the valid ones hold the last valid one (or the first row, where none is) ----
-  i4 qop[kQ];
-  {
-    const int rr = max(min(row, rows - 1), 0);
+  i4 qop[NB][kQ];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int rr = max(min(row0 + 32 * j + n, rows - 1), 0);
     const E* qp = static_cast<const E*>(p.q) + b * p.qb + (hk * p.G + rr % p.G) * p.qh + (rr / p.G) * p.ql + 8 * g;
 #pragma unroll
-    for (int s = 0; s < kQ; ++s) qop[s] = *reinterpret_cast<const i4*>(qp + 16 * s);
+    for (int s = 0; s < kQ; ++s) qop[j][s] = *reinterpret_cast<const i4*>(qp + 16 * s);
   }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) arrived(qop[j]);
 
   // ---- operand offsets from the first key and value slot ----
   int kaddr[4], vaddr[2][2];
@@ -217,15 +223,19 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
     sel = i4{pair, pair, pair, pair};
   }
 
-  f32x16 o[kDb];
+  f32x16 o[NB][kDb];
+  // Of a row: maximum of the scaled scores, less kLift; sum of the rounded probabilities;
+  // this lane's share of their sum before the rounding.
+  float mx[NB], sum[NB], raw[NB];
 #pragma unroll
-  for (int d = 0; d < kDb; ++d) o[d] = f32x16{};
-  // Of query n: maximum of the scaled scores, less kLift; sum of the rounded probabilities;
-  // this lane's share of their sum before the rounding (for lse).
-  float mx = kFloorMax, sum = 0.f, raw = 0.f;
-  f32x16 s;                          // scores of a step: element i is key 16 (i / 8) + 8 g + i % 8
+  for (int j = 0; j < NB; ++j) {
+    mx[j] = kFloorMax, sum[j] = 0.f, raw[j] = 0.f;
+#pragma unroll
+    for (int d = 0; d < kDb; ++d) o[j][d] = f32x16{};
+  }
+  f32x16 s[NB];                      // scores of a step: element i is key 16 (i / 8) + 8 g + i % 8
   constexpr int kTerms = kFine ? 2 : 1;
-  i4 pk[kTerms][2];                  // its probabilities
+  i4 pk[NB][kTerms][2];              // its probabilities
 
   // The three parts of a step.  In round u a wavefront takes the softmax of step
   // u and the product with the values of step u - 1, whose vector and matrix
@@ -239,66 +249,73 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
     kread ^= C::kSlot;
   };
   const auto scores = [&]() SIDON_INLINE {
-    f32x16 acc = {};
 #pragma unroll
-    for (int i = 0; i < kQ; ++i) acc = Half<E>::mfma(kop[i], qop[i], acc);
-    s = acc;
+    for (int j = 0; j < NB; ++j) {
+      f32x16 acc = {};
+#pragma unroll
+      for (int i = 0; i < kQ; ++i) acc = Half<E>::mfma(kop[i], qop[j][i], acc);
+      s[j] = acc;
+    }
   };
   int k0 = mine(0) * kStep;   // first key of the step in s
   const auto hide = [&]() SIDON_INLINE {
     if (k0 + kStep > lk) {
       const int left = lk - k0 - 8 * g;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (16 * (i >> 3) + (i & 7) >= left) s[i] = -INFINITY;
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (16 * (i >> 3) + (i & 7) >= left) s[j][i] = -INFINITY;
     }
     k0 += KS * kStep;
   };
-  const auto exps = [&](float (&e)[16]) SIDON_INLINE {
+  const auto exps = [&](int j, float (&e)[16]) SIDON_INLINE {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) e[i] = fast_exp2(fmaf(s[i], p.scale, -mx));
+    for (int i = 0; i < 16; ++i) e[i] = fast_exp2(fmaf(s[j][i], p.scale, -mx[j]));
   };
   const auto total_of = [&](const float (&e)[16]) SIDON_INLINE {
     float t[4] = {};
+    if constexpr (kLse) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t[i % 4] += e[i];
+      for (int i = 0; i < 16; ++i) t[i % 4] += e[i];
+    }
     return (t[0] + t[1]) + (t[2] + t[3]);
   };
   // The step's probabilities, rounded.
-  const auto round_to = [&](const float (&e)[16]) SIDON_INLINE {
+  const auto round_to = [&](int j, const float (&e)[16]) SIDON_INLINE {
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
       const v2 hi = __builtin_convertvector(f2{e[i], e[i + 1]}, v2);
-      pk[0][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, hi);
+      pk[j][0][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, hi);
       if constexpr (kFine) {
         const f2 left = {e[i] - (float)hi[0], e[i + 1] - (float)hi[1]};
-        pk[kTerms - 1][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, __builtin_convertvector(left, v2));
+        pk[j][kTerms - 1][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, __builtin_convertvector(left, v2));
       }
     }
   };
   // Their sum, on the matrix core, where the vector unit is the busier one.  Read
-  // as a 16x16x32 B operand, a lane's half of them holds query c + 16 (j % 2) of
-  // lane c + 16 j, keys 8 (j / 2) + [0, 8); the A operand is 1 where bit 4 of the
-  // lane equals bit 2, so that the four rows a lane receives are its own query's
-  // sum.  The other query of the column enters times 0: where its probabilities are
-  // infinite or NaN, so is this sum, and `settle` takes the query's own.
-  const auto matrix_sum = [&]() SIDON_INLINE {
+  // as a 16x16x32 B operand, a lane's half of them holds row c + 16 (l % 2) of
+  // lane c + 16 l, keys 8 (l / 2) + [0, 8); the A operand is 1 where bit 4 of the
+  // lane equals bit 2, so that the four numbers a lane receives are its own row's
+  // sum.  The other row of the column enters times 0: where its probabilities are
+  // infinite or NaN, so is this sum, and `settle` takes the row's own.
+  const auto matrix_sum = [&](int j) SIDON_INLINE {
     f4 total = {};
 #pragma unroll
     for (int k = 0; k < kTerms; ++k) {
-      total = Half<E>::small(sel, pk[k][0], total);
-      total = Half<E>::small(sel, pk[k][1], total);
+      total = Half<E>::small(sel, pk[j][k][0], total);
+      total = Half<E>::small(sel, pk[j][k][1], total);
     }
     return total[0];
   };
-  // The same from the lane pair that holds the query, nothing else.
-  const auto own_sum = [&]() SIDON_INLINE {
+  // The same from the lane pair that holds the row, nothing else.
+  const auto own_sum = [&](int j) SIDON_INLINE {
     float total = 0.f;
 #pragma unroll
     for (int k = 0; k < kTerms; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int pair = pk[k][i >> 2][i & 3];   // (a bit cast of the element itself takes the vector's first)
+        const int pair = pk[j][k][i >> 2][i & 3];   // (a bit cast of the element itself takes the vector's first)
         const v2 x = __builtin_bit_cast(v2, pair);
         total += (float)x[0] + (float)x[1];
       }
@@ -314,45 +331,64 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
         const i2 lo = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + vaddr[0][d & 1])));
         const i2 hi = __builtin_bit_cast(i2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(SIDON_LDS_PTR(s4, tile + vaddr[1][d & 1])));
 #pragma unroll
-        for (int k = 0; k < kTerms; ++k) o[d] = Half<E>::mfma(i4{lo[0], lo[1], hi[0], hi[1]}, pk[k][hh], o[d]);
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int k = 0; k < kTerms; ++k) o[j][d] = Half<E>::mfma(i4{lo[0], lo[1], hi[0], hi[1]}, pk[j][k][hh], o[j][d]);
       }
     vread = vread == 2 * C::kSlot ? 0 : vread + C::kSlot;
   };
-  // Raises the running maximum of the queries whose probabilities do not all
-  // fit, with what they have so far, and takes their sums apart from the other
-  // queries'.  (The condition is a lane's, not the wavefront's: behind a branch of the
-  // wavefront the compiler keeps the accumulators in two places.)
-  const auto settle = [&](float total, float exact) SIDON_INLINE {
+  // Raises the running maximum of the rows whose probabilities do not all fit, with
+  // what they have so far.  (The condition is a lane's, not the wavefront's: behind a
+  // branch of the wavefront the compiler keeps the accumulators in two places.)
+  const auto settle = [&](int j, float total, float exact) SIDON_INLINE {
     // One that left fp16 is an infinity in the sum.
     if (!(total < kSumLimit)) {
-      float top = s[0];
+      total = own_sum(j);
+      if (!(total < kSumLimit)) {
+        float top = s[j][0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-      top = fmaxf(mx, pair_max(top) * p.scale - Half<E>::kLift);
-      const float alpha = fast_exp2(mx - top);   // 0 from kFloorMax
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[j][i]);
+        top = fmaxf(mx[j], pair_max(top) * p.scale - Half<E>::kLift);
+        const float alpha = fast_exp2(mx[j] - top);   // 0 from kFloorMax
 #pragma unroll
-      for (int d = 0; d < kDb; ++d) o[d] *= alpha;
-      sum *= alpha;
-      raw *= alpha;
-      mx = top;
-      float e[16];
-      exps(e);
-      exact = total_of(e);
-      round_to(e);
-      total = own_sum();
+        for (int d = 0; d < kDb; ++d) o[j][d] *= alpha;
+        sum[j] *= alpha;
+        raw[j] *= alpha;
+        mx[j] = top;
+        float e[16];
+        exps(j, e);
+        exact = total_of(e);
+        round_to(j, e);
+        total = own_sum(j);
+      }
     }
-    sum += total;
-    raw += exact;
+    sum[j] += total;
+    raw[j] += exact;
   };
-  // Behind it, what the last round copied (the keys of step u + 1, the values
-  // of step u) is there for every wavefront of the ring, and nobody reads the
-  // keys of step u or the values of step u - 2 any more: their slots are filled
-  // with the keys of step u + 2 and the values of step u + 1.
-  const auto round = [&]() SIDON_INLINE {
-    wait_vmcnt<0>();
-    lds_barrier();
+  // Behind it the values of step u - 1 are there and, where wavefronts share the ring,
+  // for all of them, with the keys of step u + 1; nobody reads the keys of step u or the
+  // values of step u - 2 any more: their slots are filled with the keys of step u + 2
+  // and the values of step u + 1.  Copies arrive in the order in which they were issued
+  // (keys, then values, round by round), so a wait names how many of the newest it
+  // leaves under way; past the last step's none are issued, and it leaves none.
+  constexpr int kSet = C::kCopies;
+  const int mine_all = max(t1 - t0 - ks + KS - 1, 0) / KS;   // steps that this group copies
+  const auto round = [&](int u) SIDON_INLINE {
+    if constexpr (RB == 1) {
+      if (u + 1 < mine_all) wait_vmcnt<2 * kSet>(); else wait_vmcnt<0>();
+      wait_lgkm0();
+    } else {
+      if (u < mine_all) wait_vmcnt<kSet>(); else wait_vmcnt<0>();
+      lds_barrier();
+    }
     copy_k();
     copy_v();
+  };
+  // The keys of step u + 1 are there too (a ring of one wavefront waits for them late).
+  const auto keys_there = [&](int u) SIDON_INLINE {
+    if constexpr (RB == 1) {
+      if (u + 2 < mine_all) wait_vmcnt<3 * kSet>(); else wait_vmcnt<0>();
+    }
   };
 
   // ---- rounds -1 to `all` (the first needs the first keys alone) ----
@@ -364,107 +400,132 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
       load_keys();
       scores();
     }
-    round();
+    round(0);
     if (count > 0) {
       hide();
-      float e[16];
-      exps(e);
-      const float exact = total_of(e);
-      round_to(e);
-      settle(matrix_sum(), exact);
+      float exact[NB], total[NB];
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        float e[16];
+        exps(j, e);
+        exact[j] = total_of(e);
+        round_to(j, e);
+        total[j] = matrix_sum(j);
+      }
+#pragma unroll
+      for (int j = 0; j < NB; ++j) settle(j, total[j], exact[j]);
       if (count > 1) {
+        keys_there(0);
         load_keys();
         scores();
       }
     }
     for (u = 1; u < count; ++u) {
-      round();
+      round(u);
       hide();
-      float e[16];
-      exps(e);
+      float e[NB][16], exact[NB], total[NB];
+#pragma unroll
+      for (int j = 0; j < NB; ++j) exps(j, e[j]);
       values();
-      const float exact = total_of(e);
-      round_to(e);
-      const float total = matrix_sum();
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        exact[j] = total_of(e[j]);
+        round_to(j, e[j]);
+        total[j] = matrix_sum(j);
+      }
+      keys_there(u);
       load_keys();   // (of the last round: what an earlier step left in the slot, for nothing)
-      settle(total, exact);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) settle(j, total[j], exact[j]);
       scores();
     }
     for (; u <= all; ++u) {
-      round();
+      round(u);
       if (u == count && count > 0) values();
     }
   }
-  raw = pair_sum(raw);
+#pragma unroll
+  for (int j = 0; j < NB; ++j) raw[j] = kLse ? pair_sum(raw[j]) : sum[j];
 
-  // A wavefront's partial result in LDS, lane by lane: its values, then (maximum, sums).
-  float* const mem = reinterpret_cast<float*>(smem) + lane * 4;
-
-  // ---- merge the key groups, half of them into the other half at a time ----
+  // ---- merge the key groups, half of them into the other half at a time: a wavefront's
+  // partial result in LDS, lane by lane, its values, then (maximum, sums) ----
   if constexpr (KS > 1) {
+    float* const mem = reinterpret_cast<float*>(smem) + lane * 4;
 #pragma unroll
     for (int half = KS / 2; half >= 1; half >>= 1) {
       wait_vmcnt<0>();
       lds_barrier();   // the rings, or the last round's values, are done with
-      float* at = mem + ((ks % half) * RB + rb) * (C::kPart / 4);
-      float* ml = at + kDb * 4 * 256;
-      if (ks >= half) {
 #pragma unroll
-        for (int d = 0; d < kDb; ++d)
+      for (int j = 0; j < NB; ++j) {
+        float* at = mem + (((ks % half) * RB + rb) * NB + j) * (C::kPart / NB / 4);
+        if (ks >= half) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<f4*>(at + (d * 4 + i) * 256) = f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-        *reinterpret_cast<f4*>(ml) = f4{mx, sum, raw, 0.f};
+          for (int d = 0; d < kDb; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<f4*>(at + (d * 4 + i) * 256) =
+                  f4{o[j][d][4 * i], o[j][d][4 * i + 1], o[j][d][4 * i + 2], o[j][d][4 * i + 3]};
+          *reinterpret_cast<f4*>(at + kDb * 4 * 256) = f4{mx[j], sum[j], raw[j], 0.f};
+        }
       }
       lds_barrier();
       if (ks >= half) return;
-      const f4 other = *reinterpret_cast<const f4*>(ml);
-      const float top = fmaxf(mx, other[0]);
-      const float fa = fast_exp2(mx - top), fb = fast_exp2(other[0] - top);
-      mx = top;
-      sum = sum * fa + other[1] * fb;
-      raw = raw * fa + other[2] * fb;
 #pragma unroll
-      for (int d = 0; d < kDb; ++d) {
+      for (int j = 0; j < NB; ++j) {
+        const float* at = mem + (((ks % half) * RB + rb) * NB + j) * (C::kPart / NB / 4);
+        const f4 other = *reinterpret_cast<const f4*>(at + kDb * 4 * 256);
+        const float top = fmaxf(mx[j], other[0]);
+        const float fa = fast_exp2(mx[j] - top), fb = fast_exp2(other[0] - top);
+        mx[j] = top;
+        sum[j] = fmaf(sum[j], fa, other[1] * fb);
+        raw[j] = fmaf(raw[j], fa, other[2] * fb);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f4 v = *reinterpret_cast<const f4*>(at + (d * 4 + i) * 256);
+        for (int d = 0; d < kDb; ++d) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[d][4 * i + e] = o[d][4 * i + e] * fa + v[e] * fb;
+          for (int i = 0; i < 4; ++i) {
+            const f4 v = *reinterpret_cast<const f4*>(at + (d * 4 + i) * 256);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][d][4 * i + e] = fmaf(o[j][d][4 * i + e], fa, v[e] * fb);
+          }
+          if (d % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
-        if (d % 2 == 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
 
   // Lane (n, g) holds of row n the values 32 d + 8 i + 4 g + [0, 4).
-  if (row >= p.R) return;
-  if (p.splits > 1) {
-    const int64_t at = ((int64_t)bh * p.splits + split) * p.R + row;
-    float* dst = p.part_o + at * D + 4 * g;
-    if (g == 0) p.part_ml[at] = make_float4(mx, sum, raw, 0.f);
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int row = row0 + 32 * j + n;
+    if (row >= p.R) return;
+    if (p.splits > 1) {
+      const int64_t at = ((int64_t)bh * p.splits + split) * p.R + row;
+      float* dst = p.part_o + at * D + 4 * g;
+      if (g == 0) p.part_ml[at] = make_float4(mx[j], sum[j], raw[j], 0.f);
+#pragma unroll
+      for (int d = 0; d < kDb; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f4*>(dst + 32 * d + 8 * i) =
+              f4{o[j][d][4 * i], o[j][d][4 * i + 1], o[j][d][4 * i + 2], o[j][d][4 * i + 3]};
+      continue;
+    }
+    const bool there = row < rows && lk > 0;
+    const float f = there ? 1.f / sum[j] : 0.f;
+    const int head = hk * p.G + row % p.G, query = row / p.G;
+    if (p.lse != nullptr && g == 0)
+      p.lse[((int64_t)b * p.H + head) * p.L + query] = there ? (mx[j] + __log2f(raw[j])) * kLn2 : -INFINITY;
+    E* dst = static_cast<E*>(p.out) + b * p.ob + head * p.oh + query * p.ol + 4 * g;
 #pragma unroll
     for (int d = 0; d < kDb; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f4*>(dst + 32 * d + 8 * i) = f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-    return;
+      for (int i = 0; i < 4; ++i) {
+        v4 r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = there ? (E)(o[j][d][4 * i + e] * f) : (E)0.f;
+        *reinterpret_cast<v4*>(dst + 32 * d + 8 * i) = r;
+      }
   }
-  const bool there = row < rows && lk > 0;
-  const float f = there ? 1.f / sum : 0.f;
-  const int head = hk * p.G + row % p.G, query = row / p.G;
-  if (p.lse != nullptr && g == 0)
-    p.lse[((int64_t)b * p.H + head) * p.L + query] = there ? (mx + __log2f(raw)) * kLn2 : -INFINITY;
-  E* dst = static_cast<E*>(p.out) + b * p.ob + head * p.oh + query * p.ol + 4 * g;
-#pragma unroll
-  for (int d = 0; d < kDb; ++d)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v4 r;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = there ? (E)(o[d][4 * i + e] * f) : (E)0.f;
-      *reinterpret_cast<v4*>(dst + 32 * d + 8 * i) = r;
-    }
 }
 
 // Join the grid splits of a row: a workgroup per row, whose wavefronts take every
@@ -526,21 +587,60 @@ __global__ void __launch_bounds__(64 * kJoinWaves) cross_attn_join_kernel(const 
 
 // ---- host -------------------------------------------------------------------------
 
+// The kernels.
+struct Kind {
+  int dim, rows, groups;   // rows and key groups of a workgroup
+  bool fine;
+  int fit;                 // workgroups that a CU runs at once
+  double base, ends, alone, more, join, part, traffic;
+};
+// Which, and how many grid splits: the least estimate (us) of
+//
+//   base + turns (ends + rounds (alone + more running)) + what splits cost
+//
+// where a CU's share of the workgroups takes full turns of `fit` at once and one with
+// the rest, `running` is what a turn holds, and a workgroup's rounds are its steps over
+// its key groups.  Splits add a joining launch, its walk over the parts, and the partial
+// results, written and read (per MB).  Fitted to 165000 timings of 31600 shapes (1 to 32
+// items, 1 to 1400 queries, 30 to 6000 keys, in every kernel and with every number of splits):
+// the choice is on average within 1% of the best one's time, in 99 of 100 within 17%.  (32
+// rows at D 64 are for short launches: 4 x 16 heads x 224 x 1500 15.6 us, with 64 rows
+// 16.8; 1 x 16 x 4800 x 4800 151 and 123.  Rows shared by more wavefronts, 128 and 256 a
+// workgroup, took 131 and 144 there: fewer copies, but waits for one another.)
+constexpr Kind kKinds[] = {{64, 32, 4, true, 2, 1.53, 4.24, 0, .677, 2.5, .018, .744},
+                           {64, 32, 4, false, 2, 2.39, 3.98, .111, .343, 2.62, 0, .601},
+                           {64, 64, 4, false, 2, 2.58, 5.72, .05, .637, 2.29, 0, .502},
+                           {128, 32, 2, true, 2, 1.24, 5.02, .329, .484, 2.43, .022, .351},
+                           {128, 64, 2, false, 2, 1.5, 6, .4, .3, 3.2, 0, .4}};
+constexpr int kNumKinds = sizeof(kKinds) / sizeof(kKinds[0]);
+
 struct Plan {
-  int rows;     // per workgroup
+  int kind;   // -1: none yet
   int blocks, splits;
 };
 
-// Rows per workgroup and grid splits.
 Plan search(int B, int Hk, int R, int S, int D, int cus) {
   const int64_t heads = (int64_t)B * Hk;
   const int steps = (S + kStep - 1) / kStep;
-  const int rows = R <= kBlock || heads * ((R + 127) / 128) < cus ? kBlock : 4 * kBlock;
-  const int groups = rows == kBlock ? (D == 64 ? 4 : 2) : 1;
-  const int blocks = (R + rows - 1) / rows;
-  int splits = 1;
-  while (splits < kMaxGridSplits && heads * blocks * splits * 2 <= 2 * cus && splits * 2 * groups * 4 <= steps) splits *= 2;
-  return Plan{rows, blocks, splits};
+  Plan best{-1, 0, 0};
+  double best_us = 0;
+  for (int i = 0; i < kNumKinds; ++i) {
+    const Kind& k = kKinds[i];
+    // up to 32 rows keep two summands (the header says so)
+    if (k.dim != D || (R <= kBlock && !k.fine) || (R > kBlock && k.fine && D == 64)) continue;
+    const int blocks = (R + k.rows - 1) / k.rows;
+    for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, kMaxGridSplits}) {
+      const int64_t load = (heads * blocks * s + cus - 1) / cus;   // workgroups of the busiest CU
+      if (s > 1 && (s * k.groups > steps + 1 || load > 6)) break;
+      const int rounds = (steps + k.groups * s - 1) / (k.groups * s);
+      const int64_t full = load / k.fit, rest = load % k.fit;
+      double us = k.base + (double)full * (k.ends + rounds * (k.alone + k.more * k.fit));
+      if (rest > 0) us += k.ends + rounds * (k.alone + k.more * (double)rest);
+      if (s > 1) us += k.join + k.part * s + (double)heads * R * s * D * 8e-6 * k.traffic;
+      if (best.kind < 0 || us < best_us) best = Plan{i, blocks, s}, best_us = us;
+    }
+  }
+  return best;
 }
 
 // The search once per shape: one table per thread, the newest shape kept.
@@ -567,21 +667,26 @@ size_t part_bytes(int B, int Hk, int R, int D, int splits) {
   return splits > 1 ? (size_t)B * Hk * R * splits * (16 + (size_t)D * 4) : 0;
 }
 
-template <typename E>
-void launch(const CrossParams& p, int D, int rows, hipStream_t stream) {
-  const dim3 grid(p.deal.groups());
-  if (D == 64) {
-    if (rows == kBlock) {
-      hipLaunchKernelGGL((cross_attn_kernel<E, 64, 1, 4, true, 2>), grid, dim3(256), 0, stream, p);
-    } else {
-      hipLaunchKernelGGL((cross_attn_kernel<E, 64, 4, 1, false, 3>), grid, dim3(256), 0, stream, p);
-    }
+template <typename E, int D, int NB, int RB, int KS, bool kFine, int kMinWaves>
+void launch_kind(const CrossParams& p, hipStream_t stream) {
+  const dim3 grid(p.deal.groups()), block(64 * RB * KS);
+  if constexpr (kFine) {
+    hipLaunchKernelGGL((cross_attn_kernel<E, D, NB, RB, KS, true, false, kMinWaves>), grid, block, 0, stream, p);
+  } else if (p.lse != nullptr) {
+    hipLaunchKernelGGL((cross_attn_kernel<E, D, NB, RB, KS, false, true, kMinWaves>), grid, block, 0, stream, p);
   } else {
-    if (rows == kBlock) {
-      hipLaunchKernelGGL((cross_attn_kernel<E, 128, 1, 2, true, 1>), grid, dim3(128), 0, stream, p);
-    } else {
-      hipLaunchKernelGGL((cross_attn_kernel<E, 128, 4, 1, false, 2>), grid, dim3(256), 0, stream, p);
-    }
+    hipLaunchKernelGGL((cross_attn_kernel<E, D, NB, RB, KS, false, false, kMinWaves>), grid, block, 0, stream, p);
+  }
+}
+
+template <typename E>
+void launch(const CrossParams& p, int kind, int D, hipStream_t stream) {
+  switch (kind) {   // kKinds
+    case 0: launch_kind<E, 64, 1, 1, 4, true, 2>(p, stream); break;
+    case 1: launch_kind<E, 64, 1, 1, 4, false, 2>(p, stream); break;
+    case 2: launch_kind<E, 64, 2, 1, 4, false, 2>(p, stream); break;
+    case 3: launch_kind<E, 128, 1, 1, 2, true, 1>(p, stream); break;
+    default: launch_kind<E, 128, 1, 2, 2, false, 2>(p, stream); break;
   }
   if (p.splits > 1) {
     const dim3 join((unsigned)((int64_t)p.B * p.Hk * p.R));
@@ -687,9 +792,9 @@ SIDON_API int sidon_cross_attention(const void* q, const void* k, const void* v,
   p.scale = (float)(1.4426950408889634 * scale);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == SIDON_FP16) {
-    launch<_Float16>(p, D, c.rows, s);
+    launch<_Float16>(p, c.kind, D, s);
   } else {
-    launch<__bf16>(p, D, c.rows, s);
+    launch<__bf16>(p, c.kind, D, s);
   }
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return fail(SIDON_E_LAUNCH, "cross attention launch failed: %s", hipGetErrorString(err));

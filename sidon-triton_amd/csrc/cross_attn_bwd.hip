@@ -52,7 +52,7 @@ struct BwdParams {
   void* dv;
   const int32_t* lens;
   const int32_t* q_lens;
-  float* stat;           // [B, H, tiles, 2, 32]: lse in powers of two (infinite: no such row), delta
+  float* stat;           // [B, H, tiles, 2, 32]: kLift less lse in powers of two (-infinite: no such row), -delta
   float* length;         // [B, H, tiles, 32]: |dout_i|
   float* longest;        // [B, H, tiles]: of a tile
   float* longest_v;      // [B, Hk, key tiles]: |v_j|
@@ -89,6 +89,21 @@ __device__ __forceinline__ int valid(const int32_t* lens, int b, int most) {
   return lens == nullptr ? most : __builtin_amdgcn_readfirstlane(min(max(lens[b], 0), most));
 }
 
+// Sum over a team of N lanes (8 or 16), in each of them.
+template <int N>
+__device__ __forceinline__ float team_sum(float v) {
+  v += sidon::dpp_mov<0xb1>(v);                          // quad_perm [1, 0, 3, 2]
+  v += sidon::dpp_mov<0x4e>(v);                          // quad_perm [2, 3, 0, 1]
+  v += sidon::dpp_mov<0x141>(v);                         // row_half_mirror
+  if constexpr (N > 8) v += sidon::dpp_mov<0x140>(v);    // row_mirror
+  return v;
+}
+
+// Up to as many keys delta is taken as the sum of P dP, not from the rounded output:
+// the fewer keys, the more of dS cancels (of 3 keys dq was off by 0.29% in bf16, of 20 by
+// 0.24%, which is what its own and dS's rounding cost).
+constexpr int kFewKeys = 32;
+
 // ---- the first launch: a workgroup per 32 queries of a head, or (fp16) 32 keys of a key head ----
 template <typename E, int D>
 __global__ void __launch_bounds__(4 * D) cross_bwd_rows_kernel(const BwdParams p) {
@@ -119,20 +134,38 @@ __global__ void __launch_bounds__(4 * D) cross_bwd_rows_kernel(const BwdParams p
       }
     }
   }
-#pragma unroll
-  for (int d = 1; d < kTeam; d <<= 1) {
-    dot += __shfl_xor(dot, d);
-    sq += __shfl_xor(sq, d);
-  }
-  if (!keys && i == 0) {
+  dot = team_sum<kTeam>(dot);
+  sq = team_sum<kTeam>(sq);
+  if (!keys) {
     float lse = INFINITY;   // no such row, or one that sees no key: P = 0
     if (row < rows) {
       lse = p.lse[(int64_t)bh * p.L + row];
       lse = lse == -INFINITY ? INFINITY : lse * kLog2e;
     }
-    float* at = p.stat + ((int64_t)bh * p.tiles + tile) * (2 * kBlock) + r;
-    at[0] = lse;
-    at[kBlock] = dot;
+    const int lk = valid(p.lens, b, p.S);
+    if (lk <= kFewKeys && row < rows) {
+      const v8 x = *reinterpret_cast<const v8*>(static_cast<const E*>(p.q) + b * p.qb + h * p.qh + (int64_t)row * p.ql + 8 * i);
+      const v8 y = *reinterpret_cast<const v8*>(static_cast<const E*>(p.dout) + b * p.gb + h * p.gh + (int64_t)row * p.gl + 8 * i);
+      const E* const kp = static_cast<const E*>(p.k) + b * p.kb + h / p.G * p.kh + 8 * i;
+      const E* const vp = static_cast<const E*>(p.v) + b * p.vb + h / p.G * p.vh + 8 * i;
+      dot = 0.f;
+      for (int j = 0; j < lk; ++j) {
+        const v8 kk = *reinterpret_cast<const v8*>(kp + (int64_t)j * p.kl);
+        const v8 vv = *reinterpret_cast<const v8*>(vp + (int64_t)j * p.vl);
+        float s = 0.f, dp = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          s = fmaf((float)x[k], (float)kk[k], s);
+          dp = fmaf((float)y[k], (float)vv[k], dp);
+        }
+        dot = fmaf(fast_exp2(fmaf(team_sum<kTeam>(s), p.scale * kLog2e, -lse)), team_sum<kTeam>(dp), dot);
+      }
+    }
+    if (i == 0) {
+      float* at = p.stat + ((int64_t)bh * p.tiles + tile) * (2 * kBlock) + r;
+      at[0] = Range<E>::kLift - lse;
+      at[kBlock] = -dot;
+    }
   }
   if constexpr (Range<E>::kScaled) {
     const float length = sqrtf(sq);
@@ -164,14 +197,15 @@ template <int D, int W>
 struct Copies {
   static constexpr int kBytes = D / 64 * kTile;      // of a tile
   static constexpr int kCount = kBytes / 1024 / W;   // per wavefront
-  static_assert(kBytes / 1024 % W == 0 && (kCount == 1 || kCount == 2), "an even split of the copies");
+  static_assert(kBytes / 1024 % W == 0 && (kCount <= 2 || kCount % 4 == 0), "an even split of the copies");
   uint32_t off[kCount];
   int crow, lane, stride;
   uint32_t at;   // this wavefront's share of a tile in LDS
   int panel;
 
   __device__ __forceinline__ uint32_t offset(int j, int r) const {
-    return (uint32_t)r * (uint32_t)(2 * stride) + 16u * ((lane & 7) ^ tile_swz(crow + 8 * j)) + 1024u * (3 - j);
+    return (uint32_t)r * (uint32_t)(2 * stride) + 16u * ((lane & 7) ^ tile_swz(crow + 8 * (j % 4))) + j / 4 * 128u +
+           1024u * (3 - j % 4);
   }
   __device__ __forceinline__ void init(int w, int lane_, int stride_) {
     lane = lane_, stride = stride_;
@@ -179,7 +213,7 @@ struct Copies {
     crow = w * kCount % 4 * 8 + (lane >> 3);
     at = w * kCount * 1024;
 #pragma unroll
-    for (int j = 0; j < kCount; ++j) off[j] = offset(j, crow + 8 * j);
+    for (int j = 0; j < kCount; ++j) off[j] = offset(j, crow + 8 * (j % 4));
   }
   // Rows of `src` (the tile's first row) into the tile at LDS address lds; rows from
   // `rows` on read the last one again.
@@ -187,8 +221,11 @@ struct Copies {
     const char* const base = uniform(src + panel * 128 - kBack);
     uint32_t o[kCount];
 #pragma unroll
-    for (int j = 0; j < kCount; ++j) o[j] = rows >= kBlock ? off[j] : offset(j, min(crow + 8 * j, rows - 1));
-    if constexpr (kCount == 2) {
+    for (int j = 0; j < kCount; ++j) o[j] = rows >= kBlock ? off[j] : offset(j, min(crow + 8 * (j % 4), rows - 1));
+    if constexpr (kCount % 4 == 0) {
+#pragma unroll
+      for (int j = 0; j < kCount; j += 4) dma_tile(lds + at + j * 1024, base, o[j], o[j + 1], o[j + 2], o[j + 3]);
+    } else if constexpr (kCount == 2) {
       dma_2k(lds + at, base, o[0], o[1]);
     } else {
       dma_1k(lds + at, base, o[0]);
@@ -250,43 +287,47 @@ __device__ __forceinline__ void store(E* dst, const f32x16 (&x)[N], float by, bo
     }
 }
 
-// ---- dk and dv: W wavefronts of 32 keys each ----
-template <typename E, int D, int W, int kMinWaves>
-__global__ void __launch_bounds__(64 * W, kMinWaves) cross_bwd_keys_kernel(const BwdParams p) {
-  using C = Copies<D, W>;
+// ---- dk and dv: a workgroup of RB wavefronts of 32 keys each x KS row groups, which take
+// every KS-th step of 32 queries (of the heads in turn) from a ring of their own ----
+template <typename E, int D, int RB, int KS, int kWaves>
+__global__ void __launch_bounds__(64 * RB * KS) __attribute__((amdgpu_waves_per_eu(kWaves, kWaves)))
+cross_bwd_keys_kernel(const BwdParams p) {
+  using C = Copies<D, RB>;
   constexpr int kQ = D / 16, kDb = D / 32;
   constexpr int kStat = 2 * kBlock * 4, kSlot = 2 * C::kBytes + kStat;   // a step's q, dout, statistics
-  __shared__ __attribute__((aligned(16))) char smem[2 * kSlot];
+  constexpr int kMerge = KS / 2 * RB * 2 * kDb * 16 * 64 * 4;
+  constexpr int kLds = KS * 2 * kSlot > kMerge ? KS * 2 * kSlot : kMerge;
+  __shared__ __attribute__((aligned(16))) char smem[kLds];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rb = w % RB, ks = w / RB;
   const int n = lane & 31, g = lane >> 5;
   int bh;
   const int unit = dealt(p.deal, blockIdx.x, bh);
   if (unit >= p.deal.units) return;
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
-  const int key = (unit * W + w) * kBlock + n;
+  const int key = (unit * RB + rb) * kBlock + n;
   const int lk = valid(p.lens, b, p.S), lq = valid(p.q_lens, b, p.L);
-  const int tiles = unit * W * kBlock < lk ? (lq + kBlock - 1) / kBlock : 0;   // of a head
-  const int steps = tiles * p.G;
+  const int tiles = unit * RB * kBlock < lk ? (lq + kBlock - 1) / kBlock : 0;   // of a head
+  const int steps = tiles * p.G, rounds = (steps + KS - 1) / KS;
 
   C cq, cg;
-  cq.init(w, lane, p.ql);
-  cg.init(w, lane, p.gl);
-  const uint32_t lds = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem);
+  cq.init(rb, lane, p.ql);
+  cg.init(rb, lane, p.gl);
+  const uint32_t lds = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem) + ks * 2 * kSlot;
   const char* const q0 = static_cast<const char*>(p.q) + 2 * (b * p.qb + (int64_t)hk * p.G * p.qh);
   const char* const g0 = static_cast<const char*>(p.dout) + 2 * (b * p.gb + (int64_t)hk * p.G * p.gh);
-  int ch = 0, ct = 0;   // head of the group and tile that are copied next
+  const char* const s0 = reinterpret_cast<const char*>(p.stat + ((int64_t)b * p.H + hk * p.G) * p.tiles * (2 * kBlock));
+  int ch = 0, ct = ks;   // head of the group and tile that are copied next
   const auto copy = [&](int slot) SIDON_INLINE {
+    while (ct >= tiles && ch < p.G) ct -= tiles, ++ch;
     if (ch < p.G) {
       const int rows = lq - ct * kBlock;
       const uint32_t at = lds + slot * kSlot;
       cq.copy(at, q0 + 2 * (ch * p.qh + (int64_t)ct * kBlock * p.ql), rows);
       cg.copy(at + C::kBytes, g0 + 2 * (ch * p.gh + (int64_t)ct * kBlock * p.gl), rows);
-      if (w == 0)
-        dma_256(at + 2 * C::kBytes,
-                uniform(reinterpret_cast<const char*>(p.stat + (((int64_t)b * p.H + hk * p.G + ch) * p.tiles + ct) * (2 * kBlock))),
-                4 * lane);
-      if (++ct == tiles) ct = 0, ++ch;
+      if (rb == 0) dma_256(at + 2 * C::kBytes, uniform(s0 + ((int64_t)ch * p.tiles + ct) * (2 * kBlock * 4)), 4 * lane);
+      ct += KS;
     }
   };
   if (steps > 0) copy(0);
@@ -309,47 +350,81 @@ __global__ void __launch_bounds__(64 * W, kMinWaves) cross_bwd_keys_kernel(const
   if constexpr (Range<E>::kScaled)
     c = below_one(largest(p.longest + ((int64_t)b * p.H + hk * p.G) * p.tiles, p.G * p.tiles, lane),
                   largest(p.longest_v + (int64_t)bh * p.key_tiles, p.key_tiles, lane));
+  asm volatile("" : "+v"(c));
   const float scale2 = p.scale * kLog2e;
 
+  arrived(kop);
+  arrived(vop);
   f32x16 dk[kDb], dv[kDb];
 #pragma unroll
   for (int d = 0; d < kDb; ++d) dk[d] = f32x16{}, dv[d] = f32x16{};
-  for (int u = 0; u < steps; ++u) {
+  for (int u = 0; u < rounds; ++u) {
     wait_vmcnt<0>();
-    lds_barrier();   // step u is there, and step u - 1 is read
+    lds_barrier();   // round u is there, and round u - 1 is read
     copy((u + 1) & 1);
-    const char* const tq = smem + (u & 1) * kSlot;
+    if (u * KS + ks >= steps) continue;
+    const char* const tq = smem + (ks * 2 + (u & 1)) * kSlot;
     const char* const tg = tq + C::kBytes;
     // element i of an accumulator is row 16 (i / 8) + 8 g + i % 8
     const float* const st = reinterpret_cast<const float*>(tq + 2 * C::kBytes) + 8 * g;
-    f32x16 s = {}, dp = {};
-#pragma unroll
-    for (int i = 0; i < kQ; ++i) s = Half<E>::mfma(at.rows(tq, i), kop[i], s);
-#pragma unroll
-    for (int i = 0; i < kQ; ++i) dp = Half<E>::mfma(at.rows(tg, i), vop[i], dp);
+    f32x16 s = {}, dp, lse;
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
-      const f4 lse = *reinterpret_cast<const f4*>(st + 16 * (i >> 3) + (i & 7));
+      const f4 x = *reinterpret_cast<const f4*>(st + kBlock + 16 * (i >> 3) + (i & 7));
+      const f4 y = *reinterpret_cast<const f4*>(st + 16 * (i >> 3) + (i & 7));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[i + e] = fast_exp2(fmaf(s[i + e], scale2, kLift - lse[e]));
+      for (int e = 0; e < 4; ++e) dp[i + e] = x[e], lse[i + e] = y[e];   // -delta, kLift - lse
     }
-    i4 pk[2];
+    i4 qa[kQ], ga[kQ];
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) qa[i] = at.rows(tq, i), ga[i] = at.rows(tg, i);
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) {
+      s = Half<E>::mfma(qa[i], kop[i], s);
+      dp = Half<E>::mfma(ga[i], vop[i], dp);
+    }
+    i4 pk[2], dk16[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], scale2, lse[i]));
     round_to<E>(s, pk);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= Range<E>::kScaled ? dp[i] * c : dp[i];
+    round_to<E>(s, dk16);
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-      for (int d = 0; d < kDb; ++d) dv[d] = Half<E>::mfma(at.columns(tg, hh, d), pk[hh], dv[d]);
+      for (int d = 0; d < kDb; ++d) {
+        dv[d] = Half<E>::mfma(at.columns(tg, hh, d), pk[hh], dv[d]);
+        dk[d] = Half<E>::mfma(at.columns(tq, hh, d), dk16[hh], dk[d]);
+      }
+  }
+
+  // ---- sum the row groups, half of them into the other half at a time ----
+  if constexpr (KS > 1) {
+    float* const mem = reinterpret_cast<float*>(smem) + lane * 4;
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const f4 delta = *reinterpret_cast<const f4*>(st + kBlock + 16 * (i >> 3) + (i & 7));
+    for (int half = KS / 2; half >= 1; half >>= 1) {
+      lds_barrier();
+      float* const part = mem + ((ks % half) * RB + rb) * (2 * kDb * 16 * 64);
+      const auto each = [&](auto&& f) SIDON_INLINE {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[i + e] *= (dp[i + e] - delta[e]) * c;
+        for (int d = 0; d < kDb; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f(dk[d], i, reinterpret_cast<f4*>(part + (d * 8 + i) * 256));
+            f(dv[d], i, reinterpret_cast<f4*>(part + (d * 8 + 4 + i) * 256));
+          }
+      };
+      if (ks >= half)
+        each([](const f32x16& x, int i, f4* to) SIDON_INLINE { *to = f4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]}; });
+      lds_barrier();
+      if (ks >= half) return;
+      each([](f32x16& x, int i, const f4* from) SIDON_INLINE {
+        const f4 v = *from;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e];
+      });
     }
-    round_to<E>(s, pk);
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-      for (int d = 0; d < kDb; ++d) dk[d] = Half<E>::mfma(at.columns(tq, hh, d), pk[hh], dk[d]);
   }
   if (key >= p.S) return;
   const bool there = key < lk;
@@ -358,33 +433,41 @@ __global__ void __launch_bounds__(64 * W, kMinWaves) cross_bwd_keys_kernel(const
   store<E>(static_cast<E*>(p.dv) + b * p.dvb + hk * p.dvh + key * p.dvl + 4 * g, dv, down, there);
 }
 
-// ---- dq: W wavefronts of 32 queries each ----
-template <typename E, int D, int W, int kMinWaves>
-__global__ void __launch_bounds__(64 * W, kMinWaves) cross_bwd_queries_kernel(const BwdParams p) {
-  using C = Copies<D, W>;
-  constexpr int kQ = D / 16, kDb = D / 32;
+// ---- dq: a workgroup of RB wavefronts of 32 queries each x KS key groups, which take
+// every KS-th step of 32 keys from a ring of their own ----
+template <typename E, int D, int RB, int KS, int kWaves>
+__global__ void __launch_bounds__(64 * RB * KS) __attribute__((amdgpu_waves_per_eu(kWaves, kWaves)))
+cross_bwd_queries_kernel(const BwdParams p) {
+  using C = Copies<D, RB>;
+  constexpr int kQ = D / 16, kDb = D / 32, kRows = RB * kBlock;
   constexpr int kSlot = 2 * C::kBytes;   // a step's k and v
-  __shared__ __attribute__((aligned(16))) char smem[2 * kSlot];
+  constexpr int kMerge = KS / 2 * RB * kDb * 16 * 64 * 4;
+  constexpr int kLds = KS * 2 * kSlot > kMerge ? KS * 2 * kSlot : kMerge;
+  __shared__ __attribute__((aligned(16))) char smem[kLds];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rb = w % RB, ks = w / RB;
   const int n = lane & 31, g = lane >> 5;
   int bh;   // of a key head
   const int unit = dealt(p.deal, blockIdx.x, bh);
   if (unit >= p.deal.units) return;
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
-  const int head = hk * p.G + unit % p.G, row = (unit / p.G * W + w) * kBlock + n;
+  const int head = hk * p.G + unit % p.G, block0 = unit / p.G * kRows;
+  const int row = block0 + rb * kBlock + n;   // of this lane
   const int lk = valid(p.lens, b, p.S), lq = valid(p.q_lens, b, p.L);
-  const int steps = unit / p.G * W * kBlock < lq ? (lk + kBlock - 1) / kBlock : 0;
+  const int steps = block0 < lq ? (lk + kBlock - 1) / kBlock : 0;
+  const int rounds = (steps + KS - 1) / KS;
 
   C ck, cv;
-  ck.init(w, lane, p.kl);
-  cv.init(w, lane, p.vl);
-  const uint32_t lds = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem);
+  ck.init(rb, lane, p.kl);
+  cv.init(rb, lane, p.vl);
+  const uint32_t lds = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem) + ks * 2 * kSlot;
   const char* const k0 = static_cast<const char*>(p.k) + 2 * (b * p.kb + hk * p.kh);
   const char* const v0 = static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh);
-  const auto copy = [&](int t) SIDON_INLINE {
+  const auto copy = [&](int u) SIDON_INLINE {
+    const int t = u * KS + ks;
     if (t < steps) {
-      const uint32_t at = lds + (t & 1) * kSlot;
+      const uint32_t at = lds + (u & 1) * kSlot;
       ck.copy(at, k0 + (int64_t)t * kBlock * p.kl * 2, lk - t * kBlock);
       cv.copy(at + C::kBytes, v0 + (int64_t)t * kBlock * p.vl * 2, lk - t * kBlock);
     }
@@ -393,53 +476,87 @@ __global__ void __launch_bounds__(64 * W, kMinWaves) cross_bwd_queries_kernel(co
 
   Reads at;
   at.init(lane);
+  constexpr float kLift = Range<E>::kLift;
   i4 qop[kQ], gop[kQ];
   const int rr = max(min(row, lq - 1), 0);
-  {
-    const E* qp = static_cast<const E*>(p.q) + b * p.qb + head * p.qh + (int64_t)rr * p.ql + 8 * g;
-    const E* gp = static_cast<const E*>(p.dout) + b * p.gb + head * p.gh + (int64_t)rr * p.gl + 8 * g;
+  const E* const qp = static_cast<const E*>(p.q) + b * p.qb + head * p.qh + (int64_t)rr * p.ql + 8 * g;
+  const E* const gp = static_cast<const E*>(p.dout) + b * p.gb + head * p.gh + (int64_t)rr * p.gl + 8 * g;
 #pragma unroll
-    for (int s = 0; s < kQ; ++s) {
-      qop[s] = *reinterpret_cast<const i4*>(qp + 16 * s);
-      gop[s] = *reinterpret_cast<const i4*>(gp + 16 * s);
-    }
+  for (int s = 0; s < kQ; ++s) {
+    qop[s] = *reinterpret_cast<const i4*>(qp + 16 * s);
+    gop[s] = *reinterpret_cast<const i4*>(gp + 16 * s);
   }
-  constexpr float kLift = Range<E>::kLift;
   const int64_t tile = ((int64_t)b * p.H + head) * p.tiles + rr / kBlock;
-  const float lse = p.stat[tile * (2 * kBlock) + rr % kBlock] - kLift, delta = p.stat[tile * (2 * kBlock) + kBlock + rr % kBlock];
+  float lse = p.stat[tile * (2 * kBlock) + rr % kBlock];              // kLift - lse
+  float delta = p.stat[tile * (2 * kBlock) + kBlock + rr % kBlock];   // -delta
   float c = 1.f;
   if constexpr (Range<E>::kScaled)
     c = below_one(p.length[tile * kBlock + rr % kBlock], largest(p.longest_v + (int64_t)bh * p.key_tiles, p.key_tiles, lane));
+  arrived(qop);
+  arrived(gop);
+  asm volatile("" : "+v"(lse), "+v"(delta), "+v"(c));
   const float scale2 = p.scale * kLog2e;
 
   f32x16 dq[kDb];
 #pragma unroll
   for (int d = 0; d < kDb; ++d) dq[d] = f32x16{};
-  for (int u = 0; u < steps; ++u) {
+  for (int u = 0; u < rounds; ++u) {
     wait_vmcnt<0>();
     lds_barrier();
     copy(u + 1);
-    const char* const tk = smem + (u & 1) * kSlot;
+    const int t = u * KS + ks;
+    if (t >= steps) continue;
+    const char* const tk = smem + (ks * 2 + (u & 1)) * kSlot;
     const char* const tv = tk + C::kBytes;
-    f32x16 s = {}, dp = {};
+    f32x16 s = {}, dp;
 #pragma unroll
-    for (int i = 0; i < kQ; ++i) s = Half<E>::mfma(at.rows(tk, i), qop[i], s);
+    for (int i = 0; i < 16; ++i) dp[i] = delta;
 #pragma unroll
-    for (int i = 0; i < kQ; ++i) dp = Half<E>::mfma(at.rows(tv, i), gop[i], dp);
-    if ((u + 1) * kBlock > lk) {
-      const int left = lk - u * kBlock - 8 * g;
+    for (int i = 0; i < kQ; ++i) {
+      s = Half<E>::mfma(at.rows(tk, i), qop[i], s);
+      dp = Half<E>::mfma(at.rows(tv, i), gop[i], dp);
+    }
+    if ((t + 1) * kBlock > lk) {
+      const int left = lk - t * kBlock - 8 * g;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (16 * (i >> 3) + (i & 7) >= left) s[i] = -INFINITY;
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], scale2, -lse)) * ((dp[i] - delta) * c);
+    for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], scale2, lse)) * (Range<E>::kScaled ? dp[i] * c : dp[i]);
     i4 pk[2];
     round_to<E>(s, pk);
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
       for (int d = 0; d < kDb; ++d) dq[d] = Half<E>::mfma(at.columns(tk, hh, d), pk[hh], dq[d]);
+  }
+
+  // ---- sum the key groups, half of them into the other half at a time ----
+  if constexpr (KS > 1) {
+    float* const mem = reinterpret_cast<float*>(smem) + lane * 4;
+#pragma unroll
+    for (int half = KS / 2; half >= 1; half >>= 1) {
+      lds_barrier();   // the rings, or the last round's values, are done with
+      float* const part = mem + ((ks % half) * RB + rb) * (kDb * 16 * 64);
+      if (ks >= half) {
+#pragma unroll
+        for (int d = 0; d < kDb; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<f4*>(part + (d * 4 + i) * 256) = f4{dq[d][4 * i], dq[d][4 * i + 1], dq[d][4 * i + 2], dq[d][4 * i + 3]};
+      }
+      lds_barrier();
+      if (ks >= half) return;
+#pragma unroll
+      for (int d = 0; d < kDb; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f4 v = *reinterpret_cast<const f4*>(part + (d * 4 + i) * 256);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dq[d][4 * i + e] += v[e];
+        }
+    }
   }
   if (row >= p.L) return;
   store<E>(static_cast<E*>(p.dq) + b * p.dqb + head * p.dqh + row * p.dql + 4 * g, dq, p.scale * fast_exp2(-kLift) / c,
@@ -466,17 +583,76 @@ Workspace workspace(int B, int H, int Hk, int L, int S, int dtype) {
   return Workspace{tiles * 2 * kBlock, tiles * kBlock, tiles, (size_t)B * Hk * tiles_of(S)};
 }
 
+// Which form of a kernel: blocks of 32 rows or keys and groups of a workgroup, by the least
+// estimate (us) of
+//
+//   turns (ends + rounds (alone + more running))
+//
+// where a CU's share of the workgroups takes full turns of `fit` at once and one with the
+// rest, `running` is what a turn holds, and a workgroup's rounds are its steps over its
+// groups.  Fitted to 110 shapes of 1 to 24 items, 8 to 1400 queries and 30 to 6000 keys in
+// every form: the choice is on average within 2% of the best one's time.  (More groups make
+// workgroups shorter, more blocks share copies: dk and dv of 2 x 16 heads x 300 x 1463 24.1 us
+// in the first form, 20.8 in the second, 28.5 in the third; of 8 x 8 x 100 x 500 11.1, 12.2
+// and 15.2; dq of them 29.0, 19.0 and 17.9, 13.4, 10.0 and 8.5.)
+struct Form {
+  int blocks, groups, fit;
+  double base, ends, alone, more;
+};
+constexpr Form kKeys[2][3] = {
+    {{4, 1, 1, 3.37, 3.29, .629, 0}, {2, 2, 2, 1.92, 4.77, .601, .247}, {1, 4, 1, 4.47, 1.91, .623, 0}},
+    {{4, 1, 2, 1.4, 7, .55, .72}, {2, 2, 2, 0, 9.2, .777, .787}, {1, 2, 2, 3, 5.54, .805, .317}}};
+constexpr Form kQueries[2][3] = {
+    {{4, 1, 3, 0, 5.54, .19, .296}, {2, 2, 3, .85, 4.88, .215, .304}, {1, 4, 2, 1.85, 3.86, .406, .281}},
+    {{4, 1, 2, 0, 6.25, .182, .615}, {2, 2, 2, .29, 6.36, .263, .613}, {1, 2, 2, 1.39, 4.6, .859, .122}}};
+
+// heads of `units` rows or keys, each over `steps` tiles.
+int choose(const Form (&forms)[3], int64_t heads, int units, int64_t steps, int cus) {
+  int best = 0;
+  double best_us = 0;
+  for (int i = 0; i < 3; ++i) {
+    const Form& f = forms[i];
+    const int64_t load = (heads * ((units + f.blocks * kBlock - 1) / (f.blocks * kBlock)) + cus - 1) / cus;
+    const double rounds = (double)((steps + f.groups - 1) / f.groups);
+    double us = f.base + (double)(load / f.fit) * (f.ends + rounds * (f.alone + f.more * f.fit));
+    if (load % f.fit > 0) us += f.ends + rounds * (f.alone + f.more * (double)(load % f.fit));
+    if (i == 0 || us < best_us) best = i, best_us = us;
+  }
+  return best;
+}
+
+template <typename E, int D, int RB, int KS, int kWaves>
+void launch_keys(BwdParams& p, hipStream_t stream) {
+  constexpr int kKeysOf = RB * kBlock;
+  p.deal = deal((int64_t)p.B * p.Hk, (p.S + kKeysOf - 1) / kKeysOf, (int64_t)p.G * p.L * D * 4);
+  hipLaunchKernelGGL((cross_bwd_keys_kernel<E, D, RB, KS, kWaves>), dim3(p.deal.groups()), dim3(64 * RB * KS), 0, stream, p);
+}
+
+template <typename E, int D, int RB, int KS, int kWaves>
+void launch_queries(BwdParams& p, hipStream_t stream) {
+  constexpr int kRows = RB * kBlock;
+  p.deal = deal((int64_t)p.B * p.Hk, (int64_t)p.G * ((p.L + kRows - 1) / kRows), (int64_t)p.S * D * 4);
+  hipLaunchKernelGGL((cross_bwd_queries_kernel<E, D, RB, KS, kWaves>), dim3(p.deal.groups()), dim3(64 * RB * KS), 0, stream, p);
+}
+
 template <typename E, int D>
 void launch(BwdParams& p, hipStream_t stream) {
-  constexpr int W = 4;
   unsigned rows = (unsigned)p.B * p.H * p.tiles;
   if (Range<E>::kScaled) rows += (unsigned)p.B * p.Hk * p.key_tiles;
   hipLaunchKernelGGL((cross_bwd_rows_kernel<E, D>), dim3(rows), dim3(4 * D), 0, stream, p);
-  const int64_t heads = (int64_t)p.B * p.Hk;
-  p.deal = deal(heads, (p.S + W * kBlock - 1) / (W * kBlock), (int64_t)p.G * p.L * D * 4);
-  hipLaunchKernelGGL((cross_bwd_keys_kernel<E, D, W, 2>), dim3(p.deal.groups()), dim3(64 * W), 0, stream, p);
-  p.deal = deal(heads, (int64_t)p.G * ((p.L + W * kBlock - 1) / (W * kBlock)), (int64_t)p.S * D * 4);
-  hipLaunchKernelGGL((cross_bwd_queries_kernel<E, D, W, 2>), dim3(p.deal.groups()), dim3(64 * W), 0, stream, p);
+  // (as many wavefronts a SIMD as the registers allow: three of 168 at D 64, two of 256 at 128)
+  constexpr int kWaves = D == 64 ? 3 : 2, kGroups = D == 64 ? 4 : 2;
+  const int cus = sidon::compute_units();
+  switch (choose(kKeys[D == 64 ? 0 : 1], (int64_t)p.B * p.Hk, p.S, (int64_t)p.G * p.tiles, cus)) {
+    case 0: launch_keys<E, D, 4, 1, kWaves>(p, stream); break;
+    case 1: launch_keys<E, D, 2, 2, kWaves>(p, stream); break;
+    default: launch_keys<E, D, 1, kGroups, kWaves>(p, stream); break;
+  }
+  switch (choose(kQueries[D == 64 ? 0 : 1], (int64_t)p.B * p.H, p.L, p.key_tiles, cus)) {
+    case 0: launch_queries<E, D, 4, 1, kWaves>(p, stream); break;
+    case 1: launch_queries<E, D, 2, 2, kWaves>(p, stream); break;
+    default: launch_queries<E, D, 1, kGroups, kWaves>(p, stream); break;
+  }
 }
 
 }  // namespace

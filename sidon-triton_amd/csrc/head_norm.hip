@@ -369,8 +369,17 @@ __global__ void __launch_bounds__(kSumThreads) head_norm_sum_kernel(const NormPa
   const int c = threadIdx.x % kCols, row = threadIdx.x / kCols;
   const int at = blockIdx.x * kCols + c;
   float sum = 0.f;
-  if (at < p.D)
-    for (uint32_t b = row; b < s.blocks; b += kRows) sum += s.part[(int64_t)b * p.D + at];
+  constexpr int kAtOnce = 8;   // loads together, or each would wait for the one before
+  for (uint32_t b0 = row; b0 < s.blocks; b0 += kAtOnce * kRows) {
+    float v[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint32_t b = b0 + i * kRows;
+      v[i] = at < p.D && b < s.blocks ? s.part[(int64_t)b * p.D + at] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) sum += v[i];
+  }
   sums[row][c] = sum;
   __syncthreads();
   if (row == 0 && at < p.D) {

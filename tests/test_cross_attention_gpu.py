@@ -237,13 +237,19 @@ def test_strides_and_out(sidon, l):
 @pytest.mark.parametrize("kind", KINDS, ids=str)
 @pytest.mark.parametrize("l", [1, 200])
 def test_a_query_that_is_no_number(sidon, l, kind):
+    """NaN in its own row.  A row whose sum the matrix core takes in one with it has its
+    sum taken apart, its 32 fp32 terms in another order: off by less than 32 2^-24 of
+    itself, so the result moves by less than 2^-19 of itself, which its rounding turns into
+    one step (2 u) at most; every other row keeps its bits."""
     q, k, v, _ = inputs(2, 4, 2, l, 300, 64, kind, 13)
     want = sidon.cross_attention.cross_attention(q, k, v)
     q[1, 2, l // 2, 5] = float("nan")
     got = sidon.cross_attention.cross_attention(q, k, v)
     assert got[1, 2, l // 2].isnan().all()
     got[1, 2, l // 2] = want[1, 2, l // 2]
-    assert torch.equal(got, want)
+    err = (got.double() - want.double()).abs()
+    assert (err <= torch.finfo(kind).eps * want.double().abs() + tiny(kind)).all()
+    assert int((err.amax(-1) > 0).sum()) <= 1   # (of the rows)
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
@@ -274,3 +280,26 @@ def test_captured(sidon, kind):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("shape", [(1, 8, 8, 1, 4800, 64), (2, 4, 1, 1, 3000, 128), (3, 8, 4, 100, 900, 64), (4, 16, 4, 500, 1100, 64),
+                                   (3, 8, 8, 517, 700, 128)], ids=str)
+def test_repeated_calls(sidon, shape, kind):
+    """The same bits from every launch, with and without lse, both directions."""
+    b, h, hk, l, s, d = shape
+    q, k, v, dout = inputs(*shape, kind, 19)
+    lens = int32([s - 37 * i for i in range(b)])
+    ca = sidon.cross_attention
+    lse = torch.empty(b, h, l, device=DEV)
+    want = ca.cross_attention(q, k, v, lens, lse=lse)
+    grads = ca.cross_attention_backward(dout, q, k, v, want, lse, lens)
+    first = lse.clone()
+    differ = torch.zeros((), dtype=torch.int64, device=DEV)
+    for i in range(40):
+        differ += (ca.cross_attention(q, k, v, lens, lse=lse if i % 2 else None) != want).sum()
+        differ += (lse != first).sum()
+        if i % 4 == 0:
+            for x, y in zip(ca.cross_attention_backward(dout, q, k, v, want, lse, lens), grads):
+                differ += (x != y).sum()
+    assert int(differ) == 0
