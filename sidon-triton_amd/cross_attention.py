@@ -78,12 +78,6 @@ def _check(q, k, v, lens, q_lens) -> tuple:
             _strides(torch.empty(q.shape, device="meta")), workspace_bytes(*sizes, device))
 
 
-def _tensors(**named) -> None:
-    for name, t in named.items():
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
-
-
 def _scale(scale, dim) -> float:
     return dim ** -0.5 if scale is None else float(scale)
 
@@ -95,9 +89,10 @@ def _check_lse(lse, sizes, device) -> None:
         raise ValueError(f"lse must be a contiguous float32 {shape} tensor")
 
 
-def _workspace(workspace, need, device):
+def _workspace(workspace, need, like):
     if workspace is None:
-        return torch.empty(need, device=device, dtype=torch.uint8) if need else None
+        return like.new_empty(need, dtype=torch.uint8) if need else None
+    device = like.device
     _check_device_tensor("workspace", workspace, device)
     if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
         raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
@@ -107,7 +102,7 @@ def _workspace(workspace, need, device):
 def _out(name, out, like):
     """-> (tensor, strides): ``out``, or a new contiguous tensor of ``like``'s shape."""
     if out is None:
-        out = torch.empty(like.shape, device=like.device, dtype=like.dtype)
+        out = like.new_empty(like.shape)
     else:
         _check_device_tensor(name, out, like.device)
         if out.dtype != like.dtype or out.shape != like.shape or out.stride(-1) != 1:
@@ -138,7 +133,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: tor
     rounded to the inputs' type in front of v, but with H / Hk * L <= 32 (single
     tokens), where the output's rounding is the only one; with more that depends on all
     sizes."""
-    _tensors(q=q, k=k, v=v)
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+        raise TypeError("q, k and v must be torch.Tensor")
     key = _layout(q, k, v, lens, q_lens)
     sizes, dtype, strides, o_strides, need = _layouts.get(key) or _layouts.keep(key, _check(q, k, v, lens, q_lens))
     device = q.device
@@ -146,14 +142,14 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: tor
         raise ValueError("cross_attention follows no gradient: call it under torch.no_grad(), and "
                          "cross_attention_backward for the gradients")
     if out is None:
-        out = torch.empty(q.shape, device=device, dtype=q.dtype)
+        out = q.new_empty(q.shape)
     else:
         out, o_strides = _out("out", out, q)
     if lse is not None:
         _check_lse(lse, sizes, device)
     lib = _lib.load()
     with _on_device(device):
-        workspace = _workspace(workspace, need, device)
+        workspace = _workspace(workspace, need, q)
         rc = lib.sidon_cross_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lens), _ptr(q_lens), _scale(scale, sizes[-1]), out.data_ptr(),
             _ptr(lse), _ptr(workspace), 0 if workspace is None else workspace.numel(), *sizes, dtype, *strides,
@@ -190,7 +186,8 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     keys.  Heads that share a key head are summed in fp32.  workspace: a contiguous uint8
     tensor of ``backward_workspace_bytes``; allocated per call when None.  Equal calls
     give equal bits."""
-    _tensors(dout=dout, q=q, k=k, v=v, out=out, lse=lse)
+    if not all(isinstance(t, torch.Tensor) for t in (dout, q, k, v, out, lse)):
+        raise TypeError("dout, q, k, v, out and lse must be torch.Tensor")
     key = _layout(dout, q, k, v, out, lse, lens, q_lens)
     sizes, dtype, strides, contiguous, need = (
         _backward_layouts.get(key)
@@ -200,11 +197,11 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
         raise ValueError("cross_attention_backward follows no gradient: call it under torch.no_grad()")
     outs = []
     for i, (name, t, like) in enumerate((("dq", dq, q), ("dk", dk, k), ("dv", dv, v))):
-        outs.append((torch.empty(like.shape, device=device, dtype=q.dtype), contiguous[i]) if t is None
+        outs.append((like.new_empty(like.shape), contiguous[i]) if t is None
                     else _out(name, t, like))
     lib = _lib.load()
     with _on_device(device):
-        workspace = _workspace(workspace, need, device)
+        workspace = _workspace(workspace, need, q)
         rc = lib.sidon_cross_attention_bwd(
             dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(lens),
             _ptr(q_lens), _scale(scale, sizes[-1]), *[t.data_ptr() for t, _ in outs], workspace.data_ptr(),

@@ -43,18 +43,24 @@ struct Int4Params {
 };
 
 // Eight nibbles of a word (in the order 0 2 4 6 1 3 5 7 from the lowest) as an operand.
+// `mask` and `lead` in vector registers, so that an insertion is one instruction.
 template <typename E>
-__device__ __forceinline__ i4 operand(uint32_t word) {
+__device__ __forceinline__ i4 operand(uint32_t word, uint32_t mask, uint32_t lead) {
+  const auto insert = [&](uint32_t x) { return (mask & x) | (~mask & lead); };
   i4 r;
   if constexpr (__is_same(E, _Float16)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const h2 v = __builtin_bit_cast(h2, ((word >> (4 * i)) & 0x000f000fu) | 0x64006400u);
-      r[i] = __builtin_bit_cast(int, v - h2{(_Float16)1032.f, (_Float16)1032.f});
-    }
+    // The upper nibble of a byte stands 4 bits higher in the mantissa: 1024 + 16 q.
+    const uint32_t high = word >> 8;
+    const auto insert16 = [&](uint32_t x) { return ((mask << 4) & x) | (~(mask << 4) & lead); };
+    const h2 less = {(_Float16)-1032.f, (_Float16)-1032.f}, down = {(_Float16)0.0625f, (_Float16)0.0625f},
+             less16 = {(_Float16)-72.f, (_Float16)-72.f};
+    r[0] = __builtin_bit_cast(int, __builtin_bit_cast(h2, insert(word)) + less);
+    r[1] = __builtin_bit_cast(int, __builtin_elementwise_fma(__builtin_bit_cast(h2, insert16(word)), down, less16));
+    r[2] = __builtin_bit_cast(int, __builtin_bit_cast(h2, insert(high)) + less);
+    r[3] = __builtin_bit_cast(int, __builtin_elementwise_fma(__builtin_bit_cast(h2, insert16(high)), down, less16));
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = (int)(((word >> (4 * i)) & 0x000f000fu) | 0x43004300u);
+    for (int i = 0; i < 4; ++i) r[i] = (int)insert(word >> (4 * i));
   }
   return r;
 }
@@ -77,9 +83,13 @@ __global__ void __launch_bounds__(64 * WK) int4_linear_kernel(const Int4Params p
     wp[j] = static_cast<const i4*>(p.words) + tile * p.blocks * 64 + lane;
     sp[j] = p.scales + tile * p.blocks * (kGroups * 16) + c;
   }
+  // (rows past the last are that one again, and inputs past the last, whose scales are 0,
+  // the last 32: neither is stored)
   const E* xp[MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) xp[m] = static_cast<const E*>(p.x) + (row0 + 16 * m + c) * p.ldx + 8 * g;
+  for (int m = 0; m < MT; ++m) xp[m] = static_cast<const E*>(p.x) + min(row0 + 16 * m + c, p.M - 1) * p.ldx + 8 * g;
+  uint32_t mask = 0x000f000fu, lead = __is_same(E, _Float16) ? 0x64006400u : 0x43004300u;
+  asm("" : "+v"(mask), "+v"(lead));
 
   f4 total[MT][NT] = {};
   const int one2 = __is_same(E, _Float16) ? 0x3c003c00 : 0x3f803f80;
@@ -100,8 +110,7 @@ __global__ void __launch_bounds__(64 * WK) int4_linear_kernel(const Int4Params p
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         xop[m][i] = i4{};
-        if (row0 + 16 * m + c < p.M && b * kTileK + 32 * i < p.K)
-          xop[m][i] = *reinterpret_cast<const i4*>(xp[m] + b * kTileK + 32 * i);
+        if (MT > 1 || c < p.M) xop[m][i] = *reinterpret_cast<const i4*>(xp[m] + min(b * kTileK + 32 * i, p.K - 32));
       }
     f4 sums[MT][kGroups] = {};
     if constexpr (kOff) {
@@ -117,7 +126,7 @@ __global__ void __launch_bounds__(64 * WK) int4_linear_kernel(const Int4Params p
         f4 acc[MT] = {};
 #pragma unroll
         for (int i = k * SPG; i < (k + 1) * SPG; ++i) {
-          const i4 op = operand<E>((uint32_t)words[j][i]);
+          const i4 op = operand<E>((uint32_t)words[j][i], mask, lead);
 #pragma unroll
           for (int m = 0; m < MT; ++m) acc[m] = Half<E>::small(xop[m][i], op, acc[m]);
         }
@@ -163,13 +172,16 @@ struct Shape {
   int mt, nt, wk;
 };
 
-// Rows of a workgroup by what M needs; outputs of a wavefront and wavefronts along K so
-// that the launch has at least a workgroup per CU.
+// Rows of a workgroup by what M needs.  A wavefront takes four tiles of outputs where that
+// leaves every CU a workgroup (each tile more is x loaded once less: 16 x 16384 x 2048 7.1 us,
+// with one tile 11.5), one where it does not (1 x 8192 x 4096 6.1, with four 8.6), and K is
+// split over eight wavefronts, or four where there are many workgroups as it is (64 x 32768 x
+// 4096 42 us, with eight 44; 1 x 32768 x 4096 17.1 and 16.1).
 Shape shape(int M, int N, int cus) {
   const int mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  const int64_t tiles = (N + kTileN - 1) / kTileN, rows = (M + 16 * mt - 1) / (16 * mt);
-  if (tiles * rows >= 8 * (int64_t)cus) return Shape{mt, 4, 4};
-  return Shape{mt, 1, 8};
+  const int64_t units = (int64_t)((N + kTileN - 1) / kTileN) * ((M + 16 * mt - 1) / (16 * mt));
+  if (units < 4 * (int64_t)cus) return Shape{mt, 1, 8};
+  return Shape{mt, 4, units * mt > 16 * (int64_t)cus ? 4 : 8};
 }
 
 template <typename E, int MT, int NT, int WK>
@@ -192,10 +204,12 @@ void launch_groups(const Int4Params& p, int group, bool off, dim3 grid, hipStrea
 template <typename E, int MT>
 void launch_shape(const Int4Params& p, const Shape& c, int group, bool off, hipStream_t s) {
   const dim3 grid((p.tiles + c.nt - 1) / c.nt, (p.M + 16 * MT - 1) / (16 * MT));
-  if (c.nt == 4)
-    launch_groups<E, MT, 4, 4>(p, group, off, grid, s);
-  else
+  if (c.nt == 1)
     launch_groups<E, MT, 1, 8>(p, group, off, grid, s);
+  else if (c.wk == 8)
+    launch_groups<E, MT, 4, 8>(p, group, off, grid, s);
+  else
+    launch_groups<E, MT, 4, 4>(p, group, off, grid, s);
 }
 
 template <typename E>

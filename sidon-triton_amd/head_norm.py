@@ -32,7 +32,7 @@ def workspace_bytes(batch: int, heads: int, kv_heads: int, length: int, keys: in
 
 
 def _layout(*tensors) -> tuple:
-    return tuple(None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors)
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors])
 
 
 def _rows(name, t, shape, like) -> None:
@@ -111,7 +111,7 @@ def _out(name, out, like, contiguous):
             raise ValueError(f"{name} without k")
         return None, _NONE
     if out is None:
-        return torch.empty(like.shape, device=like.device, dtype=like.dtype), contiguous
+        return like.new_empty(like.shape), contiguous
     _rows(name, out, tuple(like.shape), like)
     return out, _strides(out)
 
@@ -177,12 +177,12 @@ def qk_norm_rotary_backward(dout_q: torch.Tensor, dout_k: torch.Tensor | None, q
     dq, sq = _out("dq", dq, q, contiguous[0])
     dk, sk = _out("dk", dk, k, contiguous[1])
     dim, device = sizes[-1], q.device
-    dw = torch.empty(1 if k is None else 2, dim, device=device)
+    dw = q_w.new_empty((1 if k is None else 2, dim))
     lib = _lib.load()
     with _on_device(device):
         need = lib.sidon_qk_norm_rotary_workspace_bytes(*sizes)
         if workspace is None:
-            workspace = torch.empty(need, device=device, dtype=torch.uint8)
+            workspace = q.new_empty(need, dtype=torch.uint8)
         else:
             _check_device_tensor("workspace", workspace, device)
             if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:

@@ -133,7 +133,7 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, bias: torch.Tensor | None = None
         raise ValueError("int4_linear has no backward: call it under torch.no_grad()")
     rows = x.shape[0]
     if out is None:
-        out = torch.empty(rows, w.n, device=device, dtype=w.dtype)
+        out = x.new_empty((rows, w.n))
     else:
         _check_device_tensor("out", out, device)
         if out.dtype != w.dtype or tuple(out.shape) != (rows, w.n) or (out.stride(1) != 1 and w.n > 1):
