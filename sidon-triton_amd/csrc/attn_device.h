@@ -104,7 +104,7 @@ __device__ __forceinline__ void arrived(i4 (&x)[N]) {
 // long and short items.
 struct Deal {
   int units, parts, per_xcd;   // of a head, of a head, parts of all heads on an XCD
-  unsigned groups() const { return (unsigned)(8 * per_xcd) * (unsigned)((units + parts - 1) / parts); }
+  __host__ __device__ unsigned groups() const { return (unsigned)(8 * per_xcd) * (unsigned)((units + parts - 1) / parts); }
 };
 // Parts: whole heads on an XCD where possible, and all 8 where what `heads` heads of
 // `bytes` read fits one L2 together.

@@ -5,12 +5,12 @@
 //   dv_j = sum_i P_ij dout_i          dP_ij = dout_i . v_j
 //   dS_ij = P_ij (dP_ij - delta_i)    dq_i = scale sum_j dS_ij k_j    dk_j = scale sum_i dS_ij q_i
 //
-// Three launches.  The first takes delta and lse row by row.  In the second a
-// wavefront owns 32 keys, whose k and v stay in its registers as B operands, and goes
+// Two launches.  The first takes delta and lse row by row.  In the second some
+// wavefronts own 32 keys each, whose k and v stay in their registers as B operands, and go
 // over the queries of the heads that share them: S = Q . K^T and dP = dO . V^T by
 // v_mfma_f32_32x32x16, whose accumulators, rounded, are the B operands of
-// dV^T += dO^T . P and dK^T += Q^T . dS.  In the third a wavefront owns 32 queries and
-// goes over the keys: S^T = K . Q^T, dP^T = V . dO^T, dQ^T += K^T . dS^T.  (Seven
+// dV^T += dO^T . P and dK^T += Q^T . dS; others own 32 queries and
+// go over the keys: S^T = K . Q^T, dP^T = V . dO^T, dQ^T += K^T . dS^T.  (Seven
 // products where one pass would do with five and add dq up across workgroups: no
 // atomics, so the same bits every time.)  The tiles of 32 rows that the wavefronts of
 // a workgroup share are copied global -> LDS by global_load_lds_dwordx4 one step
@@ -61,7 +61,7 @@ struct BwdParams {
   int ql, kl, vl, gl;    // row strides (< 2^25)
   int B, H, Hk, G, L, S;
   int tiles, key_tiles;  // of 32 queries, of 32 keys
-  Deal deal;
+  Deal keys, queries;    // blocks of keys, of queries of a group's heads
   float scale;
 };
 
@@ -287,24 +287,29 @@ __device__ __forceinline__ void store(E* dst, const f32x16 (&x)[N], float by, bo
     }
 }
 
+// LDS of a workgroup: KS rings of two slots, which hold a step's q, dout and statistics or
+// its k and v; then the partial results of half of the groups.
+template <int D, int RB, int KS>
+struct Lds {
+  static constexpr int kStat = 2 * kBlock * 4;
+  static constexpr int kTiles = 2 * Copies<D, RB>::kBytes, kKeysSlot = kTiles + kStat;
+  static constexpr int kMerge = KS / 2 * RB * 2 * (D / 32) * 16 * 64 * 4;
+  static constexpr int kBytes = KS * 2 * kKeysSlot > kMerge ? KS * 2 * kKeysSlot : kMerge;
+};
+
 // ---- dk and dv: a workgroup of RB wavefronts of 32 keys each x KS row groups, which take
 // every KS-th step of 32 queries (of the heads in turn) from a ring of their own ----
-template <typename E, int D, int RB, int KS, int kWaves>
-__global__ void __launch_bounds__(64 * RB * KS) __attribute__((amdgpu_waves_per_eu(kWaves, kWaves)))
-cross_bwd_keys_kernel(const BwdParams p) {
+template <typename E, int D, int RB, int KS>
+__device__ __forceinline__ void keys_body(const BwdParams& p, char* smem, int block) {
   using C = Copies<D, RB>;
-  constexpr int kQ = D / 16, kDb = D / 32;
-  constexpr int kStat = 2 * kBlock * 4, kSlot = 2 * C::kBytes + kStat;   // a step's q, dout, statistics
-  constexpr int kMerge = KS / 2 * RB * 2 * kDb * 16 * 64 * 4;
-  constexpr int kLds = KS * 2 * kSlot > kMerge ? KS * 2 * kSlot : kMerge;
-  __shared__ __attribute__((aligned(16))) char smem[kLds];
+  constexpr int kQ = D / 16, kDb = D / 32, kSlot = Lds<D, RB, KS>::kKeysSlot;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rb = w % RB, ks = w / RB;
   const int n = lane & 31, g = lane >> 5;
   int bh;
-  const int unit = dealt(p.deal, blockIdx.x, bh);
-  if (unit >= p.deal.units) return;
+  const int unit = dealt(p.keys, block, bh);
+  if (unit >= p.keys.units) return;
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
   const int key = (unit * RB + rb) * kBlock + n;
   const int lk = valid(p.lens, b, p.S), lq = valid(p.q_lens, b, p.L);
@@ -435,22 +440,17 @@ cross_bwd_keys_kernel(const BwdParams p) {
 
 // ---- dq: a workgroup of RB wavefronts of 32 queries each x KS key groups, which take
 // every KS-th step of 32 keys from a ring of their own ----
-template <typename E, int D, int RB, int KS, int kWaves>
-__global__ void __launch_bounds__(64 * RB * KS) __attribute__((amdgpu_waves_per_eu(kWaves, kWaves)))
-cross_bwd_queries_kernel(const BwdParams p) {
+template <typename E, int D, int RB, int KS>
+__device__ __forceinline__ void queries_body(const BwdParams& p, char* smem, int block) {
   using C = Copies<D, RB>;
-  constexpr int kQ = D / 16, kDb = D / 32, kRows = RB * kBlock;
-  constexpr int kSlot = 2 * C::kBytes;   // a step's k and v
-  constexpr int kMerge = KS / 2 * RB * kDb * 16 * 64 * 4;
-  constexpr int kLds = KS * 2 * kSlot > kMerge ? KS * 2 * kSlot : kMerge;
-  __shared__ __attribute__((aligned(16))) char smem[kLds];
+  constexpr int kQ = D / 16, kDb = D / 32, kRows = RB * kBlock, kSlot = Lds<D, RB, KS>::kTiles;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rb = w % RB, ks = w / RB;
   const int n = lane & 31, g = lane >> 5;
   int bh;   // of a key head
-  const int unit = dealt(p.deal, blockIdx.x, bh);
-  if (unit >= p.deal.units) return;
+  const int unit = dealt(p.queries, block, bh);
+  if (unit >= p.queries.units) return;
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
   const int head = hk * p.G + unit % p.G, block0 = unit / p.G * kRows;
   const int row = block0 + rb * kBlock + n;   // of this lane
@@ -563,6 +563,21 @@ cross_bwd_queries_kernel(const BwdParams p) {
            row < lq && lk > 0);
 }
 
+// Both in one launch: neither needs the other's results, and the workgroups of the second
+// fill what the last ones of the first leave idle (1 x 16 heads x 4800 x 4800, D 128: 652 us,
+// one after the other 751).
+template <typename E, int D, int RB, int KS, int kWaves>
+__global__ void __launch_bounds__(64 * RB * KS) __attribute__((amdgpu_waves_per_eu(kWaves, kWaves)))
+cross_bwd_kernel(const BwdParams p) {
+  __shared__ __attribute__((aligned(16))) char smem[Lds<D, RB, KS>::kBytes];
+  const int first = (int)p.keys.groups();   // (a multiple of 8: the XCDs go on in turn)
+  if ((int)blockIdx.x < first) {
+    keys_body<E, D, RB, KS>(p, smem, blockIdx.x);
+  } else {
+    queries_body<E, D, RB, KS>(p, smem, blockIdx.x - first);
+  }
+}
+
 // ---- host -------------------------------------------------------------------------
 
 bool shape_ok(int B, int H, int Hk, int L, int S, int D) {
@@ -583,56 +598,56 @@ Workspace workspace(int B, int H, int Hk, int L, int S, int dtype) {
   return Workspace{tiles * 2 * kBlock, tiles * kBlock, tiles, (size_t)B * Hk * tiles_of(S)};
 }
 
-// Which form of a kernel: blocks of 32 rows or keys and groups of a workgroup, by the least
-// estimate (us) of
+// Which form: blocks of 32 rows or keys and groups of a workgroup, by the least estimate (us)
 //
-//   turns (ends + rounds (alone + more running))
+//   base + keys n_k + queries n_q + keys_round n_k r_k + queries_round n_q r_q + alone r_k + longest max(r_k, r_q)
 //
-// where a CU's share of the workgroups takes full turns of `fit` at once and one with the
-// rest, `running` is what a turn holds, and a workgroup's rounds are its steps over its
-// groups.  Fitted to 110 shapes of 1 to 24 items, 8 to 1400 queries and 30 to 6000 keys in
-// every form: the choice is on average within 2% of the best one's time.  (More groups make
-// workgroups shorter, more blocks share copies: dk and dv of 2 x 16 heads x 300 x 1463 24.1 us
-// in the first form, 20.8 in the second, 28.5 in the third; of 8 x 8 x 100 x 500 11.1, 12.2
-// and 15.2; dq of them 29.0, 19.0 and 17.9, 13.4, 10.0 and 8.5.)
+// with n workgroups a CU of either kind, of r rounds each (its steps over its groups): what
+// all of them take together, and what one takes alone, which the last ones do.  Fitted to
+// 19400 shapes of 1 to 24 items, 8 to 1400 queries and 30 to 5000 keys in every form: the
+// choice is on average within 2% of the best one's time, in 99 of 100 within 25%.  (More
+// groups make workgroups shorter, more blocks share copies: 4 x 16 heads (4 key heads) x 1200
+// x 4800 363 us in the first form, 378 in the second, 445 in the third; 8 x 8 x 100 x 500
+// 22.0, 19.8 and 22.8.)
 struct Form {
-  int blocks, groups, fit;
-  double base, ends, alone, more;
+  int dim, blocks, groups;
+  double base, keys, queries, keys_round, queries_round, alone, longest;
 };
-constexpr Form kKeys[2][3] = {
-    {{4, 1, 1, 3.37, 3.29, .629, 0}, {2, 2, 2, 1.92, 4.77, .601, .247}, {1, 4, 1, 4.47, 1.91, .623, 0}},
-    {{4, 1, 2, 1.4, 7, .55, .72}, {2, 2, 2, 0, 9.2, .777, .787}, {1, 2, 2, 3, 5.54, .805, .317}}};
-constexpr Form kQueries[2][3] = {
-    {{4, 1, 3, 0, 5.54, .19, .296}, {2, 2, 3, .85, 4.88, .215, .304}, {1, 4, 2, 1.85, 3.86, .406, .281}},
-    {{4, 1, 2, 0, 6.25, .182, .615}, {2, 2, 2, .29, 6.36, .263, .613}, {1, 2, 2, 1.39, 4.6, .859, .122}}};
+constexpr Form kForms[] = {{64, 4, 1, 7.86, 3.7, .225, .457, .202, .251, .412},
+                           {64, 2, 2, 8.29, 2.64, 1.43, .564, .172, .376, .429},
+                           {64, 1, 4, 8.12, 2.27, 1.47, .294, .637, .059, .553},
+                           {128, 4, 1, 8.45, 7.87, .552, .902, .324, .616, .607},
+                           {128, 2, 2, 9.66, 5.65, 2.86, 1.16, .225, .635, .68},
+                           {128, 1, 2, 8.37, 3.12, 1.89, .187, .593, .248, .826}};
 
-// heads of `units` rows or keys, each over `steps` tiles.
-int choose(const Form (&forms)[3], int64_t heads, int units, int64_t steps, int cus) {
-  int best = 0;
+int choose(const BwdParams& p, int D, int cus) {
+  int best = -1;
   double best_us = 0;
-  for (int i = 0; i < 3; ++i) {
-    const Form& f = forms[i];
-    const int64_t load = (heads * ((units + f.blocks * kBlock - 1) / (f.blocks * kBlock)) + cus - 1) / cus;
-    const double rounds = (double)((steps + f.groups - 1) / f.groups);
-    double us = f.base + (double)(load / f.fit) * (f.ends + rounds * (f.alone + f.more * f.fit));
-    if (load % f.fit > 0) us += f.ends + rounds * (f.alone + f.more * (double)(load % f.fit));
-    if (i == 0 || us < best_us) best = i, best_us = us;
+  for (int i = 0; i < (int)(sizeof(kForms) / sizeof(kForms[0])); ++i) {
+    const Form& f = kForms[i];
+    if (f.dim != D) continue;
+    const int64_t rows = f.blocks * kBlock;
+    const double nk = (double)((int64_t)p.B * p.Hk * ((p.S + rows - 1) / rows)) / cus;
+    const double nq = (double)((int64_t)p.B * p.H * ((p.L + rows - 1) / rows)) / cus;
+    const double rk = (double)(((int64_t)p.G * p.tiles + f.groups - 1) / f.groups);
+    const double rq = (double)((p.key_tiles + f.groups - 1) / f.groups);
+    const double us = f.base + f.keys * nk + f.queries * nq + f.keys_round * nk * rk + f.queries_round * nq * rq +
+                      f.alone * rk + f.longest * (rk > rq ? rk : rq);
+    if (best < 0 || us < best_us) best = i, best_us = us;
   }
   return best;
 }
 
-template <typename E, int D, int RB, int KS, int kWaves>
-void launch_keys(BwdParams& p, hipStream_t stream) {
-  constexpr int kKeysOf = RB * kBlock;
-  p.deal = deal((int64_t)p.B * p.Hk, (p.S + kKeysOf - 1) / kKeysOf, (int64_t)p.G * p.L * D * 4);
-  hipLaunchKernelGGL((cross_bwd_keys_kernel<E, D, RB, KS, kWaves>), dim3(p.deal.groups()), dim3(64 * RB * KS), 0, stream, p);
-}
-
-template <typename E, int D, int RB, int KS, int kWaves>
-void launch_queries(BwdParams& p, hipStream_t stream) {
+template <typename E, int D, int RB, int KS>
+void launch_form(BwdParams& p, hipStream_t stream) {
   constexpr int kRows = RB * kBlock;
-  p.deal = deal((int64_t)p.B * p.Hk, (int64_t)p.G * ((p.L + kRows - 1) / kRows), (int64_t)p.S * D * 4);
-  hipLaunchKernelGGL((cross_bwd_queries_kernel<E, D, RB, KS, kWaves>), dim3(p.deal.groups()), dim3(64 * RB * KS), 0, stream, p);
+  // (as many wavefronts a SIMD as the registers allow: three of 168 at D 64, two of 256 at 128)
+  constexpr int kWaves = D == 64 ? 3 : 2;
+  const int64_t heads = (int64_t)p.B * p.Hk;
+  p.keys = deal(heads, (p.S + kRows - 1) / kRows, (int64_t)p.G * p.L * D * 4);
+  p.queries = deal(heads, (int64_t)p.G * ((p.L + kRows - 1) / kRows), (int64_t)p.S * D * 4);
+  hipLaunchKernelGGL((cross_bwd_kernel<E, D, RB, KS, kWaves>), dim3(p.keys.groups() + p.queries.groups()),
+                     dim3(64 * RB * KS), 0, stream, p);
 }
 
 template <typename E, int D>
@@ -640,19 +655,13 @@ void launch(BwdParams& p, hipStream_t stream) {
   unsigned rows = (unsigned)p.B * p.H * p.tiles;
   if (Range<E>::kScaled) rows += (unsigned)p.B * p.Hk * p.key_tiles;
   hipLaunchKernelGGL((cross_bwd_rows_kernel<E, D>), dim3(rows), dim3(4 * D), 0, stream, p);
-  // (as many wavefronts a SIMD as the registers allow: three of 168 at D 64, two of 256 at 128)
-  constexpr int kWaves = D == 64 ? 3 : 2, kGroups = D == 64 ? 4 : 2;
-  const int cus = sidon::compute_units();
-  switch (choose(kKeys[D == 64 ? 0 : 1], (int64_t)p.B * p.Hk, p.S, (int64_t)p.G * p.tiles, cus)) {
-    case 0: launch_keys<E, D, 4, 1, kWaves>(p, stream); break;
-    case 1: launch_keys<E, D, 2, 2, kWaves>(p, stream); break;
-    default: launch_keys<E, D, 1, kGroups, kWaves>(p, stream); break;
-  }
-  switch (choose(kQueries[D == 64 ? 0 : 1], (int64_t)p.B * p.H, p.L, p.key_tiles, cus)) {
-    case 0: launch_queries<E, D, 4, 1, kWaves>(p, stream); break;
-    case 1: launch_queries<E, D, 2, 2, kWaves>(p, stream); break;
-    default: launch_queries<E, D, 1, kGroups, kWaves>(p, stream); break;
-  }
+  const Form& f = kForms[choose(p, D, sidon::compute_units())];
+  if (f.blocks == 4)
+    launch_form<E, D, 4, 1>(p, stream);
+  else if (f.blocks == 2)
+    launch_form<E, D, 2, 2>(p, stream);
+  else
+    launch_form<E, D, 1, D == 64 ? 4 : 2>(p, stream);
 }
 
 }  // namespace
@@ -728,8 +737,8 @@ SIDON_API int sidon_cross_attention_bwd(const void* dout, const void* q, const v
       return fail(SIDON_E_SHAPE, "ws must lie apart from %s", flat[i].name);
   }
   const int64_t heads = (int64_t)B * Hk;
-  if ((int64_t)B * H * tiles_of(L) + heads * tiles_of(S) > INT32_MAX / 256 || !deal_fits(heads, tiles_of(S)) ||
-      !deal_fits(heads, (int64_t)(H / Hk) * tiles_of(L)))
+  if ((int64_t)B * H * tiles_of(L) + heads * tiles_of(S) > INT32_MAX / 512 ||
+      !deal_fits(heads, tiles_of(S) + (int64_t)(H / Hk) * tiles_of(L) + 8))
     return fail(SIDON_E_SHAPE, "too many rows for one launch");
   const int rc = sidon::check_device();
   if (rc) return rc;
