@@ -492,9 +492,10 @@ __device__ __forceinline__ void queries_body(const BwdParams& p, char* smem, int
   float c = 1.f;
   if constexpr (Range<E>::kScaled)
     c = below_one(p.length[tile * kBlock + rr % kBlock], largest(p.longest_v + (int64_t)bh * p.key_tiles, p.key_tiles, lane));
+  lse += __log2f(c);   // (P itself is not wanted here: its exponent takes the power of two)
   arrived(qop);
   arrived(gop);
-  asm volatile("" : "+v"(lse), "+v"(delta), "+v"(c));
+  asm volatile("" : "+v"(lse), "+v"(delta));
   const float scale2 = p.scale * kLog2e;
 
   f32x16 dq[kDb];
@@ -523,7 +524,7 @@ __device__ __forceinline__ void queries_body(const BwdParams& p, char* smem, int
         if (16 * (i >> 3) + (i & 7) >= left) s[i] = -INFINITY;
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], scale2, lse)) * (Range<E>::kScaled ? dp[i] * c : dp[i]);
+    for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], scale2, lse)) * dp[i];
     i4 pk[2];
     round_to<E>(s, pk);
 #pragma unroll
@@ -600,25 +601,26 @@ Workspace workspace(int B, int H, int Hk, int L, int S, int dtype) {
 
 // Which form: blocks of 32 rows or keys and groups of a workgroup, by the least estimate (us)
 //
-//   base + keys n_k + queries n_q + keys_round n_k r_k + queries_round n_q r_q + alone r_k + longest max(r_k, r_q)
+//   base + keys n_k + queries n_q + keys_round n_k r_k + queries_round n_q r_q
+//        + keys_turn r_k ceil(n_k / fit) + queries_turn r_q ceil(n_q / fit) + longest max(r_k, r_q)
 //
 // with n workgroups a CU of either kind, of r rounds each (its steps over its groups): what
-// all of them take together, and what one takes alone, which the last ones do.  Fitted to
+// all of them take together, and what the busiest CU's and the longest one take.  Fitted to
 // 19400 shapes of 1 to 24 items, 8 to 1400 queries and 30 to 5000 keys in every form: the
-// choice is on average within 2% of the best one's time, in 99 of 100 within 25%.  (More
+// choice is on average within 2% of the best one's time, in 99 of 100 within 24%.  (More
 // groups make workgroups shorter, more blocks share copies: 4 x 16 heads (4 key heads) x 1200
 // x 4800 363 us in the first form, 378 in the second, 445 in the third; 8 x 8 x 100 x 500
 // 22.0, 19.8 and 22.8.)
 struct Form {
-  int dim, blocks, groups;
-  double base, keys, queries, keys_round, queries_round, alone, longest;
+  int dim, blocks, groups, fit;
+  double base, keys, queries, keys_round, queries_round, keys_turn, queries_turn, longest;
 };
-constexpr Form kForms[] = {{64, 4, 1, 7.86, 3.7, .225, .457, .202, .251, .412},
-                           {64, 2, 2, 8.29, 2.64, 1.43, .564, .172, .376, .429},
-                           {64, 1, 4, 8.12, 2.27, 1.47, .294, .637, .059, .553},
-                           {128, 4, 1, 8.45, 7.87, .552, .902, .324, .616, .607},
-                           {128, 2, 2, 9.66, 5.65, 2.86, 1.16, .225, .635, .68},
-                           {128, 1, 2, 8.37, 3.12, 1.89, .187, .593, .248, .826}};
+constexpr Form kForms[] = {{64, 4, 1, 1, 7.75, 3.59, .446, .308, .148, .28, 0, .445},
+                           {64, 2, 2, 2, 8.14, 2.44, 1.29, .46, .165, .508, 0, .435},
+                           {64, 1, 4, 1, 7.74, 2.28, 1.64, 0, .193, .484, .383, .19},
+                           {128, 4, 1, 1, 8.48, 8.86, 2.16, .536, .016, .646, .092, .504},
+                           {128, 2, 2, 2, 9.57, 5.72, 3.1, 1.1, 0, .83, .147, .508},
+                           {128, 1, 2, 1, 8.04, 3.06, 2.09, 0, .058, .629, .294, .532}};
 
 int choose(const BwdParams& p, int D, int cus) {
   int best = -1;
@@ -632,7 +634,8 @@ int choose(const BwdParams& p, int D, int cus) {
     const double rk = (double)(((int64_t)p.G * p.tiles + f.groups - 1) / f.groups);
     const double rq = (double)((p.key_tiles + f.groups - 1) / f.groups);
     const double us = f.base + f.keys * nk + f.queries * nq + f.keys_round * nk * rk + f.queries_round * nq * rq +
-                      f.alone * rk + f.longest * (rk > rq ? rk : rq);
+                      f.keys_turn * rk * ceil(nk / f.fit) + f.queries_turn * rq * ceil(nq / f.fit) +
+                      f.longest * (rk > rq ? rk : rq);
     if (best < 0 || us < best_us) best = i, best_us = us;
   }
   return best;
