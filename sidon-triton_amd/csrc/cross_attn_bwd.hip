@@ -492,7 +492,7 @@ __device__ __forceinline__ void queries_body(const BwdParams& p, char* smem, int
   float c = 1.f;
   if constexpr (Range<E>::kScaled)
     c = below_one(p.length[tile * kBlock + rr % kBlock], largest(p.longest_v + (int64_t)bh * p.key_tiles, p.key_tiles, lane));
-  lse += __log2f(c);   // (P itself is not wanted here: its exponent takes the power of two)
+  if constexpr (Range<E>::kScaled) lse += __log2f(c);   // (P itself is not wanted here: its exponent takes the power of two)
   arrived(qop);
   arrived(gop);
   asm volatile("" : "+v"(lse), "+v"(delta));

@@ -37,7 +37,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256;
 constexpr int kVec = 8;           // values of a lane
 constexpr int kMaxBlocks = 1024;  // workgroups of a side in the backward pass: rows of partial sums
-constexpr int kSumThreads = 1024;
+constexpr int kSumThreads = 1024, kSumCols = 16;
 constexpr uint32_t kMostBlocks = (1u << 24) - 1;   // (a launch holds less than 2^32 threads)
 
 struct Side {
@@ -361,9 +361,9 @@ __global__ void __launch_bounds__(kThreads) head_norm_bwd_kernel(const NormParam
   }
 }
 
-// dw of a side from its workgroups' sums: a workgroup per 32 values.
+// dw of a side from its workgroups' sums: a workgroup per 16 values.
 __global__ void __launch_bounds__(kSumThreads) head_norm_sum_kernel(const NormParams p) {
-  constexpr int kCols = 32, kRows = kSumThreads / kCols;
+  constexpr int kCols = kSumCols, kRows = kSumThreads / kCols;
   __shared__ float sums[kRows][kCols];
   const Side& s = p.side[blockIdx.y];
   const int c = threadIdx.x % kCols, row = threadIdx.x / kCols;
@@ -375,15 +375,16 @@ __global__ void __launch_bounds__(kSumThreads) head_norm_sum_kernel(const NormPa
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       const uint32_t b = b0 + i * kRows;
-      v[i] = at < p.D && b < s.blocks ? s.part[(int64_t)b * p.D + at] : 0.f;
+      v[i] = b < s.blocks ? s.part[(int64_t)b * p.D + at] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) sum += v[i];
   }
   sums[row][c] = sum;
   __syncthreads();
-  if (row == 0 && at < p.D) {
+  if (row == 0) {
     sum = 0.f;
+#pragma unroll 16
     for (int j = 0; j < kRows; ++j) sum += sums[j][c];
     s.dw[at] = sum;
   }
@@ -410,7 +411,8 @@ Blocks backward_blocks(int64_t tokens, int heads, int nh, int D) {
   const int64_t chunks = (heads + nh - 1) / nh;
   int64_t turns = (tokens + teams - 1) / teams;
   const int64_t most = chunks >= kMaxBlocks ? 1 : kMaxBlocks / chunks;
-  if (turns > most) turns = most;
+  const int64_t each = (turns + most - 1) / most;   // tokens of a team, the same for nearly all of them
+  turns = (turns + each - 1) / each;
   return Blocks{(uint32_t)chunks, (uint32_t)(chunks * turns)};
 }
 
@@ -646,7 +648,7 @@ SIDON_API int sidon_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, c
   }
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   launch_any(p, nh, true, blocks, dtype, st);
-  hipLaunchKernelGGL(head_norm_sum_kernel, dim3((D + 31) / 32, Hk == 0 ? 1 : 2), dim3(kSumThreads), 0, st, p);
+  hipLaunchKernelGGL(head_norm_sum_kernel, dim3(D / kSumCols, Hk == 0 ? 1 : 2), dim3(kSumThreads), 0, st, p);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return fail(SIDON_E_LAUNCH, "norm and rotation gradient launch failed: %s", hipGetErrorString(err));
   return SIDON_OK;
