@@ -22,8 +22,6 @@ from .conformer import plain
 from .flexrel import _check_device_tensor, _on_device, _stream_handle
 
 _TILE_N, _TILE_K = 16, 128
-# Where a word holds input k of its eight: from the lowest nibble.
-_NIBBLES = (0, 2, 4, 6, 1, 3, 5, 7)
 
 
 @dataclasses.dataclass(frozen=True)
@@ -89,21 +87,25 @@ def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | 
         zeros = None if zeros is None else zeros.repeat_interleave(group // 128, 1)
         group = 128
     tiles, blocks, per = -(-n // _TILE_N), -(-k // _TILE_K), _TILE_K // group
-    full = values.new_zeros(tiles * _TILE_N, blocks * _TILE_K)
-    full[:n, :k] = values
-    # [tile, row, block, step, lane quarter, input] -> [tile, block, quarter, row, step] of words
-    nib = full.view(tiles, _TILE_N, blocks, 4, 4, 8).permute(0, 2, 4, 1, 3, 5).to(torch.int32)
-    words = torch.zeros(nib.shape[:-1], dtype=torch.int32, device=values.device)
-    for at, i in enumerate(_NIBBLES):
-        words |= nib[..., i] << (4 * at)
+    if n % _TILE_N or k % _TILE_K:
+        full = values.new_zeros(tiles * _TILE_N, blocks * _TILE_K)
+        full[:n, :k] = values
+        values = full
+    # input 4 a + 2 p + s of a word's eight goes to byte 2 s + a, nibble p
+    nib = values.unflatten(1, (-1, 2, 2, 2))
+    words = values.new_empty(*nib.shape[:2], 2, 2)
+    torch.add(nib[..., 0, :], nib[..., 1, :], alpha=16, out=words.transpose(-1, -2))
+    # [tile, row, block, step, lane quarter] -> [tile, block, quarter, row, step] of words
+    words = words.flatten(2).view(torch.int32).view(tiles, _TILE_N, blocks, 4, 4).permute(0, 2, 4, 1, 3).contiguous()
     # the scale, and above it what goes off the operand that a value becomes: fp16 v - 8, bf16 128 + v
+    scales = scales.detach()
     zero = torch.full_like(scales, 8) if zeros is None else zeros.to(scales.dtype)
     off = zero - 8 if scales.dtype == torch.float16 else zero + 128
     pair = torch.stack((scales, off), -1).contiguous().view(torch.int32).squeeze(-1)
     both = pair.new_zeros(tiles * _TILE_N, blocks * per)
     both[:n, :pair.shape[1]] = pair
     both = both.view(tiles, _TILE_N, blocks, per).permute(0, 2, 3, 1).contiguous()
-    return Int4Weight(words.view(tiles, blocks, 64, 4).contiguous(), both, n, k, group, scales.dtype, zeros is not None)
+    return Int4Weight(words.view(tiles, blocks, 64, 4), both, n, k, group, scales.dtype, zeros is not None)
 
 
 def int4_linear(x: torch.Tensor, w: Int4Weight, bias: torch.Tensor | None = None, act: str | None = None,
