@@ -53,13 +53,14 @@ struct CrossParams {
   float* lse;            // [B, H, L] or null
   const int32_t* lens;
   const int32_t* q_lens;
-  float4* part_ml;       // [B Hk, splits, R] (maximum, sum, sum before the rounding, -)
-  float* part_o;         // [B Hk, splits, R, D]
+  float4* part_ml;       // [B Hk, splits, rest] (maximum, sum, sum before the rounding, -)
+  float* part_o;         // [B Hk, splits, rest, D]
   int64_t qb, qh, ql, kb, kh, vb, vh, ob, oh, ol;   // strides (elements): batch, head, row
   int kl, vl;            // row strides (< 2^25)
   int B, H, Hk, G, L, S, R;
-  int blocks, splits;
-  Deal deal;             // a key head's (row block, split) units
+  int whole, cut, splits;   // row blocks of a key head that a workgroup takes whole, those that `splits` share
+  int first, rest;          // the rows of the latter: from `first` on, `rest` of them
+  Deal deal;                // a key head's units: blocks, then (split, block)
   float scale;           // log2(e) times the caller's
 };
 
@@ -104,8 +105,10 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
   int bh;
   const int unit = dealt(p.deal, blockIdx.x, bh);
   if (unit >= p.deal.units) return;
-  const int split = unit / p.blocks;
-  const int blk = unit - split * p.blocks;
+  const bool alone = unit < p.whole;
+  const int split = alone ? 0 : (unit - p.whole) / p.cut;
+  const int blk = alone ? unit : unit - split * p.cut;
+  const uint32_t splits = alone ? 1 : p.splits;
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
   const int row0 = (blk * RB + rb) * (NB * kBlock);   // of this wavefront
   // Lane n holds the rows row0 + 32 j + n, j < NB: query row / G, head row % G of the group.
@@ -115,8 +118,8 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
   if (p.q_lens != nullptr) rows = p.G * __builtin_amdgcn_readfirstlane(min(max(p.q_lens[b], 0), p.L));
 
   const int steps = blk * RB * NB * kBlock < rows ? (lk + kStep - 1) / kStep : 0;   // of the workgroup
-  const int t0 = (int)((uint32_t)steps * (uint32_t)split / (uint32_t)p.splits);   // (steps <= 2^25, splits <= 2^6)
-  const int t1 = (int)((uint32_t)steps * (uint32_t)(split + 1) / (uint32_t)p.splits);
+  const int t0 = (int)((uint32_t)steps * (uint32_t)split / splits);   // (steps <= 2^25, splits <= 2^6)
+  const int t1 = (int)((uint32_t)steps * (uint32_t)(split + 1) / splits);
   const auto mine = [&](int u) SIDON_INLINE { return t0 + u * KS + ks; };   // step u of this group
   const int all = (t1 - t0 + KS - 1) / KS;         // most steps of a group: the workgroup's rounds
   const int count = row0 < rows ? max(t1 - t0 - ks + KS - 1, 0) / KS : 0;    // of this wavefront
@@ -498,8 +501,8 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
   for (int j = 0; j < NB; ++j) {
     const int row = row0 + 32 * j + n;
     if (row >= p.R) return;
-    if (p.splits > 1) {
-      const int64_t at = ((int64_t)bh * p.splits + split) * p.R + row;
+    if (splits > 1) {
+      const int64_t at = ((int64_t)bh * p.splits + split) * p.rest + (row - p.first);
       float* dst = p.part_o + at * D + 4 * g;
       if (g == 0) p.part_ml[at] = make_float4(mx[j], sum[j], raw[j], 0.f);
 #pragma unroll
@@ -528,7 +531,7 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
   }
 }
 
-// Join the grid splits of a row: a workgroup per row, whose wavefronts take every
+// Join the grid splits of a row: a workgroup per row that has them, whose wavefronts take every
 // fourth part; a lane has D / 64 of the values.
 constexpr int kJoinWaves = 4;
 template <typename E, int D>
@@ -538,8 +541,8 @@ __global__ void __launch_bounds__(64 * kJoinWaves) cross_attn_join_kernel(const 
   __shared__ fn part[kJoinWaves][64];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int bh = blockIdx.x / p.R;
-  const int row = blockIdx.x - bh * p.R;
+  const int bh = blockIdx.x / p.rest;
+  const int at = blockIdx.x - bh * p.rest, row = p.first + at;
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
   const int head = hk * p.G + row % p.G, query = row / p.G;
   bool there = p.lens == nullptr || p.lens[b] > 0;
@@ -547,8 +550,8 @@ __global__ void __launch_bounds__(64 * kJoinWaves) cross_attn_join_kernel(const 
 
   // Lane s < splits holds the statistics of part s (kMaxGridSplits <= 64).
   float4 ml = make_float4(kFloorMax, 0.f, 0.f, 0.f);
-  if (lane < p.splits) ml = p.part_ml[((int64_t)bh * p.splits + lane) * p.R + row];
-  const float* src = p.part_o + ((int64_t)bh * p.splits * p.R + row) * D + N * lane;
+  if (lane < p.splits) ml = p.part_ml[((int64_t)bh * p.splits + lane) * p.rest + at];
+  const float* src = p.part_o + ((int64_t)bh * p.splits * p.rest + at) * D + N * lane;
   float top = ml.x;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -563,7 +566,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) cross_attn_join_kernel(const 
     fn u[kAtOnce];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i)
-      u[i] = *reinterpret_cast<const fn*>(src + (int64_t)min(s0 + i * kJoinWaves, p.splits - 1) * p.R * D);
+      u[i] = *reinterpret_cast<const fn*>(src + (int64_t)min(s0 + i * kJoinWaves, p.splits - 1) * p.rest * D);
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       const int s = s0 + i * kJoinWaves;
@@ -593,6 +596,7 @@ struct Kind {
   bool fine;
   int fit;                 // workgroups that a CU runs at once
   double base, ends, alone, more, join, part, traffic;
+  double cut, cut_round;   // of cut row blocks (0: none of this kernel's)
 };
 // Which, and how many grid splits: the least estimate (us) of
 //
@@ -607,37 +611,60 @@ struct Kind {
 // rows at D 64 are for short launches: 4 x 16 heads x 224 x 1500 15.6 us, with 64 rows
 // 16.8; 1 x 16 x 4800 x 4800 151 and 123.  Rows shared by more wavefronts, 128 and 256 a
 // workgroup, took 131 and 144 there: fewer copies, but waits for one another.)
-constexpr Kind kKinds[] = {{64, 32, 4, true, 2, 1.53, 4.24, 0, .677, 2.5, .018, .744},
-                           {64, 32, 4, false, 2, 2.39, 3.98, .111, .343, 2.62, 0, .601},
-                           {64, 64, 4, false, 2, 2.58, 5.72, .05, .637, 2.29, 0, .502},
-                           {128, 32, 2, true, 2, 1.24, 5.02, .329, .484, 2.43, .022, .351},
-                           {128, 64, 2, false, 2, 1.5, 6, .4, .3, 3.2, 0, .4}};
+//
+// Where one or two workgroups a CU leave a few row blocks over, whose turn would hold few CUs,
+// those alone are split, and run beside the others. Their estimate is the others' and
+//   cut + cut_round rounds workgroups a CU
+// for heads that divide evenly over the XCDs, 40 steps and more and a quarter of a turn at
+// most; fitted to 45000 shapes, of which it takes 622, to 0.86 of their time on average and 1.06 at
+// worst (2 x 8 heads (2 key heads) x 1037 x 4800, D 128, 260 row blocks on 256 CUs: 78 -> 58 us).
+constexpr Kind kKinds[] = {{64, 32, 4, true, 2, 1.53, 4.24, 0, .677, 2.5, .018, .744, 0, 0},
+                           {64, 32, 4, false, 2, 2.39, 3.98, .111, .343, 2.62, 0, .601, 0, 0},
+                           {64, 64, 4, false, 2, 2.58, 5.72, .05, .637, 2.29, 0, .502, 9, .5},
+                           {128, 32, 2, true, 2, 1.24, 5.02, .329, .484, 2.43, .022, .351, 0, 0},
+                           {128, 64, 2, false, 2, 1.5, 6, .4, .3, 3.2, 0, .4, 6, .3}};
 constexpr int kNumKinds = sizeof(kKinds) / sizeof(kKinds[0]);
 
 struct Plan {
   int kind;   // -1: none yet
-  int blocks, splits;
+  int whole, cut, splits;   // row blocks of a workgroup each, and of `splits` workgroups each
 };
 
 Plan search(int B, int Hk, int R, int S, int D, int cus) {
   const int64_t heads = (int64_t)B * Hk;
   const int steps = (S + kStep - 1) / kStep;
-  Plan best{-1, 0, 0};
+  Plan best{-1, 0, 0, 1};
   double best_us = 0;
   for (int i = 0; i < kNumKinds; ++i) {
     const Kind& k = kKinds[i];
     // up to 32 rows keep two summands (the header says so)
     if (k.dim != D || (R <= kBlock && !k.fine) || (R > kBlock && k.fine && D == 64)) continue;
     const int blocks = (R + k.rows - 1) / k.rows;
+    const auto turns = [&](int64_t load, int rounds) {
+      const int64_t full = load / k.fit, rest = load % k.fit;
+      double us = (double)full * (k.ends + rounds * (k.alone + k.more * k.fit));
+      if (rest > 0) us += k.ends + rounds * (k.alone + k.more * (double)rest);
+      return us;
+    };
     for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, kMaxGridSplits}) {
       const int64_t load = (heads * blocks * s + cus - 1) / cus;   // workgroups of the busiest CU
       if (s > 1 && (s * k.groups > steps + 1 || load > 6)) break;
       const int rounds = (steps + k.groups * s - 1) / (k.groups * s);
-      const int64_t full = load / k.fit, rest = load % k.fit;
-      double us = k.base + (double)full * (k.ends + rounds * (k.alone + k.more * k.fit));
-      if (rest > 0) us += k.ends + rounds * (k.alone + k.more * (double)rest);
+      double us = k.base + turns(load, rounds);
       if (s > 1) us += k.join + k.part * s + (double)heads * R * s * D * 8e-6 * k.traffic;
-      if (best.kind < 0 || us < best_us) best = Plan{i, blocks, s}, best_us = us;
+      if (best.kind < 0 || us < best_us) best = s > 1 ? Plan{i, 0, blocks, s} : Plan{i, blocks, 0, 1}, best_us = us;
+    }
+    if (k.cut == 0 || steps < 40 || (heads % 8 != 0 && 8 % heads != 0)) continue;
+    for (int load = 1; load <= k.fit; ++load) {
+      const int whole = (int)(load * (int64_t)cus / heads), cut = blocks - whole;
+      if (whole < 1 || cut < 1 || 4 * heads * cut > cus) continue;
+      for (const int s : {4, 8, 16}) {
+        const int64_t more = (heads * cut * s + cus - 1) / cus;
+        if (more > k.fit) break;
+        const int rounds = (steps + k.groups * s - 1) / (k.groups * s);
+        const double us = k.base + turns(load, (steps + k.groups - 1) / k.groups) + k.cut + k.cut_round * rounds * (double)more;
+        if (us < best_us) best = Plan{i, whole, cut, s}, best_us = us;
+      }
     }
   }
   return best;
@@ -663,8 +690,9 @@ bool shape_ok(int B, int H, int Hk, int L, int S, int D) {
          S <= (1 << 30) && (int64_t)(H / Hk) * L <= (1 << 24) && (int64_t)B * Hk <= (1 << 24);
 }
 
-size_t part_bytes(int B, int Hk, int R, int D, int splits) {
-  return splits > 1 ? (size_t)B * Hk * R * splits * (16 + (size_t)D * 4) : 0;
+size_t part_bytes(int B, int Hk, int R, int D, const Plan& c) {
+  if (c.splits == 1) return 0;
+  return (size_t)B * Hk * (R - c.whole * kKinds[c.kind].rows) * c.splits * (16 + (size_t)D * 4);
 }
 
 template <typename E, int D, int NB, int RB, int KS, bool kFine, int kMinWaves>
@@ -689,7 +717,7 @@ void launch(const CrossParams& p, int kind, int D, hipStream_t stream) {
     default: launch_kind<E, 128, 1, 2, 2, false, 2>(p, stream); break;
   }
   if (p.splits > 1) {
-    const dim3 join((unsigned)((int64_t)p.B * p.Hk * p.R));
+    const dim3 join((unsigned)((int64_t)p.B * p.Hk * p.rest));
     if (D == 64) {
       hipLaunchKernelGGL((cross_attn_join_kernel<E, 64>), join, dim3(64 * kJoinWaves), 0, stream, p);
     } else {
@@ -703,7 +731,7 @@ void launch(const CrossParams& p, int kind, int D, hipStream_t stream) {
 SIDON_API size_t sidon_cross_attention_workspace_bytes(int B, int H, int Hk, int L, int S, int D) {
   if (!shape_ok(B, H, Hk, L, S, D)) return 0;
   const int R = H / Hk * L;
-  return part_bytes(B, Hk, R, D, plan(B, Hk, R, S, D, sidon::compute_units()).splits);
+  return part_bytes(B, Hk, R, D, plan(B, Hk, R, S, D, sidon::compute_units()));
 }
 
 SIDON_API int sidon_cross_attention(const void* q, const void* k, const void* v, const int32_t* lens,
@@ -746,7 +774,7 @@ SIDON_API int sidon_cross_attention(const void* q, const void* k, const void* v,
   if (!sidon::apart(rows[3].n, rows[3].st, 3, D)) return fail(SIDON_E_STRIDE, "rows of out overlap one another");
   const int R = H / Hk * L;
   const Plan c = plan(B, Hk, R, S, D, sidon::compute_units());
-  const size_t need = part_bytes(B, Hk, R, D, c.splits);
+  const size_t need = part_bytes(B, Hk, R, D, c);
   if (ws_bytes < need || (need > 0 && ws == nullptr))
     return fail(SIDON_E_SHAPE, "ws holds %zu bytes, the call needs %zu", ws_bytes, need);
   // Workgroups read the inputs while others already write out, lse, or ws.
@@ -773,7 +801,7 @@ SIDON_API int sidon_cross_attention(const void* q, const void* k, const void* v,
           return fail(SIDON_E_SHAPE, "%s must lie apart from %s", flat[i].name, flat[j].name);
     }
   }
-  const int64_t heads = (int64_t)B * Hk, units = (int64_t)c.blocks * c.splits;
+  const int64_t heads = (int64_t)B * Hk, units = c.whole + (int64_t)c.cut * c.splits;
   if (!deal_fits(heads, units) || (c.splits > 1 && heads * R > INT32_MAX / 256))
     return fail(SIDON_E_SHAPE, "too many rows for one launch");
   const int rc = sidon::check_device();
@@ -781,13 +809,14 @@ SIDON_API int sidon_cross_attention(const void* q, const void* k, const void* v,
   CrossParams p{};
   p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse, p.lens = lens, p.q_lens = q_lens;
   p.part_ml = static_cast<float4*>(ws);
-  p.part_o = static_cast<float*>(ws) + (size_t)B * Hk * R * c.splits * 4;
+  p.whole = c.whole, p.cut = c.cut, p.splits = c.splits;
+  p.first = c.whole * kKinds[c.kind].rows, p.rest = c.cut > 0 ? R - p.first : 0;
+  p.part_o = static_cast<float*>(ws) + (size_t)B * Hk * p.rest * c.splits * 4;
   p.qb = q_strides[0], p.qh = q_strides[1], p.ql = q_strides[2];
   p.kb = k_strides[0], p.kh = k_strides[1], p.kl = (int)k_strides[2];
   p.vb = v_strides[0], p.vh = v_strides[1], p.vl = (int)v_strides[2];
   p.ob = o_strides[0], p.oh = o_strides[1], p.ol = o_strides[2];
   p.B = B, p.H = H, p.Hk = Hk, p.G = H / Hk, p.L = L, p.S = S, p.R = R;
-  p.blocks = c.blocks, p.splits = c.splits;
   p.deal = deal(heads, units, (int64_t)S * D * 4);
   p.scale = (float)(1.4426950408889634 * scale);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -116,6 +116,29 @@ def test_forward(sidon, shape, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("shape", [(1, 4, 4, 4136, 1330, 128), (2, 4, 4, 2060, 1300, 64), (1, 8, 8, 4110, 1409, 64),
+                                   (2, 8, 2, 1037, 2600, 128), (1, 4, 4, 4136, 2650, 128), (2, 4, 4, 2060, 3300, 64),
+                                   (1, 8, 8, 4110, 3299, 64), (2, 8, 2, 1037, 4800, 128)], ids=str)
+def test_row_blocks_left_over(sidon, shape, kind):
+    """A few row blocks more than 256 CUs take at once, whose keys are split, where there are many, while the others' are not."""
+    b, h, hk, l, s, d = shape
+    q, k, v, dout = inputs(*shape, kind, 31 * l + s + d)
+    lens, q_lens = ([s - 3], [l - 5]) if b == 1 else ([s, s - 70], [l - 11, l])
+    poison(lens, q_lens, q, k, v, dout)
+    ca = sidon.cross_attention
+    if s > 2600 and torch.cuda.get_device_properties(DEV).multi_processor_count == 256:
+        # parts of fewer rows than there are (16 + 4 D bytes each)
+        assert 0 < ca.workspace_bytes(b, h, hk, l, s, d, DEV) < b * h * l * (16 + 4 * d)
+    lse = torch.full((b, h, l), 5.0, device=DEV)
+    got = ca.cross_attention(q, k, v, int32(lens), int32(q_lens), lse=lse)
+    check_forward(got, lse, q, k, v, lens, q_lens, d ** -0.5)
+    assert torch.equal(got, ca.cross_attention(q, k, v, int32(lens), int32(q_lens)))
+    lse.zero_()
+    got = ca.cross_attention(q, k, v, int32([0] * b), int32(q_lens), lse=lse)
+    assert (got == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
 @pytest.mark.parametrize("shape", [(1, 2, 2, 200, 300, 64), (6, 8, 8, 700, 700, 64), (6, 8, 8, 700, 700, 128),
                                    (2, 4, 1, 1, 900, 128)], ids=str)
 def test_rising_scores(sidon, shape, kind):
