@@ -567,15 +567,15 @@ __device__ __forceinline__ void queries_body(const BwdParams& p, char* smem, int
 // Both in one launch: neither needs the other's results, and the workgroups of the second
 // fill what the last ones of the first leave idle (1 x 16 heads x 4800 x 4800, D 128: 652 us,
 // one after the other 751).
-template <typename E, int D, int RB, int KS, int kWaves>
+template <typename E, int D, int RB, int KS, int kWaves, bool kQueriesFirst>
 __global__ void __launch_bounds__(64 * RB * KS) __attribute__((amdgpu_waves_per_eu(kWaves, kWaves)))
 cross_bwd_kernel(const BwdParams p) {
   __shared__ __attribute__((aligned(16))) char smem[Lds<D, RB, KS>::kBytes];
-  const int first = (int)p.keys.groups();   // (a multiple of 8: the XCDs go on in turn)
-  if ((int)blockIdx.x < first) {
-    keys_body<E, D, RB, KS>(p, smem, blockIdx.x);
+  const int first = (int)(kQueriesFirst ? p.queries.groups() : p.keys.groups());   // (a multiple of 8: the XCDs go on in turn)
+  if (((int)blockIdx.x < first) != kQueriesFirst) {
+    keys_body<E, D, RB, KS>(p, smem, blockIdx.x - (kQueriesFirst ? first : 0));
   } else {
-    queries_body<E, D, RB, KS>(p, smem, blockIdx.x - first);
+    queries_body<E, D, RB, KS>(p, smem, blockIdx.x - (kQueriesFirst ? 0 : first));
   }
 }
 
@@ -649,8 +649,11 @@ void launch_form(BwdParams& p, hipStream_t stream) {
   const int64_t heads = (int64_t)p.B * p.Hk;
   p.keys = deal(heads, (p.S + kRows - 1) / kRows, (int64_t)p.G * p.L * D * 4);
   p.queries = deal(heads, (int64_t)p.G * ((p.L + kRows - 1) / kRows), (int64_t)p.S * D * 4);
-  hipLaunchKernelGGL((cross_bwd_kernel<E, D, RB, KS, kWaves>), dim3(p.keys.groups() + p.queries.groups()),
-                     dim3(64 * RB * KS), 0, stream, p);
+  const dim3 grid(p.keys.groups() + p.queries.groups()), block(64 * RB * KS);
+  if (3 * (int64_t)p.key_tiles > 4 * (int64_t)p.G * p.tiles)   // (products of their steps)
+    hipLaunchKernelGGL((cross_bwd_kernel<E, D, RB, KS, kWaves, true>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((cross_bwd_kernel<E, D, RB, KS, kWaves, false>), grid, block, 0, stream, p);
 }
 
 template <typename E, int D>
