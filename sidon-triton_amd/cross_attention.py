@@ -102,7 +102,7 @@ def _workspace(workspace, need, like):
 def _out(name, out, like):
     """-> (tensor, strides): ``out``, or a new contiguous tensor of ``like``'s shape."""
     if out is None:
-        out = like.new_empty(like.shape)
+        out = torch.empty_like(like, memory_format=torch.contiguous_format)
     else:
         _check_device_tensor(name, out, like.device)
         if out.dtype != like.dtype or out.shape != like.shape or out.stride(-1) != 1:
@@ -142,7 +142,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: tor
         raise ValueError("cross_attention follows no gradient: call it under torch.no_grad(), and "
                          "cross_attention_backward for the gradients")
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         out, o_strides = _out("out", out, q)
     if lse is not None:
@@ -197,7 +197,7 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
         raise ValueError("cross_attention_backward follows no gradient: call it under torch.no_grad()")
     outs = []
     for i, (name, t, like) in enumerate((("dq", dq, q), ("dk", dk, k), ("dv", dv, v))):
-        outs.append((like.new_empty(like.shape), contiguous[i]) if t is None
+        outs.append((torch.empty_like(like, memory_format=torch.contiguous_format), contiguous[i]) if t is None
                     else _out(name, t, like))
     lib = _lib.load()
     with _on_device(device):

@@ -111,7 +111,7 @@ def _out(name, out, like, contiguous):
             raise ValueError(f"{name} without k")
         return None, _NONE
     if out is None:
-        return like.new_empty(like.shape), contiguous
+        return torch.empty_like(like, memory_format=torch.contiguous_format), contiguous
     _rows(name, out, tuple(like.shape), like)
     return out, _strides(out)
 
