@@ -19,6 +19,11 @@
 // fp16 holds P times 2^15, and dS times a power of two that keeps it below 2^15: the
 // bound |dS_ij| <= 2 |dout_i| |v_j| needs the longest v, and for dk the longest dout,
 // of a key head, which the first launch leaves.  bf16 has fp32's exponents.
+//
+// What bounds it, and what it reached.  16 heads x 4800 x 4800 take 350 us at D 64 (the five
+// products at 0.67 PFLOP/s) and 627 at D 128 (0.75): matrix cores and vector units are each
+// busy a third of the time and overlap little, LDS a fifth.  2 x 16 heads x 300 x 1463 takes 37 us: a
+// wavefront's longest chain of steps, and some 14 us of launches, first copies and merges.
 #include <hip/hip_runtime.h>
 
 #include <float.h>
@@ -607,7 +612,8 @@ Workspace workspace(int B, int H, int Hk, int L, int S, int dtype) {
 // with n workgroups a CU of either kind, of r rounds each (its steps over its groups): what
 // all of them take together, and what the busiest CU's and the longest one take.  Fitted to
 // 19400 shapes of 1 to 24 items, 8 to 1400 queries and 30 to 5000 keys in every form: the
-// choice is on average within 2% of the best one's time, in 99 of 100 within 24%.  (More
+// choice is on average within 2% of the best one's time, in 99 of 100 within 24% (launched
+// in the better order too).  (More
 // groups make workgroups shorter, more blocks share copies: 4 x 16 heads (4 key heads) x 1200
 // x 4800 363 us in the first form, 378 in the second, 445 in the third; 8 x 8 x 100 x 500
 // 22.0, 19.8 and 22.8.)

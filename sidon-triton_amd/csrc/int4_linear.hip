@@ -14,6 +14,10 @@
 //
 // A wavefront has 16 NT outputs of 16 MT rows and every WK-th block of 128 inputs;
 // the WK wavefronts of a workgroup are summed through LDS.
+//
+// Reached: 1 x 32768 x 4096 (71 MB) 16 us, 4.4 TB/s; 32 rows of it 21 to 24, where every
+// wavefront's loads of x, as many bytes as its weights, and 40 matrix and 200 vector
+// instructions a block come between the loads of weights; 1 x 4096 x 1024 2.8, latency.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>

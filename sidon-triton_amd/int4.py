@@ -80,7 +80,7 @@ def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | 
         raise ValueError(f"groups of {group} inputs: need 32, 64 or a multiple of 128")
     if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
         raise ValueError(f"zeros must be a uint8 {tuple(scales.shape)} tensor")
-    if int(values.max()) > 15 or (zeros is not None and int(zeros.max()) > 15):
+    if int(values.max() if zeros is None else torch.maximum(values.max(), zeros.max())) > 15:
         raise ValueError("values and zeros must be from 0 to 15")
     if group > 128:
         scales = scales.repeat_interleave(group // 128, 1)
