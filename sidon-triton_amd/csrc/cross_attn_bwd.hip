@@ -20,9 +20,9 @@
 // bound |dS_ij| <= 2 |dout_i| |v_j| needs the longest v, and for dk the longest dout,
 // of a key head, which the first launch leaves.  bf16 has fp32's exponents.
 //
-// What bounds it, and what it reached.  16 heads x 4800 x 4800 take 350 us at D 64 (the five
-// products at 0.67 PFLOP/s) and 627 at D 128 (0.75): matrix cores and vector units are each
-// busy a third of the time and overlap little, LDS a fifth.  2 x 16 heads x 300 x 1463 takes 37 us: a
+// What bounds it, and what it reached.  16 heads x 4800 x 4800 take 330 us at D 64 (the five
+// products at 0.71 PFLOP/s) and 620 at D 128 (0.76): matrix cores and vector units are each
+// busy a third of the time and overlap little, LDS a fifth.  2 x 16 heads x 300 x 1463 takes 33 us: a
 // wavefront's longest chain of steps, and some 14 us of launches, first copies and merges.
 #include <hip/hip_runtime.h>
 
@@ -291,6 +291,9 @@ __device__ __forceinline__ void store(E* dst, const f32x16 (&x)[N], float by, bo
       *reinterpret_cast<v4*>(dst + 32 * d + 8 * i) = r;
     }
 }
+
+// Groups of a workgroup of so many blocks: four wavefronts, two for a block alone at D 128.
+constexpr int groups_of(int dim, int blocks) { return dim == 128 && blocks == 1 ? 2 : 4 / blocks; }
 
 // LDS of a workgroup: KS rings of two slots, which hold a step's q, dout and statistics or
 // its k and v; then the partial results of half of the groups.
@@ -570,17 +573,20 @@ __device__ __forceinline__ void queries_body(const BwdParams& p, char* smem, int
 }
 
 // Both in one launch: neither needs the other's results, and the workgroups of the second
-// fill what the last ones of the first leave idle (1 x 16 heads x 4800 x 4800, D 128: 652 us,
+// fill what the last ones of the first leave idle (1 x 16 heads x 4800 x 4800, D 128: 620 us,
 // one after the other 751).
-template <typename E, int D, int RB, int KS, int kWaves, bool kQueriesFirst>
-__global__ void __launch_bounds__(64 * RB * KS) __attribute__((amdgpu_waves_per_eu(kWaves, kWaves)))
+template <typename E, int D, int KB, int QB, int kWaves, bool kQueriesFirst>
+__global__ void __launch_bounds__(64 * KB * groups_of(D, KB)) __attribute__((amdgpu_waves_per_eu(kWaves, kWaves)))
 cross_bwd_kernel(const BwdParams p) {
-  __shared__ __attribute__((aligned(16))) char smem[Lds<D, RB, KS>::kBytes];
+  constexpr int KS = groups_of(D, KB), QS = groups_of(D, QB);
+  static_assert(KB * KS == QB * QS, "as many wavefronts");
+  constexpr int kKeys = Lds<D, KB, KS>::kBytes, kQueries = Lds<D, QB, QS>::kBytes;
+  __shared__ __attribute__((aligned(16))) char smem[kKeys > kQueries ? kKeys : kQueries];
   const int first = (int)(kQueriesFirst ? p.queries.groups() : p.keys.groups());   // (a multiple of 8: the XCDs go on in turn)
   if (((int)blockIdx.x < first) != kQueriesFirst) {
-    keys_body<E, D, RB, KS>(p, smem, blockIdx.x - (kQueriesFirst ? first : 0));
+    keys_body<E, D, KB, KS>(p, smem, blockIdx.x - (kQueriesFirst ? first : 0));
   } else {
-    queries_body<E, D, RB, KS>(p, smem, blockIdx.x - (kQueriesFirst ? 0 : first));
+    queries_body<E, D, QB, QS>(p, smem, blockIdx.x - (kQueriesFirst ? 0 : first));
   }
 }
 
@@ -604,29 +610,43 @@ Workspace workspace(int B, int H, int Hk, int L, int S, int dtype) {
   return Workspace{tiles * 2 * kBlock, tiles * kBlock, tiles, (size_t)B * Hk * tiles_of(S)};
 }
 
-// Which form: blocks of 32 rows or keys and groups of a workgroup, by the least estimate (us)
+// Which form: blocks of 32 keys and of 32 rows of a workgroup, and whose are launched first, by
+// the least estimate (us)
 //
 //   base + keys n_k + queries n_q + keys_round n_k r_k + queries_round n_q r_q
-//        + keys_turn r_k ceil(n_k / fit) + queries_turn r_q ceil(n_q / fit) + longest max(r_k, r_q)
+//        + keys_turn r_k ceil(n_k / fit) + queries_turn r_q ceil(n_q / fit) + longest max(r_k, r_q) + last r
 //
-// with n workgroups a CU of either kind, of r rounds each (its steps over its groups): what
-// all of them take together, and what the busiest CU's and the longest one take.  Fitted to
-// 19400 shapes of 1 to 24 items, 8 to 1400 queries and 30 to 5000 keys in every form: the
-// choice is on average within 2% of the best one's time, in 99 of 100 within 24% (launched
-// in the better order too).  (More
-// groups make workgroups shorter, more blocks share copies: 4 x 16 heads (4 key heads) x 1200
-// x 4800 363 us in the first form, 378 in the second, 445 in the third; 8 x 8 x 100 x 500
-// 22.0, 19.8 and 22.8.)
+// with n workgroups a CU of either kind, of r rounds each (its steps over its groups), the
+// last ones' r: what all of them take together, and what the busiest CU's, the longest one and
+// the last take.  (More groups make a workgroup shorter, more blocks share copies, and where the
+// longer kind waits for the other it ends late.)  20000 shapes of 1 to 24 items, 8 to 2400
+// queries and 30 to 5000 keys were timed in 18 forms at D 64 and 10 at 128; these are the ones
+// that the others rarely beat, and their numbers chosen for the choice: it takes 1.02 times the
+// best one's time on average, 1.2 in 99 of 100 (one form for both kinds, in the better order: 1.06 at
+// best, at D 64; 4 x 16 heads (4 key heads) x 1200 x 4800 306 us, with one form 324; 1 x 16 x 300 x 4800 42 and 55).
 struct Form {
-  int dim, blocks, groups, fit;
-  double base, keys, queries, keys_round, queries_round, keys_turn, queries_turn, longest;
+  int dim, key_blocks, query_blocks;
+  bool queries_first;
+  int fit;
+  double base, keys, queries, keys_round, queries_round, keys_turn, queries_turn, longest, last;
 };
-constexpr Form kForms[] = {{64, 4, 1, 1, 7.75, 3.59, .446, .308, .148, .28, 0, .445},
-                           {64, 2, 2, 2, 8.14, 2.44, 1.29, .46, .165, .508, 0, .435},
-                           {64, 1, 4, 1, 7.74, 2.28, 1.64, 0, .193, .484, .383, .19},
-                           {128, 4, 1, 1, 8.48, 8.86, 2.16, .536, .016, .646, .092, .504},
-                           {128, 2, 2, 2, 9.57, 5.72, 3.1, 1.1, 0, .83, .147, .508},
-                           {128, 1, 2, 1, 8.04, 3.06, 2.09, 0, .058, .629, .294, .532}};
+constexpr Form kForms[] = {{64, 4, 2, false, 1, 9.55, 1.59, 1.15, .00519, .00611, .233, 0, .825, 0},
+                           {64, 4, 2, true, 1, 9.02, 1.42, 2.19, 0, 0, .00427, .253, .109, 1.06},
+                           {64, 4, 1, false, 1, 3.58, 6.06, .777, 0, .00899, .736, .665, 1.13, 0},
+                           {64, 4, 1, true, 1, 7.5, .0957, 6.87, .00644, .477, .538, .0867, .011, .215},
+                           {64, 2, 4, false, 2, 9.01, 3.63, .0469, .0182, .328, .471, 0, .722, 0},
+                           {64, 2, 4, true, 1, 8.19, 1.53, 4.57, .0645, 0, .566, .173, .0621, .77},
+                           {64, 2, 1, false, 1, 4.99, 7.03, 2.32, 0, .00386, .449, .11, .754, 0},
+                           {64, 2, 1, true, 1, 5.46, 1.62, 7.92, 0, .0103, .625, .0126, .543, .191},
+                           {64, 1, 4, false, 1, 6.43, 5.11, 1.18, .362, 0, .468, .229, .0192, .297},
+                           {64, 1, 4, true, 1, 7.73, 1.87, 3.37, .38, .681, .0298, .161, .126, .448},
+                           {64, 1, 2, false, 1, 5.42, 4.87, 2.18, .211, .404, .307, .00446, .284, .449},
+                           {64, 1, 2, true, 1, 5.86, 2.6, 5.61, .457, .0501, .635, .161, .364, 0},
+                           {128, 4, 2, false, 1, 8.66, 3.39, 3.88, .00365, .00429, .661, 0, 1.18, .383},
+                           {128, 4, 2, true, 1, 9.01, .391, 7.66, .00418, 0, .527, .0384, .932, .946},
+                           {128, 2, 4, false, 2, 10.6, 5.42, .081, .705, .607, 1.35, 0, .447, 0},
+                           {128, 1, 1, false, 1, 7.85, 3.8, 1.31, .241, .845, .0651, .178, .466, .761},
+                           {128, 1, 1, true, 1, 8.52, 1.72, 5.33, 1.52, 0, .0846, .379, .0187, .332}};
 
 int choose(const BwdParams& p, int D, int cus) {
   int best = -1;
@@ -634,32 +654,35 @@ int choose(const BwdParams& p, int D, int cus) {
   for (int i = 0; i < (int)(sizeof(kForms) / sizeof(kForms[0])); ++i) {
     const Form& f = kForms[i];
     if (f.dim != D) continue;
-    const int64_t rows = f.blocks * kBlock;
-    const double nk = (double)((int64_t)p.B * p.Hk * ((p.S + rows - 1) / rows)) / cus;
+    const int keys = f.key_blocks * kBlock, rows = f.query_blocks * kBlock;
+    const int ks = groups_of(D, f.key_blocks), qs = groups_of(D, f.query_blocks);
+    const double nk = (double)((int64_t)p.B * p.Hk * ((p.S + keys - 1) / keys)) / cus;
     const double nq = (double)((int64_t)p.B * p.H * ((p.L + rows - 1) / rows)) / cus;
-    const double rk = (double)(((int64_t)p.G * p.tiles + f.groups - 1) / f.groups);
-    const double rq = (double)((p.key_tiles + f.groups - 1) / f.groups);
+    const double rk = (double)(((int64_t)p.G * p.tiles + ks - 1) / ks), rq = (double)((p.key_tiles + qs - 1) / qs);
     const double us = f.base + f.keys * nk + f.queries * nq + f.keys_round * nk * rk + f.queries_round * nq * rq +
                       f.keys_turn * rk * ceil(nk / f.fit) + f.queries_turn * rq * ceil(nq / f.fit) +
-                      f.longest * (rk > rq ? rk : rq);
+                      f.longest * (rk > rq ? rk : rq) + f.last * (f.queries_first ? rk : rq);
     if (best < 0 || us < best_us) best = i, best_us = us;
   }
   return best;
 }
 
-template <typename E, int D, int RB, int KS>
-void launch_form(BwdParams& p, hipStream_t stream) {
-  constexpr int kRows = RB * kBlock;
+template <typename E, int D, int KB, int QB>
+void launch_form(BwdParams& p, bool queries_first, hipStream_t stream) {
+  constexpr int kKeys = KB * kBlock, kRows = QB * kBlock;
   // (as many wavefronts a SIMD as the registers allow: three of 168 at D 64, two of 256 at 128)
   constexpr int kWaves = D == 64 ? 3 : 2;
   const int64_t heads = (int64_t)p.B * p.Hk;
-  p.keys = deal(heads, (p.S + kRows - 1) / kRows, (int64_t)p.G * p.L * D * 4);
+  p.keys = deal(heads, (p.S + kKeys - 1) / kKeys, (int64_t)p.G * p.L * D * 4);
   p.queries = deal(heads, (int64_t)p.G * ((p.L + kRows - 1) / kRows), (int64_t)p.S * D * 4);
-  const dim3 grid(p.keys.groups() + p.queries.groups()), block(64 * RB * KS);
-  if (3 * (int64_t)p.key_tiles > 4 * (int64_t)p.G * p.tiles)   // (products of their steps)
-    hipLaunchKernelGGL((cross_bwd_kernel<E, D, RB, KS, kWaves, true>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((cross_bwd_kernel<E, D, RB, KS, kWaves, false>), grid, block, 0, stream, p);
+  const dim3 grid(p.keys.groups() + p.queries.groups()), block(64 * KB * groups_of(D, KB));
+  if constexpr (D == 64 || KB != 2) {   // (not of kForms)
+    if (queries_first) {
+      hipLaunchKernelGGL((cross_bwd_kernel<E, D, KB, QB, kWaves, true>), grid, block, 0, stream, p);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((cross_bwd_kernel<E, D, KB, QB, kWaves, false>), grid, block, 0, stream, p);
 }
 
 template <typename E, int D>
@@ -668,12 +691,21 @@ void launch(BwdParams& p, hipStream_t stream) {
   if (Range<E>::kScaled) rows += (unsigned)p.B * p.Hk * p.key_tiles;
   hipLaunchKernelGGL((cross_bwd_rows_kernel<E, D>), dim3(rows), dim3(4 * D), 0, stream, p);
   const Form& f = kForms[choose(p, D, sidon::compute_units())];
-  if (f.blocks == 4)
-    launch_form<E, D, 4, 1>(p, stream);
-  else if (f.blocks == 2)
-    launch_form<E, D, 2, 2>(p, stream);
-  else
-    launch_form<E, D, 1, D == 64 ? 4 : 2>(p, stream);
+  switch (f.key_blocks * 10 + f.query_blocks) {   // (those of kForms)
+    case 42: return launch_form<E, D, 4, 2>(p, f.queries_first, stream);
+    case 24: return launch_form<E, D, 2, 4>(p, f.queries_first, stream);
+    default: break;
+  }
+  if constexpr (D == 64) {
+    switch (f.key_blocks * 10 + f.query_blocks) {
+      case 41: return launch_form<E, D, 4, 1>(p, f.queries_first, stream);
+      case 21: return launch_form<E, D, 2, 1>(p, f.queries_first, stream);
+      case 14: return launch_form<E, D, 1, 4>(p, f.queries_first, stream);
+      default: return launch_form<E, D, 1, 2>(p, f.queries_first, stream);
+    }
+  } else {
+    launch_form<E, D, 1, 1>(p, f.queries_first, stream);
+  }
 }
 
 }  // namespace

@@ -180,6 +180,37 @@ def test_backward(sidon, shape, kind):
     assert all(torch.equal(x, y) for x, y in zip(grads, again))
 
 
+# (batch, heads, key heads, queries, keys, D): one for each form of the gradients' launch, on 256 CUs (blocks of keys, of
+# queries, and whose come first)
+FORMS = [
+    (20, 8, 8, 42, 44, 64), (19, 8, 8, 49, 129, 64), (10, 4, 4, 41, 72, 64), (2, 1, 1, 42, 820, 64), (17, 16, 8, 41, 36, 64),
+    (11, 8, 8, 112, 101, 64), (2, 1, 1, 39, 36, 64), (2, 1, 1, 48, 312, 64), (2, 3, 1, 594, 38, 64), (13, 8, 8, 68, 37, 64),
+    (2, 2, 1, 37, 36, 64), (2, 2, 1, 107, 296, 64), (34, 2, 2, 40, 74, 128), (27, 2, 2, 34, 207, 128),
+    (38, 8, 4, 37, 35, 128), (2, 1, 1, 37, 34, 128), (2, 1, 1, 35, 79, 128),
+]
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("shape", FORMS, ids=str)
+def test_backward_forms(sidon, shape, kind):
+    b, h, hk, l, s, d = shape
+    q, k, v, dout = inputs(*shape, kind, l + s + b)
+    lens, q_lens = lengths(b, l, s, 0)
+    poison(lens, q_lens, q, k, v, dout)
+    lens32, q_lens32 = int32(lens), int32(q_lens)
+    lse, ca = torch.empty(b, h, l, device=DEV), sidon.cross_attention
+    out = ca.cross_attention(q, k, v, lens32, q_lens32, lse=lse)
+    outs = [torch.full_like(t, 7.0) for t in (q, k, v)]
+    grads = ca.cross_attention_backward(dout, q, k, v, out, lse, lens32, q_lens32, dq=outs[0], dk=outs[1], dv=outs[2])
+    assert all(x is y for x, y in zip(grads, outs))
+    check_backward(grads, dout, q, k, v, lens, q_lens, d ** -0.5, whole=False)
+    for i in range(b):
+        n, m = min(max(lens[i], 0), s), min(max(q_lens[i], 0), l)
+        assert (grads[0][i, :, m:] == 0).all() and (grads[1][i, :, n:] == 0).all() and (grads[2][i, :, n:] == 0).all()
+    again = ca.cross_attention_backward(dout, q, k, v, out, lse, lens32, q_lens32)
+    assert all(torch.equal(x, y) for x, y in zip(grads, again))
+
+
 @pytest.mark.parametrize("kind", KINDS, ids=str)
 def test_gradient_is_the_difference(sidon, kind):
     """Along random directions, against differences of the float64 definition: each
