@@ -176,15 +176,16 @@ struct Shape {
   int mt, nt, wk;
 };
 
-// Rows of a workgroup by what M needs.  A wavefront takes four tiles of outputs where that
-// leaves every CU a workgroup (each tile more is x loaded once less: 16 x 16384 x 2048 7.1 us,
-// with one tile 11.5), one where it does not (1 x 8192 x 4096 6.1, with four 8.6), and K is
-// split over eight wavefronts, or four where there are many workgroups as it is (64 x 32768 x
-// 4096 42 us, with eight 44; 1 x 32768 x 4096 17.1 and 16.1).
+// Rows of a workgroup by what M needs.  A wavefront takes one tile of outputs where that gives no
+// CU more than one workgroup, two where two do, else four (each tile more is x loaded once less,
+// and a CU with two workgroups takes twice as long: 64 x 8192 x 4096 in one, two, four tiles 33, 19
+// and 23 us; 16 x 16384 x 2048 11.2, 7.9 and 6.7; 1 x 4096 x 14336 10.9, 13.1 and 18.1), and K is
+// split over eight wavefronts, or four where there are many workgroups as it is (64 x 32768 x 4096
+// 46 us, with eight 47; 32 x 32768 x 4096 27.5 and 23.7).
 Shape shape(int M, int N, int cus) {
   const int mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
   const int64_t units = (int64_t)((N + kTileN - 1) / kTileN) * ((M + 16 * mt - 1) / (16 * mt));
-  if (units < 4 * (int64_t)cus) return Shape{mt, 1, 8};
+  if (units <= 2 * (int64_t)cus) return Shape{mt, units <= cus ? 1 : 2, 8};
   return Shape{mt, 4, units * mt > 16 * (int64_t)cus ? 4 : 8};
 }
 
@@ -210,6 +211,8 @@ void launch_shape(const Int4Params& p, const Shape& c, int group, bool off, hipS
   const dim3 grid((p.tiles + c.nt - 1) / c.nt, (p.M + 16 * MT - 1) / (16 * MT));
   if (c.nt == 1)
     launch_groups<E, MT, 1, 8>(p, group, off, grid, s);
+  else if (c.nt == 2)
+    launch_groups<E, MT, 2, 8>(p, group, off, grid, s);
   else if (c.wk == 8)
     launch_groups<E, MT, 4, 8>(p, group, off, grid, s);
   else

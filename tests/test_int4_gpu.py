@@ -56,6 +56,18 @@ def test_against_float64(sidon, shape, kind, zeros):
     close(got, *oracle.int4(x, values, scales, zero, bias, act))
 
 
+@pytest.mark.parametrize("zeros", [False, True], ids=["plain", "zeros"])
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(1, 4500, 128, 128), (16, 8190, 1184, 32), (20, 6001, 256, 64), (50, 5000, 160, 32), (64, 8177, 2048, 128),
+                                   (300, 1000, 640, 128), (33, 16500, 64, 64), (7, 16400, 256, 64)], ids=str)
+def test_tiles_of_a_wavefront(sidon, shape, kind, zeros):
+    """Two tiles of outputs, and four with K over eight wavefronts, with tails of rows, outputs and inputs."""
+    m, n, k, group = shape
+    x, values, scales, zero, bias = inputs(m, n, k, group, zeros, kind, m + n + k)
+    got = sidon.int4.int4_linear(x, sidon.int4.pack_int4(values, scales, zero), bias)
+    close(got, *oracle.int4(x, values, scales, zero, bias, None))
+
+
 @pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16], ids=str)
 def test_every_value_and_place(sidon, kind):
     """One-hot rows read single weights exactly: every nibble of a word, every value."""
