@@ -36,6 +36,18 @@ class Int4Weight:
     dtype: torch.dtype
     zeros: bool
 
+    def __post_init__(self):
+        """The kernel reads as far as n, k and group say."""
+        if self.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"weights are for float16 or bfloat16 (got {self.dtype})")
+        if self.group not in (32, 64, 128) or min(self.n, self.k) < 1 or self.k % self.group:
+            raise ValueError(f"weights [{self.n}, {self.k}] in groups of {self.group}: need 32, 64 or 128 that divide k")
+        tiles, blocks = -(-self.n // _TILE_N), -(-self.k // _TILE_K)
+        for name, t, shape in (("words", self.words, (tiles, blocks, 64, 4)),
+                               ("scales", self.scales, (tiles, blocks, _TILE_K // self.group, 16))):
+            if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous int32 {shape} tensor (got {t.dtype} {tuple(t.shape)})")
+
     def to(self, device) -> "Int4Weight":
         return dataclasses.replace(self, words=self.words.to(device), scales=self.scales.to(device))
 

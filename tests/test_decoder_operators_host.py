@@ -339,3 +339,18 @@ def test_quantize(sidon, zeros):
     back = (values.float().unflatten(1, (3, 32)) - (zero.float().unsqueeze(-1) if zeros else 8)) * scales.unsqueeze(-1)
     assert ((back.flatten(1) - w).abs() <= 1.01 * scales.repeat_interleave(32, 1)).all()
     assert (back.flatten(1)[3] == 0).all()
+
+
+def test_int4_weights_of_other_sizes_are_refused(sidon):
+    """Built or changed by hand, as from a file: what the kernel would read past its tensors."""
+    import dataclasses
+
+    w = sidon.int4.pack_int4(torch.zeros(20, 160, dtype=torch.uint8), torch.ones(20, 5, dtype=torch.float16))
+    assert dataclasses.replace(w, n=17).n == 17   # (the same tiles)
+    for bad in (dict(n=33), dict(n=0), dict(k=288), dict(k=170), dict(group=64), dict(group=256), dict(words=w.words[:1]),
+                dict(words=w.words.long()), dict(scales=w.scales[:, :, :2]), dict(scales=w.scales.float()),
+                dict(words=w.words.transpose(0, 1).contiguous().transpose(0, 1))):
+        with pytest.raises(ValueError):
+            dataclasses.replace(w, **bad)
+    with pytest.raises(TypeError):
+        dataclasses.replace(w, dtype=torch.float32)
