@@ -83,6 +83,7 @@ def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | 
         raise TypeError(f"values must be uint8 (got {values.dtype})")
     if scales.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"scales must be float16 or bfloat16 (got {scales.dtype})")
+    scales = scales.detach()
     n, k = values.shape
     groups = scales.shape[1]
     if scales.shape[0] != n or k % groups:
@@ -100,9 +101,13 @@ def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | 
         group = 128
     tiles, blocks, per = -(-n // _TILE_N), -(-k // _TILE_K), _TILE_K // group
     if n % _TILE_N or k % _TILE_K:
-        full = values.new_zeros(tiles * _TILE_N, blocks * _TILE_K)
-        full[:n, :k] = values
-        values = full
+        def padded(t, width):
+            full = t.new_zeros(tiles * _TILE_N, width)
+            full[:n, :t.shape[1]] = t
+            return full
+
+        values, scales = padded(values, blocks * _TILE_K), padded(scales, blocks * per)
+        zeros = None if zeros is None else padded(zeros, blocks * per)
     # input 4 a + 2 p + s of a word's eight goes to byte 2 s + a, nibble p
     nib = values.unflatten(1, (-1, 2, 2, 2))
     words = values.new_empty(*nib.shape[:2], 2, 2)
@@ -110,13 +115,15 @@ def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | 
     # [tile, row, block, step, lane quarter] -> [tile, block, quarter, row, step] of words
     words = words.flatten(2).view(torch.int32).view(tiles, _TILE_N, blocks, 4, 4).permute(0, 2, 4, 1, 3).contiguous()
     # the scale, and above it what goes off the operand that a value becomes: fp16 v - 8, bf16 128 + v
-    scales = scales.detach()
-    zero = torch.full_like(scales, 8) if zeros is None else zeros.to(scales.dtype)
-    off = zero - 8 if scales.dtype == torch.float16 else zero + 128
-    pair = torch.stack((scales, off), -1).contiguous().view(torch.int32).squeeze(-1)
-    both = pair.new_zeros(tiles * _TILE_N, blocks * per)
-    both[:n, :pair.shape[1]] = pair
-    both = both.view(tiles, _TILE_N, blocks, per).permute(0, 2, 3, 1).contiguous()
+    less = -8.0 if scales.dtype == torch.float16 else 128.0
+    pair = scales.new_empty(tiles, blocks, per, _TILE_N, 2)
+    placed = lambda t: t.unflatten(1, (blocks, per)).unflatten(0, (tiles, _TILE_N)).permute(0, 2, 3, 1)  # noqa: E731
+    pair[..., 0] = placed(scales)
+    if zeros is None:
+        pair[..., 1] = 8 + less
+    else:
+        torch.add(placed(zeros), less, out=pair[..., 1])
+    both = pair.view(torch.int32).squeeze(-1)
     return Int4Weight(words.view(tiles, blocks, 64, 4), both, n, k, group, scales.dtype, zeros is not None)
 
 
