@@ -90,6 +90,16 @@ __device__ __forceinline__ void dma_256(uint32_t lds_addr, const char* gbase, ui
 }
 #pragma clang diagnostic pop
 
+// One copy of 1 KB, 16 bytes a lane from an address of its own, to LDS lds_addr + 16 l of lane l
+// (of those that take part).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma_lanes(uint32_t lds_addr, const void* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(lds_addr), "v"(from) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 // Waits for the loads of x here.  Left to its first use, within a loop, the compiler's
 // wait would come round with every turn and take the loop's own copies with it.
 template <int N>

@@ -71,9 +71,11 @@ __device__ __forceinline__ i4 operand(uint32_t word, uint32_t mask, uint32_t lea
 
 // SPG: steps of 32 inputs per group within a block.  kOff: something goes off the weights.
 template <typename E, int MT, int NT, int WK, int SPG, bool kOff>
-__global__ void __launch_bounds__(64 * WK) int4_linear_kernel(const Int4Params p) {
+__global__ void __launch_bounds__(64 * WK, 2) int4_linear_kernel(const Int4Params p) {
   constexpr int kGroups = 4 / SPG;
-  __shared__ f4 part[WK][MT * NT][64];
+  constexpr int kX = MT * 16 * kTileK * 2;   // bytes of a block's inputs
+  static_assert(sizeof(E) == 2, "16-bit inputs");
+  __shared__ __attribute__((aligned(16))) char smem[WK * (kX > MT * NT * 1024 ? kX : MT * NT * 1024)];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -87,46 +89,76 @@ __global__ void __launch_bounds__(64 * WK) int4_linear_kernel(const Int4Params p
     wp[j] = static_cast<const i4*>(p.words) + tile * p.blocks * 64 + lane;
     sp[j] = p.scales + tile * p.blocks * (kGroups * 16) + c;
   }
-  // (rows past the last are that one again, and inputs past the last, whose scales are 0,
-  // the last 32: neither is stored)
-  const E* xp[MT];
+  // A block's inputs go through LDS, 4 rows x 256 bytes a copy: lanes that lie side by side read
+  // one row, where the operand's are of 16 rows, whose loads would go through the cache one by
+  // one.  Chunk q of 16 bytes of row r lies at q ^ (r % 16).  (Rows past the last are not copied
+  // and not stored; inputs past the last, whose scales are 0, are the last 32.)
+  const char* const xs = smem + w * kX;
+  const uint32_t xat = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem) + w * kX;
+  const int xr = lane >> 4, left = p.M - row0 - xr;
+  const E* const xl = static_cast<const E*>(p.x) + (int64_t)(row0 + xr) * p.ldx + 8 * ((lane & 3) ^ xr);
+  const auto copy_x = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
-  for (int m = 0; m < MT; ++m) xp[m] = static_cast<const E*>(p.x) + min(row0 + 16 * m + c, p.M - 1) * p.ldx + 8 * g;
-  uint32_t mask = 0x000f000fu, lead = __is_same(E, _Float16) ? 0x64006400u : 0x43004300u;
-  asm("" : "+v"(mask), "+v"(lead));
-
-  f4 total[MT][NT] = {};
-  const int one2 = __is_same(E, _Float16) ? 0x3c003c00 : 0x3f803f80;
-  const i4 ones = {one2, one2, one2, one2};
-#pragma unroll 2
-  for (int b = w; b < p.blocks; b += WK) {
-    i4 words[NT];
-    uint32_t scale[NT][kGroups];
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (16 * m + 4 * j < left) {
+          const int k = min(b * kTileK + 32 * (((lane >> 2) & 3) ^ j), p.K - 32);
+          dma_lanes(xat + (4 * m + j) * 1024, xl + (16 * m + 4 * j) * p.ldx + k);
+        }
+  };
+  const auto load_w = [&](int b, i4 (&words)[NT], uint32_t (&scale)[NT][kGroups]) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       words[j] = wp[j][(int64_t)b * 64];
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) scale[j][k] = sp[j][(int64_t)b * (kGroups * 16) + k * 16];
     }
+  };
+  uint32_t mask = 0x000f000fu, lead = __is_same(E, _Float16) ? 0x64006400u : 0x43004300u;
+  asm("" : "+v"(mask), "+v"(lead));
+
+  f4 total[MT][NT] = {};
+  const int one2 = __is_same(E, _Float16) ? 0x3c003c00 : 0x3f803f80;
+  const i4 ones = {one2, one2, one2, one2};
+  i4 words[NT];
+  uint32_t scale[NT][kGroups];
+  if (w < p.blocks) {
+    load_w(w, words, scale);
+    copy_x(w);
+  }
+#pragma unroll 1
+  for (int b = w; b < p.blocks; b += WK) {
+    wait_vmcnt<0>();
+    arrived(words);   // (or the compiler would wait for them again, and for what is sent for below)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) asm volatile("" : "+v"(scale[j][k]));
     i4 xop[MT][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        xop[m][i] = i4{};
-        if (MT > 1 || c < p.M) xop[m][i] = *reinterpret_cast<const i4*>(xp[m] + min(b * kTileK + 32 * i, p.K - 32));
-      }
-    f4 sums[MT][kGroups] = {};
-    if constexpr (kOff) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sums[m][i / SPG] = Half<E>::small(xop[m][i], ones, sums[m][i / SPG]);
+      for (int i = 0; i < 4; ++i)
+        xop[m][i] = *reinterpret_cast<const i4*>(xs + m * 4096 + c * 256 + (((4 * i + g) ^ c) << 4));
+    wait_lgkm0();
+    i4 next[NT] = {};
+    uint32_t next_scale[NT][kGroups] = {};
+    if (b + WK < p.blocks) {   // a block ahead
+      load_w(b + WK, next, next_scale);
+      copy_x(b + WK);
     }
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+    for (int k = 0; k < kGroups; ++k) {
+      f4 sums[MT] = {};
+      if constexpr (kOff) {
 #pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = k * SPG; i < (k + 1) * SPG; ++i) sums[m] = Half<E>::small(xop[m][i], ones, sums[m]);
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
         f4 acc[MT] = {};
 #pragma unroll
         for (int i = k * SPG; i < (k + 1) * SPG; ++i) {
@@ -142,12 +174,22 @@ __global__ void __launch_bounds__(64 * WK) int4_linear_kernel(const Int4Params p
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float a = acc[m][e];
-            if constexpr (kOff) a = fmaf(off, sums[m][k][e], a);
+            if constexpr (kOff) a = fmaf(off, sums[m][e], a);
             total[m][j][e] = fmaf(s, a, total[m][j][e]);
           }
       }
+    }
+    __builtin_amdgcn_sched_barrier(0);   // (or these would wait for the next block among the products)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      words[j] = next[j];
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) scale[j][k] = next_scale[j][k];
+    }
   }
 
+  __syncthreads();   // (the inputs are done with)
+  f4(*const part)[MT * NT][64] = reinterpret_cast<f4(*)[MT * NT][64]>(smem);
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
