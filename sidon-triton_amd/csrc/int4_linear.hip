@@ -12,12 +12,14 @@
 // inputs, which a product with ones gives in the accumulator's own layout, is taken
 // off in fp32 with the group's scale.
 //
-// A wavefront has 16 NT outputs of 16 MT rows and every WK-th block of 128 inputs;
-// the WK wavefronts of a workgroup are summed through LDS.
+// A wavefront has 16 NT outputs of 16 MT rows and every WK-th block of 128 inputs, and
+// sends for the next one's weights and inputs before it takes a block's products; the WK
+// wavefronts of a workgroup are summed through LDS.  Inputs come through LDS too, copied as
+// whole rows: the operand's own lanes are of 16 rows, whose loads the cache takes one at a time
+// (32 x 4096 x 14336 33 us; so 16).
 //
-// Reached: 1 x 32768 x 4096 (71 MB) 16 us, 4.4 TB/s; 32 rows of it 21 to 24, where every
-// wavefront's loads of x, as many bytes as its weights, and 40 matrix and 200 vector
-// instructions a block come between the loads of weights; 1 x 4096 x 1024 2.8, latency.
+// Reached: 1 x 32768 x 4096 (71 MB) 16 us, 4.4 TB/s; 32 rows of it 21 to 23, where 40 matrix and 200
+// vector instructions a block stand beside the weights' 4 KB; 1 x 4096 x 1024 2.8, latency.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -220,15 +222,14 @@ struct Shape {
 
 // Rows of a workgroup by what M needs.  A wavefront takes one tile of outputs where that gives no
 // CU more than one workgroup, two where two do, else four (each tile more is x loaded once less,
-// and a CU with two workgroups takes twice as long: 64 x 8192 x 4096 in one, two, four tiles 33, 19
-// and 23 us; 16 x 16384 x 2048 11.2, 7.9 and 6.7; 1 x 4096 x 14336 10.9, 13.1 and 18.1), and K is
-// split over eight wavefronts, or four where there are many workgroups as it is (64 x 32768 x 4096
-// 46 us, with eight 47; 32 x 32768 x 4096 27.5 and 23.7).
+// and a CU with two workgroups takes longer: 64 x 8192 x 4096 in one, two, four tiles 17.9, 13.0
+// and 15.2 us; 64 x 16384 x 2048 22.3, 15.1 and 12.0; 32 x 4096 x 14336 15.6, 16.7 and 22.5), and K is
+// split over eight wavefronts, or four where four tiles give CUs several workgroups (32 x 32768 x
+// 4096 21.8 us, with eight 23.9; 64 x 16384 x 2048 12.8 and 12.0).
 Shape shape(int M, int N, int cus) {
   const int mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
   const int64_t units = (int64_t)((N + kTileN - 1) / kTileN) * ((M + 16 * mt - 1) / (16 * mt));
-  if (units <= 2 * (int64_t)cus) return Shape{mt, units <= cus ? 1 : 2, 8};
-  return Shape{mt, 4, units * mt > 16 * (int64_t)cus ? 4 : 8};
+  return Shape{mt, units <= cus ? 1 : units <= 2 * (int64_t)cus ? 2 : 4, units <= 4 * (int64_t)cus ? 8 : 4};
 }
 
 template <typename E, int MT, int NT, int WK>
