@@ -18,7 +18,7 @@
 // whole rows: the operand's own lanes are of 16 rows, whose loads the cache takes one at a time
 // (32 x 4096 x 14336 33 us; so 16).
 //
-// Reached: 1 x 32768 x 4096 (71 MB) 16 us, 4.4 TB/s; 32 rows of it 21 to 23, where 40 matrix and 200
+// Reached: 1 x 32768 x 4096 (71 MB) 16 us, 4.4 TB/s; 32 rows of it 18 to 23, where 40 matrix and 200
 // vector instructions a block stand beside the weights' 4 KB; 1 x 4096 x 1024 2.8, latency.
 #include <hip/hip_runtime.h>
 
