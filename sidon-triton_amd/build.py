@@ -66,7 +66,8 @@ def build(verbose: bool = False) -> Path:
     generate(verbose)
     out = PKG_DIR / LIB_NAME
     tmp = out.with_name(out.name + f".tmp{os.getpid()}")
-    cmd = [hipcc(), *HIP_FLAGS, f"-I{REPO_DIR / 'include'}", "-o", str(tmp), *map(str, SOURCES), *LIBS]
+    jobs = min(8, os.cpu_count() or 1)   # files at a time
+    cmd = [hipcc(), *HIP_FLAGS, f"-parallel-jobs={jobs}", f"-I{REPO_DIR / 'include'}", "-o", str(tmp), *map(str, SOURCES), *LIBS]
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)

@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(64 * RB * KS, kMinWaves) cross_attn_kernel(con
   static_assert(!(kFine && kLse), "the sums of two summands are as good");
   typedef typename Half<E>::v2 v2;
   typedef typename Half<E>::v4 v4;
-  constexpr int P = C::kP, kDb = C::kDb;
+  constexpr int kDb = C::kDb;
   constexpr int kQ = D / 16;          // Q operands
   __shared__ __attribute__((aligned(16))) char smem[C::kLds];
 

@@ -670,8 +670,9 @@ int choose(const BwdParams& p, int D, int cus) {
 template <typename E, int D, int KB, int QB>
 void launch_form(BwdParams& p, bool queries_first, hipStream_t stream) {
   constexpr int kKeys = KB * kBlock, kRows = QB * kBlock;
-  // (as many wavefronts a SIMD as the registers allow: three of 168 at D 64, two of 256 at 128)
-  constexpr int kWaves = D == 64 ? 3 : 2;
+  // (as many wavefronts a SIMD as the registers allow, three of 168 at D 64 and two of 256 at
+  // 128, or the LDS of a block alone, whose four groups have rings of their own)
+  constexpr int kWaves = (D == 64 ? 3 : 2) - (KB == 1 || QB == 1 ? 1 : 0);
   const int64_t heads = (int64_t)p.B * p.Hk;
   p.keys = deal(heads, (p.S + kKeys - 1) / kKeys, (int64_t)p.G * p.L * D * 4);
   p.queries = deal(heads, (int64_t)p.G * ((p.L + kRows - 1) / kRows), (int64_t)p.S * D * 4);
