@@ -213,7 +213,9 @@ int sidon_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * otherwise.  What dout holds past LQ does not matter.  Products in
  * `dtype` with fp32 sums: probabilities and dS are rounded once in front of them (fp16
  * scales both by powers of two, so that neither leaves its range whatever the size of
- * dout).  The same bits every time.  ws: sidon_cross_attention_bwd_workspace_bytes bytes.
+ * dout).  sum_j P dP, which dS holds the distance from, is taken in fp32 over the keys, not from the
+ * rounded out, so that dS is right to its own rounding where one key has nearly all of P.
+ * The same bits every time.  ws: sidon_cross_attention_bwd_workspace_bytes bytes.
  */
 size_t sidon_cross_attention_workspace_bytes(int B, int H, int Hk, int L, int S, int D);
 int sidon_cross_attention(const void* q, const void* k, const void* v, const int32_t* lens, const int32_t* q_lens,

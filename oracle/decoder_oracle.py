@@ -119,6 +119,48 @@ def cross_grads(dout, q, k, v, lens, q_lens, scale, u):
     return {name: (value, bound + u * value.abs()) for name, (value, bound) in grads.items()}
 
 
+def sharp_cross_grads(dout, q, k, v, lens, q_lens, scale, u):
+    """cross_grads' gradients -> {name: (gradient, bound)} with bounds that hold delta to fp32.
+
+    Scores s of at most A = max scale |q| . |k| (over a query's keys) go through D / 16 <= 8 sums of 16 products, a
+    scale, lse (its logarithm, two scalings) and an exponential: under 32 half steps of fp32 of A + 1, so
+    P is off by e = 2^-19 (A + 1) of itself, dP (8 sums) by m = 2^-20 |dout| . |v|.  delta starts
+    from dout . out, off by 2 u |dout| . softmax |v| at most (the forward call's roundings of P and out), and is
+    corrected by the sum of P (dP - dout . out), of up to 2^11 terms one after another:
+      delta is off by (e + 2^-12) (P |dP - delta| + 2 u |dout| . softmax |v|) + P m.
+    dS = P (dP - delta) is off by (u + e) of itself and P (m + delta's).  fp16 holds P times 2^15, off by
+    2^-40 where it is small, and dS times the power of two that brings 2 |dout| |v| of the longest rows
+    (dk: of all the heads that share the key) to 1/2 or more, off by 2^-38 |dout| |v|."""
+    b, h, l, d = q.shape
+    g, s = k.shape[1], k.shape[2]
+    zero = lambda t: torch.zeros(t.shape, dtype=torch.float64, device=t.device)  # noqa: E731
+    grads = {name: [zero(t), zero(t)] for name, t in (("dq", q), ("dk", k), ("dv", v))}
+    small = u == 2.0 ** -11
+    for i, (n, m) in enumerate(zip(_lengths(lens, b, s), _lengths(q_lens, b, l))):
+        for j in range(h if n and m else 0):
+            c = j // (h // g)
+            qq, do, kk, vv = (t.double() for t in (q[i, j, :m], dout[i, j, :m], k[i, c, :n], v[i, c, :n]))
+            p = torch.softmax(scale * (qq @ kk.t()), -1)
+            e = 2.0 ** -19 * (1 + (scale * (qq.abs() @ kk.abs().t())).amax(-1, keepdim=True))
+            dp, dp_off = do @ vv.t(), 2.0 ** -20 * (do.abs() @ vv.abs().t())
+            from_delta = dp - (p * dp).sum(-1, keepdim=True)
+            ds = p * from_delta
+            start = 2 * u * (do.abs() * (p @ vv.abs())).sum(-1, keepdim=True)
+            off = (e + 2.0 ** -12) * (ds.abs().sum(-1, keepdim=True) + start) + (p * dp_off).sum(-1, keepdim=True)
+            off = (u + e) * ds.abs() + p * (dp_off + off)
+            heads = slice(c * (h // g), (c + 1) * (h // g))
+            longest_v, longest = vv.norm(dim=-1).max(), dout[i, heads, :m].double().norm(dim=-1).max()
+            dq_off = off + small * 2.0 ** -38 * do.norm(dim=-1, keepdim=True) * longest_v
+            dk_off = off + small * 2.0 ** -38 * longest * longest_v
+            p_off = (u + e) * p + small * 2.0 ** -40
+            for name, at, value, bound in (("dq", (i, j, slice(m)), scale * (ds @ kk), scale * (dq_off @ kk.abs())),
+                                           ("dk", (i, c, slice(n)), scale * (ds.t() @ qq), scale * (dk_off.t() @ qq.abs())),
+                                           ("dv", (i, c, slice(n)), p.t() @ do, p_off.t() @ do.abs())):
+                grads[name][0][at] += value
+                grads[name][1][at] += bound
+    return {name: (value, bound + u * value.abs()) for name, (value, bound) in grads.items()}
+
+
 # ---- 4-bit projection --------------------------------------------------------------
 
 

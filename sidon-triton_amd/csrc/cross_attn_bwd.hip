@@ -1,18 +1,19 @@
 // cross_attn_bwd.hip -- gradients of the attention over states of another length
 // (MI355X / gfx950).  With P_ij = exp(scale q_i . k_j - lse_i) from the forward
-// call's lse, and delta_i = dout_i . out_i (= sum_j P_ij dP_ij):
+// call's lse, and delta_i = sum_j P_ij dP_ij (= dout_i . out_i, but for out's rounding):
 //
 //   dv_j = sum_i P_ij dout_i          dP_ij = dout_i . v_j
 //   dS_ij = P_ij (dP_ij - delta_i)    dq_i = scale sum_j dS_ij k_j    dk_j = scale sum_i dS_ij q_i
 //
-// Two launches.  The first takes delta and lse row by row.  In the second some
+// Two launches.  In the first, wavefronts that own 32 queries each go over the keys for delta: S and dP,
+// and the sum of P (dP - dout . out).  In the second some
 // wavefronts own 32 keys each, whose k and v stay in their registers as B operands, and go
 // over the queries of the heads that share them: S = Q . K^T and dP = dO . V^T by
 // v_mfma_f32_32x32x16, whose accumulators, rounded, are the B operands of
 // dV^T += dO^T . P and dK^T += Q^T . dS; others own 32 queries and
-// go over the keys: S^T = K . Q^T, dP^T = V . dO^T, dQ^T += K^T . dS^T.  (Seven
-// products where one pass would do with five and add dq up across workgroups: no
-// atomics, so the same bits every time.)  The tiles of 32 rows that the wavefronts of
+// go over the keys: S^T = K . Q^T, dP^T = V . dO^T, dQ^T += K^T . dS^T.  (Nine
+// products where one pass would do with five, delta from the rounded output and dq added up
+// across workgroups: no atomics, so the same bits every time.)  The tiles of 32 rows that the wavefronts of
 // a workgroup share are copied global -> LDS by global_load_lds_dwordx4 one step
 // ahead, and read as they are and transposed.
 //
@@ -20,10 +21,11 @@
 // bound |dS_ij| <= 2 |dout_i| |v_j| needs the longest v, and for dk the longest dout,
 // of a key head, which the first launch leaves.  bf16 has fp32's exponents.
 //
-// What bounds it, and what it reached.  16 heads x 4800 x 4800 take 330 us at D 64 (the five
-// products at 0.71 PFLOP/s) and 620 at D 128 (0.76): matrix cores and vector units are each
-// busy a third of the time and overlap little, LDS a fifth.  2 x 16 heads x 300 x 1463 takes 33 us: a
-// wavefront's longest chain of steps, and some 14 us of launches, first copies and merges.
+// What bounds it, and what it reached.  16 heads x 4800 x 4800 take 444 us at D 64 (112 of them the first
+// launch; the five products at 0.53 PFLOP/s) and 835 at D 128 (212; 0.57).  First launch: a tile's 16 exponentials and 32 other
+// vector instructions beside 8 products (16 at D 128).  Second: matrix cores and vector units are each
+// busy a third of the time and overlap little, LDS a fifth.  2 x 16 heads x 300 x 1463 takes 44 us: a
+// wavefront's longest chains of steps, and some 14 us of launches, first copies and merges.
 #include <hip/hip_runtime.h>
 
 #include <float.h>
@@ -67,6 +69,7 @@ struct BwdParams {
   int B, H, Hk, G, L, S;
   int tiles, key_tiles;  // of 32 queries, of 32 keys
   Deal keys, queries;    // blocks of keys, of queries of a group's heads
+  Deal rows;             // of the first launch
   float scale;
 };
 
@@ -102,89 +105,6 @@ __device__ __forceinline__ float team_sum(float v) {
   v += sidon::dpp_mov<0x141>(v);                         // row_half_mirror
   if constexpr (N > 8) v += sidon::dpp_mov<0x140>(v);    // row_mirror
   return v;
-}
-
-// Up to as many keys delta is taken as the sum of P dP, not from the rounded output:
-// the fewer keys, the more of dS cancels (of 3 keys dq was off by 0.29% in bf16, of 20 by
-// 0.24%, which is what its own and dS's rounding cost).
-constexpr int kFewKeys = 32;
-
-// ---- the first launch: a workgroup per 32 queries of a head, or (fp16) 32 keys of a key head ----
-template <typename E, int D>
-__global__ void __launch_bounds__(4 * D) cross_bwd_rows_kernel(const BwdParams p) {
-  typedef typename Half<E>::v8 v8;
-  constexpr int kTeam = D / 8;   // lanes of a row
-  __shared__ float most[D / 16];
-  const int tid = threadIdx.x, i = tid % kTeam, r = tid / kTeam;
-  const int groups = p.B * p.H * p.tiles;
-  const bool keys = (int)blockIdx.x >= groups;
-  int block = keys ? blockIdx.x - groups : blockIdx.x;
-  const int per = keys ? p.key_tiles : p.tiles, heads = keys ? p.Hk : p.H;
-  const int tile = block % per, bh = block / per, b = bh / heads, h = bh - b * heads;
-  const int row = tile * kBlock + r;
-  const int rows = keys ? valid(p.lens, b, p.S) : valid(p.q_lens, b, p.L);
-  float dot = 0.f, sq = 0.f;
-  if (row < rows) {
-    if (keys) {
-      const v8 x = *reinterpret_cast<const v8*>(static_cast<const E*>(p.v) + b * p.vb + h * p.vh + (int64_t)row * p.vl + 8 * i);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sq = fmaf((float)x[k], (float)x[k], sq);
-    } else {
-      const v8 x = *reinterpret_cast<const v8*>(static_cast<const E*>(p.dout) + b * p.gb + h * p.gh + (int64_t)row * p.gl + 8 * i);
-      const v8 y = *reinterpret_cast<const v8*>(static_cast<const E*>(p.out) + b * p.ob + h * p.oh + row * p.ol + 8 * i);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        dot = fmaf((float)x[k], (float)y[k], dot);
-        sq = fmaf((float)x[k], (float)x[k], sq);
-      }
-    }
-  }
-  dot = team_sum<kTeam>(dot);
-  sq = team_sum<kTeam>(sq);
-  if (!keys) {
-    float lse = INFINITY;   // no such row, or one that sees no key: P = 0
-    if (row < rows) {
-      lse = p.lse[(int64_t)bh * p.L + row];
-      lse = lse == -INFINITY ? INFINITY : lse * kLog2e;
-    }
-    const int lk = valid(p.lens, b, p.S);
-    if (lk <= kFewKeys && row < rows) {
-      const v8 x = *reinterpret_cast<const v8*>(static_cast<const E*>(p.q) + b * p.qb + h * p.qh + (int64_t)row * p.ql + 8 * i);
-      const v8 y = *reinterpret_cast<const v8*>(static_cast<const E*>(p.dout) + b * p.gb + h * p.gh + (int64_t)row * p.gl + 8 * i);
-      const E* const kp = static_cast<const E*>(p.k) + b * p.kb + h / p.G * p.kh + 8 * i;
-      const E* const vp = static_cast<const E*>(p.v) + b * p.vb + h / p.G * p.vh + 8 * i;
-      dot = 0.f;
-      for (int j = 0; j < lk; ++j) {
-        const v8 kk = *reinterpret_cast<const v8*>(kp + (int64_t)j * p.kl);
-        const v8 vv = *reinterpret_cast<const v8*>(vp + (int64_t)j * p.vl);
-        float s = 0.f, dp = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          s = fmaf((float)x[k], (float)kk[k], s);
-          dp = fmaf((float)y[k], (float)vv[k], dp);
-        }
-        dot = fmaf(fast_exp2(fmaf(team_sum<kTeam>(s), p.scale * kLog2e, -lse)), team_sum<kTeam>(dp), dot);
-      }
-    }
-    if (i == 0) {
-      float* at = p.stat + ((int64_t)bh * p.tiles + tile) * (2 * kBlock) + r;
-      at[0] = Range<E>::kLift - lse;
-      at[kBlock] = -dot;
-    }
-  }
-  if constexpr (Range<E>::kScaled) {
-    const float length = sqrtf(sq);
-    if (!keys && i == 0) p.length[((int64_t)bh * p.tiles + tile) * kBlock + r] = length;
-    float top = length;
-#pragma unroll
-    for (int d = kTeam; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (tid % 64 == 0) most[tid / 64] = top;
-    __syncthreads();
-    if (tid == 0) {
-      for (int k = 1; k < D / 16; ++k) top = fmaxf(top, most[k]);
-      (keys ? p.longest_v : p.longest)[(int64_t)bh * per + tile] = top;
-    }
-  }
 }
 
 // The largest of `count` numbers, by a wavefront.
@@ -304,6 +224,177 @@ struct Lds {
   static constexpr int kMerge = KS / 2 * RB * 2 * (D / 32) * 16 * 64 * 4;
   static constexpr int kBytes = KS * 2 * kKeysSlot > kMerge ? KS * 2 * kKeysSlot : kMerge;
 };
+
+// ---- the first launch: delta and lse of every query, and (fp16) the longest rows ----
+
+// A workgroup of RB wavefronts of 32 queries each x KS key groups.  delta is the sum of P dP, taken
+// as dout . out plus the sum of P (dP - dout . out): from the rounded output alone it is off by half a
+// step of |dout| |out|, which is all of dS where a query's softmax is nearly one key (dP - delta is
+// what the other keys leave).  The difference that is summed up is small, so that what lse's
+// and the products' roundings do to P does not matter beside it.
+template <typename E, int D, int RB, int KS>
+__device__ __forceinline__ void rows_body(const BwdParams& p, char* smem, int block) {
+  typedef typename Half<E>::v8 v8;
+  using C = Copies<D, RB>;
+  constexpr int kQ = D / 16, kRows = RB * kBlock, kSlot = Lds<D, RB, KS>::kTiles;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rb = w % RB, ks = w / RB;
+  const int n = lane & 31, g = lane >> 5;
+  int bh;   // of a key head
+  const int unit = dealt(p.rows, block, bh);
+  if (unit >= p.rows.units) return;
+  const int b = bh / p.Hk, hk = bh - b * p.Hk;
+  const int head = hk * p.G + unit % p.G, block0 = unit / p.G * kRows;
+  const int row = block0 + rb * kBlock + n;   // of this lane
+  const int lk = valid(p.lens, b, p.S), lq = valid(p.q_lens, b, p.L);
+  const int steps = block0 < lq ? (lk + kBlock - 1) / kBlock : 0;
+  const int rounds = (steps + KS - 1) / KS;
+
+  C ck, cv;
+  ck.init(rb, lane, p.kl);
+  cv.init(rb, lane, p.vl);
+  const uint32_t lds = (uint32_t)(uintptr_t)SIDON_LDS_PTR(char, smem) + ks * 2 * kSlot;
+  const char* const k0 = static_cast<const char*>(p.k) + 2 * (b * p.kb + hk * p.kh);
+  const char* const v0 = static_cast<const char*>(p.v) + 2 * (b * p.vb + hk * p.vh);
+  const auto copy = [&](int u) SIDON_INLINE {
+    const int t = u * KS + ks;
+    if (t < steps) {
+      const uint32_t at = lds + (u & 1) * kSlot;
+      ck.copy(at, k0 + (int64_t)t * kBlock * p.kl * 2, lk - t * kBlock);
+      cv.copy(at + C::kBytes, v0 + (int64_t)t * kBlock * p.vl * 2, lk - t * kBlock);
+    }
+  };
+  copy(0);
+
+  Reads at;
+  at.init(lane);
+  i4 qop[kQ], gop[kQ];
+  float dot = 0.f, sq = 0.f, lse = INFINITY;   // lse of no such row, or of one that sees no key: P = 0
+  const int rr = max(min(row, lq - 1), 0);
+  {
+    const E* const qp = static_cast<const E*>(p.q) + b * p.qb + head * p.qh + (int64_t)rr * p.ql + 8 * g;
+    const E* const gp = static_cast<const E*>(p.dout) + b * p.gb + head * p.gh + (int64_t)rr * p.gl + 8 * g;
+    const E* const op = static_cast<const E*>(p.out) + b * p.ob + head * p.oh + rr * p.ol + 8 * g;
+    i4 oop[kQ];
+#pragma unroll
+    for (int s = 0; s < kQ; ++s) {
+      qop[s] = *reinterpret_cast<const i4*>(qp + 16 * s);
+      gop[s] = *reinterpret_cast<const i4*>(gp + 16 * s);
+      oop[s] = *reinterpret_cast<const i4*>(op + 16 * s);
+    }
+    if (row < lq) {
+      lse = p.lse[((int64_t)b * p.H + head) * p.L + row];
+      lse = lse == -INFINITY ? INFINITY : lse * kLog2e;
+#pragma unroll
+      for (int s = 0; s < kQ; ++s) {
+        const v8 x = __builtin_bit_cast(v8, gop[s]), y = __builtin_bit_cast(v8, oop[s]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          dot = fmaf((float)x[k], (float)y[k], dot);
+          sq = fmaf((float)x[k], (float)x[k], sq);
+        }
+      }
+    }
+  }
+  dot = pair_sum(dot);
+  sq = pair_sum(sq);
+  arrived(qop);
+  arrived(gop);
+  asm volatile("" : "+v"(lse), "+v"(dot), "+v"(sq));
+  const float scale2 = p.scale * kLog2e;
+
+  float more[4] = {};   // sum of P (dP - dout . out), of this lane's keys
+  for (int u = 0; u < rounds; ++u) {
+    wait_vmcnt<0>();
+    lds_barrier();   // round u is there, and round u - 1 is read
+    copy(u + 1);
+    const int t = u * KS + ks;
+    if (t >= steps) continue;
+    const char* const tk = smem + (ks * 2 + (u & 1)) * kSlot;
+    const char* const tv = tk + C::kBytes;
+    f32x16 s = {}, dp;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dp[i] = -dot;
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) {
+      s = Half<E>::mfma(at.rows(tk, i), qop[i], s);
+      dp = Half<E>::mfma(at.rows(tv, i), gop[i], dp);
+    }
+    if ((t + 1) * kBlock > lk) {
+      const int left = lk - t * kBlock - 8 * g;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (16 * (i >> 3) + (i & 7) >= left) s[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) more[i % 4] = fmaf(fast_exp2(fmaf(s[i], scale2, -lse)), dp[i], more[i % 4]);
+  }
+  float sum = pair_sum((more[0] + more[1]) + (more[2] + more[3]));
+  if constexpr (KS > 1) {
+    float* const part = reinterpret_cast<float*>(smem);
+    lds_barrier();   // the rings are done with
+    if (g == 0) part[w * kBlock + n] = sum;
+    lds_barrier();
+    if (ks > 0) return;
+    sum = part[rb * kBlock + n];
+#pragma unroll
+    for (int k = 1; k < KS; ++k) sum += part[(k * RB + rb) * kBlock + n];
+  }
+  const int tile = block0 / kBlock + rb;
+  if (tile >= p.tiles) return;
+  const int64_t to = ((int64_t)b * p.H + head) * p.tiles + tile;
+  const float length = sqrtf(sq);
+  if (g == 0) {
+    p.stat[to * (2 * kBlock) + n] = Range<E>::kLift - lse;
+    p.stat[to * (2 * kBlock) + kBlock + n] = row < lq ? -(dot + sum) : 0.f;
+    if (Range<E>::kScaled) p.length[to * kBlock + n] = length;
+  }
+  if constexpr (Range<E>::kScaled) {
+    float top = length;
+#pragma unroll
+    for (int d = 1; d < kBlock; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (lane == 0) p.longest[to] = top;
+  }
+}
+
+// The longest v of a tile of 32 keys, by a wavefront.
+template <typename E, int D>
+__device__ __forceinline__ void longest_key(const BwdParams& p, int64_t at) {
+  typedef typename Half<E>::v8 v8;
+  constexpr int kTeam = D / 8, kAtOnce = 64 / kTeam;   // lanes of a row, rows
+  const int lane = threadIdx.x & 63, i = lane % kTeam;
+  const int tile = (int)(at % p.key_tiles), bh = (int)(at / p.key_tiles), b = bh / p.Hk, h = bh - b * p.Hk;
+  const int rows = valid(p.lens, b, p.S);
+  const E* const vp = static_cast<const E*>(p.v) + b * p.vb + h * p.vh + 8 * i;
+  float top = 0.f;
+#pragma unroll
+  for (int r0 = 0; r0 < kBlock; r0 += kAtOnce) {
+    const int row = tile * kBlock + r0 + lane / kTeam;
+    float sq = 0.f;
+    if (row < rows) {
+      const v8 x = *reinterpret_cast<const v8*>(vp + (int64_t)row * p.vl);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sq = fmaf((float)x[k], (float)x[k], sq);
+    }
+    top = fmaxf(top, team_sum<kTeam>(sq));
+  }
+  for (int d = kTeam; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if (lane == 0) p.longest_v[at] = sqrtf(top);
+}
+
+template <typename E, int D, int RB>
+__global__ void __launch_bounds__(256, 2) cross_bwd_rows_kernel(const BwdParams p) {
+  constexpr int KS = 4 / RB;
+  __shared__ __attribute__((aligned(16))) char smem[KS * 2 * Lds<D, RB, KS>::kTiles];
+  const int first = (int)p.rows.groups();
+  if ((int)blockIdx.x < first) {
+    rows_body<E, D, RB, KS>(p, smem, blockIdx.x);
+  } else if constexpr (Range<E>::kScaled) {
+    const int64_t at = (int64_t)(blockIdx.x - first) * 4 + (threadIdx.x >> 6);
+    if (at < (int64_t)p.B * p.Hk * p.key_tiles) longest_key<E, D>(p, at);
+  }
+}
 
 // ---- dk and dv: a workgroup of RB wavefronts of 32 keys each x KS row groups, which take
 // every KS-th step of 32 queries (of the heads in turn) from a ring of their own ----
@@ -686,11 +777,31 @@ void launch_form(BwdParams& p, bool queries_first, hipStream_t stream) {
   hipLaunchKernelGGL((cross_bwd_kernel<E, D, KB, QB, kWaves, false>), grid, block, 0, stream, p);
 }
 
+template <typename E, int D, int RB>
+void launch_row_blocks(BwdParams& p, hipStream_t stream) {
+  constexpr int kRows = RB * kBlock;
+  const int64_t heads = (int64_t)p.B * p.Hk;
+  p.rows = deal(heads, (int64_t)p.G * ((p.L + kRows - 1) / kRows), (int64_t)p.S * D * 4);
+  unsigned groups = p.rows.groups();
+  if (Range<E>::kScaled) groups += (unsigned)((heads * p.key_tiles + 3) / 4);
+  hipLaunchKernelGGL((cross_bwd_rows_kernel<E, D, RB>), dim3(groups), dim3(256), 0, stream, p);
+}
+
+// A block of 32 queries of four key groups while all of them run at once (the LDS of their rings lets
+// a CU hold two at D 64, one at 128), else two blocks of two groups: us of both launches, 1 x 16 heads x 300 x 4800
+// 70 and 79, 2 x 16 x 300 x 1463 43.6 and 44.4, but 8 x 16 x 448 x 1500 174 and 151, 4 x 16 (4 key heads) x 1200 x 4800
+// 439 and 408; at D 128 2 x 16 (4) x 128 x 3000 82 and 92, 2 x 16 x 300 x 1463 85 and 75.
+template <typename E, int D>
+void launch_rows(BwdParams& p, hipStream_t stream) {
+  if ((int64_t)p.B * p.H * p.tiles <= (int64_t)(D == 64 ? 2 : 1) * sidon::compute_units())
+    launch_row_blocks<E, D, 1>(p, stream);
+  else
+    launch_row_blocks<E, D, 2>(p, stream);
+}
+
 template <typename E, int D>
 void launch(BwdParams& p, hipStream_t stream) {
-  unsigned rows = (unsigned)p.B * p.H * p.tiles;
-  if (Range<E>::kScaled) rows += (unsigned)p.B * p.Hk * p.key_tiles;
-  hipLaunchKernelGGL((cross_bwd_rows_kernel<E, D>), dim3(rows), dim3(4 * D), 0, stream, p);
+  launch_rows<E, D>(p, stream);
   const Form& f = kForms[choose(p, D, sidon::compute_units())];
   switch (f.key_blocks * 10 + f.query_blocks) {   // (those of kForms)
     case 42: return launch_form<E, D, 4, 2>(p, f.queries_first, stream);
