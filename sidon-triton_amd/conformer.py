@@ -36,6 +36,7 @@ import ctypes
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .flexrel import _check_device_tensor, _on_device, _stream_handle
@@ -301,6 +302,14 @@ def plain(*tensors: torch.Tensor) -> bool:
                 return False
     return (getattr(forward_ad, "_current_level", 0) < 0
             or all(forward_ad.unpack_dual(t).tangent is None for t in tensors))
+
+
+def written(*tensors: torch.Tensor | None) -> None:
+    """Counts a caller's tensors that a kernel has written (None: not given) as changed in
+    place, so that a graph that saved one says so at its backward call."""
+    given = [t for t in tensors if t is not None]
+    if given:
+        increment_version(given)
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, out: torch.Tensor) -> torch.Tensor:

@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .conformer import plain
+from .conformer import plain, written
 from .diff_attention import _strides
 from .flexrel import _check_device_tensor, _on_device, _stream_handle
 
@@ -137,16 +137,16 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: tor
         raise TypeError("q, k and v must be torch.Tensor")
     key = _layout(q, k, v, lens, q_lens)
     sizes, dtype, strides, o_strides, need = _layouts.get(key) or _layouts.keep(key, _check(q, k, v, lens, q_lens))
-    device = q.device
-    if not plain(q, k, v):
-        raise ValueError("cross_attention follows no gradient: call it under torch.no_grad(), and "
-                         "cross_attention_backward for the gradients")
+    device, given = q.device, out
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         out, o_strides = _out("out", out, q)
     if lse is not None:
         _check_lse(lse, sizes, device)
+    if not (plain(q, k, v, out) if lse is None else plain(q, k, v, out, lse)):
+        raise ValueError("cross_attention follows no gradient: call it under torch.no_grad(), and "
+                         "cross_attention_backward for the gradients")
     lib = _lib.load()
     with _on_device(device):
         workspace = _workspace(workspace, need, q)
@@ -156,6 +156,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: tor
             o_strides, _stream_handle(device))
     if rc:
         _lib.check("sidon_cross_attention", rc)
+    written(given, lse)
     return out
 
 
@@ -192,13 +193,13 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     sizes, dtype, strides, contiguous, need = (
         _backward_layouts.get(key)
         or _backward_layouts.keep(key, _check_backward(dout, q, k, v, out, lse, lens, q_lens)))
-    device = q.device
-    if not plain(dout, q, k, v, out, lse):
-        raise ValueError("cross_attention_backward follows no gradient: call it under torch.no_grad()")
+    device, given = q.device, (dq, dk, dv)
     outs = []
     for i, (name, t, like) in enumerate((("dq", dq, q), ("dk", dk, k), ("dv", dv, v))):
         outs.append((torch.empty_like(like, memory_format=torch.contiguous_format), contiguous[i]) if t is None
                     else _out(name, t, like))
+    if not plain(dout, q, k, v, out, lse, *[t for t, _ in outs]):
+        raise ValueError("cross_attention_backward follows no gradient: call it under torch.no_grad()")
     lib = _lib.load()
     with _on_device(device):
         workspace = _workspace(workspace, need, q)
@@ -208,4 +209,5 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
             workspace.numel(), *sizes, dtype, *strides, *[s for _, s in outs], _stream_handle(device))
     if rc:
         _lib.check("sidon_cross_attention_bwd", rc)
+    written(*given)
     return tuple(t for t, _ in outs)

@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .conformer import plain
+from .conformer import plain, written
 from .diff_attention import _strides
 from .flexrel import _check_device_tensor, _on_device, _stream_handle
 
@@ -137,9 +137,10 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_w: torch.Tensor, k
     one past the tables gives NaN in the rotated dimensions.  out_q may be q itself,
     out_k k; they must not share other memory with an operand."""
     sizes, dtype, rot, places, strides, contiguous = _found(q, k, q_w, k_w, cos, sin, q_pos, k_pos)
-    _plain("qk_norm_rotary", q, k, q_w, k_w, cos, sin)
+    given = (out_q, out_k)
     out_q, oq = _out("out_q", out_q, q, contiguous[0])
     out_k, ok = _out("out_k", out_k, k, contiguous[1])
+    _plain("qk_norm_rotary", q, k, q_w, k_w, cos, sin, out_q, out_k)
     lib = _lib.load()
     with _on_device(q.device):
         rc = lib.sidon_qk_norm_rotary(
@@ -148,6 +149,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_w: torch.Tensor, k
             _stream_handle(q.device))
     if rc:
         _lib.check("sidon_qk_norm_rotary", rc)
+    written(*given)
     return out_q, out_k
 
 
@@ -168,7 +170,7 @@ def qk_norm_rotary_backward(dout_q: torch.Tensor, dout_k: torch.Tensor | None, q
     uint8 tensor of ``workspace_bytes``; allocated per call when None.  Without k the
     second and fourth are None."""
     sizes, dtype, rot, places, strides, contiguous = _found(q, k, q_w, k_w, cos, sin, q_pos, k_pos)
-    _plain("qk_norm_rotary_backward", dout_q, dout_k, q, k, q_w, k_w, cos, sin)
+    given = (dq, dk)
     _rows("dout_q", dout_q, tuple(q.shape), q)
     if (dout_k is None) != (k is None):
         raise ValueError("dout_k and k belong together")
@@ -176,6 +178,7 @@ def qk_norm_rotary_backward(dout_q: torch.Tensor, dout_k: torch.Tensor | None, q
         _rows("dout_k", dout_k, tuple(k.shape), k)
     dq, sq = _out("dq", dq, q, contiguous[0])
     dk, sk = _out("dk", dk, k, contiguous[1])
+    _plain("qk_norm_rotary_backward", dout_q, dout_k, q, k, q_w, k_w, cos, sin, dq, dk)
     dim, device = sizes[-1], q.device
     dw = q_w.new_empty((1 if k is None else 2, dim))
     lib = _lib.load()
@@ -194,4 +197,5 @@ def qk_norm_rotary_backward(dout_q: torch.Tensor, dout_k: torch.Tensor | None, q
             dtype, _strides(dout_q), _NONE if k is None else _strides(dout_k), *strides, sq, sk, _stream_handle(device))
     if rc:
         _lib.check("sidon_qk_norm_rotary_bwd", rc)
+    written(*given)
     return dq, dk, dw[0], None if k is None else dw[1]

@@ -18,7 +18,7 @@ import dataclasses
 import torch
 
 from . import _lib
-from .conformer import plain
+from .conformer import plain, written
 from .flexrel import _check_device_tensor, _on_device, _stream_handle
 
 _TILE_N, _TILE_K = 16, 128
@@ -150,15 +150,15 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, bias: torch.Tensor | None = None
         _check_device_tensor("bias", bias, device)
         if bias.dtype != w.dtype or tuple(bias.shape) != (w.n,) or not bias.is_contiguous():
             raise ValueError(f"bias must be a contiguous {w.dtype} [{w.n}] tensor")
-    if not (plain(x) if bias is None else plain(x, bias)):
-        raise ValueError("int4_linear has no backward: call it under torch.no_grad()")
-    rows = x.shape[0]
+    rows, given = x.shape[0], out
     if out is None:
         out = x.new_empty((rows, w.n))
     else:
         _check_device_tensor("out", out, device)
         if out.dtype != w.dtype or tuple(out.shape) != (rows, w.n) or (out.stride(1) != 1 and w.n > 1):
             raise ValueError(f"out must be a {w.dtype} [{rows}, {w.n}] tensor with rows contiguous")
+    if not (plain(x, out) if bias is None else plain(x, bias, out)):
+        raise ValueError("int4_linear has no backward: call it under torch.no_grad()")
     _lib.ints(rows=rows)
     lib = _lib.load()
     with _on_device(device):
@@ -169,4 +169,5 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, bias: torch.Tensor | None = None
                                    _lib.ACTIVATIONS[act], _lib.DTYPES[w.dtype], _stream_handle(device))
     if rc:
         _lib.check("sidon_int4_linear", rc)
+    written(given)
     return out
