@@ -52,18 +52,22 @@ class Int4Weight:
         return dataclasses.replace(self, words=self.words.to(device), scales=self.scales.to(device))
 
 
-def quantize_int4(w: torch.Tensor, group: int = 128, zeros: bool = True):
-    """w [N, K] -> (values uint8 [N, K] from 0 to 15, scales [N, K / group] of w's
-    type, zero points uint8 [N, K / group] or None): each group's range in 15 steps,
-    to the nearest.  Without zero points the values are 8 + w / scale."""
+def quantize_int4(w: torch.Tensor, group: int = 128, zeros: bool = True, dtype: torch.dtype | None = None):
+    """w [N, K] -> (values uint8 [N, K] from 0 to 15, scales [N, K / group] of ``dtype``
+    (None: w's), zero points uint8 [N, K / group] or None): each group's range in 15 steps
+    of the scale as it is rounded, to the nearest.  Without zero points the values are 8 + w / scale.
+    ``pack_int4`` takes fp16 and bf16 scales: name one of them for weights of another type."""
+    dtype = w.dtype if dtype is None else dtype
+    if not dtype.is_floating_point:
+        raise TypeError(f"scales must be of a floating point type (got {dtype})")
     if w.dim() != 2 or group < 1 or w.shape[1] % group:
         raise ValueError(f"w must be [N, K] with K a multiple of {group}")
     g = w.detach().float().unflatten(1, (-1, group))
     if zeros:
         low, high = g.amin(-1).clamp_max(0), g.amax(-1).clamp_min(0)
-        scale = ((high - low) / 15).to(w.dtype)
+        scale = ((high - low) / 15).to(dtype)
     else:
-        scale = (g.abs().amax(-1) / 7).to(w.dtype)
+        scale = (g.abs().amax(-1) / 7).to(dtype)
     # (a group of zeros, or one whose steps the type does not hold: any scale)
     scale = torch.where(scale > 0, scale, torch.ones_like(scale))
     step = scale.float()
@@ -82,7 +86,7 @@ def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | 
     if values.dtype != torch.uint8:
         raise TypeError(f"values must be uint8 (got {values.dtype})")
     if scales.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"scales must be float16 or bfloat16 (got {scales.dtype})")
+        raise TypeError(f"scales must be float16 or bfloat16 (got {scales.dtype}; quantize_int4's dtype)")
     scales = scales.detach()
     n, k = values.shape
     groups = scales.shape[1]
