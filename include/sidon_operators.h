@@ -193,7 +193,7 @@ int sidon_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * head, row) in elements, multiples of 8 from 0 to 2^40, rows of k and v less than 2^25
  * apart; D 64 or 128; 0 < scale <= 2^100.  lse fp32 [B, H, L] contiguous, or NULL.  out's
  * rows must not overlap one another, and out, lse and ws hold nothing of another operand
- * (out may be a column block of one tensor with q).
+ * (out may be a column block of one tensor with q, or lie in turn with it).
  *
  * Scores, softmax statistics and sums in fp32; |scale q . k| up to 2^24.  Probabilities
  * are rounded to `dtype` in front of the product with v: each off by half a step of
@@ -209,8 +209,8 @@ int sidon_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * `dtype` from the output's, dout, and the forward call's q, k, v, out and lse under the
  * same lens, q_lens and scale; written, not added to; zeros past LQ and LK.  Rows of
  * dout and q less than 2^25 apart, S <= 2^24, B * H <= 2^20, the rest as above; an output
- * may be a column block of one tensor with another operand, and shares no memory
- * otherwise.  What dout holds past LQ does not matter.  Products in
+ * may be a column block of one tensor with another operand, or lie in turn with it, and shares
+ * no memory.  What dout holds past LQ does not matter.  Products in
  * `dtype` with fp32 sums: probabilities and dS are rounded once in front of them (fp16
  * scales both by powers of two, so that neither leaves its range whatever the size of
  * dout).  sum_j P dP, which dS holds the distance from, is taken in fp32 over the keys, not from the

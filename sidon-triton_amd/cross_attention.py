@@ -125,7 +125,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: tor
     (None: all S), q_lens: int32 [B] valid queries (None: all L); what lies past
     either does not matter.  A query without keys, or past q_lens, gives zeros.
     scale: of the scores, positive (None: 1 / sqrt D).  out: optional [B, H, L, D], in
-    memory apart from the inputs (a column block of one tensor with q is).  lse: optional
+    memory apart from the inputs (a column block of one tensor with q is, and items in turn with it).  lse: optional
     contiguous fp32 [B, H, L] that takes the logarithm of the sums of exponentials,
     which ``cross_attention_backward`` wants.  workspace: a contiguous uint8 tensor of
     ``workspace_bytes``, apart from all of them; allocated per call when None.
@@ -183,7 +183,7 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     q, k, v, lens, q_lens and scale as the forward call had them, out and lse as it
     left them; dout [B, H, L, D] of the same type (any strides as q's; what it holds past
     q_lens does not matter).  dq like q, dk and dv like k, optional, in memory apart from the other operands
-    (column blocks of one tensor are); they are written, zeros past the valid queries and
+    (column blocks of one tensor are, and items in turn); they are written, zeros past the valid queries and
     keys.  Heads that share a key head are summed in fp32.  workspace: a contiguous uint8
     tensor of ``backward_workspace_bytes``; allocated per call when None.  Equal calls
     give equal bits."""

@@ -85,28 +85,29 @@ struct Rows {
   int last, size;
   __int128 bytes() const { return span(n, st, 3, last) * size; }
 };
-// Whether two such tensors may share memory.  Column blocks of one wider tensor do
-// not, though their ranges meet: where every (batch, row) step of both is a multiple
-// of the smallest one, the heads of each stay within it, and so do their columns.
+// Whether two such tensors may share memory.  Those whose ranges meet do not where some step
+// of theirs divides them: dimensions of steps that are multiples of it shift either tensor
+// by whole pitches, the others stay within one, and there in columns apart (column blocks of one
+// wider tensor, items of two tensors in turn).
 inline bool tensors_meet(const Rows& a, const Rows& b) {
   if (!ranges_meet(a.at, (int64_t)a.bytes(), b.at, (int64_t)b.bytes())) return false;
-  int64_t pitch = 0;
-  for (const Rows* t : {&a, &b})
-    for (const int d : {0, 2})
-      if (t->n[d] > 1 && t->st[d] > 0 && (pitch == 0 || t->st[d] * t->size < pitch)) pitch = t->st[d] * t->size;
-  if (pitch == 0) return true;
-  int64_t width[2];
-  int i = 0;
-  for (const Rows* t : {&a, &b}) {
-    for (const int d : {0, 2})
-      if (t->n[d] > 1 && t->st[d] * t->size % pitch != 0) return true;
-    const __int128 w = ((__int128)(t->n[1] - 1) * t->st[1] + t->last) * t->size;
-    if (w > pitch) return true;
-    width[i++] = (int64_t)w;
-  }
-  const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(b.at) - reinterpret_cast<uintptr_t>(a.at)) % pitch;
-  const int64_t on = d < 0 ? d + pitch : d;   // from a's column to b's
-  return on < width[0] || pitch - on < width[1];
+  for (const Rows* by : {&a, &b})
+    for (int i = 0; i < 3; ++i) {
+      if (by->n[i] == 1 || by->st[i] <= 0) continue;
+      const int64_t pitch = by->st[i] * by->size;
+      __int128 width[2];
+      int k = 0;
+      for (const Rows* t : {&a, &b}) {
+        __int128 w = t->last;
+        for (int d = 0; d < 3; ++d)
+          if (t->st[d] * t->size % pitch != 0) w += (__int128)(t->n[d] - 1) * t->st[d];
+        width[k++] = w * t->size;
+      }
+      const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(b.at) - reinterpret_cast<uintptr_t>(a.at)) % pitch;
+      const int64_t on = d < 0 ? d + pitch : d;   // from a's column to b's
+      if (on >= width[0] && pitch - on >= width[1]) return false;
+    }
+  return true;
 }
 
 }  // namespace sidon
