@@ -253,6 +253,9 @@ int sidon_cross_attention_bwd(const void* dout, const void* q, const void* k, co
 int sidon_int4_linear(const void* x, int64_t ldx, const void* words, const void* scales, const void* bias, void* y,
                       int64_t ldy, int M, int N, int K, int group, int zeros, int act, int dtype,
                       sidon_stream_t stream);
+/* How a call of these sizes is cut on the current device (256 compute units without one): tiles of 16 rows and of
+ * 16 outputs of a wavefront, wavefronts that K is split over. */
+int sidon_int4_linear_tiles(int M, int N, int* rows, int* outputs, int* splits);
 
 #ifdef __cplusplus
 }

@@ -109,6 +109,7 @@ SIGNATURES = {
                                                  *[ctypes.c_int] * 7, *[_I64P] * 8, _VP]),
     "sidon_int4_linear": (ctypes.c_int, [_VP, ctypes.c_int64, _VP, _VP, _VP, _VP, ctypes.c_int64, *[ctypes.c_int] * 7,
                                          _VP]),
+    "sidon_int4_linear_tiles": (ctypes.c_int, [ctypes.c_int] * 2 + [_IP] * 3),
     "sidon_last_error": (ctypes.c_char_p, []),
     "sidon_version": (ctypes.c_char_p, []),
 }

@@ -274,6 +274,16 @@ void launch(const Int4Params& p, const Shape& c, int group, bool off, hipStream_
 
 }  // namespace
 
+SIDON_API int sidon_int4_linear_tiles(int M, int N, int* rows, int* outputs, int* splits) {
+  sidon::clear_error();
+  if (!rows || !outputs || !splits) return sidon::fail(SIDON_E_NULL, "rows, outputs and splits must be non-NULL");
+  if (M < 1 || N < 1 || M > (1 << 21) || N > (1 << 24))
+    return sidon::fail(SIDON_E_SHAPE, "M=%d N=%d: need 1 <= M <= 2^21, N <= 2^24", M, N);
+  const Shape c = shape(M, N, sidon::compute_units());
+  *rows = c.mt, *outputs = c.nt, *splits = c.wk;
+  return SIDON_OK;
+}
+
 SIDON_API int sidon_int4_linear(const void* x, int64_t ldx, const void* words, const void* scales, const void* bias,
                                 void* y, int64_t ldy, int M, int N, int K, int group, int zeros, int act, int dtype,
                                 sidon_stream_t stream) {
