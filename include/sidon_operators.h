@@ -201,7 +201,8 @@ int sidon_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * H / Hk * L <= 32 what the rounding left is multiplied too, and the result is off by
  * its own rounding; with more it may be or not, as the kernel that is fastest for the
  * sizes and the device has it.  One rounding at the end.  lse sums what was not rounded.
- * A query that is no number gives NaN and reaches no other.  ws:
+ * A query that is no number gives NaN; another's sum of probabilities may be added up in another order
+ * beside it, which is a step of its result at most, and nothing else reaches another.  ws:
  * sidon_cross_attention_workspace_bytes bytes for these sizes on the current device
  * (0: ws may be NULL), 16-byte aligned, contents irrelevant.
  *
