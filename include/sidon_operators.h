@@ -212,9 +212,12 @@ int sidon_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * dout and q less than 2^25 apart, S <= 2^24, B * H <= 2^20, the rest as above; an output
  * may be a column block of one tensor with another operand, or lie in turn with it, and shares
  * no memory.  What dout holds past LQ does not matter.  Products in
- * `dtype` with fp32 sums: probabilities and dS are rounded once in front of them (fp16
- * scales both by powers of two, so that neither leaves its range whatever the size of
- * dout).  sum_j P dP, which dS holds the distance from, is taken in fp32 over the keys, not from the
+ * `dtype` with fp32 sums: probabilities and dS are rounded once in front of them.  fp16
+ * scales both by powers of two, so that neither overflows whatever the size of dout: P keeps
+ * its digits down to 2^-29 and vanishes below 2^-40; dS does so relative to 2 |dout| |v| of the longest rows
+ * below 2^-28 and 2^-39, of an item's v for the key head, and for dk of the dout of all the heads that share it
+ * (so where some rows' dout is a million times shorter than others', what only they add to dk loses digits), for dq
+ * of the query's own.  sum_j P dP, which dS holds the distance from, is taken in fp32 over the keys, not from the
  * rounded out, so that dS is right to its own rounding where one key has nearly all of P.
  * The same bits every time.  ws: sidon_cross_attention_bwd_workspace_bytes bytes.
  */

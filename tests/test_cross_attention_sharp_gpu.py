@@ -36,3 +36,53 @@ def test_sharp_gradients(sidon, shape, size, kind):
         cross_test.within(got, value, tol + cross_test.tiny(kind))
     again = ca.cross_attention_backward(dout, q, k, v, out, lse, n, m)
     assert all(torch.equal(x, y) for x, y in zip(grads, again))
+
+
+@pytest.mark.parametrize("less", [2.0 ** -6, 2.0 ** -12, 2.0 ** -20], ids=str)
+@pytest.mark.parametrize("shape", [(2, 4, 2, 70, 300, 64), (1, 2, 1, 40, 96, 128), (1, 4, 4, 160, 500, 64)], ids=str)
+def test_fp16_rows_far_apart_in_size(sidon, shape, less):
+    """Rows of dout a million times shorter than others', and keys that only such rows see: what
+    fp16's power of two leaves of them (one for all rows of a key in dk, one for a row in dq)."""
+    b, h, hk, l, s, d = shape
+    q, k, v, dout = cross_test.inputs(*shape, torch.float16, 23)
+    q, dout = q.contiguous(), (64 * dout).contiguous()
+    dout[:, :, ::2] *= less
+    # even queries see the first half of the keys, odd ones the rest
+    q[..., 0], k[..., 0] = 0, 0
+    q[:, :, ::2, 0], q[:, :, 1::2, 0] = 16, -16
+    k[:, :, :s // 2, 0], k[:, :, s // 2:, 0] = 8, -8
+    ca, lse = sidon.cross_attention, torch.empty(b, h, l, device=DEV)
+    out = ca.cross_attention(q, k, v, lse=lse)
+    grads = ca.cross_attention_backward(dout, q, k, v, out, lse)
+    want = oracle.sharp_cross_grads(dout, q, k, v, None, None, d ** -0.5, 2.0 ** -11)
+    for got, (value, tol) in zip(grads, want.values()):
+        cross_test.within(got, value, tol + cross_test.tiny(torch.float16))
+
+
+@pytest.mark.parametrize("kind", cross_test.KINDS, ids=str)
+@pytest.mark.parametrize("size", [32, 512])
+def test_gradients_of_large_scores(sidon, size, kind):
+    """Scores of a standard deviation of ``size``, within the bounds of their fp32 values."""
+    b, h, hk, l, s, d = 2, 2, 1, 40, 90, 64
+    q, k, v, dout = cross_test.inputs(b, h, hk, l, s, d, kind, 29)
+    q = (q * size).contiguous()
+    ca, lse = sidon.cross_attention, torch.empty(b, h, l, device=DEV)
+    out = ca.cross_attention(q, k, v, lse=lse)
+    assert float(lse.max()) > 2 * size
+    grads = ca.cross_attention_backward(dout, q, k, v, out, lse)
+    want = oracle.sharp_cross_grads(dout, q, k, v, None, None, d ** -0.5, torch.finfo(kind).eps / 2)
+    for got, (value, tol) in zip(grads, want.values()):
+        cross_test.within(got, value, tol + cross_test.tiny(kind))
+
+
+@pytest.mark.parametrize("kind", cross_test.KINDS, ids=str)
+@pytest.mark.parametrize("shape", [(2, 2, 1, 40, 90, 64), (1, 2, 2, 33, 70, 128)], ids=str)
+def test_gradients_of_the_largest_scores(sidon, shape, kind):
+    """Scores of up to some 2^20, whose fp32 values are right to 2^-4: numbers, if no more than that."""
+    b, h, hk, l, s, d = shape
+    q, k, v, dout = cross_test.inputs(*shape, kind, 31)
+    q, k = (8192 * q).contiguous(), (16 * k).contiguous()
+    ca, lse = sidon.cross_attention, torch.empty(b, h, l, device=DEV)
+    out = ca.cross_attention(q, k, v, scale=0.25, lse=lse)
+    assert 2.0 ** 21 > float(lse.max()) > 2.0 ** 19   # (standard deviations of 2^18 and 2^18.5)
+    assert all(torch.isfinite(t).all() for t in (out, *ca.cross_attention_backward(dout, q, k, v, out, lse, scale=0.25)))
