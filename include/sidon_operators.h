@@ -219,7 +219,8 @@ int sidon_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * (so where some rows' dout is a million times shorter than others', what only they add to dk loses digits), for dq
  * of the query's own.  sum_j P dP, which dS holds the distance from, is taken in fp32 over the keys, not from the
  * rounded out, so that dS is right to its own rounding where one key has nearly all of P.
- * The same bits every time.  ws: sidon_cross_attention_bwd_workspace_bytes bytes.
+ * P is formed anew from lse, off by what fp32 leaves of it, some 2^-21 |lse| of itself; |scale q . k| up to 2^20
+ * here.  The same bits every time.  ws: sidon_cross_attention_bwd_workspace_bytes bytes.
  */
 size_t sidon_cross_attention_workspace_bytes(int B, int H, int Hk, int L, int S, int D);
 int sidon_cross_attention(const void* q, const void* k, const void* v, const int32_t* lens, const int32_t* q_lens,
