@@ -245,7 +245,8 @@ int sidon_cross_attention_bwd(const void* dout, const void* q, const void* k, co
  * SIDON_ACT_NONE or SIDON_ACT_SILU.  group 32, 64 or 128, K a multiple of it; M <= 2^21,
  * N <= 2^24, K <= 2^20.  y shares no memory with an operand (it may be a column block
  * of one tensor with x).  Sums in fp32, one rounding at the end; a row's sums of |x|
- * over a group times 143 must be fp32 numbers.
+ * over a group times 143 must be fp32 numbers.  A row that holds an infinity or a NaN gives infinities
+ * or NaN in all of its outputs, and no other row does.
  *
  * The weights w (0 to 15) and (s, z) as they are laid out once, for N and K rounded up
  * to 16 and 128 with zeros, 16-byte aligned:
