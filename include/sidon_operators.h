@@ -213,11 +213,11 @@ int sidon_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * may be a column block of one tensor with another operand, or lie in turn with it, and shares
  * no memory.  What dout holds past LQ does not matter.  Products in
  * `dtype` with fp32 sums: probabilities and dS are rounded once in front of them.  fp16
- * scales both by powers of two, so that neither overflows whatever the size of dout: P keeps
- * its digits down to 2^-29 and vanishes below 2^-40; dS does so relative to 2 |dout| |v| of the longest rows
- * below 2^-28 and 2^-39, of an item's v for the key head, and for dk of the dout of all the heads that share it
- * (so where some rows' dout is a million times shorter than others', what only they add to dk loses digits), for dq
- * of the query's own.  sum_j P dP, which dS holds the distance from, is taken in fp32 over the keys, not from the
+ * scales both by powers of two, so that neither overflows whatever the size of dout.  P keeps
+ * its digits down to 2^-29 and vanishes below 2^-40; dS does so down to 2^-28 and 2^-39 of 2 |dout| |v|, with
+ * the longest v of the item's key head, and dout of the query itself for dq, the longest of all heads
+ * that share the key for dk: what rows a million times shorter than others add there loses digits.
+ * sum_j P dP, the number that dS holds the distance from, is taken in fp32 over the keys, not from the
  * rounded out, so that dS is right to its own rounding where one key has nearly all of P.
  * P is formed anew from lse, off by what fp32 leaves of it, some 2^-21 |lse| of itself; |scale q . k| up to 2^20
  * here.  The same bits every time.  ws: sidon_cross_attention_bwd_workspace_bytes bytes.

@@ -6,16 +6,16 @@
 //   dS_ij = P_ij (dP_ij - delta_i)    dq_i = scale sum_j dS_ij k_j    dk_j = scale sum_i dS_ij q_i
 //
 // Two launches.  In the first, wavefronts that own 32 queries each go over the keys for delta: S and dP,
-// and the sum of P (dP - dout . out).  In the second some
-// wavefronts own 32 keys each, whose k and v stay in their registers as B operands, and go
-// over the queries of the heads that share them: S = Q . K^T and dP = dO . V^T by
-// v_mfma_f32_32x32x16, whose accumulators, rounded, are the B operands of
-// dV^T += dO^T . P and dK^T += Q^T . dS; others own 32 queries and
-// go over the keys: S^T = K . Q^T, dP^T = V . dO^T, dQ^T += K^T . dS^T.  (Nine
-// products where one pass would do with five, delta from the rounded output and dq added up
-// across workgroups: no atomics, so the same bits every time.)  The tiles of 32 rows that the wavefronts of
-// a workgroup share are copied global -> LDS by global_load_lds_dwordx4 one step
-// ahead, and read as they are and transposed.
+// and the sum of P (dP - dout . out).  In the second some wavefronts own 32 keys each, whose k
+// and v stay in their registers as B operands, and go over the queries of the heads that share them:
+// S = Q . K^T and dP = dO . V^T by v_mfma_f32_32x32x16, whose accumulators, rounded, are the B
+// operands of dV^T += dO^T . P and dK^T += Q^T . dS; others own 32 queries and go over the keys:
+// S^T = K . Q^T, dP^T = V . dO^T, dQ^T += K^T . dS^T.  (Nine products, where one pass would do with five
+// if delta came from the rounded output and dq were added up across workgroups: here no atomics, so the
+// same bits every time.)  The tiles of 32 rows that the wavefronts of a workgroup share are copied global -> LDS by global_load_lds_dwordx4 one step
+// ahead, and read as they are and transposed.  (Where the second launch spills `4 * lane`, at D 128 but for one block of
+// either kind, at D 64 in two blocks of keys by four of queries and, queries first, in four by two of bf16, its reload
+// stands between the copies and waits for the ones just issued.)
 //
 // fp16 holds P times 2^15, and dS times a power of two that keeps it below 2^15: the
 // bound |dS_ij| <= 2 |dout_i| |v_j| needs the longest v, and for dk the longest dout,
@@ -708,13 +708,14 @@ Workspace workspace(int B, int H, int Hk, int L, int S, int dtype) {
 //        + keys_turn r_k ceil(n_k / fit) + queries_turn r_q ceil(n_q / fit) + longest max(r_k, r_q) + last r
 //
 // with n workgroups a CU of either kind, of r rounds each (its steps over its groups), the
-// last ones' r: what all of them take together, and what the busiest CU's, the longest one and
+// last ones' r (with a first launch of 5 us, the same for all of them): what all of them take together, and what the busiest CU's, the longest one and
 // the last take.  (More groups make a workgroup shorter, more blocks share copies, and where the
 // longer kind waits for the other it ends late.)  20000 shapes of 1 to 24 items, 8 to 2400
 // queries and 30 to 5000 keys were timed in 18 forms at D 64 and 10 at 128; these are the ones
 // that the others rarely beat, and their numbers chosen for the choice: it takes 1.02 times the
 // best one's time on average, 1.2 in 99 of 100 (one form for both kinds, in the better order: 1.06 at
-// best, at D 64; 4 x 16 heads (4 key heads) x 1200 x 4800 306 us, with one form 324; 1 x 16 x 300 x 4800 42 and 55).
+// best, at D 64; 4 x 16 heads (4 key heads) x 1200 x 4800 306 us, with one form 324; 1 x 16 x 300 x 4800 42 and 55; the first launch
+// is 15 to 115 now, whichever form).
 struct Form {
   int dim, key_blocks, query_blocks;
   bool queries_first;
@@ -761,8 +762,9 @@ int choose(const BwdParams& p, int D, int cus) {
 template <typename E, int D, int KB, int QB>
 void launch_form(BwdParams& p, bool queries_first, hipStream_t stream) {
   constexpr int kKeys = KB * kBlock, kRows = QB * kBlock;
-  // (as many wavefronts a SIMD as the registers allow, three of 168 at D 64 and two of 256 at
-  // 128, or the LDS of a block alone, whose four groups have rings of their own)
+  // (wavefronts a SIMD: three of 168 registers at D 64 and two of 256 at 128, for which most of these
+  // kernels spill 1 to 13 of them, or as the LDS of a block alone allows, whose four groups have rings
+  // of their own)
   constexpr int kWaves = (D == 64 ? 3 : 2) - (KB == 1 || QB == 1 ? 1 : 0);
   const int64_t heads = (int64_t)p.B * p.Hk;
   p.keys = deal(heads, (p.S + kKeys - 1) / kKeys, (int64_t)p.G * p.L * D * 4);
