@@ -307,9 +307,9 @@ def plain(*tensors: torch.Tensor) -> bool:
 def written(*tensors: torch.Tensor | None) -> None:
     """Counts a caller's tensors that a kernel has written (None: not given) as changed in
     place, so that a graph that saved one says so at its backward call."""
-    given = [t for t in tensors if t is not None]
-    if given:
-        increment_version(given)
+    for t in tensors:
+        if t is not None:
+            increment_version(t)
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, out: torch.Tensor) -> torch.Tensor:

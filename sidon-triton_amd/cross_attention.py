@@ -144,7 +144,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: tor
         out, o_strides = _out("out", out, q)
     if lse is not None:
         _check_lse(lse, sizes, device)
-    if not (plain(q, k, v, out) if lse is None else plain(q, k, v, out, lse)):
+    if not (plain(q, k, v) if given is lse is None else plain(q, k, v, out, *(() if lse is None else (lse,)))):
         raise ValueError("cross_attention follows no gradient: call it under torch.no_grad(), and "
                          "cross_attention_backward for the gradients")
     lib = _lib.load()
@@ -198,7 +198,7 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     for i, (name, t, like) in enumerate((("dq", dq, q), ("dk", dk, k), ("dv", dv, v))):
         outs.append((torch.empty_like(like, memory_format=torch.contiguous_format), contiguous[i]) if t is None
                     else _out(name, t, like))
-    if not plain(dout, q, k, v, out, lse, *[t for t, _ in outs]):
+    if not plain(dout, q, k, v, out, lse, *[t for t in given if t is not None]):
         raise ValueError("cross_attention_backward follows no gradient: call it under torch.no_grad()")
     lib = _lib.load()
     with _on_device(device):

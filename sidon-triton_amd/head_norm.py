@@ -140,7 +140,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_w: torch.Tensor, k
     given = (out_q, out_k)
     out_q, oq = _out("out_q", out_q, q, contiguous[0])
     out_k, ok = _out("out_k", out_k, k, contiguous[1])
-    _plain("qk_norm_rotary", q, k, q_w, k_w, cos, sin, out_q, out_k)
+    _plain("qk_norm_rotary", q, k, q_w, k_w, cos, sin, *given)
     lib = _lib.load()
     with _on_device(q.device):
         rc = lib.sidon_qk_norm_rotary(
@@ -178,7 +178,7 @@ def qk_norm_rotary_backward(dout_q: torch.Tensor, dout_k: torch.Tensor | None, q
         _rows("dout_k", dout_k, tuple(k.shape), k)
     dq, sq = _out("dq", dq, q, contiguous[0])
     dk, sk = _out("dk", dk, k, contiguous[1])
-    _plain("qk_norm_rotary_backward", dout_q, dout_k, q, k, q_w, k_w, cos, sin, dq, dk)
+    _plain("qk_norm_rotary_backward", dout_q, dout_k, q, k, q_w, k_w, cos, sin, *given)
     dim, device = sizes[-1], q.device
     dw = q_w.new_empty((1 if k is None else 2, dim))
     lib = _lib.load()

@@ -161,7 +161,7 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, bias: torch.Tensor | None = None
         _check_device_tensor("out", out, device)
         if out.dtype != w.dtype or tuple(out.shape) != (rows, w.n) or (out.stride(1) != 1 and w.n > 1):
             raise ValueError(f"out must be a {w.dtype} [{rows}, {w.n}] tensor with rows contiguous")
-    if not (plain(x, out) if bias is None else plain(x, bias, out)):
+    if not plain(*[t for t in (x, bias, given) if t is not None]):
         raise ValueError("int4_linear has no backward: call it under torch.no_grad()")
     _lib.ints(rows=rows)
     lib = _lib.load()
