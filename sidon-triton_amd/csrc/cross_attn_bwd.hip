@@ -11,11 +11,12 @@
 // S = Q . K^T and dP = dO . V^T by v_mfma_f32_32x32x16, whose accumulators, rounded, are the B
 // operands of dV^T += dO^T . P and dK^T += Q^T . dS; others own 32 queries and go over the keys:
 // S^T = K . Q^T, dP^T = V . dO^T, dQ^T += K^T . dS^T.  (Nine products, where one pass would do with five
-// if delta came from the rounded output and dq were added up across workgroups: here no atomics, so the
-// same bits every time.)  The tiles of 32 rows that the wavefronts of a workgroup share are copied global -> LDS by global_load_lds_dwordx4 one step
-// ahead, and read as they are and transposed.  (Where the second launch spills `4 * lane`, at D 128 but for one block of
-// either kind, at D 64 in two blocks of keys by four of queries and, queries first, in four by two of bf16, its reload
-// stands between the copies and waits for the ones just issued.)
+// if delta came from the rounded output and dq were added up across workgroups: here no atomics, so
+// the same bits every time.)  The tiles of 32 rows that the wavefronts of a workgroup share are
+// copied global -> LDS by global_load_lds_dwordx4 one step ahead, and read as they are and
+// transposed.  (Where the second launch spills `4 * lane`, at D 128 but for one block of either
+// kind, at D 64 in two blocks of keys by four of queries and, queries first, in four by two of
+// bf16, its reload stands between the copies and waits for the ones just issued.)
 //
 // fp16 holds P times 2^15, and dS times a power of two that keeps it below 2^15: the
 // bound |dS_ij| <= 2 |dout_i| |v_j| needs the longest v, and for dk the longest dout,
